@@ -5,16 +5,17 @@ Operator API; the work is done by hand-written CUDA behind a C ABI
 (``include/bsgemm.h``, loaded by ``cutlass_b200.lib``)."""
 from .arguments import (DenseTensor, EpilogueDescriptor, GemmArguments, GemmProblemSize, GroupedGemmArguments,
                         Mxfp8Quant, Nvfp4Quant, ScaledOperand, ScaleMode, ScaleSwizzleMode)
+from .int8 import int8_linear, quantize_int8
 from .operator import (AllocationRequirement, BlockScaledGemmOperator, CompiledArtifact,
-                       GroupedBlockScaledGemmOperator, NativeProvider, Operator, OperatorMetadata, Workspace, all_operators,
+                       GroupedBlockScaledGemmOperator, GroupedInt8GemmOperator, Int8GemmOperator, NativeProvider, Operator, OperatorMetadata, Workspace, all_operators,
                        get_operators, to_cuda_stream)
 from .quantize import quantize_blockscaled
 from .status import Status
 
 __all__ = [
     "AllocationRequirement", "BlockScaledGemmOperator", "CompiledArtifact", "DenseTensor", "EpilogueDescriptor",
-    "GemmArguments", "GemmProblemSize", "GroupedBlockScaledGemmOperator", "GroupedGemmArguments", "Mxfp8Quant", "NativeProvider", "Nvfp4Quant",
+    "GemmArguments", "GemmProblemSize", "GroupedBlockScaledGemmOperator", "GroupedGemmArguments", "GroupedInt8GemmOperator", "Int8GemmOperator", "Mxfp8Quant", "NativeProvider", "Nvfp4Quant",
     "Operator", "OperatorMetadata", "ScaleMode", "ScaleSwizzleMode", "ScaledOperand", "Status", "Workspace",
-    "all_operators", "get_operators", "quantize_blockscaled", "to_cuda_stream",
+    "all_operators", "get_operators", "int8_linear", "quantize_blockscaled", "quantize_int8", "to_cuda_stream",
 ]
 __version__ = "0.1.0"

@@ -7,6 +7,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
@@ -18,35 +19,56 @@ def lib_name(profile: bool) -> str:
 
 
 OUT = os.path.join(_HERE, "lib", lib_name(PROFILE))
-SOURCES = ["bsgemm.cu"]
-HEADERS = ["gemm_kernel.cuh", "quant_kernel.cuh", "ptx.cuh", os.path.join("..", "..", "include", "bsgemm.h")]
+SOURCES = {      # translation unit -> the headers it includes
+    "bsgemm.cu": ["gemm_kernel.cuh", "quant_kernel.cuh", "ptx.cuh", "host.h"],
+    "int8.cu": ["int8_kernel.cuh", "gemm_kernel.cuh", "ptx.cuh", "host.h"],
+}
+ABI_HEADER = os.path.join("..", "..", "include", "bsgemm.h")
 NVCC_FLAGS = [
-    "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "--shared", "-Xcompiler", "-fPIC", "-cudart", "static",
+    "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-cudart", "static",
 ]
+
+
+def _objects() -> list[tuple[str, str, bool]]:
+    """(source, object, is the object missing or older than what it is made from) of every translation unit."""
+    out = []
+    for src, headers in SOURCES.items():
+        obj = os.path.join(_HERE, "build", src + (".profile" if PROFILE else "") + ".o")
+        deps = [os.path.join(CSRC, f) for f in [src, ABI_HEADER] + headers]
+        fresh = os.path.exists(obj) and all(os.path.getmtime(d) <= os.path.getmtime(obj) for d in deps if os.path.exists(d))
+        out.append((os.path.join(CSRC, src), obj, not fresh))
+    return out
 
 
 def _stale() -> bool:
     if not os.path.exists(OUT):
         return True
     t = os.path.getmtime(OUT)
-    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
+    deps = {os.path.join(CSRC, f) for src, headers in SOURCES.items() for f in [src, ABI_HEADER] + headers}
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the CUDA library if it is missing or older than its sources; return its path."""
-    if not force and not _stale():
-        return OUT
-    nvcc = os.environ.get("NVCC", "nvcc")
-    os.makedirs(os.path.dirname(OUT), exist_ok=True)
-    extra = ["-DBSG_PROFILE"] if PROFILE else []
-    cmd = [nvcc] + NVCC_FLAGS + extra + (["-Xptxas", "-v"] if verbose else []) + ["-o", OUT] + [os.path.join(CSRC, f) for f in SOURCES]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
+def _nvcc(args: list[str]) -> str:
+    proc = subprocess.run([os.environ.get("NVCC", "nvcc")] + NVCC_FLAGS + args, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError("nvcc failed:\n" + proc.stdout + proc.stderr)
+    return proc.stderr
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    """Compile the CUDA library if it is missing or older than its sources; return its path.  Translation units are
+    compiled side by side, and only those whose sources changed."""
+    if not force and not _stale():
+        return OUT
+    units = _objects()
+    os.makedirs(os.path.dirname(OUT), exist_ok=True)
+    os.makedirs(os.path.join(_HERE, "build"), exist_ok=True)
+    extra = (["-DBSG_PROFILE"] if PROFILE else []) + (["-Xptxas", "-v"] if verbose else [])
+    with ThreadPoolExecutor() as pool:
+        logs = list(pool.map(lambda u: _nvcc(extra + ["-c", "-o", u[1], u[0]]), [u for u in units if force or u[2]]))
+    _nvcc(["--shared", "-o", OUT] + [u[1] for u in units])
     if verbose:
-        sys.stderr.write(proc.stderr)
+        sys.stderr.write("".join(logs))
     return OUT
 
 

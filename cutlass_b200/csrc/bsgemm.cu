@@ -16,6 +16,7 @@
 
 #include "../../include/bsgemm.h"
 #include "gemm_kernel.cuh"
+#include "host.h"
 #include "quant_kernel.cuh"
 
 namespace {
@@ -891,6 +892,24 @@ static int32_t rs_upload_out_maps(bsg_rs_comm* c) {
   c->maps_uploaded = true;
   return BSG_OK;
 }
+
+// Host helpers of the other translation units (host.h).
+namespace bsg {
+int32_t host_fail(int32_t code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+int32_t host_operand_map(CUtensorMap* map, const void* base, uint64_t row_bytes, uint64_t rows, uint64_t batches, uint64_t pitch_bytes,
+                         uint64_t batch_stride_bytes, uint32_t box_rows) {
+  return make_operand_map(map, base, row_bytes, rows, batches, pitch_bytes, batch_stride_bytes, box_rows);
+}
+int32_t host_out_map(CUtensorMap* map, const void* base, int32_t out_kind, uint64_t cols, uint64_t rows, uint64_t pitch_elems) {
+  return make_out_map(map, base, out_kind, cols, rows, 1, pitch_elems, rows * pitch_elems);
+}
+}  // namespace bsg
 
 extern "C" {
 

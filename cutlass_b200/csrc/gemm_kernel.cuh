@@ -313,7 +313,7 @@ __device__ __forceinline__ TileInfo decode_tile(const Ctl* ctl, const GemmParams
 
 // Slow path of a barrier wait; only reached when the fast spin gave up, i.e. when
 // something is wrong or the machine is badly oversubscribed.  Bounded by SM cycles.
-__device__ __noinline__ uint32_t slow_wait(uint32_t bar, uint32_t parity, Ctl* ctl) {
+static __device__ __noinline__ uint32_t slow_wait(uint32_t bar, uint32_t parity, Ctl* ctl) {
   const long long t0 = clock64();
   while (true) {
     if (ptx::mbar_spin(bar, parity, 64)) return 1;
@@ -477,7 +477,7 @@ __device__ __forceinline__ void tp_wait_read(uint32_t n) {
 
 // Side-stream helpers of the copy-engine mode of the tensor-parallel GEMM.
 // Waits (bounded) until every peer has launched call `epoch`, i.e. its gathered buffer may be overwritten.
-__global__ void tp_wait_peers_kernel(const uint32_t* sync, int world, int rank, uint32_t epoch, uint32_t* status) {
+static __global__ void tp_wait_peers_kernel(const uint32_t* sync, int world, int rank, uint32_t epoch, uint32_t* status) {
   if (threadIdx.x != 0) return;
   const long long t0 = clock64();
   for (int q = 0; q < world; ++q) {
@@ -490,7 +490,7 @@ __global__ void tp_wait_peers_kernel(const uint32_t* sync, int world, int rank, 
 }
 // Announces `blocks` row blocks (starting at `first`) as arrived in a peer's buffer: stream order puts
 // this after the copy-engine transfers that filled them.
-__global__ void tp_announce_kernel(uint32_t* peer_flags, int first, int blocks, uint32_t add) {
+static __global__ void tp_announce_kernel(uint32_t* peer_flags, int first, int blocks, uint32_t add) {
   const int i = threadIdx.x;
   if (i < blocks) {
     __threadfence_system();

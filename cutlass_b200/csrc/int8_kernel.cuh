@@ -1,0 +1,858 @@
+// Matrix product in 8-bit integers with one scale per token (row of A) and one per output channel (row of B):
+//
+//   q[m,k] = sign(x) floor(127 |x[m,k]| / a_m + 1/2),  a_m = max_k |x[m,k]|,  sa[m] = a_m / 127
+//   D[m,n] = act(sa[m] * sb[n] * sum_k q[m,k] w[n,k] + bias[n])
+//
+// The sum is a 32-bit integer and exact (K <= 131071: 127 * 127 * K < 2^31), so neither the order of the additions nor
+// a split of K changes a result.  Three kernels:
+//
+//   bsg_i8_quant_kernel   tokens -> 8 bits; bound by HBM
+//   bsg_i8_rows_kernel    many rows: tokens are the M side of the MMA; bound by the tensor pipe
+//   bsg_i8_few_kernel     few rows (one token to a few hundred): the output channels are the M side of the MMA and the
+//                         tokens its N side, so that the tile carries no padding rows; bound by reading the weights
+//
+// The two products are dense (one group of rows) or grouped (ragged rows per group, end rows on the device).
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cstdint>
+
+#include "gemm_kernel.cuh"
+#include "ptx.cuh"
+
+namespace bsg {
+
+constexpr int kI8MaxK = 131071;
+
+// ------------------------------------------------------------------------------------------------ quantiser
+struct I8QuantParams {
+  const uint16_t* X;         // bf16 or fp16 bits
+  const int32_t* index;      // row r of Q is made from row index[r] of X; null: from row r
+  int8_t* Q;
+  float* scale;
+  int64_t ldx, ldq;          // elements
+  int32_t rows, tokens, K;
+  int32_t fp16;
+  int32_t wide;              // rows of X and Q start on 16- / 8-byte boundaries
+};
+
+__device__ __forceinline__ float i8_unpack(uint32_t bits16, bool fp16) {
+  return fp16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(bits16))) : __uint_as_float(bits16 << 16);
+}
+
+// max(|a|, |b|) of two packed pairs; a NaN operand gives NaN.  (The sign bits of the result are not meaningful.)
+template <bool FP16>
+__device__ __forceinline__ uint32_t i8_maxabs2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (FP16) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a & 0x7FFF7FFFu), "r"(b & 0x7FFF7FFFu));
+  else asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// Level of one value.  `inv` is 127 / amax, enlarged by 2^-21: the distance of 127 |x| / amax from the next half
+// k + 1/2 is 0 or, for 16-bit x and amax, at least 2^-19 of its size (254 |x| - (2k + 1) amax is a multiple of the
+// smaller operand's last place), so the enlarged product, whose own roundings amount to 2^-23, lies above every half
+// that the exact ratio reaches and below every half that it does not: rounding to nearest gives
+// floor(127 |x| / amax + 1/2) without a division per value.
+__device__ __forceinline__ int i8_level(float x, float pre, float inv) { return __float2int_rn(__fmul_rn(__fmul_rn(x, pre), inv)); }
+
+struct I8Scale {
+  float scale;     // amax / 127; NaN for a row that holds a NaN or an infinity, 0 for a row of zeros
+  float pre, inv;  // levels are rn(x * pre * inv); both 0 where the scale is 0 or NaN
+};
+__device__ __forceinline__ I8Scale i8_scale(float amax) {
+  I8Scale s;
+  s.scale = __fdiv_rn(amax, 127.0f);
+  s.pre = 1.0f;
+  if (!(amax < __uint_as_float(0x7F800000u))) {
+    s.scale = __uint_as_float(0x7FC00000u);
+    s.pre = s.inv = 0.0f;
+  } else if (amax == 0.0f) {
+    s.pre = s.inv = 0.0f;
+  } else {
+    // 127 / amax leaves fp32's range below 2^-121: such rows are scaled by 2^64 first (exact)
+    if (amax < 0x1p-64f) s.pre = 0x1p64f;
+    s.inv = __fmul_rn(__fdiv_rn(127.0f, __fmul_rn(amax, s.pre)), 1.0f + 0x1p-21f);
+  }
+  return s;
+}
+
+__device__ __forceinline__ uint32_t i8_pack4(int a, int b, int c, int d) {
+  return (uint32_t(a) & 0xFFu) | ((uint32_t(b) & 0xFFu) << 8) | ((uint32_t(c) & 0xFFu) << 16) | (uint32_t(d) << 24);
+}
+
+// Eight consecutive values of a row, zeros past its end.
+__device__ __forceinline__ uint4 i8_load8(const uint16_t* row, int32_t k, int32_t K, bool wide) {
+  if (wide && k + 8 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t lo = k + 2 * j < K ? uint32_t(__ldg(row + k + 2 * j)) : 0u;
+    const uint32_t hi = k + 2 * j + 1 < K ? uint32_t(__ldg(row + k + 2 * j + 1)) : 0u;
+    w[j] = lo | (hi << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <bool FP16>
+__device__ __forceinline__ uint2 i8_levels8(const uint4& v, const I8Scale& s) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  int q[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    q[2 * j] = i8_level(i8_unpack(w[j] & 0xFFFFu, FP16), s.pre, s.inv);
+    q[2 * j + 1] = i8_level(i8_unpack(w[j] >> 16, FP16), s.pre, s.inv);
+  }
+  // A NaN or infinity times 0 is NaN, which converts to 0.
+  return make_uint2(i8_pack4(q[0], q[1], q[2], q[3]), i8_pack4(q[4], q[5], q[6], q[7]));
+}
+
+// TPR threads own a row; a thread holds kI8Chunks groups of 8 values in registers between the maximum and the rounding, so
+// a row of up to TPR * 64 values is read once.  Longer rows are read a second time (from L2).
+constexpr int kI8Chunks = 8;
+constexpr int kI8QuantThreads = 256;
+template <int TPR, bool FP16>
+__global__ void __launch_bounds__(TPR > kI8QuantThreads ? TPR : kI8QuantThreads) bsg_i8_quant_kernel(const I8QuantParams p) {
+  constexpr int kThreads = TPR > kI8QuantThreads ? TPR : kI8QuantThreads;
+  constexpr int kRows = kThreads / TPR;
+  const int t = threadIdx.x % TPR;
+  const int32_t r = blockIdx.x * kRows + threadIdx.x / TPR;
+  __shared__ float s_max[kThreads / 32];
+  // The product behind may start its set-up now (and fetch weights: what it reads besides this kernel's results is older).
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  const bool row_ok = r < p.rows;
+  int32_t src = r;
+  if (row_ok && p.index) src = __ldg(p.index + r);
+  const bool src_ok = row_ok && src >= 0 && src < p.tokens;
+  const uint16_t* row = p.X + (src_ok ? int64_t(src) * p.ldx : 0);
+  const int32_t K = src_ok ? p.K : 0;
+  const bool wide = p.wide != 0;
+  uint4 v[kI8Chunks];
+  uint32_t m = 0;
+#pragma unroll
+  for (int c = 0; c < kI8Chunks; ++c) v[c] = i8_load8(row, (c * TPR + t) * 8, K, wide);
+#pragma unroll
+  for (int c = 0; c < kI8Chunks; ++c)
+    m = i8_maxabs2<FP16>(m, i8_maxabs2<FP16>(i8_maxabs2<FP16>(v[c].x, v[c].y), i8_maxabs2<FP16>(v[c].z, v[c].w)));
+  for (int32_t k = (kI8Chunks * TPR + t) * 8; k < K; k += TPR * 8) {
+    const uint4 u = i8_load8(row, k, K, wide);
+    m = i8_maxabs2<FP16>(m, i8_maxabs2<FP16>(i8_maxabs2<FP16>(u.x, u.y), i8_maxabs2<FP16>(u.z, u.w)));
+  }
+  m &= 0x7FFF7FFFu;
+  float amax = ptx::fmax_nan(i8_unpack(m & 0xFFFFu, FP16), i8_unpack(m >> 16, FP16));
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) amax = ptx::fmax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if constexpr (TPR > 32) {
+    if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = amax;
+    __syncthreads();
+    const int w0 = (threadIdx.x / TPR) * (TPR / 32);
+    amax = s_max[w0];
+#pragma unroll
+    for (int w = 1; w < TPR / 32; ++w) amax = ptx::fmax_nan(amax, s_max[w0 + w]);
+  }
+  if (!row_ok) return;
+  I8Scale s = i8_scale(amax);
+  // a row whose index names no token: zeros with a NaN scale, so that a product that uses it shows it
+  if (!src_ok) s.scale = __uint_as_float(0x7FC00000u);
+  if (t == 0) p.scale[r] = s.scale;
+  int8_t* out = p.Q + int64_t(r) * p.ldq;
+  auto store = [&](int32_t k, const uint4& u) {
+    const uint2 q = i8_levels8<FP16>(u, s);
+    if (wide && k + 8 <= p.K) {
+      *reinterpret_cast<uint2*>(out + k) = q;
+    } else {
+      for (int j = 0; j < 8 && k + j < p.K; ++j) out[k + j] = int8_t((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
+    }
+  };
+#pragma unroll
+  for (int c = 0; c < kI8Chunks; ++c) {
+    const int32_t k = (c * TPR + t) * 8;
+    if (k < p.K) store(k, v[c]);
+  }
+  for (int32_t k = (kI8Chunks * TPR + t) * 8; k < p.K; k += TPR * 8) store(k, i8_load8(row, k, K, wide));
+}
+
+// ------------------------------------------------------------------------------------------------ products
+struct I8GemmParams {
+  int32_t num_groups;         // 1 for a dense product
+  int32_t total_rows, N, K;
+  const int32_t* offsets;     // grouped: end row of each group (device); null: one group with all rows
+  int32_t tiles_n, band;
+  int32_t out_kind;           // kOutBf16, kOutF16 or kOutF32
+  int32_t activation;
+  int32_t tma_out;            // rows kernel: D's address and pitch allow TMA stores
+  int32_t tma_edge;           // ... and a row is whole 16-byte pieces: a store that crosses the last column writes up to the next
+                              // 16-byte boundary, so otherwise the last columns are copied
+  const float* sa;            // [total_rows]
+  const float* sb;            // [num_groups][N]
+  const float* bias;          // [num_groups][N] or null
+  void* D;
+  int64_t ldd;                // elements
+  uint32_t* status;
+};
+
+struct alignas(16) I8Ctl {
+  uint64_t full[8];
+  uint64_t empty[8];
+  uint64_t tmem_full[2];
+  uint64_t tmem_empty[2];
+  uint32_t tmem_base;
+  volatile uint32_t abort;
+  int32_t total_tiles;
+  int32_t pad;
+  int32_t tile_start[kMaxGroups + 1];
+  int32_t end[kMaxGroups];
+};
+constexpr int kI8CtlBytes = 3072;
+static_assert(sizeof(I8Ctl) <= kI8CtlBytes, "control block");
+
+static __device__ __noinline__ uint32_t i8_slow_wait(uint32_t bar, uint32_t parity, I8Ctl* ctl) {
+  const long long t0 = clock64();
+  while (true) {
+    if (ptx::mbar_spin(bar, parity, 64)) return 1;
+    if (clock64() - t0 > (ctl->abort ? 40000ll : 4000000000ll)) break;      // ~20 us once aborting, else ~2 s
+  }
+  ctl->abort = 1;
+  return 0;
+}
+// Bounded wait; `dead` makes later waits of this thread short once one has run out.
+__device__ __forceinline__ void i8_wait(uint32_t bar, uint32_t parity, I8Ctl* ctl, uint32_t& dead) {
+  uint32_t ok = ptx::mbar_spin(bar, parity, dead ? 16u : 100000u);
+  if (!ok) {
+    ok = dead ? 0u : i8_slow_wait(bar, parity, ctl);
+    if (!ok) dead = 1;
+  }
+}
+
+// kind::i8: signed 8-bit operands, 32-bit integer accumulator, K = 32 per instruction.
+template <int CG>
+__device__ __forceinline__ void i8_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 2)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__host__ __device__ constexpr uint32_t i8_idesc(uint32_t m, uint32_t n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);      // D s32, A s8, B s8, both K-major
+}
+__device__ __forceinline__ void i8_tmem_ld_x16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Group table, built by one whole warp: end row and first tile of every group.  End rows that fall, or that leave
+// [0, total_rows], are clamped and reported.
+__device__ __forceinline__ void i8_build_groups(I8Ctl* ctl, const I8GemmParams& p, int32_t tile_rows) {
+  const int lane = threadIdx.x & 31;
+  int32_t prev_end = 0, tiles = 0;
+  bool bad = false;
+  for (int base = 0; base < p.num_groups; base += 32) {
+    const int g = base + lane;
+    const bool in = g < p.num_groups;
+    const int32_t raw = !in ? 0 : p.offsets ? __ldg(p.offsets + g) : p.total_rows;
+    int32_t end = min(max(raw, 0), p.total_rows);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int32_t up = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end = max(end, up);
+    }
+    end = max(end, prev_end);
+    if (in && end != raw) bad = true;
+    int32_t begin = __shfl_up_sync(0xffffffffu, end, 1);
+    if (lane == 0) begin = prev_end;
+    const int32_t mine = in ? ((end - begin + tile_rows - 1) / tile_rows) * p.tiles_n : 0;
+    int32_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int32_t up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    if (in) {
+      ctl->end[g] = end;
+      ctl->tile_start[g] = tiles + upto - mine;
+    }
+    tiles += __shfl_sync(0xffffffffu, upto, 31);
+    prev_end = __shfl_sync(0xffffffffu, end, 31);
+  }
+  if (lane == 0) {
+    ctl->tile_start[p.num_groups] = tiles;
+    ctl->total_tiles = tiles;
+  }
+  if (bad) atomicOr(p.status, kStBadOffsets);
+}
+
+struct I8Tile {
+  int32_t g, tm, tn, row0, row_end;
+};
+// Tile t of the walk: groups in order; inside a group bands of `band` row tiles, rows fastest.
+__device__ __forceinline__ I8Tile i8_decode(const I8Ctl* ctl, const I8GemmParams& p, int32_t t, int32_t tile_rows) {
+  int lo = 0, hi = p.num_groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (ctl->tile_start[mid] <= t) lo = mid; else hi = mid;
+  }
+  I8Tile ti;
+  ti.g = lo;
+  const int32_t begin = lo ? ctl->end[lo - 1] : 0;
+  ti.row_end = ctl->end[lo];
+  const int32_t local = t - ctl->tile_start[lo];
+  const int32_t tiles_m = (ti.row_end - begin + tile_rows - 1) / tile_rows;
+  const int32_t per_band = p.band * p.tiles_n;
+  const int32_t b = local / per_band, rem = local - b * per_band;
+  const int32_t bh = min(p.band, tiles_m - b * p.band);
+  ti.tm = b * p.band + rem % bh;
+  ti.tn = rem / bh;
+  ti.row0 = begin + ti.tm * tile_rows;
+  return ti;
+}
+
+// The bias is 0 where there is none: adding it then changes nothing (a sum of -0 becomes +0).
+__device__ __forceinline__ float i8_finish(uint32_t acc, float sa, float sb, float bias) {
+  return __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(int32_t(acc)), sa), sb), bias);
+}
+// Activation of a register tile, behind one branch and in a loop that is not unrolled: inlined at every value, its code was
+// larger than the instruction caches and a 256-column epilogue took 28 us instead of 2.
+template <int N>
+__device__ __forceinline__ void i8_activate(float (&x)[N], int act) {
+  if (act == kActIdentity) return;
+  if (act == kActRelu) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = apply_activation(x[j], kActRelu);
+  } else if (act == kActGelu) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = apply_activation(x[j], kActGelu);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = apply_activation(x[j], kActSilu);
+  }
+}
+
+// ---- many rows: D tile = (128 * CG rows) x BN columns, persistent, two accumulators of BN columns in tensor memory
+template <int CG, int BN>
+struct I8RowsCfg {
+  static constexpr int kTileM = 128 * CG;
+  static constexpr int kABytes = 128 * 128;
+  static constexpr int kBRows = BN / CG;
+  static constexpr int kBBytes = kBRows * 128;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kEpiBytes = 4 * 4096;
+  static constexpr int kColBytes = 2 * 2 * BN * 4;        // scale and bias of the tile's columns, two tiles
+  static constexpr int kStagesRaw = (232448 - 1024 - kI8CtlBytes - kEpiBytes - kColBytes) / kStageBytes;
+  static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + kColBytes + kI8CtlBytes + 1024;
+  static constexpr int kTmemCols = 2 * BN;
+  static_assert(kTmemCols == 64 || kTmemCols == 128 || kTmemCols == 256 || kTmemCols == 512, "tensor-memory columns");
+};
+
+template <int CG, int BN>
+__global__ void __launch_bounds__(192, 1)
+bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ CUtensorMap tmD, const I8GemmParams p) {
+  using C = I8RowsCfg<CG, BN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + C::kStages * C::kABytes;
+  uint8_t* sEpi = sB + C::kStages * C::kBBytes;
+  float* sCol = reinterpret_cast<float*>(sEpi + C::kEpiBytes);
+  I8Ctl* ctl = reinterpret_cast<I8Ctl*>(sEpi + C::kEpiBytes + C::kColBytes);
+
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const uint32_t cta_rank = CG == 2 ? ptx::cluster_ctarank() : 0u;
+  const bool is_leader = cta_rank == 0;
+  const int32_t cluster_idx = CG == 2 ? int32_t(ptx::cluster_id_x()) : int32_t(blockIdx.x);
+  const int32_t num_clusters = CG == 2 ? int32_t(ptx::num_clusters_x()) : int32_t(gridDim.x);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&ctl->full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&ctl->empty[s]), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&ctl->tmem_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&ctl->tmem_empty[s]), 4 * CG);
+    }
+    ctl->abort = 0;
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async();
+  }
+  if (warp == 5 && lane == 0) {
+    ptx::prefetch_tmap(&tmA);
+    ptx::prefetch_tmap(&tmB);
+    ptx::prefetch_tmap(&tmD);
+  }
+  if (warp == 4) {
+    ptx::tmem_alloc<CG>(ptx::smem_u32(&ctl->tmem_base), C::kTmemCols);
+    ptx::tmem_relinquish<CG>();
+  }
+  // Launched behind the quantiser with programmatic stream serialisation: from here on its results are read.
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  if (warp == 0) i8_build_groups(ctl, p, C::kTileM);
+  __syncwarp();
+  ptx::tc_fence_before();
+  if constexpr (CG == 2) { ptx::cluster_arrive(); ptx::cluster_wait(); } else { __syncthreads(); }
+  ptx::tc_fence_after();
+
+  const uint32_t tmem_base = bcast(ctl->tmem_base);
+  const int32_t total_tiles = bcast(ctl->total_tiles);
+  const int32_t k_tiles = (p.K + 127) / 128;
+  uint32_t dead = 0;
+
+  if (warp == 5) {
+    // ---------------------------------------------------------------- TMA producer
+    const uint32_t elected = ptx::elect_one_sync();
+    const uint32_t sA0 = ptx::smem_u32(sA), sB0 = ptx::smem_u32(sB);
+    const uint32_t full0 = ptx::smem_u32(&ctl->full[0]), empty0 = ptx::smem_u32(&ctl->empty[0]);
+    const uint32_t full0_leader = CG == 2 ? ptx::mapa(full0, 0) : full0;
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int32_t t = cluster_idx; t < total_tiles; t += num_clusters) {
+      const I8Tile ti = i8_decode(ctl, p, t, C::kTileM);
+      const int32_t a_row = bcast(ti.row0 + int32_t(cta_rank) * 128);
+      const int32_t b_row = bcast(ti.tn * BN + int32_t(cta_rank) * C::kBRows);
+      const int32_t g = bcast(ti.g);
+      for (int32_t kt = 0; kt < k_tiles; ++kt) {
+        i8_wait(empty0 + stage * 8, phase ^ 1u, ctl, dead);
+        if (elected && !dead) {
+          if (is_leader) ptx::mbar_arrive_expect_tx(full0 + stage * 8, uint32_t(C::kStageBytes) * CG);
+          const uint32_t bar = full0_leader + stage * 8;
+          ptx::tma_load_3d<CG>(sA0 + stage * C::kABytes, &tmA, bar, kt * 128, a_row, 0);
+          ptx::tma_load_3d<CG>(sB0 + stage * C::kBBytes, &tmB, bar, kt * 128, b_row, g);
+        }
+        if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    // Every stage must have been released before this CTA leaves: no commit is then in flight towards it.
+    for (int s = 0; s < C::kStages; ++s) {
+      i8_wait(empty0 + stage * 8, phase ^ 1u, ctl, dead);
+      if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+    }
+    if (dead) atomicOr(p.status, kStTimeoutEmpty);
+  } else if (warp == 4) {
+    // ---------------------------------------------------------------- MMA issue
+    if (is_leader) {
+      constexpr uint32_t idesc = i8_idesc(C::kTileM, BN);
+      const uint32_t elected = ptx::elect_one_sync();
+      const uint32_t sA0 = ptx::smem_u32(sA), sB0 = ptx::smem_u32(sB);
+      const uint32_t full0 = ptx::smem_u32(&ctl->full[0]), empty0 = ptx::smem_u32(&ctl->empty[0]);
+      const uint32_t tfull0 = ptx::smem_u32(&ctl->tmem_full[0]), tempty0 = ptx::smem_u32(&ctl->tmem_empty[0]);
+      int stage = 0;
+      uint32_t phase = 0, ready = 0;
+      int32_t it = 0;
+      for (int32_t t = cluster_idx; t < total_tiles; t += num_clusters, ++it) {
+        const int acc = it & 1;
+        const uint32_t d_tmem = tmem_base + uint32_t(acc) * BN;
+        i8_wait(tempty0 + acc * 8, (uint32_t(it >> 1) & 1u) ^ 1u, ctl, dead);
+        ptx::tc_fence_after();
+        for (int32_t kt = 0; kt < k_tiles; ++kt) {
+          if (!ready) i8_wait(full0 + stage * 8, phase, ctl, dead);
+          int next_stage = stage + 1;
+          uint32_t next_phase = phase;
+          if (next_stage == C::kStages) { next_stage = 0; next_phase ^= 1u; }
+          ready = ptx::mbar_spin_test(full0 + next_stage * 8, next_phase, 1);
+          ptx::tc_fence_after();
+          const uint64_t a_desc = make_desc_sw128(sA0 + stage * C::kABytes);
+          const uint64_t b_desc = make_desc_sw128(sB0 + stage * C::kBBytes);
+          if (elected && !dead) {
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb) i8_mma<CG>(d_tmem, a_desc + 2 * kb, b_desc + 2 * kb, idesc, kb > 0 || kt > 0);
+            ptx::umma_commit<CG>(empty0 + stage * 8);
+          }
+          stage = next_stage;
+          phase = next_phase;
+        }
+        if (elected && !dead) ptx::umma_commit<CG>(tfull0 + acc * 8);
+      }
+      if (dead) atomicOr(p.status, kStTimeoutFull | kStTimeoutTmemEmpty);
+    }
+  } else {
+    // ---------------------------------------------------------------- epilogue (warps 0-3: one quarter of the rows each)
+    const uint32_t tfull0 = ptx::smem_u32(&ctl->tmem_full[0]), tempty0 = ptx::smem_u32(&ctl->tmem_empty[0]);
+    uint8_t* stage_buf = sEpi + warp * 4096;
+    const int out_kind = p.out_kind, act = p.activation;
+    const bool f32 = out_kind == kOutF32, has_bias = p.bias != nullptr;
+    int32_t it = 0;
+    for (int32_t t = cluster_idx; t < total_tiles; t += num_clusters, ++it) {
+      const I8Tile ti = i8_decode(ctl, p, t, C::kTileM);
+      const int acc = it & 1;
+      const int32_t col0 = ti.tn * BN;
+      // scales and bias of the tile's columns, while its products are still being summed
+      float* cs = sCol + acc * 2 * BN;
+      for (int c = threadIdx.x; c < BN; c += 128) {
+        const bool in = col0 + c < p.N;
+        const int64_t at = int64_t(ti.g) * p.N + col0 + c;
+        cs[c] = in ? __ldg(p.sb + at) : 0.0f;
+        cs[BN + c] = in && has_bias ? __ldg(p.bias + at) : 0.0f;
+      }
+      const int32_t warp_row0 = ti.row0 + int32_t(cta_rank) * 128 + warp * 32;
+      const int32_t rows_here = min(32, ti.row_end - warp_row0);
+      const float sa = lane < rows_here ? __ldcg(p.sa + warp_row0 + lane) : 0.0f;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      i8_wait(tfull0 + acc * 8, uint32_t(it >> 1) & 1u, ctl, dead);
+      __syncwarp();
+      ptx::tc_fence_after();
+      const uint32_t lane_addr = tmem_base + (uint32_t(warp * 32) << 16) + uint32_t(acc) * BN;
+      // Whole warps of rows leave by TMA; the warp that holds a group's last rows, and outputs whose rows do not start
+      // on 16 bytes, are copied row by row from the same staging tile.
+      const bool tma = p.tma_out != 0 && rows_here == 32;
+#pragma unroll 1
+      for (int c0 = 0; c0 < BN; c0 += 32) {
+        uint32_t v[32];
+        ptx::tmem_ld_32x32b_x32(lane_addr + c0, v);
+        ptx::tmem_ld_wait();
+        if (c0 + 32 == BN) {
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {       // relaxed: what is handed back is tensor memory, whose reads have completed
+            if constexpr (CG == 2) ptx::mbar_arrive_remote_relaxed(ptx::mapa(tempty0 + acc * 8, 0));
+            else ptx::mbar_arrive_relaxed(tempty0 + acc * 8);
+          }
+        }
+        if (rows_here <= 0 || col0 + c0 >= p.N) continue;
+        float x[32];
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 s4 = *reinterpret_cast<const float4*>(cs + c0 + j);
+          const float4 b4 = *reinterpret_cast<const float4*>(cs + BN + c0 + j);
+          x[j + 0] = i8_finish(v[j + 0], sa, s4.x, b4.x);
+          x[j + 1] = i8_finish(v[j + 1], sa, s4.y, b4.y);
+          x[j + 2] = i8_finish(v[j + 2], sa, s4.z, b4.z);
+          x[j + 3] = i8_finish(v[j + 3], sa, s4.w, b4.w);
+        }
+        i8_activate(x, act);
+        // Staging tile: 32 rows of 128 bytes (64 columns of 16 bits or 32 of 32 bits), 16-byte chunk c of row r at chunk c ^ (r & 7).
+        const int half = f32 ? 0 : (c0 >> 5) & 1;
+        if (half == 0) {
+          if (tma && lane == 0) ptx::bulk_wait_group_read<0>();
+          __syncwarp();
+        }
+        if (f32) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<float4*>(stage_buf + lane * 128 + ((q ^ (lane & 7)) * 16)) = make_float4(x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint4 o;
+            if (out_kind == kOutBf16)
+              o = make_uint4(pack_bf16x2(x[q * 8], x[q * 8 + 1]), pack_bf16x2(x[q * 8 + 2], x[q * 8 + 3]), pack_bf16x2(x[q * 8 + 4], x[q * 8 + 5]), pack_bf16x2(x[q * 8 + 6], x[q * 8 + 7]));
+            else
+              o = make_uint4(pack_f16x2(x[q * 8], x[q * 8 + 1]), pack_f16x2(x[q * 8 + 2], x[q * 8 + 3]), pack_f16x2(x[q * 8 + 4], x[q * 8 + 5]), pack_f16x2(x[q * 8 + 6], x[q * 8 + 7]));
+            *reinterpret_cast<uint4*>(stage_buf + lane * 128 + (((half * 4 + q) ^ (lane & 7)) * 16)) = o;
+          }
+        }
+        // 16-bit output: the tile is full after two steps, or at the last columns of the matrix
+        const bool full = f32 || half == 1 || col0 + c0 + 32 >= p.N;
+        if (!full) continue;
+        const int32_t out_col = col0 + c0 - 32 * half;
+        if (tma && (p.tma_edge || out_col + (f32 ? 32 : 64) <= p.N)) {
+          ptx::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            ptx::tma_store_3d(&tmD, ptx::smem_u32(stage_buf), out_col, warp_row0, 0);
+            ptx::bulk_commit_group();
+          }
+        } else {
+          __syncwarp();
+          const int32_t cols = min(f32 ? 32 : 64, p.N - out_col);
+          for (int r = 0; r < rows_here; ++r) {
+            const uint8_t* srow = stage_buf + r * 128;
+            for (int c = lane; c < cols; c += 32) {
+              if (f32)
+                reinterpret_cast<float*>(p.D)[int64_t(warp_row0 + r) * p.ldd + out_col + c] =
+                    *reinterpret_cast<const float*>(srow + (((c >> 2) ^ (r & 7)) * 16) + (c & 3) * 4);
+              else
+                reinterpret_cast<uint16_t*>(p.D)[int64_t(warp_row0 + r) * p.ldd + out_col + c] =
+                    *reinterpret_cast<const uint16_t*>(srow + (((c >> 3) ^ (r & 7)) * 16) + (c & 7) * 2);
+            }
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) ptx::bulk_wait_group<0>();
+    if (dead) atomicOr(p.status, kStTimeoutTmemFull);
+  }
+
+  if (ctl->abort) {      // copies and MMAs that may still be in flight land before the memory is handed back
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000ll) __nanosleep(1000);
+  }
+  __syncwarp();
+  ptx::tc_fence_before();
+  if constexpr (CG == 2) { ptx::cluster_arrive(); ptx::cluster_wait(); } else { __syncthreads(); }
+  if (warp == 4) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<CG>(tmem_base, C::kTmemCols);
+  }
+}
+
+// ---- few rows: D^T tile = 128 channels x BT tokens.  The CTAs of a cluster (`split` of them) take consecutive parts of K of
+// one tile; each sends the columns that another one finishes into that CTA's shared memory, and each finishes BT / split.
+template <int BT>
+struct I8FewCfg {
+  static constexpr int kWBytes = 128 * 128;
+  static constexpr int kTBytes = BT * 128;
+  static constexpr int kStageBytes = kWBytes + kTBytes;
+  static constexpr int kRedBytes = BT <= 64 ? BT * 512 : 0;           // [split][BT / split][128] int32; wider tiles do not split
+  static constexpr int kStagesRaw = (115712 - 1024 - kI8CtlBytes - kRedBytes) / kStageBytes;     // two CTAs per SM
+  static constexpr int kStages = kStagesRaw > 6 ? 6 : kStagesRaw;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kRedBytes + kI8CtlBytes + 1024;
+  static constexpr int kTmemCols = 2 * BT;
+  static_assert(kStages >= 3, "stages");
+};
+
+// Column of N values (tokens) of one channel; consecutive lanes hold consecutive channels.
+template <int N>
+__device__ __forceinline__ void i8_put(const I8GemmParams& p, const float (&x)[N], int n_here, int64_t at) {
+  if (p.out_kind == kOutBf16) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j < n_here) reinterpret_cast<__nv_bfloat16*>(p.D)[at + j * p.ldd] = __float2bfloat16_rn(x[j]);
+    }
+  } else if (p.out_kind == kOutF16) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j < n_here) reinterpret_cast<__half*>(p.D)[at + j * p.ldd] = __float2half_rn(x[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j < n_here) reinterpret_cast<float*>(p.D)[at + j * p.ldd] = x[j];
+    }
+  }
+}
+
+template <int BT>
+__global__ void __launch_bounds__(192, 2)
+bsg_i8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const I8GemmParams p, const int32_t split) {
+  using C = I8FewCfg<BT>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sW = smem;
+  uint8_t* sT = sW + C::kStages * C::kWBytes;
+  uint8_t* sRed = sT + C::kStages * C::kTBytes;
+  I8Ctl* ctl = reinterpret_cast<I8Ctl*>(sRed + C::kRedBytes);
+
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0);
+  const int lane = threadIdx.x & 31;
+  const int32_t rank = split > 1 ? int32_t(ptx::cluster_ctarank()) : 0;
+  const int32_t worker = int32_t(blockIdx.x) / split, workers = int32_t(gridDim.x) / split;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&ctl->full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&ctl->empty[s]), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&ctl->tmem_full[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&ctl->tmem_empty[s]), 4);
+    }
+    ctl->abort = 0;
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async();
+  }
+  if (warp == 5 && lane == 0) {
+    ptx::prefetch_tmap(&tmW);
+    ptx::prefetch_tmap(&tmX);
+  }
+  if (warp == 4) {
+    ptx::tmem_alloc<1>(ptx::smem_u32(&ctl->tmem_base), C::kTmemCols);
+    ptx::tmem_relinquish<1>();
+  }
+  // The group table needs the end rows only, which are older than the quantiser this kernel may overlap with.
+  if (warp == 0) i8_build_groups(ctl, p, BT);
+  __syncwarp();
+  ptx::tc_fence_before();
+  if (split > 1) { ptx::cluster_arrive(); ptx::cluster_wait(); } else { __syncthreads(); }
+  ptx::tc_fence_after();
+
+  const uint32_t tmem_base = bcast(ctl->tmem_base);
+  const int32_t total_tiles = bcast(ctl->total_tiles);
+  const int32_t k_all = (p.K + 127) / 128;
+  const int32_t kt0 = int32_t(int64_t(k_all) * rank / split), kt1 = int32_t(int64_t(k_all) * (rank + 1) / split);
+  uint32_t dead = 0;
+
+  if (warp == 5) {
+    // ---------------------------------------------------------------- TMA producer
+    // The weights do not depend on the quantiser in front: the first stages' weights are asked for before waiting for it.
+    const uint32_t elected = ptx::elect_one_sync();
+    const uint32_t sW0 = ptx::smem_u32(sW), sT0 = ptx::smem_u32(sT);
+    const uint32_t full0 = ptx::smem_u32(&ctl->full[0]), empty0 = ptx::smem_u32(&ctl->empty[0]);
+    int stage = 0;
+    uint32_t phase = 0;
+    int32_t early = 0;
+    if (worker < total_tiles) {
+      const I8Tile ti = i8_decode(ctl, p, worker, BT);
+      early = bcast(min(kt1 - kt0, C::kStages));
+      const int32_t w_row = bcast(ti.tn * 128), g = bcast(ti.g);
+      if (elected) {
+        for (int32_t i = 0; i < early; ++i) {
+          ptx::mbar_arrive_expect_tx(full0 + i * 8, C::kStageBytes);
+          ptx::tma_load_3d<1>(sW0 + i * C::kWBytes, &tmW, full0 + i * 8, (kt0 + i) * 128, w_row, g);
+        }
+      }
+    }
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    for (int32_t t = worker; t < total_tiles; t += workers) {
+      const I8Tile ti = i8_decode(ctl, p, t, BT);
+      const int32_t w_row = bcast(ti.tn * 128), t_row = bcast(ti.row0), g = bcast(ti.g);
+      for (int32_t kt = kt0; kt < kt1; ++kt) {
+        const bool first = early > 0;
+        if (first) --early;
+        else i8_wait(empty0 + stage * 8, phase ^ 1u, ctl, dead);
+        if (elected && !dead) {
+          const uint32_t bar = full0 + stage * 8;
+          if (!first) {
+            ptx::mbar_arrive_expect_tx(bar, C::kStageBytes);
+            ptx::tma_load_3d<1>(sW0 + stage * C::kWBytes, &tmW, bar, kt * 128, w_row, g);
+          }
+          ptx::tma_load_3d<1>(sT0 + stage * C::kTBytes, &tmX, bar, kt * 128, t_row, 0);
+        }
+        if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+      }
+    }
+    for (int s = 0; s < C::kStages; ++s) {
+      i8_wait(empty0 + stage * 8, phase ^ 1u, ctl, dead);
+      if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+    }
+    if (dead) atomicOr(p.status, kStTimeoutEmpty);
+  } else if (warp == 4) {
+    // ---------------------------------------------------------------- MMA issue
+    constexpr uint32_t idesc = i8_idesc(128, BT);
+    const uint32_t elected = ptx::elect_one_sync();
+    const uint32_t sW0 = ptx::smem_u32(sW), sT0 = ptx::smem_u32(sT);
+    const uint32_t full0 = ptx::smem_u32(&ctl->full[0]), empty0 = ptx::smem_u32(&ctl->empty[0]);
+    const uint32_t tfull0 = ptx::smem_u32(&ctl->tmem_full[0]), tempty0 = ptx::smem_u32(&ctl->tmem_empty[0]);
+    int stage = 0;
+    uint32_t phase = 0;
+    int32_t it = 0;
+    for (int32_t t = worker; t < total_tiles; t += workers, ++it) {
+      const int acc = it & 1;
+      const uint32_t d_tmem = tmem_base + uint32_t(acc) * BT;
+      i8_wait(tempty0 + acc * 8, (uint32_t(it >> 1) & 1u) ^ 1u, ctl, dead);
+      ptx::tc_fence_after();
+      for (int32_t kt = kt0; kt < kt1; ++kt) {
+        i8_wait(full0 + stage * 8, phase, ctl, dead);
+        ptx::tc_fence_after();
+        const uint64_t a_desc = make_desc_sw128(sW0 + stage * C::kWBytes);
+        const uint64_t b_desc = make_desc_sw128(sT0 + stage * C::kTBytes);
+        if (elected && !dead) {
+#pragma unroll
+          for (int kb = 0; kb < 4; ++kb) i8_mma<1>(d_tmem, a_desc + 2 * kb, b_desc + 2 * kb, idesc, kb > 0 || kt > kt0);
+          ptx::umma_commit<1>(empty0 + stage * 8);
+        }
+        if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+      }
+      if (elected && !dead) ptx::umma_commit<1>(tfull0 + acc * 8);
+    }
+    if (dead) atomicOr(p.status, kStTimeoutFull | kStTimeoutTmemEmpty);
+  } else {
+    // ---------------------------------------------------------------- epilogue: a lane is an output channel
+    const uint32_t tfull0 = ptx::smem_u32(&ctl->tmem_full[0]), tempty0 = ptx::smem_u32(&ctl->tmem_empty[0]);
+    const int act = p.activation;
+    const bool has_bias = p.bias != nullptr;
+    ptx::grid_dependency_wait();          // the token scales come from the quantiser, and D may still be read by what ran before
+    int32_t it = 0;
+    for (int32_t t = worker; t < total_tiles; t += workers, ++it) {
+      const I8Tile ti = i8_decode(ctl, p, t, BT);
+      const int acc = it & 1;
+      const int32_t n = ti.tn * 128 + warp * 32 + lane;
+      const bool n_ok = n < p.N;
+      const int64_t at = int64_t(ti.g) * p.N + n;
+      const float sb = n_ok ? __ldg(p.sb + at) : 0.0f;
+      const float bias = n_ok && has_bias ? __ldg(p.bias + at) : 0.0f;
+      i8_wait(tfull0 + acc * 8, uint32_t(it >> 1) & 1u, ctl, dead);
+      __syncwarp();
+      ptx::tc_fence_after();
+      const uint32_t lane_addr = tmem_base + (uint32_t(warp * 32) << 16) + uint32_t(acc) * BT;
+      const int32_t cols = min(BT, ti.row_end - ti.row0);
+#pragma unroll 1
+      for (int c0 = 0; c0 < BT; c0 += 16) {
+        uint32_t v[16];
+        i8_tmem_ld_x16(lane_addr + c0, v);
+        ptx::tmem_ld_wait();
+        if (c0 + 16 == BT) {
+          ptx::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive_relaxed(tempty0 + acc * 8);
+        }
+        if (split == 1) {
+          if (n_ok && c0 < cols) {
+            float x[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = i8_finish(v[j], c0 + j < cols ? __ldcg(p.sa + ti.row0 + c0 + j) : 0.0f, sb, bias);
+            i8_activate(x, act);
+            i8_put(p, x, min(16, cols - c0), int64_t(ti.row0 + c0) * p.ldd + n);
+          }
+        } else {
+          const int per = BT / split;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int c = c0 + j, owner = c / per;
+            if (c < cols)
+              ptx::st_shared_cluster_u32(ptx::mapa(ptx::smem_u32(sRed) + uint32_t(((rank * per + c - owner * per) * 128 + warp * 32 + lane) * 4), uint32_t(owner)), v[j]);
+          }
+        }
+      }
+    }
+    if (dead) atomicOr(p.status, kStTimeoutTmemFull);
+  }
+
+  if (split > 1) {
+    // One tile per cluster: every part of it has been sent once all CTAs are here.
+    __syncwarp();
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+    if (warp < 4 && worker < total_tiles) {
+      const I8Tile ti = i8_decode(ctl, p, worker, BT);
+      const int32_t n = ti.tn * 128 + warp * 32 + lane;
+      const int per = BT / split;
+      if (n < p.N) {
+        const int64_t at = int64_t(ti.g) * p.N + n;
+        const bool has_bias = p.bias != nullptr;
+        const float sb = __ldg(p.sb + at), bias = has_bias ? __ldg(p.bias + at) : 0.0f;
+        const int32_t* red = reinterpret_cast<const int32_t*>(sRed) + warp * 32 + lane;
+        const int32_t left = ti.row_end - (ti.row0 + rank * per);
+        for (int c0 = 0; c0 < per && c0 < left; c0 += 4) {
+          const int n_here = min(4, min(per, left) - c0);
+          float x[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            int32_t sum = 0;
+            if (j < n_here) {
+              for (int s = 0; s < split; ++s) sum += red[(s * per + c0 + j) * 128];
+            }
+            x[j] = i8_finish(uint32_t(sum), j < n_here ? __ldcg(p.sa + ti.row0 + rank * per + c0 + j) : 0.0f, sb, bias);
+          }
+          i8_activate(x, p.activation);
+          i8_put(p, x, n_here, int64_t(ti.row0 + rank * per + c0) * p.ldd + n);
+        }
+      }
+    }
+  }
+  if (ctl->abort) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000ll) __nanosleep(1000);
+  }
+  __syncwarp();
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc<1>(tmem_base, C::kTmemCols);
+  }
+}
+
+}  // namespace bsg

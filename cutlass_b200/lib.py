@@ -29,6 +29,7 @@ KIND_NVFP4 = 0
 KIND_MXFP8 = 1
 KIND_MXFP4 = 2          # e2m1 data, ue8m0 scale per 32
 KIND_MXFP8_MXFP4 = 3    # A e4m3, B e2m1, ue8m0 scale per 32
+KIND_INT8 = 16          # signed 8-bit integers, fp32 scale per row of A and per row of B (no kind of bsg_gemm_args)
 OUT_BF16 = 0
 OUT_NVFP4 = 1
 OUT_MXFP8 = 2
@@ -105,6 +106,18 @@ class QuantArgs(C.Structure):
                 ("ldx", C.c_int64), ("Q", C.c_void_p), ("SF", C.c_void_p), ("norm_constant", C.c_void_p)]
 
 
+class Int8Args(C.Structure):
+    """``bsg_int8_args`` of include/bsgemm.h, field for field."""
+    _fields_ = [
+        ("in_kind", C.c_int32), ("out_kind", C.c_int32), ("num_groups", C.c_int32), ("activation", C.c_int32),
+        ("rows", C.c_int64), ("tokens", C.c_int64), ("N", C.c_int64), ("K", C.c_int64),
+        ("X", C.c_void_p), ("ldx", C.c_int64), ("index", C.c_void_p), ("Q", C.c_void_p), ("ldq", C.c_int64), ("q_scale", C.c_void_p),
+        ("W", C.c_void_p), ("ldw", C.c_int64), ("group_stride_w", C.c_int64), ("w_scale", C.c_void_p), ("bias", C.c_void_p),
+        ("offsets", C.c_void_p), ("D", C.c_void_p), ("ldd", C.c_int64),
+        ("kernel", C.c_int32), ("tile", C.c_int32), ("split", C.c_int32), ("reserved0", C.c_int32),
+    ]
+
+
 SYMBOLS = {
     "bsg_version": (C.c_int32, []),
     "bsg_last_error_string": (C.c_char_p, []),
@@ -122,6 +135,10 @@ SYMBOLS = {
     "bsg_ptr_array_initialize_from_device": (C.c_int32, [C.POINTER(PtrArrayArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "bsg_ptr_array_run": (C.c_int32, [C.POINTER(PtrArrayArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "bsg_quantize": (C.c_int32, [C.POINTER(QuantArgs), C.c_void_p]),
+    "bsg_int8_query": (C.c_int32, [C.POINTER(Int8Args), C.POINTER(Caps)]),
+    "bsg_int8_quantize": (C.c_int32, [C.POINTER(Int8Args), C.c_void_p]),
+    "bsg_int8_gemm_run": (C.c_int32, [C.POINTER(Int8Args), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "bsg_int8_linear_run": (C.c_int32, [C.POINTER(Int8Args), C.c_void_p, C.c_size_t, C.c_void_p]),
     "bsg_tp_create": (C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_int64, C.POINTER(C.c_void_p), C.c_void_p]),
     "bsg_tp_connect": (C.c_int32, [C.c_void_p, C.c_void_p]),
     "bsg_tp_buffers": (C.c_int32, [C.c_void_p] + [C.POINTER(C.c_void_p)] * 4),

@@ -69,6 +69,7 @@ class CompiledArtifact:
 
 
 _WORKSPACE_BYTES = 16
+MAX_INT8_K = 131071       # 127 * 127 * K stays below 2^31
 _default_workspaces: dict[int, torch.Tensor] = {}
 
 
@@ -488,6 +489,91 @@ class GroupedBlockScaledGemmOperator(Operator):
         L.check(artifact.library.bsg_grouped_run(C.byref(a), ws.data_ptr(), ws.numel() * ws.element_size(), stream))
 
 
+def _int8_operand_error(name: str, op, rows: int, K: int) -> str | None:
+    """What keeps ``op`` from being a signed 8-bit operand with one fp32 scale per row, or None."""
+    if not isinstance(op, ScaledOperand) or op.quantized.dtype != torch.int8:
+        return f"{name} must be a ScaledOperand of int8 values"
+    mode = ScaleMode.as_tuple(op.mode)
+    if op.swizzle != ScaleSwizzleMode.SwizzleNone or mode[:-1] != (1,) * (len(mode) - 1) or mode[-1] != K:
+        return f"{name}: an int8 operand has one scale per row (mode (1, 1, {K}), SwizzleNone), got mode {mode}, {op.swizzle}"
+    if op.scale.dtype != torch.float32 or op.scale.numel() != rows or not op.scale.tensor.is_contiguous():
+        return f"{name}: scale must be a contiguous fp32 tensor of {rows} entries"
+    return None
+
+
+class Int8GemmOperator(Operator):
+    """Product of signed 8-bit operands with one fp32 scale per token (row of A) and one per output channel (column of B),
+    exact 32-bit sums; bf16, fp16 or fp32 output with optional bias and activation.  Dense (``GemmArguments``)."""
+
+    supported_args_type = GemmArguments
+
+    def _check(self, args, b_rows: int) -> Status:
+        ps = args.problem_size
+        epi = args.epilogue or EpilogueDescriptor()
+        out = args.out.tensor
+        if args.accumulator_type not in (torch.int32, int, "int32"):
+            return Status.fail(f"accumulator type {args.accumulator_type} is not supported (int32 only)")
+        for error in (_int8_operand_error("A", args.A, ps.M, ps.K), _int8_operand_error("B", args.B, b_rows, ps.K)):
+            if error:
+                return Status.fail(error)
+        if not _k_major_rows(args.A.quantized.tensor, -2, -1) or not _k_major_rows(args.B.quantized.tensor, -1, -2):
+            return Status.fail("A and B must be K-major with 16-byte aligned rows")
+        if args.A.quantized.data_ptr() % 16 != 0 or args.B.quantized.data_ptr() % 16 != 0:
+            return Status.fail("A and B must be 16-byte aligned")
+        if out.dtype not in (torch.bfloat16, torch.float16, torch.float32) or out.stride(-1) != 1 or (ps.M > 1 and out.stride(-2) < ps.N):
+            return Status.fail("out must be a row-major bf16, fp16 or fp32 tensor")
+        if epi.C is not None or epi.out_quant is not None or epi.bias_per_row:
+            return Status.fail("the 8-bit integer product takes a per-column bias and an activation, no C and no quantised output")
+        if isinstance(epi.alpha, torch.Tensor) or isinstance(epi.beta, torch.Tensor) or float(epi.alpha) != 1.0 or float(epi.beta) != 0.0:
+            return Status.fail("alpha and beta are 1 and 0 in the 8-bit integer product (fold alpha into a scale)")
+        if epi.activation not in ACTIVATIONS:
+            return Status.fail(f"unknown activation {epi.activation!r}: one of {sorted(ACTIVATIONS)}")
+        if epi.bias is not None and (epi.bias.dtype != torch.float32 or epi.bias.numel() != b_rows or not epi.bias.is_contiguous()):
+            return Status.fail(f"bias must be a contiguous fp32 tensor of {b_rows} entries")
+        if ps.K > MAX_INT8_K:
+            return Status.fail(f"K={ps.K} exceeds {MAX_INT8_K} (32-bit sums)")
+        return Status.success()
+
+    def _supports(self, args: GemmArguments) -> Status:
+        if len(args.A.shape) != 2:
+            return Status.fail("the 8-bit integer product is not batched")
+        return self._check(args, args.problem_size.N)
+
+    def build_args(self, args) -> L.Int8Args:
+        ps = args.problem_size
+        epi = args.epilogue or EpilogueDescriptor()
+        grouped = isinstance(args, GroupedGemmArguments)
+        q, w, out = args.A.quantized.tensor, args.B.quantized.tensor, args.out.tensor
+        a = L.Int8Args()
+        a.out_kind, a.num_groups, a.activation = _plain_out_kind(out), ps.L if grouped else 1, ACTIVATIONS[epi.activation]
+        a.rows, a.tokens, a.N, a.K = ps.M, ps.M, ps.N, ps.K
+        a.Q, a.ldq, a.q_scale = q.data_ptr(), q.stride(-2) if ps.M > 1 else -(-ps.K // 16) * 16, args.A.scale.data_ptr()
+        a.W, a.ldw, a.w_scale = w.data_ptr(), w.stride(-1) if ps.N > 1 else -(-ps.K // 16) * 16, args.B.scale.data_ptr()
+        a.group_stride_w = w.stride(0) if grouped and ps.L > 1 else 0
+        a.bias = epi.bias.data_ptr() if epi.bias is not None else None
+        a.offsets = args.offsets.data_ptr() if grouped else None
+        a.D, a.ldd = out.data_ptr(), out.stride(-2) if ps.M > 1 else ps.N
+        return a
+
+    def _run(self, args, artifact: CompiledArtifact, stream: int, workspace) -> None:
+        ws = self._resolve_workspace(workspace, args.out.tensor.device)
+        a = self.build_args(args)
+        L.check(artifact.library.bsg_int8_gemm_run(C.byref(a), ws.data_ptr(), ws.numel() * ws.element_size(), stream))
+
+
+class GroupedInt8GemmOperator(Int8GemmOperator):
+    """The same product over ragged groups of rows (``GroupedGemmArguments``): scales of B and bias per group."""
+
+    supported_args_type = GroupedGemmArguments
+
+    def _supports(self, args: GroupedGemmArguments) -> Status:
+        if args.problem_size.L > L.MAX_GROUPS:
+            return Status.fail(f"at most {L.MAX_GROUPS} groups are supported, got {args.problem_size.L}")
+        if not args.offsets.tensor.is_contiguous():
+            return Status.fail("offsets must be contiguous")
+        return self._check(args, args.problem_size.L * args.problem_size.N)
+
+
 _TILE_CHOICES = ((2, 256), (2, 128), (1, 256), (1, 128), (2, 192), (2, 64))   # (cta_group, tile_n), best first; the last two
 # (the reference's mma_tiler_n also takes 64 and 192) exist for the two main kinds and unquantised-type-bf16 / re-quantised outputs
 
@@ -500,7 +586,7 @@ def _name(kind: int, grouped: bool, cg: int, tn: int) -> str:
 
 
 def all_operators() -> list[Operator]:
-    """Every operator configuration the library offers."""
+    """Every configuration of the block-scaled operators."""
     ops: list[Operator] = []
     for kind in (L.KIND_NVFP4, L.KIND_MXFP8, L.KIND_MXFP4, L.KIND_MXFP8_MXFP4):
         for cg, tn in _TILE_CHOICES:
@@ -511,6 +597,12 @@ def all_operators() -> list[Operator]:
     return ops
 
 
+def int8_operators() -> list[Operator]:
+    """The 8-bit integer operators; kernel and tile follow from the problem inside the library."""
+    return [Int8GemmOperator(OperatorMetadata("native.Int8Gemm_sm100_tn_s8_acc_s32", L.KIND_INT8, 256, 2, False)),
+            GroupedInt8GemmOperator(OperatorMetadata("native.GroupedInt8Gemm_sm100_tn_s8_acc_s32", L.KIND_INT8, 256, 2, True))]
+
+
 class NativeProvider:
     """The one source of operators here: the hand-written sm_100a library.  Takes the place of the reference's
     provider classes (operators/cutlass/operators/providers/provider.py:43) in ``get_operators(providers=...)``."""
@@ -519,7 +611,7 @@ class NativeProvider:
 
     @staticmethod
     def operators() -> list["Operator"]:
-        return all_operators()
+        return all_operators() + int8_operators()
 
 
 def get_operators(args=None, metadata_filter: Callable[[OperatorMetadata], bool] | None = None,
@@ -530,7 +622,7 @@ def get_operators(args=None, metadata_filter: Callable[[OperatorMetadata], bool]
     if providers is not None and NativeProvider not in providers and not any(isinstance(p, NativeProvider) for p in providers):
         return []
     out = []
-    for op in all_operators():
+    for op in NativeProvider.operators():
         if metadata_filter is not None and not metadata_filter(op.metadata):
             continue
         if args is not None and not op.supports(args, target_sm=target_sm):

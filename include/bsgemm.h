@@ -295,6 +295,54 @@ int32_t bsg_ptr_array_initialize_from_device(const bsg_ptr_array_args* args, voi
 int32_t bsg_ptr_array_run(const bsg_ptr_array_args* args, void* workspace, size_t workspace_bytes, void* cuda_stream);
 
 /*
+ * Matrix product in 8-bit integers with one scale per token and one per output channel:
+ *     q[m,k] = sign(x) floor(127 |x[m,k]| / a_m + 1/2),  a_m = max_k |x[m,k]|,  q_scale[m] = a_m / 127
+ *     D[m,n] = act(q_scale[m] * w_scale[n] * sum_k q[m,k] W[n,k] + bias[n])
+ * with exact 32-bit integer sums (K <= 131071).  A token that holds a NaN or an infinity gets the scale NaN and zeros,
+ * so that its outputs are NaN; a token of zeros gets the scale 0.  Dense, or grouped by device-side end rows like
+ * bsg_grouped_args (W, w_scale and bias per group); rows of D at or behind the last end row are not written.
+ *
+ * Rows of Q and W start on 16-byte boundaries; K, N, ldd and the alignment of X, D, bias and the scales are free
+ * (whole elements).  Nothing is allocated.
+ */
+typedef struct bsg_int8_args {
+  int32_t in_kind;          /* type of X: BSG_OUT_BF16 or BSG_OUT_F16 */
+  int32_t out_kind;         /* type of D: BSG_OUT_BF16, BSG_OUT_F16 or BSG_OUT_F32 */
+  int32_t num_groups;       /* 1 (dense, offsets NULL) .. BSG_MAX_GROUPS */
+  int32_t activation;       /* BSG_ACT_* */
+  int64_t rows;             /* rows of Q and D */
+  int64_t tokens;           /* rows of X (== rows without an index) */
+  int64_t N, K;
+  const void* X;            /* (tokens, K); quantise and linear only */
+  int64_t ldx;
+  const int32_t* index;     /* device int32[rows]: row of X that row r of Q is made from; an index outside [0, tokens) gives
+                               zeros with the scale NaN; NULL: row r */
+  void* Q;                  /* (rows, K) int8: written by quantise and linear, read by the product */
+  int64_t ldq;
+  float* q_scale;           /* device fp32[rows], likewise */
+  const void* W;            /* (num_groups, N, K) int8, K contiguous */
+  int64_t ldw;
+  int64_t group_stride_w;   /* elements between the matrices of two groups */
+  const float* w_scale;     /* device fp32[num_groups][N] */
+  const float* bias;        /* device fp32[num_groups][N] or NULL */
+  const int32_t* offsets;   /* device int32[num_groups], cumulative END rows; NULL: dense */
+  void* D;                  /* (rows, N) */
+  int64_t ldd;
+  int32_t kernel;           /* 0: chosen by the library; 1: the kernel for few rows; 2: the kernel for many rows */
+  int32_t tile;             /* 0: chosen; few rows: tokens per tile (16, 32, 64, 128); many rows: columns per tile (128, 256) */
+  int32_t split;            /* 0: chosen; few rows, dense, tile <= 64: CTAs of a cluster that share the K of one tile (1, 2, 4, 8) */
+  int32_t reserved0;
+} bsg_int8_args;
+
+int32_t bsg_int8_query(const bsg_int8_args* args, bsg_caps* caps);
+/* X -> Q, q_scale. */
+int32_t bsg_int8_quantize(const bsg_int8_args* args, void* cuda_stream);
+/* Q, q_scale, W, ... -> D.  Workspace and device status as in bsg_gemm_run. */
+int32_t bsg_int8_gemm_run(const bsg_int8_args* args, void* workspace, size_t workspace_bytes, void* cuda_stream);
+/* Both steps; the product's set-up and its first weights overlap the quantiser. */
+int32_t bsg_int8_linear_run(const bsg_int8_args* args, void* workspace, size_t workspace_bytes, void* cuda_stream);
+
+/*
  * The same dense / batched GEMM as bsg_gemm_run for callers that have no device memory to hand over
  * as workspace and are not allowed to create any: code running under a framework that has frozen or
  * pre-reserved all device memory (an inference server after warm-up, a plug-in whose enqueue hook
