@@ -118,6 +118,14 @@ class Int8Args(C.Structure):
     ]
 
 
+class ActArgs(C.Structure):
+    """``bsg_act_args`` of include/bsgemm.h, field for field."""
+    _fields_ = [
+        ("type", C.c_int32), ("activation", C.c_int32), ("gated", C.c_int32), ("reserved0", C.c_int32), ("rows", C.c_int64), ("width", C.c_int64),
+        ("in_", C.c_void_p), ("ld_in", C.c_int64), ("out", C.c_void_p), ("ld_out", C.c_int64), ("kept", C.c_void_p), ("kept_scale", C.c_void_p),
+    ]
+
+
 SYMBOLS = {
     "bsg_version": (C.c_int32, []),
     "bsg_last_error_string": (C.c_char_p, []),
@@ -139,6 +147,8 @@ SYMBOLS = {
     "bsg_int8_quantize": (C.c_int32, [C.POINTER(Int8Args), C.c_void_p]),
     "bsg_int8_gemm_run": (C.c_int32, [C.POINTER(Int8Args), C.c_void_p, C.c_size_t, C.c_void_p]),
     "bsg_int8_linear_run": (C.c_int32, [C.POINTER(Int8Args), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "bsg_act_forward": (C.c_int32, [C.POINTER(ActArgs), C.c_void_p]),
+    "bsg_act_backward": (C.c_int32, [C.POINTER(ActArgs), C.c_void_p]),
     "bsg_tp_create": (C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_int64, C.POINTER(C.c_void_p), C.c_void_p]),
     "bsg_tp_connect": (C.c_int32, [C.c_void_p, C.c_void_p]),
     "bsg_tp_buffers": (C.c_int32, [C.c_void_p] + [C.POINTER(C.c_void_p)] * 4),

@@ -343,6 +343,30 @@ int32_t bsg_int8_gemm_run(const bsg_int8_args* args, void* workspace, size_t wor
 int32_t bsg_int8_linear_run(const bsg_int8_args* args, void* workspace, size_t workspace_bytes, void* cuda_stream);
 
 /*
+ * Activation between the two products of an MLP layer whose input is kept in 8 bits for the backward pass.  X is
+ * (rows, 2 width) = (g | u) when gated, else (rows, width) = g:
+ *     forward   h = act(g) u (or act(g)); kept: per row and block of 128 columns of g and of u
+ *               s = max|.| / 127, q = sign(.) floor(127 |.| / max|.| + 1/2)
+ *     backward  with g^ = s q, u^ = s q:  dg = dh u^ act'(g^), du = dh act(g^)  (or dg = dh act'(g^))
+ * A block with a NaN or an infinity is kept as NaN.  act and its order of operations: BSG_ACT_*.
+ */
+typedef struct bsg_act_args {
+  int32_t type;             /* BSG_OUT_BF16 or BSG_OUT_F16: X, h and their gradients */
+  int32_t activation;       /* BSG_ACT_* */
+  int32_t gated;            /* 0 or 1 */
+  int32_t reserved0;
+  int64_t rows, width;
+  const void* in;           /* forward: X; backward: gradient of h */
+  int64_t ld_in;            /* elements */
+  void* out;                /* forward: h; backward: gradient of X */
+  int64_t ld_out;
+  void* kept;               /* int8 [rows][1 + gated][width rounded up to 16]: written by forward, read by backward */
+  float* kept_scale;        /* fp32 [rows][1 + gated][ceil(width / 128)] */
+} bsg_act_args;
+int32_t bsg_act_forward(const bsg_act_args* args, void* cuda_stream);
+int32_t bsg_act_backward(const bsg_act_args* args, void* cuda_stream);
+
+/*
  * The same dense / batched GEMM as bsg_gemm_run for callers that have no device memory to hand over
  * as workspace and are not allowed to create any: code running under a framework that has frozen or
  * pre-reserved all device memory (an inference server after warm-up, a plug-in whose enqueue hook
