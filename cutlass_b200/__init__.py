@@ -11,12 +11,13 @@ from .operator import (AllocationRequirement, BlockScaledGemmOperator, CompiledA
                        GroupedBlockScaledGemmOperator, GroupedInt8GemmOperator, Int8GemmOperator, NativeProvider, Operator, OperatorMetadata, Workspace, all_operators,
                        get_operators, to_cuda_stream)
 from .quantize import quantize_blockscaled
+from .routing import Routing, route_tokens, route_tokens_backward
 from .status import Status
 
 __all__ = [
     "ActivationCheckpoint", "AllocationRequirement", "BlockScaledGemmOperator", "CompiledArtifact", "DenseTensor", "EpilogueDescriptor",
     "GemmArguments", "GemmProblemSize", "GroupedBlockScaledGemmOperator", "GroupedGemmArguments", "GroupedInt8GemmOperator", "Int8GemmOperator", "Mxfp8Quant", "NativeProvider", "Nvfp4Quant",
-    "Operator", "OperatorMetadata", "ScaleMode", "ScaleSwizzleMode", "ScaledOperand", "Status", "Workspace",
-    "all_operators", "checkpoint_activation", "checkpoint_activation_backward", "checkpointed_activation", "get_operators", "int8_linear", "quantize_blockscaled", "quantize_int8", "to_cuda_stream",
+    "Operator", "OperatorMetadata", "Routing", "ScaleMode", "ScaleSwizzleMode", "ScaledOperand", "Status", "Workspace",
+    "all_operators", "checkpoint_activation", "checkpoint_activation_backward", "checkpointed_activation", "get_operators", "int8_linear", "quantize_blockscaled", "quantize_int8", "route_tokens", "route_tokens_backward", "to_cuda_stream",
 ]
 __version__ = "0.1.0"

@@ -23,6 +23,7 @@ SOURCES = {      # translation unit -> the headers it includes
     "bsgemm.cu": ["gemm_kernel.cuh", "quant_kernel.cuh", "ptx.cuh", "host.h"],
     "int8.cu": ["int8_kernel.cuh", "gemm_kernel.cuh", "ptx.cuh", "host.h"],
     "activation.cu": ["activation_kernel.cuh", "int8_kernel.cuh", "gemm_kernel.cuh", "ptx.cuh", "host.h"],
+    "route.cu": ["route_kernel.cuh", "gemm_kernel.cuh", "ptx.cuh", "host.h"],
 }
 ABI_HEADER = os.path.join("..", "..", "include", "bsgemm.h")
 NVCC_FLAGS = [

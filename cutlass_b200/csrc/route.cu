@@ -1,0 +1,133 @@
+// Host side of the router (bsg_route_*): argument checks and launches.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstring>
+
+#include "../../include/bsgemm.h"
+#include "gemm_kernel.cuh"
+#include "host.h"
+#include "route_kernel.cuh"
+
+namespace {
+
+using bsg::host_aligned;
+using bsg::host_fail;
+
+constexpr int64_t kBlocksMax = 4 * 148;
+
+int64_t route_blocks(int64_t tokens) {
+  const int64_t b = (tokens + 31) / 32;      // at least four tokens a warp
+  return b < 1 ? 1 : b > kBlocksMax ? kBlocksMax : b;
+}
+
+int32_t check(const bsg_route_args* a, bool forward) {
+  if (!a) return host_fail(BSG_ERR_INVALID_PROBLEM, "args is null");
+  if (a->type != BSG_OUT_BF16 && a->type != BSG_OUT_F16 && a->type != BSG_OUT_F32) return host_fail(BSG_ERR_NOT_SUPPORTED, "logits must be bf16, fp16 or fp32 (type %d)", a->type);
+  if (a->experts < 1 || a->experts > bsg::kRouteMaxExperts) return host_fail(BSG_ERR_INVALID_PROBLEM, "expert count %d outside [1, %d]", a->experts, bsg::kRouteMaxExperts);
+  if (a->k < 1 || a->k > bsg::kRouteMaxK || a->k > a->experts) return host_fail(BSG_ERR_INVALID_PROBLEM, "k = %d outside [1, min(%d, %d experts)]", a->k, bsg::kRouteMaxK, a->experts);
+  if (a->tokens < 0 || a->tokens * a->k > 0x7FFFFFFFll) return host_fail(BSG_ERR_INVALID_PROBLEM, "%lld tokens with %d choices exceed 2^31 rows", (long long)a->tokens, a->k);
+  if (a->normalize != 0 && a->normalize != 1) return host_fail(BSG_ERR_INVALID_PROBLEM, "normalize must be 0 or 1");
+  if (!a->counts || !a->live || (forward && (!a->offsets || !a->loss))) return host_fail(BSG_ERR_INVALID_PROBLEM, "per-expert tensors and the loss must not be null");
+  if (a->tokens > 0) {
+    if (!a->logits || !a->chosen || !a->weights) return host_fail(BSG_ERR_INVALID_PROBLEM, "logits, chosen and weights must not be null");
+    if (forward && (!a->rows || !a->positions)) return host_fail(BSG_ERR_INVALID_PROBLEM, "rows and positions must not be null");
+    if (!forward && !a->grad_logits) return host_fail(BSG_ERR_INVALID_PROBLEM, "grad_logits must not be null");
+    if (a->ld < a->experts || (!forward && a->ld_grad < a->experts)) return host_fail(BSG_ERR_INVALID_PROBLEM, "a row pitch is smaller than the %d experts", a->experts);
+    const int esz = a->type == BSG_OUT_F32 ? 4 : 2;
+    if (!host_aligned(a->logits, esz) || !host_aligned(a->grad_logits, esz)) return host_fail(BSG_ERR_MISALIGNED_OPERAND, "tensors must be aligned to their elements");
+  }
+  return BSG_OK;
+}
+
+int64_t scratch_words(const bsg_route_args* a) {
+  const int64_t b = route_blocks(a->tokens);
+  return b * (a->experts + 1) + b * a->experts + a->experts;
+}
+
+bsg::RouteParams params(const bsg_route_args* a, void* scratch) {
+  bsg::RouteParams p;
+  memset(&p, 0, sizeof(p));
+  const int esz = a->type == BSG_OUT_F32 ? 4 : 2;
+  p.logits = a->logits; p.ld = a->ld; p.mask = a->mask; p.tokens = int32_t(a->tokens); p.experts = a->experts; p.k = a->k;
+  p.normalize = a->normalize; p.wide = host_aligned(a->logits, 16) && (a->ld * esz) % 16 == 0;
+  p.chosen = a->chosen; p.weights = a->weights; p.counts = a->counts; p.offsets = a->offsets; p.rows = a->rows;
+  p.positions = a->positions; p.loss = a->loss; p.live = a->live;
+  p.grad_weights = a->grad_weights; p.grad_loss = a->grad_loss; p.grad_logits = a->grad_logits; p.ld_grad = a->ld_grad;
+  p.wide_grad = host_aligned(a->grad_logits, 16) && (a->ld_grad * esz) % 16 == 0;
+  const int64_t b = route_blocks(a->tokens);
+  p.per_block = int32_t((a->tokens + b - 1) / b);
+  p.blocks = int32_t(p.per_block > 0 ? (a->tokens + p.per_block - 1) / p.per_block : 1);
+  if (p.blocks < 1) p.blocks = 1;
+  int32_t* w = static_cast<int32_t*>(scratch);
+  p.block_counts = w;
+  p.block_sums = reinterpret_cast<float*>(w + b * (a->experts + 1));
+  p.sums = p.block_sums + b * a->experts;
+  return p;
+}
+
+template <int TYPE, int V>
+int32_t forward_v(const bsg::RouteParams& p, cudaStream_t s) {
+  const size_t shared1 = size_t(p.experts + 1 + bsg::kRouteWarps * p.experts) * 4;
+  bsg::bsg_route_tokens_kernel<TYPE, V><<<p.blocks, bsg::kRouteThreads, shared1, s>>>(p);
+  bsg::bsg_route_scan_kernel<<<(p.experts + 1 + bsg::kRouteWarps - 1) / bsg::kRouteWarps, bsg::kRouteThreads, 0, s>>>(p);
+  bsg::bsg_route_order_kernel<<<p.blocks, bsg::kRouteThreads, size_t(1 + bsg::kRouteWarps) * p.experts * 4, s>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "router launch: %s", cudaGetErrorString(e));
+  return BSG_OK;
+}
+template <int TYPE, int V>
+int32_t backward_v(const bsg::RouteParams& p, int sms, cudaStream_t s) {
+  const int64_t want = (int64_t(p.tokens) + bsg::kRouteWarps - 1) / bsg::kRouteWarps, most = 8 * int64_t(sms);
+  bsg::bsg_route_backward_kernel<TYPE, V><<<unsigned(want < most ? want : most), bsg::kRouteThreads, size_t(bsg::kRouteWarps) * 32 * V * 4, s>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "router launch: %s", cudaGetErrorString(e));
+  return BSG_OK;
+}
+template <int TYPE>
+int32_t pick(const bsg::RouteParams& p, bool forward, int sms, cudaStream_t s) {
+#define BSG_ROUTE_V(V) return forward ? forward_v<TYPE, V>(p, s) : backward_v<TYPE, V>(p, sms, s)
+  if (p.experts <= 32) BSG_ROUTE_V(1);
+  if (p.experts <= 64) BSG_ROUTE_V(2);
+  if (p.experts <= 128) BSG_ROUTE_V(4);
+  if (p.experts <= 256) BSG_ROUTE_V(8);
+  if (p.experts <= 512) BSG_ROUTE_V(16);
+  BSG_ROUTE_V(32);
+#undef BSG_ROUTE_V
+}
+int32_t run(const bsg::RouteParams& p, int32_t type, bool forward, int sms, cudaStream_t s) {
+  if (type == BSG_OUT_BF16) return pick<bsg::kRouteBf16>(p, forward, sms, s);
+  if (type == BSG_OUT_F16) return pick<bsg::kRouteF16>(p, forward, sms, s);
+  return pick<bsg::kRouteF32>(p, forward, sms, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t bsg_route_scratch_size(const bsg_route_args* args, size_t* bytes) {
+  if (!args || !bytes) return host_fail(BSG_ERR_INVALID_PROBLEM, "args and bytes must not be null");
+  if (args->tokens < 0 || args->experts < 1 || args->experts > bsg::kRouteMaxExperts) return host_fail(BSG_ERR_INVALID_PROBLEM, "extents out of range");
+  *bytes = size_t(scratch_words(args)) * 4;
+  return BSG_OK;
+}
+
+int32_t bsg_route_forward(const bsg_route_args* args, void* scratch, size_t scratch_bytes, void* cuda_stream) {
+  int32_t rc = check(args, true);
+  if (rc != BSG_OK) return rc;
+  if (!scratch || scratch_bytes < size_t(scratch_words(args)) * 4) return host_fail(BSG_ERR_WORKSPACE_NULL, "the router needs %lld bytes of scratch", (long long)scratch_words(args) * 4);
+  if (!host_aligned(scratch, 4)) return host_fail(BSG_ERR_MISALIGNED_OPERAND, "scratch must be 4-byte aligned");
+  int dev = 0, sms = 0;
+  if ((rc = bsg::host_device(BSG_ERR_ARCH_MISMATCH, BSG_ERR_CUDA, &dev, &sms)) != BSG_OK) return rc;
+  return run(params(args, scratch), args->type, true, sms, static_cast<cudaStream_t>(cuda_stream));
+}
+
+int32_t bsg_route_backward(const bsg_route_args* args, void* cuda_stream) {
+  int32_t rc = check(args, false);
+  if (rc != BSG_OK || args->tokens == 0) return rc;
+  int dev = 0, sms = 0;
+  if ((rc = bsg::host_device(BSG_ERR_ARCH_MISMATCH, BSG_ERR_CUDA, &dev, &sms)) != BSG_OK) return rc;
+  return run(params(args, nullptr), args->type, false, sms, static_cast<cudaStream_t>(cuda_stream));
+}
+
+}  // extern "C"

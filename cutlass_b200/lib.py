@@ -126,6 +126,17 @@ class ActArgs(C.Structure):
     ]
 
 
+class RouteArgs(C.Structure):
+    """``bsg_route_args`` of include/bsgemm.h, field for field."""
+    _fields_ = [
+        ("type", C.c_int32), ("experts", C.c_int32), ("k", C.c_int32), ("normalize", C.c_int32), ("tokens", C.c_int64),
+        ("logits", C.c_void_p), ("ld", C.c_int64), ("mask", C.c_void_p),
+        ("chosen", C.c_void_p), ("weights", C.c_void_p), ("counts", C.c_void_p), ("live", C.c_void_p),
+        ("offsets", C.c_void_p), ("rows", C.c_void_p), ("positions", C.c_void_p), ("loss", C.c_void_p),
+        ("grad_weights", C.c_void_p), ("grad_loss", C.c_void_p), ("grad_logits", C.c_void_p), ("ld_grad", C.c_int64),
+    ]
+
+
 SYMBOLS = {
     "bsg_version": (C.c_int32, []),
     "bsg_last_error_string": (C.c_char_p, []),
@@ -149,6 +160,9 @@ SYMBOLS = {
     "bsg_int8_linear_run": (C.c_int32, [C.POINTER(Int8Args), C.c_void_p, C.c_size_t, C.c_void_p]),
     "bsg_act_forward": (C.c_int32, [C.POINTER(ActArgs), C.c_void_p]),
     "bsg_act_backward": (C.c_int32, [C.POINTER(ActArgs), C.c_void_p]),
+    "bsg_route_scratch_size": (C.c_int32, [C.POINTER(RouteArgs), C.POINTER(C.c_size_t)]),
+    "bsg_route_forward": (C.c_int32, [C.POINTER(RouteArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "bsg_route_backward": (C.c_int32, [C.POINTER(RouteArgs), C.c_void_p]),
     "bsg_tp_create": (C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_int64, C.POINTER(C.c_void_p), C.c_void_p]),
     "bsg_tp_connect": (C.c_int32, [C.c_void_p, C.c_void_p]),
     "bsg_tp_buffers": (C.c_int32, [C.c_void_p] + [C.POINTER(C.c_void_p)] * 4),

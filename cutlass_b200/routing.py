@@ -1,0 +1,141 @@
+"""Router in front of a layer of experts.
+
+    r = route_tokens(logits, top_k)                       # logits (T, E)
+    y = int8_linear(x, W, W_scale, offsets=r.offsets, rows=r.rows)      # (T * top_k, N), rows sorted by expert
+    loss = task_loss + 0.01 * r.balance_loss
+
+``r.offsets`` are the end rows that ``GroupedGemmArguments`` and ``int8_linear`` take.  ``r.weights`` and ``r.balance_loss``
+carry gradients to the logits when those require them.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+
+from . import lib as L
+from .int8 import _OUT_KINDS as _KINDS
+from .int8 import _on_stream
+
+MAX_EXPERTS, MAX_TOP_K = 1024, 32
+
+
+class Routing(NamedTuple):
+    """What ``route_tokens`` returns.  A slot that chose nothing (a token that does not count, or fewer than k logits above
+    -inf) has expert -1, weight 0 and position -1; rows at or behind ``offsets[-1]`` name token -1."""
+
+    experts: torch.Tensor         # (T, k) int32, largest logit first
+    weights: torch.Tensor         # (T, k) fp32
+    counts: torch.Tensor          # (E,) int32: rows of every expert
+    offsets: torch.Tensor         # (E,) int32: cumulative end rows
+    rows: torch.Tensor            # (T * k,) int32: token of every row, rows sorted by expert, stable in (token, slot)
+    positions: torch.Tensor       # (T, k) int32: row of every slot
+    balance_loss: torch.Tensor    # () fp32
+    num_tokens: torch.Tensor      # (1,) int32: tokens that count
+    normalize: bool
+
+
+def _scratch_words(T: int, E: int) -> int:
+    blocks = min(max(-(-T // 32), 1), 592)
+    return blocks * (2 * E + 1) + E
+
+
+def _check_logits(logits, top_k, token_mask) -> None:
+    if logits.dim() != 2 or logits.dtype not in _KINDS or not logits.is_cuda or (logits.shape[1] > 1 and logits.stride(1) != 1) \
+            or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
+        raise ValueError("logits must be a 2-D row-major bf16, fp16 or fp32 CUDA tensor")
+    T, E = logits.shape
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"between 1 and {MAX_EXPERTS} experts are supported, got {E}")
+    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 1 <= top_k <= min(MAX_TOP_K, E):
+        raise ValueError(f"top_k must be an int between 1 and min({MAX_TOP_K}, {E}), got {top_k!r}")
+    if T * top_k > 0x7FFFFFFF:
+        raise ValueError(f"{T} tokens with {top_k} choices exceed 2^31 rows")
+    if token_mask is not None and (token_mask.dtype != torch.bool or tuple(token_mask.shape) != (T,) or not token_mask.is_contiguous()
+                                   or token_mask.device != logits.device):
+        raise ValueError(f"token_mask must be a contiguous bool tensor of shape {(T,)} on {logits.device}")
+
+
+def _forward(logits, top_k, token_mask, normalize, stream) -> Routing:
+    T, E = logits.shape
+    device = logits.device
+    n = T * top_k
+    # what is whole comes from one allocation; the two results that carry gradients are tensors of their own
+    whole = torch.empty(3 * n + 2 * E + 1, dtype=torch.int32, device=device)
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=device)
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    scratch = torch.empty(_scratch_words(T, E), dtype=torch.int32, device=device)
+    w = whole.data_ptr()
+    a = L.RouteArgs(_KINDS[logits.dtype], E, top_k, int(normalize), T, logits.data_ptr(), logits.stride(0) if T > 1 else E,
+                    token_mask.data_ptr() if token_mask is not None else None,
+                    w, weights.data_ptr(), w + 12 * n, w + 12 * n + 8 * E, w + 12 * n + 4 * E, w + 4 * n, w + 8 * n, loss.data_ptr())
+    _on_stream(device, stream, lambda s: L.check(L.load().bsg_route_forward(C.byref(a), scratch.data_ptr(), 4 * scratch.numel(), s)),
+               whole, weights, loss, scratch)
+    experts, rows, positions, counts, offsets, live = whole.split_with_sizes([n, n, n, E, E, 1])
+    return Routing(experts.view(T, top_k), weights, counts, offsets, rows, positions.view(T, top_k), loss, live, bool(normalize))
+
+
+def route_tokens_backward(logits, routing: Routing, grad_weights=None, grad_balance_loss=None, *, stream=None) -> torch.Tensor:
+    """Gradient of ``logits`` (in their type) for the gradients of ``routing.weights`` (T, k) fp32 and ``routing.balance_loss``
+    () fp32, either of which may be None (zero).  The counts are constants.  Asynchronous on ``stream`` (None: torch's current
+    stream)."""
+    k = routing.experts.shape[1]
+    _check_logits(logits, k, None)
+    T, E = logits.shape
+    device = logits.device
+    if tuple(routing.experts.shape) != (T, k) or tuple(routing.counts.shape) != (E,) or routing.experts.device != device:
+        raise ValueError("routing does not belong to these logits")
+    if grad_weights is not None and (grad_weights.dtype != torch.float32 or tuple(grad_weights.shape) != (T, k)
+                                     or not grad_weights.is_contiguous() or grad_weights.device != device):
+        raise ValueError(f"grad_weights must be a contiguous fp32 tensor of shape {(T, k)} on {device}")
+    if grad_balance_loss is not None and (grad_balance_loss.dtype != torch.float32 or grad_balance_loss.numel() != 1
+                                          or grad_balance_loss.device != device):
+        raise ValueError(f"grad_balance_loss must be a one-element fp32 tensor on {device}")
+    out = torch.empty((T, E), dtype=logits.dtype, device=device)
+    a = L.RouteArgs(_KINDS[logits.dtype], E, k, int(routing.normalize), T, logits.data_ptr(), logits.stride(0) if T > 1 else E, None,
+                    routing.experts.data_ptr(), routing.weights.data_ptr(), routing.counts.data_ptr(), routing.num_tokens.data_ptr(),
+                    None, None, None, None, grad_weights.data_ptr() if grad_weights is not None else None,
+                    grad_balance_loss.data_ptr() if grad_balance_loss is not None else None, out.data_ptr(), E)
+    _on_stream(device, stream, lambda s: L.check(L.load().bsg_route_backward(C.byref(a), s)), out)
+    return out
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_k, token_mask, normalize, stream):
+        r = _forward(logits, top_k, token_mask, normalize, stream)
+        ctx.save_for_backward(logits, r.experts, r.weights, r.counts, r.num_tokens)
+        ctx.normalize = r.normalize
+        whole = (r.experts, r.counts, r.offsets, r.rows, r.positions, r.num_tokens)
+        ctx.mark_non_differentiable(*whole)
+        ctx.set_materialize_grads(False)
+        return (r.weights, r.balance_loss) + whole
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_weights, grad_loss, *_):
+        logits, experts, weights, counts, live = ctx.saved_tensors
+        if grad_weights is None and grad_loss is None:
+            return None, None, None, None, None
+        r = Routing(experts, weights, counts, None, None, None, None, live, ctx.normalize)
+        grad = route_tokens_backward(logits, r, grad_weights.contiguous() if grad_weights is not None else None, grad_loss)
+        return grad, None, None, None, None
+
+
+def route_tokens(logits, top_k: int, *, token_mask=None, normalize: bool = True, stream=None) -> Routing:
+    """Choose ``top_k`` experts for every token of ``logits`` (T, E) bf16 / fp16 / fp32.
+
+    The probabilities are ``softmax(logits)`` in fp32.  The k largest logits are chosen, ties to the lower index; -inf is never
+    chosen (a masked expert), NaN ranks above all.  ``weights`` are the chosen probabilities, divided by their sum when
+    ``normalize``.  ``token_mask`` (T,) bool: False marks padding, which is not routed and does not count; neither does a token
+    whose logits are all -inf.  ``balance_loss = E * sum_e f_e P_e`` with f_e the share of the n * k choices that fell on expert
+    e and P_e the mean probability over the n tokens that count: 1 when balanced, 0 when n = 0.
+
+    E is at most 1024 and k at most 32.  Results do not depend on the order in which anything runs.  Asynchronous on ``stream``
+    (None: torch's current stream); the backward pass runs on the stream that autograd makes current."""
+    _check_logits(logits, top_k, token_mask)
+    if not (torch.is_grad_enabled() and logits.requires_grad):
+        return _forward(logits, top_k, token_mask, normalize, stream)
+    weights, loss, experts, counts, offsets, rows, positions, live = _Route.apply(logits, top_k, token_mask, normalize, stream)
+    return Routing(experts, weights, counts, offsets, rows, positions, loss, live, bool(normalize))

@@ -367,6 +367,43 @@ int32_t bsg_act_forward(const bsg_act_args* args, void* cuda_stream);
 int32_t bsg_act_backward(const bsg_act_args* args, void* cuda_stream);
 
 /*
+ * Router of a layer of experts: p = softmax(logits); the k largest logits of a token are chosen (ties to the lower index, NaN
+ * above all, -inf never), with weights p / sum of the chosen p (normalize) or p; the chosen (token, slot) pairs are ordered by
+ * expert, stably; offsets are the cumulative END rows that the grouped products take.  Tokens whose mask is 0 or whose
+ * logits are all -inf do not count and are not routed.  With n tokens that count, f_e = counts_e / (n k) and
+ * P_e = sum_t p_te / n, loss = experts * sum_e f_e P_e (f is a constant for the gradient).
+ * Slots that chose nothing: chosen -1, weight 0, position -1; rows at or behind the last end row: -1.
+ */
+typedef struct bsg_route_args {
+  int32_t type;             /* BSG_OUT_BF16, BSG_OUT_F16 or BSG_OUT_F32: logits and their gradient */
+  int32_t experts, k;       /* up to 1024; up to min(32, experts) */
+  int32_t normalize;        /* 0 or 1 */
+  int64_t tokens;
+  const void* logits;       /* (tokens, experts) */
+  int64_t ld;               /* elements */
+  const uint8_t* mask;      /* device [tokens], 0: the token does not count; or NULL */
+  /* written by forward, read by backward */
+  int32_t* chosen;          /* (tokens, k) */
+  float* weights;           /* (tokens, k) */
+  int32_t* counts;          /* [experts] */
+  int32_t* live;            /* [1]: n */
+  /* written by forward */
+  int32_t* offsets;         /* [experts] */
+  int32_t* rows;            /* [tokens * k]: token of every row */
+  int32_t* positions;       /* (tokens, k): row of every slot */
+  float* loss;              /* [1] */
+  /* backward */
+  const float* grad_weights;    /* (tokens, k) or NULL (zeros) */
+  const float* grad_loss;       /* [1], device, or NULL (0) */
+  void* grad_logits;            /* (tokens, experts) */
+  int64_t ld_grad;
+} bsg_route_args;
+int32_t bsg_route_scratch_size(const bsg_route_args* args, size_t* bytes);
+/* `scratch` need not be initialised; calls that may overlap need scratch of their own. */
+int32_t bsg_route_forward(const bsg_route_args* args, void* scratch, size_t scratch_bytes, void* cuda_stream);
+int32_t bsg_route_backward(const bsg_route_args* args, void* cuda_stream);
+
+/*
  * The same dense / batched GEMM as bsg_gemm_run for callers that have no device memory to hand over
  * as workspace and are not allowed to create any: code running under a framework that has frozen or
  * pre-reserved all device memory (an inference server after warm-up, a plug-in whose enqueue hook
