@@ -8,14 +8,13 @@ What is kept is one byte per value of ``x`` and one fp32 scale per 128 of them, 
 """
 from __future__ import annotations
 
-import ctypes as C
 from dataclasses import dataclass
 
 import torch
 
 from . import lib as L
 from .arguments import ACTIVATIONS
-from .int8 import _IN_KINDS, _no_gradient, _on_stream
+from .int8 import _IN_KINDS, _launch, _matrix, _no_gradient
 
 BLOCK = 128      # columns of a row that share one scale
 
@@ -36,13 +35,12 @@ class ActivationCheckpoint:
         return self.quantized.numel() + 4 * self.scale.numel()
 
 
-def _check_matrix(name, t, cols, dtype=None, rows=None, device=None) -> None:
-    if t.dim() != 2 or t.dtype not in _IN_KINDS or not t.is_cuda or (t.shape[1] > 1 and t.stride(1) != 1) \
-            or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        raise ValueError(f"{name} must be a 2-D row-major bf16 or fp16 CUDA tensor")
-    if t.shape[1] < 1 or (cols is not None and t.shape[1] != cols) or (rows is not None and t.shape[0] != rows) \
-            or (dtype is not None and t.dtype != dtype) or (device is not None and t.device != device):
-        raise ValueError(f"{name} must be a {dtype} tensor of shape {(rows, cols)} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _given(name, t, kind, device, rows, cols) -> int:
+    """Row pitch of a matrix of the caller's that has to have this type, place and shape."""
+    k, d, r, c, pitch = _matrix(name, t, _IN_KINDS)
+    if (k, d, r, c) != (kind, device, rows, cols):
+        raise ValueError(f"{name} must have the type of x, on CUDA device {device}, and shape {(rows, cols)}; got {t.dtype} {(r, c)} on {t.device}")
+    return pitch
 
 
 def checkpoint_activation(x, activation: str = "silu", *, gated: bool = True, out=None, stream=None):
@@ -50,46 +48,43 @@ def checkpoint_activation(x, activation: str = "silu", *, gated: bool = True, ou
     itself, and the ``ActivationCheckpoint`` that ``checkpoint_activation_backward`` takes.  ``x`` is (T, 2F) or (T, F) bf16 /
     fp16; ``activation``: "identity", "relu", "gelu" (erf form) or "silu"; ``out`` (T, F) may be given.  A block of 128 values
     with a NaN or an infinity is kept as NaN.  Asynchronous on ``stream`` (None: torch's current stream)."""
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"unknown activation {activation!r}: one of {sorted(ACTIVATIONS)}")
-    _check_matrix("x", x, None)
+    kind, device, T, cols, ldx = _matrix("x", x, _IN_KINDS)
     _no_gradient("checkpoint_activation", x)
-    T, cols = x.shape
+    gated = bool(gated)
     if gated and cols % 2 != 0:
         raise ValueError(f"a gated activation needs an even number of columns (gate | up), got {cols}")
-    parts = 2 if gated else 1
-    F = cols // parts
-    device = x.device
-    made = [torch.empty((T, parts, -(-F // 16) * 16), dtype=torch.int8, device=device),
-            torch.empty((T, parts, -(-F // BLOCK)), dtype=torch.float32, device=device)]
-    kept = ActivationCheckpoint(made[0], made[1], activation, bool(gated), F, x.dtype)
+    parts, F = (2, cols // 2) if gated else (1, cols)
+    q = x.new_empty((T, parts, (F + 15) & ~15), dtype=torch.int8)
+    scale = x.new_empty((T, parts, (F + BLOCK - 1) // BLOCK), dtype=torch.float32)
     if out is None:
-        out = torch.empty((T, F), dtype=x.dtype, device=device)
-        made.append(out)
+        out, ldh = x.new_empty((T, F)), F
+        made = (q, scale, out)
     else:
-        _check_matrix("out", out, F, x.dtype, T, device)
-    a = L.ActArgs(_IN_KINDS[x.dtype], ACTIVATIONS[activation], parts - 1, 0, T, F, x.data_ptr(), x.stride(0) if T > 1 else cols,
-                  out.data_ptr(), out.stride(0) if T > 1 else F, made[0].data_ptr(), made[1].data_ptr())
-    _on_stream(device, stream, lambda s: L.check(L.load().bsg_act_forward(C.byref(a), s)), *made)
-    return out, kept
+        ldh = _given("out", out, kind, device, T, F)
+        made = (q, scale)
+    pack, call = L.direct("bsg_act_forward", L.ACT_LAYOUT)
+    _launch(device, stream, made, call, pack(kind, act, parts - 1, 0, T, F, x.data_ptr(), ldx, out.data_ptr(), ldh, q.data_ptr(), scale.data_ptr()))
+    return out, ActivationCheckpoint(q, scale, activation, gated, F, x.dtype)
 
 
 def checkpoint_activation_backward(grad, kept: ActivationCheckpoint, *, out=None, stream=None) -> torch.Tensor:
     """Gradient of ``x`` for the gradient ``grad`` (T, F) of ``h``, from what ``checkpoint_activation`` kept: (T, 2F) or (T, F)
     in the type of ``x``.  ``out`` may be given.  Asynchronous on ``stream`` (None: torch's current stream)."""
-    T, parts, F = kept.quantized.shape[0], 2 if kept.gated else 1, kept.width
-    device = kept.quantized.device
-    _check_matrix("grad", grad, F, kept.dtype, T, device)
+    q, F = kept.quantized, kept.width
+    kind, device, (T, parts, _) = _IN_KINDS[kept.dtype], q.get_device(), q.shape
+    ldg = _given("grad", grad, kind, device, T, F)
     _no_gradient("checkpoint_activation_backward", grad)
-    made = []
     if out is None:
-        out = torch.empty((T, parts * F), dtype=kept.dtype, device=device)
-        made.append(out)
+        out, ldx = grad.new_empty((T, parts * F)), parts * F
+        made = (out,)
     else:
-        _check_matrix("out", out, parts * F, kept.dtype, T, device)
-    a = L.ActArgs(_IN_KINDS[kept.dtype], ACTIVATIONS[kept.activation], parts - 1, 0, T, F, grad.data_ptr(), grad.stride(0) if T > 1 else F,
-                  out.data_ptr(), out.stride(0) if T > 1 else parts * F, kept.quantized.data_ptr(), kept.scale.data_ptr())
-    _on_stream(device, stream, lambda s: L.check(L.load().bsg_act_backward(C.byref(a), s)), *made)
+        ldx, made = _given("out", out, kind, device, T, parts * F), ()
+    pack, call = L.direct("bsg_act_backward", L.ACT_LAYOUT)
+    _launch(device, stream, made, call, pack(kind, ACTIVATIONS[kept.activation], parts - 1, 0, T, F, grad.data_ptr(), ldg, out.data_ptr(), ldx,
+                                             q.data_ptr(), kept.scale.data_ptr()))
     return out
 
 

@@ -909,6 +909,26 @@ int32_t host_operand_map(CUtensorMap* map, const void* base, uint64_t row_bytes,
 int32_t host_out_map(CUtensorMap* map, const void* base, int32_t out_kind, uint64_t cols, uint64_t rows, uint64_t pitch_elems) {
   return make_out_map(map, base, out_kind, cols, rows, 1, pitch_elems, rows * pitch_elems);
 }
+int32_t host_device(int32_t not_sm100, int32_t cuda_error, int* dev, int* sms) {
+  static std::mutex mu;
+  static int known[64];      // SM count of a device that was looked up and is sm_100
+  cudaError_t e = cudaGetDevice(dev);
+  if (e != cudaSuccess) return host_fail(cuda_error, "cudaGetDevice: %s", cudaGetErrorString(e));
+  const bool small = *dev >= 0 && *dev < 64;
+  if (small) {
+    std::lock_guard<std::mutex> lock(mu);
+    if ((*sms = known[*dev]) > 0) return BSG_OK;
+  }
+  int major = 0;
+  cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, *dev);
+  cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, *dev);
+  if (major != 10) return host_fail(not_sm100, "device compute capability %d.x is not sm_100", major);
+  if (small) {
+    std::lock_guard<std::mutex> lock(mu);
+    known[*dev] = *sms;
+  }
+  return BSG_OK;
+}
 }  // namespace bsg
 
 extern "C" {

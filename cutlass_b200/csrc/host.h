@@ -19,14 +19,6 @@ BSG_HIDDEN int32_t host_out_map(CUtensorMap* map, const void* base, int32_t out_
 inline bool host_aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 // Current device and its SM count; refuses devices that are not sm_100.
-inline int32_t host_device(int32_t not_sm100, int32_t cuda_error, int* dev, int* sms) {
-  cudaError_t e = cudaGetDevice(dev);
-  if (e != cudaSuccess) return host_fail(cuda_error, "cudaGetDevice: %s", cudaGetErrorString(e));
-  int major = 0;
-  cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, *dev);
-  cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, *dev);
-  if (major != 10) return host_fail(not_sm100, "device compute capability %d.x is not sm_100", major);
-  return 0;
-}
+BSG_HIDDEN int32_t host_device(int32_t not_sm100, int32_t cuda_error, int* dev, int* sms);
 
 }  // namespace bsg

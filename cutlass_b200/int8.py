@@ -9,48 +9,66 @@ experts.  Operands that are already quantised go through ``GemmArguments`` / ``G
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import lib as L
 from .arguments import ACTIVATIONS, ScaledOperand, ScaleSwizzleMode
-from .operator import MAX_INT8_K, _default_workspace, to_cuda_stream
+from .operator import MAX_INT8_K, _default_workspace, _default_workspaces, to_cuda_stream
 
 _IN_KINDS = {torch.bfloat16: L.OUT_BF16, torch.float16: L.OUT_F16}
 _OUT_KINDS = {torch.bfloat16: L.OUT_BF16, torch.float16: L.OUT_F16, torch.float32: L.OUT_F32}
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def _on_stream(device, stream, run, *made):
-    """Calls ``run(handle)`` with ``device`` current and the raw handle of ``stream`` (None: torch's current stream of that
-    device).  ``made`` are tensors this module allocated on the current stream: another stream's use of them is recorded."""
-    if device.index != torch.cuda.current_device():
+def _launch(device: int, stream, made, call, *args) -> None:
+    """``call(*args, handle)`` with ``device`` current and the raw handle of ``stream`` (None: torch's current stream of that
+    device).  ``made`` are tensors that were allocated for the call on the current stream: if it runs on another one, the
+    allocator is told."""
+    if device != _current_device():
         with torch.cuda.device(device):
-            return _on_stream(device, stream, run, *made)
-    handle = torch.cuda.current_stream().cuda_stream
-    if stream is not None and to_cuda_stream(stream) != handle:
-        handle = to_cuda_stream(stream)
-        other = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
-        for t in made:
-            t.record_stream(other)
-    return run(handle)
+            return _launch(device, stream, made, call, *args)
+    handle = _current_stream(device)
+    if stream is not None:
+        other = to_cuda_stream(stream)
+        if other != handle:
+            s = torch.cuda.ExternalStream(other, device=device) if other else torch.cuda.default_stream(device)
+            for t in made:
+                t.record_stream(s)
+            handle = other
+    code = call(*args, handle)
+    if code:
+        L.check(code)
 
 
-def _no_gradient(name, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{name} has no gradient: call it under torch.no_grad() or detach its inputs")
+def _no_gradient(name, *tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} has no gradient: call it under torch.no_grad() or detach its inputs")
 
 
-def _check_tokens(x) -> None:
-    if x.dim() != 2 or x.dtype not in _IN_KINDS or not x.is_cuda or (x.stride(1) != 1 and x.shape[1] > 1):
-        raise ValueError("x must be a 2-D bf16 or fp16 CUDA tensor with unit stride along K")
-    if x.shape[1] < 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-        raise ValueError("x must have at least one column and rows that do not overlap")
+def _matrix(name, t, kinds):
+    """(kind, device index, rows, columns, row pitch) of a row-major CUDA matrix; columns that do not overlap."""
+    shape, kind, device = t.shape, kinds.get(t.dtype), t.get_device()
+    if len(shape) != 2 or kind is None or device < 0:
+        raise ValueError(f"{name} must be a 2-D CUDA tensor of type {', '.join(str(k) for k in kinds)}, got {t.dtype} {tuple(shape)} on {t.device}")
+    rows, cols = shape
+    pitch, step = t.stride()
+    if cols < 1 or (step != 1 and cols > 1) or (rows > 1 and pitch < cols):
+        raise ValueError(f"{name} must have at least one column, unit stride along its columns and rows that do not overlap")
+    return kind, device, rows, cols, (pitch if rows > 1 else cols)
 
 
-def _check_vector(name, t, dtype, shape, device) -> None:
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}")
+def _check_array(name, t, dtype, shape, device) -> None:
+    if t.dtype != dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on CUDA device {device}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _check_rows(rows, device) -> int:
+    if rows.dtype != torch.int32 or rows.dim() != 1 or rows.get_device() != device or not rows.is_contiguous():
+        raise ValueError("rows must be a contiguous 1-D int32 tensor on the device of x")
+    return rows.shape[0]
 
 
 def quantize_int8(x, *, rows=None, out=None, scale_out=None, stream=None) -> ScaledOperand:
@@ -61,12 +79,9 @@ def quantize_int8(x, *, rows=None, out=None, scale_out=None, stream=None) -> Sca
     scale NaN), as a grouped product wants its tokens.  The result's rows start on 16-byte boundaries, whatever K is.
     ``out`` (R, K) int8 with such rows and ``scale_out`` (R,) fp32 may be given.  Asynchronous on ``stream`` (None: torch's
     current stream)."""
-    _check_tokens(x)
+    kind, device, M, K, ldx = _matrix("x", x, _IN_KINDS)
     _no_gradient("quantize_int8", x)
-    M, K = x.shape
-    if rows is not None and (rows.dim() != 1 or rows.dtype != torch.int32 or not rows.is_contiguous() or rows.device != x.device):
-        raise ValueError("rows must be a contiguous 1-D int32 tensor on the device of x")
-    R = M if rows is None else rows.shape[0]
+    R = M if rows is None else _check_rows(rows, device)
     made = []
     if out is None:
         made.append(torch.empty((R, -(-K // 16) * 16), dtype=torch.int8, device=x.device))
@@ -77,13 +92,11 @@ def quantize_int8(x, *, rows=None, out=None, scale_out=None, stream=None) -> Sca
     if scale_out is None:
         scale_out = torch.empty(R, dtype=torch.float32, device=x.device)
         made.append(scale_out)
-    _check_vector("scale_out", scale_out, torch.float32, (R,), x.device)
-    a = L.Int8Args()
-    a.in_kind, a.rows, a.tokens, a.K = _IN_KINDS[x.dtype], R, M, K
-    a.X, a.ldx = x.data_ptr(), x.stride(0) if M > 1 else K
-    a.index = rows.data_ptr() if rows is not None else None
-    a.Q, a.ldq, a.q_scale = out.data_ptr(), out.stride(0) if R > 1 else -(-K // 16) * 16, scale_out.data_ptr()
-    _on_stream(x.device, stream, lambda s: L.check(L.load().bsg_int8_quantize(C.byref(a), s)), *made)
+    _check_array("scale_out", scale_out, torch.float32, (R,), device)
+    pack, call = L.direct("bsg_int8_quantize", L.INT8_LAYOUT)
+    args = pack(kind, 0, 1, 0, R, M, 1, K, x.data_ptr(), ldx, 0 if rows is None else rows.data_ptr(), out.data_ptr(),
+                out.stride(0) if R > 1 else -(-K // 16) * 16, scale_out.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    _launch(device, stream, made, call, args)
     return ScaledOperand(out, scale_out, (1, 1, K), ScaleSwizzleMode.SwizzleNone)
 
 
@@ -100,53 +113,57 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
     written.  Offsets that fall or leave the rows are clamped and reported by ``check_device_status`` of an operator.
 
     No gradient is kept.  Asynchronous on ``stream`` (None: torch's current stream)."""
-    _check_tokens(x)
+    in_kind, device, M, K, ldx = _matrix("x", x, _IN_KINDS)
     _no_gradient("int8_linear", x, weight_scale, bias)
-    M, K = x.shape
-    device = x.device
-    grouped = offsets is not None
-    if weight.dim() != (3 if grouped else 2) or weight.dtype != torch.int8 or weight.device != device or weight.shape[-1] != K:
-        raise ValueError(f"weight must be an int8 tensor of shape {'(experts, N, K)' if grouped else '(N, K)'} with K = {K} on {device}")
-    N = weight.shape[-2]
-    strides = weight.stride()
-    if N < 1 or (K > 1 and strides[-1] != 1) or (N > 1 and (strides[-2] < K or strides[-2] % 16 != 0)) or weight.data_ptr() % 16 != 0 \
-            or (grouped and weight.shape[0] > 1 and strides[0] % 16 != 0):
+    shape, strides, w = weight.shape, weight.stride(), weight.data_ptr()
+    if offsets is None:
+        if rows is not None:
+            raise ValueError("rows goes with offsets")
+        if len(shape) != 2:
+            raise ValueError(f"weight must be (N, K), or (experts, N, K) with offsets; got {tuple(shape)}")
+        experts, group_stride, R, per_channel = 1, 0, M, shape[:1]
+    else:
+        if len(shape) != 3 or not 1 <= shape[0] <= L.MAX_GROUPS:
+            raise ValueError(f"with offsets, weight must be (experts, N, K) with 1 to {L.MAX_GROUPS} experts; got {tuple(shape)}")
+        experts, per_channel = shape[0], shape[:2]
+        group_stride = strides[0] if experts > 1 else 0
+        _check_array("offsets", offsets, torch.int32, shape[:1], device)
+        R = M if rows is None else _check_rows(rows, device)
+    N, pitch = shape[-2], (K + 15) & ~15
+    ldw = strides[-2] if N > 1 else pitch
+    if weight.dtype != torch.int8 or weight.get_device() != device or shape[-1] != K or N < 1:
+        raise ValueError(f"weight must be an int8 tensor on CUDA device {device} whose last extent is K = {K}, got {weight.dtype} {tuple(shape)} on {weight.device}")
+    if (strides[-1] != 1 and K > 1) or ldw < K or ldw & 15 or w & 15 or group_stride & 15:
         raise ValueError("the rows of weight must have unit stride along K and start on 16-byte boundaries (quantize_int8 lays them out so)")
-    per_channel = (weight.shape[0], N) if grouped else (N,)
-    _check_vector("weight_scale", weight_scale, torch.float32, per_channel, device)
+    _check_array("weight_scale", weight_scale, torch.float32, per_channel, device)
     if bias is not None:
-        _check_vector("bias", bias, torch.float32, per_channel, device)
-    if grouped:
-        if not 1 <= weight.shape[0] <= L.MAX_GROUPS:
-            raise ValueError(f"between 1 and {L.MAX_GROUPS} experts are supported, got {weight.shape[0]}")
-        _check_vector("offsets", offsets, torch.int32, (weight.shape[0],), device)
-    if rows is not None and (not grouped or rows.dim() != 1 or rows.dtype != torch.int32 or not rows.is_contiguous() or rows.device != device):
-        raise ValueError("rows must be a contiguous 1-D int32 tensor on the device of x, and goes with offsets")
+        _check_array("bias", bias, torch.float32, per_channel, device)
     if K > MAX_INT8_K:
         raise ValueError(f"K={K} exceeds {MAX_INT8_K} (32-bit sums)")
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise ValueError(f"unknown activation {activation!r}: one of {sorted(ACTIVATIONS)}")
-    R = M if rows is None else rows.shape[0]
-    pitch = -(-K // 16) * 16
-    scratch = torch.empty(R * (pitch + 4), dtype=torch.int8, device=device)        # 8-bit tokens, then their scales
-    made = [scratch]
+    scratch = x.new_empty(R * (pitch + 4), dtype=torch.int8)        # 8-bit tokens, then their scales
     if out is None:
-        out = torch.empty((R, N), dtype=out_dtype or x.dtype, device=device)
-        made.append(out)
-    elif tuple(out.shape) != (R, N) or out.device != device or (out_dtype is not None and out.dtype != out_dtype) \
-            or (N > 1 and out.stride(1) != 1) or (R > 1 and out.stride(0) < N):
-        raise ValueError(f"out must be a row-major {out_dtype or 'bf16, fp16 or fp32'} tensor of shape {(R, N)} on {device}")
-    if out.dtype not in _OUT_KINDS:
+        out = x.new_empty((R, N), dtype=out_dtype)
+        made, ldd = (scratch, out), N
+        out_kind = _OUT_KINDS.get(out.dtype)
+    else:
+        out_kind, out_device, out_rows, out_cols, ldd = _matrix("out", out, _OUT_KINDS)
+        made = (scratch,)
+        if (out_rows, out_cols, out_device) != (R, N, device) or (out_dtype is not None and out.dtype != out_dtype):
+            raise ValueError(f"out must be a {out_dtype or ''} tensor of shape {(R, N)} on CUDA device {device}")
+    if out_kind is None:
         raise ValueError(f"out dtype {out.dtype} is not supported (bf16, fp16 or fp32)")
     if R == 0:
         return out
     q = scratch.data_ptr()
-    a = L.Int8Args(
-        _IN_KINDS[x.dtype], _OUT_KINDS[out.dtype], weight.shape[0] if grouped else 1, ACTIVATIONS[activation], R, M, N, K,
-        x.data_ptr(), x.stride(0) if M > 1 else K, rows.data_ptr() if rows is not None else None, q, pitch, q + R * pitch,
-        weight.data_ptr(), strides[-2] if N > 1 else pitch, strides[0] if grouped and weight.shape[0] > 1 else 0,
-        weight_scale.data_ptr(), bias.data_ptr() if bias is not None else None, offsets.data_ptr() if grouped else None,
-        out.data_ptr(), out.stride(0) if R > 1 else N)
-    ws = _default_workspace(device)
-    _on_stream(device, stream, lambda s: L.check(L.load().bsg_int8_linear_run(C.byref(a), ws.data_ptr(), 16, s)), *made)
+    status = _default_workspaces.get(device)
+    if status is None:
+        status = _default_workspace(x.device)
+    pack, call = L.direct("bsg_int8_linear_run", L.INT8_LAYOUT)
+    args = pack(in_kind, out_kind, experts, act, R, M, N, K, x.data_ptr(), ldx, 0 if rows is None else rows.data_ptr(), q, pitch,
+                q + R * pitch, w, ldw, group_stride, weight_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                0 if offsets is None else offsets.data_ptr(), out.data_ptr(), ldd, 0, 0, 0, 0)
+    _launch(device, stream, made, call, args, status.data_ptr(), 16)
     return out

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # BSG_PROFILE=1 selects the instrumented build (python -m cutlass_b200.build with the same variable set).
@@ -106,6 +107,11 @@ class QuantArgs(C.Structure):
                 ("ldx", C.c_int64), ("Q", C.c_void_p), ("SF", C.c_void_p), ("norm_constant", C.c_void_p)]
 
 
+INT8_LAYOUT = "4i4qPqPPqPPqqPPPPq4i"      # Int8Args, ActArgs and RouteArgs below as struct formats
+ACT_LAYOUT = "4i2qPqPqPP"
+ROUTE_LAYOUT = "4iqPq12Pq"
+
+
 class Int8Args(C.Structure):
     """``bsg_int8_args`` of include/bsgemm.h, field for field."""
     _fields_ = [
@@ -177,6 +183,20 @@ SYMBOLS = {
 }
 
 _lib = None
+_direct: dict = {}
+
+
+def direct(name: str, layout: str):
+    """(pack, call) of an entry point whose argument struct is passed as packed bytes: ``pack(*fields)`` lays the fields out as
+    ``layout`` (native alignment) says, ``call(bytes, ...)`` takes the other arguments as integers.  A call through
+    ``ctypes.Structure`` costs several microseconds more, which a kernel of a few microseconds does not hide."""
+    found = _direct.get(name)
+    if found is None:
+        fn = load()[name]                    # a function object of its own: the prototypes of SYMBOLS stay as they are
+        fn.restype = C.c_int32
+        fn.argtypes = [C.c_char_p] + [C.c_void_p if t is not C.c_size_t else t for t in SYMBOLS[name][1][1:]]
+        found = _direct[name] = (struct.Struct("@" + layout).pack, fn)
+    return found
 
 
 class BsgError(RuntimeError):

@@ -9,14 +9,13 @@ carry gradients to the logits when those require them.
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import NamedTuple
 
 import torch
 
 from . import lib as L
 from .int8 import _OUT_KINDS as _KINDS
-from .int8 import _on_stream
+from .int8 import _check_array, _launch, _matrix
 
 MAX_EXPERTS, MAX_TOP_K = 1024, 32
 
@@ -41,63 +40,57 @@ def _scratch_words(T: int, E: int) -> int:
     return blocks * (2 * E + 1) + E
 
 
-def _check_logits(logits, top_k, token_mask) -> None:
-    if logits.dim() != 2 or logits.dtype not in _KINDS or not logits.is_cuda or (logits.shape[1] > 1 and logits.stride(1) != 1) \
-            or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
-        raise ValueError("logits must be a 2-D row-major bf16, fp16 or fp32 CUDA tensor")
-    T, E = logits.shape
-    if not 1 <= E <= MAX_EXPERTS:
+def _check_logits(logits, top_k):
+    kind, device, T, E, ld = _matrix("logits", logits, _KINDS)
+    if E > MAX_EXPERTS:
         raise ValueError(f"between 1 and {MAX_EXPERTS} experts are supported, got {E}")
-    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 1 <= top_k <= min(MAX_TOP_K, E):
+    if type(top_k) is not int or not 1 <= top_k <= min(MAX_TOP_K, E):
         raise ValueError(f"top_k must be an int between 1 and min({MAX_TOP_K}, {E}), got {top_k!r}")
     if T * top_k > 0x7FFFFFFF:
         raise ValueError(f"{T} tokens with {top_k} choices exceed 2^31 rows")
-    if token_mask is not None and (token_mask.dtype != torch.bool or tuple(token_mask.shape) != (T,) or not token_mask.is_contiguous()
-                                   or token_mask.device != logits.device):
-        raise ValueError(f"token_mask must be a contiguous bool tensor of shape {(T,)} on {logits.device}")
+    return kind, device, T, E, ld
 
 
 def _forward(logits, top_k, token_mask, normalize, stream) -> Routing:
-    T, E = logits.shape
-    device = logits.device
+    kind, device, T, E, ld = _check_logits(logits, top_k)
+    if token_mask is not None:
+        _check_array("token_mask", token_mask, torch.bool, (T,), device)
+    normalize = bool(normalize)
     n = T * top_k
     # what is whole comes from one allocation; the two results that carry gradients are tensors of their own
-    whole = torch.empty(3 * n + 2 * E + 1, dtype=torch.int32, device=device)
-    weights = torch.empty((T, top_k), dtype=torch.float32, device=device)
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    scratch = torch.empty(_scratch_words(T, E), dtype=torch.int32, device=device)
+    whole = logits.new_empty(3 * n + 2 * E + 1, dtype=torch.int32)
+    weights = logits.new_empty((T, top_k), dtype=torch.float32)
+    loss = logits.new_empty((), dtype=torch.float32)
+    scratch = logits.new_empty(_scratch_words(T, E), dtype=torch.int32)
     w = whole.data_ptr()
-    a = L.RouteArgs(_KINDS[logits.dtype], E, top_k, int(normalize), T, logits.data_ptr(), logits.stride(0) if T > 1 else E,
-                    token_mask.data_ptr() if token_mask is not None else None,
-                    w, weights.data_ptr(), w + 12 * n, w + 12 * n + 8 * E, w + 12 * n + 4 * E, w + 4 * n, w + 8 * n, loss.data_ptr())
-    _on_stream(device, stream, lambda s: L.check(L.load().bsg_route_forward(C.byref(a), scratch.data_ptr(), 4 * scratch.numel(), s)),
-               whole, weights, loss, scratch)
+    pack, call = L.direct("bsg_route_forward", L.ROUTE_LAYOUT)
+    args = pack(kind, E, top_k, normalize, T, logits.data_ptr(), ld, 0 if token_mask is None else token_mask.data_ptr(),
+                w, weights.data_ptr(), w + 12 * n, w + 12 * n + 8 * E, w + 12 * n + 4 * E, w + 4 * n, w + 8 * n, loss.data_ptr(), 0, 0, 0, 0)
+    _launch(device, stream, (whole, weights, loss, scratch), call, args, scratch.data_ptr(), 4 * scratch.numel())
     experts, rows, positions, counts, offsets, live = whole.split_with_sizes([n, n, n, E, E, 1])
-    return Routing(experts.view(T, top_k), weights, counts, offsets, rows, positions.view(T, top_k), loss, live, bool(normalize))
+    return Routing(experts.view(T, top_k), weights, counts, offsets, rows, positions.view(T, top_k), loss, live, normalize)
 
 
 def route_tokens_backward(logits, routing: Routing, grad_weights=None, grad_balance_loss=None, *, stream=None) -> torch.Tensor:
     """Gradient of ``logits`` (in their type) for the gradients of ``routing.weights`` (T, k) fp32 and ``routing.balance_loss``
     () fp32, either of which may be None (zero).  The counts are constants.  Asynchronous on ``stream`` (None: torch's current
     stream)."""
-    k = routing.experts.shape[1]
-    _check_logits(logits, k, None)
-    T, E = logits.shape
-    device = logits.device
-    if tuple(routing.experts.shape) != (T, k) or tuple(routing.counts.shape) != (E,) or routing.experts.device != device:
+    experts, counts = routing.experts, routing.counts
+    k = experts.shape[1]
+    kind, device, T, E, ld = _check_logits(logits, k)
+    if experts.shape[0] != T or counts.shape[0] != E or experts.get_device() != device:
         raise ValueError("routing does not belong to these logits")
-    if grad_weights is not None and (grad_weights.dtype != torch.float32 or tuple(grad_weights.shape) != (T, k)
-                                     or not grad_weights.is_contiguous() or grad_weights.device != device):
-        raise ValueError(f"grad_weights must be a contiguous fp32 tensor of shape {(T, k)} on {device}")
+    if grad_weights is not None:
+        _check_array("grad_weights", grad_weights, torch.float32, experts.shape, device)
     if grad_balance_loss is not None and (grad_balance_loss.dtype != torch.float32 or grad_balance_loss.numel() != 1
-                                          or grad_balance_loss.device != device):
-        raise ValueError(f"grad_balance_loss must be a one-element fp32 tensor on {device}")
-    out = torch.empty((T, E), dtype=logits.dtype, device=device)
-    a = L.RouteArgs(_KINDS[logits.dtype], E, k, int(routing.normalize), T, logits.data_ptr(), logits.stride(0) if T > 1 else E, None,
-                    routing.experts.data_ptr(), routing.weights.data_ptr(), routing.counts.data_ptr(), routing.num_tokens.data_ptr(),
-                    None, None, None, None, grad_weights.data_ptr() if grad_weights is not None else None,
-                    grad_balance_loss.data_ptr() if grad_balance_loss is not None else None, out.data_ptr(), E)
-    _on_stream(device, stream, lambda s: L.check(L.load().bsg_route_backward(C.byref(a), s)), out)
+                                          or grad_balance_loss.get_device() != device):
+        raise ValueError(f"grad_balance_loss must be a one-element fp32 tensor on CUDA device {device}")
+    out = logits.new_empty((T, E))
+    pack, call = L.direct("bsg_route_backward", L.ROUTE_LAYOUT)
+    args = pack(kind, E, k, routing.normalize, T, logits.data_ptr(), ld, 0, experts.data_ptr(), routing.weights.data_ptr(),
+                counts.data_ptr(), routing.num_tokens.data_ptr(), 0, 0, 0, 0, 0 if grad_weights is None else grad_weights.data_ptr(),
+                0 if grad_balance_loss is None else grad_balance_loss.data_ptr(), out.data_ptr(), E)
+    _launch(device, stream, (out,), call, args)
     return out
 
 
@@ -134,7 +127,6 @@ def route_tokens(logits, top_k: int, *, token_mask=None, normalize: bool = True,
 
     E is at most 1024 and k at most 32.  Results do not depend on the order in which anything runs.  Asynchronous on ``stream``
     (None: torch's current stream); the backward pass runs on the stream that autograd makes current."""
-    _check_logits(logits, top_k, token_mask)
     if not (torch.is_grad_enabled() and logits.requires_grad):
         return _forward(logits, top_k, token_mask, normalize, stream)
     weights, loss, experts, counts, offsets, rows, positions, live = _Route.apply(logits, top_k, token_mask, normalize, stream)
