@@ -14,16 +14,17 @@ namespace {
 using bsg::host_aligned;
 using bsg::host_fail;
 
-int32_t check_quantise(const bsg_int8_args& a) {
+// `own_q`: Q and q_scale are the caller's (false for the kernel that quantises on the way and has none).
+int32_t check_quantise(const bsg_int8_args& a, bool own_q) {
   if (a.in_kind != BSG_OUT_BF16 && a.in_kind != BSG_OUT_F16) return host_fail(BSG_ERR_NOT_SUPPORTED, "X must be bf16 or fp16 (kind %d)", a.in_kind);
   if (a.rows < 0 || a.tokens < 0 || a.K < 1) return host_fail(BSG_ERR_INVALID_PROBLEM, "extents must be positive (rows=%lld tokens=%lld K=%lld)", (long long)a.rows, (long long)a.tokens, (long long)a.K);
   if (a.rows > 0x3FFFFFFF || a.tokens > 0x3FFFFFFF || a.K > 0x3FFFFFFF) return host_fail(BSG_ERR_INVALID_PROBLEM, "extent exceeds 2^30");
   if (!a.index && a.rows != a.tokens) return host_fail(BSG_ERR_INVALID_PROBLEM, "without an index the %lld rows must be the %lld tokens", (long long)a.rows, (long long)a.tokens);
   if (a.rows == 0) return BSG_OK;
-  if (!a.Q || !a.q_scale || (!a.X && a.tokens > 0)) return host_fail(BSG_ERR_INVALID_PROBLEM, "X, Q and q_scale must not be null");
+  if ((own_q && (!a.Q || !a.q_scale)) || (!a.X && a.tokens > 0)) return host_fail(BSG_ERR_INVALID_PROBLEM, "X, Q and q_scale must not be null");
   if (!host_aligned(a.X, 2) || !host_aligned(a.q_scale, 4)) return host_fail(BSG_ERR_MISALIGNED_OPERAND, "X and q_scale must be aligned to their elements");
   if (a.ldx < a.K && a.tokens > 1) return host_fail(BSG_ERR_INVALID_PROBLEM, "ldx=%lld is smaller than K", (long long)a.ldx);
-  if (a.ldq < a.K || a.ldq % 16 != 0 || !host_aligned(a.Q, 16)) return host_fail(BSG_ERR_MISALIGNED_OPERAND, "rows of Q must start on 16-byte boundaries (ldq=%lld, at least K)", (long long)a.ldq);
+  if (own_q && (a.ldq < a.K || a.ldq % 16 != 0 || !host_aligned(a.Q, 16))) return host_fail(BSG_ERR_MISALIGNED_OPERAND, "rows of Q must start on 16-byte boundaries (ldq=%lld, at least K)", (long long)a.ldq);
   return BSG_OK;
 }
 
@@ -33,7 +34,62 @@ struct I8Plan {
   int32_t split;   // few: CTAs of a cluster that share one tile's K
 };
 
-int32_t check_product(const bsg_int8_args& a, I8Plan* plan) {
+// Kernel, tile and split, by a model of the time.  A CTA (or pair) streams its part of K through a pipeline that is bound by the
+// latency of a TMA round trip, so a k-tile of 128 values takes a time that depends on the tile alone; two CTAs of the kernel
+// for few rows are resident on an SM, one pair of the other kernel on two SMs; a grid runs in whole waves.  The constants were
+// fitted to 60 problems from 16 x 512 x 512 to 777 x 14336 x 8192 (rows x N x K), where the choice is within 10 % of the best
+// of all variants in all but six: e.g. 777 x 5000 x 8192: 128-token tiles 34.5 us, 64-token tiles 43.7, 256 x 128 44.5,
+// 256 x 256 48.8; 256 x 5000 x 8192: 256 x 128 20.7 us, 64-token tiles 25.2, 256 x 256 27.2, 128-token tiles 30.7.
+struct Variant {
+  bool few;
+  int32_t tile;
+  double per_k_tile, fixed;      // microseconds
+};
+constexpr Variant kVariants[] = {{true, 16, 0.20, 4.5}, {true, 32, 0.235, 4.5}, {true, 64, 0.29, 4.6}, {true, 128, 0.40, 4.8},
+                                 {false, 128, 0.19, 7.0}, {false, 256, 0.30, 8.0}};
+constexpr double kHbmBytesPerUs = 6.5e6;
+
+int32_t choose(const bsg_int8_args& a, I8Plan* plan) {
+  const int64_t k_tiles = (a.K + 127) / 128;
+  const int64_t active = a.rows < a.num_groups ? a.rows : a.num_groups;      // groups that can have rows
+  const double weights = double(a.N) * double(a.K) * double(active > 0 ? active : 1) / kHbmBytesPerUs;
+  double best = 1e300;
+  bool found = false;
+  for (const Variant& v : kVariants) {
+    if ((a.kernel == 1 && !v.few) || (a.kernel == 2 && v.few) || (a.tile && a.tile != v.tile)) continue;
+    const int64_t tile_m = v.few ? v.tile : 256, tile_n = v.few ? 128 : v.tile;
+    // row tiles: grouped, half of a group's last tile is empty on average
+    double tiles_m = double((a.rows + tile_m - 1) / tile_m);
+    if (a.offsets) {
+      tiles_m = double(a.rows) / double(tile_m) + 0.5 * double(active);
+      if (tiles_m < double(active)) tiles_m = double(active);
+    }
+    const double tiles = tiles_m * double((a.N + tile_n - 1) / tile_n);
+    for (int split = 1; split <= 8; split *= 2) {
+      if (split > 1 && (!v.few || v.tile > 64 || a.offsets || split > k_tiles)) break;
+      if (a.split ? a.split != split : split > 1 && (tiles * split > 296 || k_tiles < split * 2)) continue;
+      const double slots = v.few ? 296.0 : 74.0;
+      double waves = double(int64_t(tiles * split / slots));
+      if (waves * slots < tiles * split) waves += 1.0;
+      double t = waves * double((k_tiles + split - 1) / split) * v.per_k_tile;
+      if (t < weights) t = weights;
+      t += v.fixed + 0.1 * split;
+      if (t < best) {
+        best = t;
+        found = true;
+        plan->few = v.few;
+        plan->tile = v.tile;
+        plan->split = split;
+      }
+    }
+  }
+  if (!found)
+    return host_fail(BSG_ERR_NOT_SUPPORTED, "no variant with kernel %d, tile %d and split %d (few rows: 16, 32, 64 or 128 tokens, up to 64 of them "
+                     "with a split of 2, 4 or 8, dense, over at least as many 128-value pieces of K; many rows: 128 or 256 columns)", a.kernel, a.tile, a.split);
+  return BSG_OK;
+}
+
+int32_t check_product(const bsg_int8_args& a, bool own_q, I8Plan* plan) {
   if (a.out_kind != BSG_OUT_BF16 && a.out_kind != BSG_OUT_F16 && a.out_kind != BSG_OUT_F32)
     return host_fail(BSG_ERR_NOT_SUPPORTED, "the 8-bit integer product writes bf16, fp16 or fp32 (output kind %d)", a.out_kind);
   if (a.num_groups < 1 || a.num_groups > BSG_MAX_GROUPS) return host_fail(BSG_ERR_INVALID_PROBLEM, "group count %d outside [1, %d]", a.num_groups, BSG_MAX_GROUPS);
@@ -44,37 +100,15 @@ int32_t check_product(const bsg_int8_args& a, I8Plan* plan) {
   if (a.activation < BSG_ACT_IDENTITY || a.activation > BSG_ACT_SILU) return host_fail(BSG_ERR_NOT_SUPPORTED, "unknown activation %d", a.activation);
   if (a.kernel < 0 || a.kernel > 2) return host_fail(BSG_ERR_NOT_SUPPORTED, "unknown kernel %d", a.kernel);
   if (!a.W || !a.w_scale) return host_fail(BSG_ERR_INVALID_PROBLEM, "W and w_scale must not be null");
-  if (a.rows > 0 && (!a.Q || !a.q_scale || !a.D)) return host_fail(BSG_ERR_INVALID_PROBLEM, "Q, q_scale and D must not be null");
-  if (!host_aligned(a.W, 16) || a.ldw % 16 != 0 || !host_aligned(a.Q, 16) || a.ldq % 16 != 0)
+  if (a.rows > 0 && (!a.D || (own_q && (!a.Q || !a.q_scale)))) return host_fail(BSG_ERR_INVALID_PROBLEM, "Q, q_scale and D must not be null");
+  if (!host_aligned(a.W, 16) || a.ldw % 16 != 0 || (own_q && (!host_aligned(a.Q, 16) || a.ldq % 16 != 0)))
     return host_fail(BSG_ERR_MISALIGNED_OPERAND, "rows of Q and W must start on 16-byte boundaries (ldq=%lld, ldw=%lld)", (long long)a.ldq, (long long)a.ldw);
-  if (a.ldw < a.K || a.ldq < a.K || a.ldd < a.N) return host_fail(BSG_ERR_INVALID_PROBLEM, "ldq, ldw or ldd is smaller than a row");
+  if (a.ldw < a.K || (own_q && a.ldq < a.K) || a.ldd < a.N) return host_fail(BSG_ERR_INVALID_PROBLEM, "ldq, ldw or ldd is smaller than a row");
   if (a.num_groups > 1 && (a.group_stride_w % 16 != 0 || a.group_stride_w < 0)) return host_fail(BSG_ERR_MISALIGNED_OPERAND, "group_stride_w must be a multiple of 16");
   const int esz = a.out_kind == BSG_OUT_F32 ? 4 : 2;
   if (!host_aligned(a.D, esz) || !host_aligned(a.w_scale, 4) || !host_aligned(a.q_scale, 4) || !host_aligned(a.bias, 4) || !host_aligned(a.offsets, 4))
     return host_fail(BSG_ERR_MISALIGNED_OPERAND, "tensors must be aligned to their elements");
-  // Tiles.  Grouped: the ragged rows per group live on the device; the mean is what the host knows.
-  const int64_t mean = (a.rows + a.num_groups - 1) / a.num_groups;
-  plan->few = a.kernel ? a.kernel == 1 : mean <= 128;
-  if (plan->few) {
-    plan->tile = a.tile ? a.tile : mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
-    if (plan->tile != 16 && plan->tile != 32 && plan->tile != 64 && plan->tile != 128) return host_fail(BSG_ERR_NOT_SUPPORTED, "token tile %d: 16, 32, 64 or 128", plan->tile);
-    plan->split = 1;
-    if (!a.offsets && plan->tile <= 64) {
-      const int64_t tiles = ((a.N + 127) / 128) * ((a.rows + plan->tile - 1) / plan->tile), k_tiles = (a.K + 127) / 128;
-      while (plan->split < 8 && tiles * plan->split * 2 <= 296 && k_tiles >= plan->split * 4) plan->split *= 2;
-    }
-    if (a.split > 1) {
-      if (a.offsets || plan->tile > 64 || (a.split != 2 && a.split != 4 && a.split != 8) || a.split > (a.K + 127) / 128)
-        return host_fail(BSG_ERR_NOT_SUPPORTED, "split %d: 2, 4 or 8 parts of at least 128 values, dense, token tile up to 64", a.split);
-      plan->split = a.split;
-    }
-  } else {
-    plan->tile = a.tile ? a.tile : a.N <= 128 ? 128 : 256;
-    plan->split = 1;
-    if (plan->tile != 128 && plan->tile != 256) return host_fail(BSG_ERR_NOT_SUPPORTED, "column tile %d: 128 or 256", plan->tile);
-    if (a.split > 1) return host_fail(BSG_ERR_NOT_SUPPORTED, "only the kernel for few rows splits K");
-  }
-  return BSG_OK;
+  return choose(a, plan);
 }
 
 // Raises the dynamic shared-memory limit of a kernel once per device.
@@ -158,18 +192,20 @@ int32_t launch_rows(const bsg_int8_args& a, bsg::I8GemmParams& p, cudaStream_t s
   return BSG_OK;
 }
 
-template <int BT>
-int32_t launch_few(const bsg_int8_args& a, bsg::I8GemmParams& p, int split, cudaStream_t s, int sms, int dev, bool pdl) {
-  using C = bsg::I8FewCfg<BT>;
+template <int BT, int SPLIT>
+int32_t launch_few(const bsg_int8_args& a, bsg::I8GemmParams& p, cudaStream_t s, int sms, int dev, bool pdl) {
+  using C = bsg::I8FewCfg<BT, SPLIT>;
+  constexpr int split = SPLIT;
   static SmemOnce once;
-  auto kernel = bsg::bsg_i8_few_kernel<BT>;
+  auto kernel = bsg::bsg_i8_few_kernel<BT, SPLIT>;
   int32_t rc = once.set(reinterpret_cast<const void*>(kernel), C::kSmemBytes, dev);
   if (rc != BSG_OK) return rc;
   CUtensorMap tmW, tmX;
   if ((rc = bsg::host_operand_map(&tmW, a.W, a.K, a.N, a.num_groups, a.ldw, a.num_groups > 1 ? a.group_stride_w : a.N * a.ldw, 128)) != BSG_OK) return rc;
   if ((rc = bsg::host_operand_map(&tmX, a.Q, a.K, a.rows, 1, a.ldq, a.rows * a.ldq, BT)) != BSG_OK) return rc;
   p.tiles_n = int32_t((a.N + 127) / 128);
-  p.band = 0x3FFFFF / p.tiles_n + 1;      // all token tiles of a channel tile in a row: its weights are then in L2
+  p.band = int32_t((a.rows + BT - 1) / BT);      // all token tiles of a channel tile in a row: its weights are then in L2
+  if (p.band > 0x7FFFFFFF / p.tiles_n) return host_fail(BSG_ERR_INVALID_PROBLEM, "too many tiles for one launch");
   p.tma_out = 0;
   int64_t workers = int64_t(2) * sms;
   const int64_t tiles = a.offsets ? (a.rows / BT + a.num_groups) * p.tiles_n : ((a.rows + BT - 1) / BT) * p.tiles_n;
@@ -182,9 +218,57 @@ int32_t launch_few(const bsg_int8_args& a, bsg::I8GemmParams& p, int split, cuda
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   launch_ex(cfg, split, pdl, attr);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmW, tmX, p, int32_t(split));
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmW, tmX, p);
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   return BSG_OK;
+}
+
+template <int BT>
+int32_t launch_few_split(const bsg_int8_args& a, bsg::I8GemmParams& p, int split, cudaStream_t s, int sms, int dev, bool pdl) {
+  switch (split) {
+    case 1: return launch_few<BT, 1>(a, p, s, sms, dev, pdl);
+    case 2: return launch_few<BT, 2>(a, p, s, sms, dev, pdl);
+    case 4: return launch_few<BT, 4>(a, p, s, sms, dev, pdl);
+    default: return launch_few<BT, 8>(a, p, s, sms, dev, pdl);
+  }
+}
+
+// Up to four dense tokens of at most 64 KB in 8 bits: the kernel that quantises on the way.
+bool fits_token_kernel(const bsg_int8_args& a) {
+  return !a.offsets && !a.index && a.num_groups == 1 && a.rows >= 1 && a.rows <= bsg::kI8TokenMost &&
+         int64_t(a.rows <= 1 ? 1 : a.rows <= 2 ? 2 : 4) * ((a.K + 15) / 16 * 16) <= bsg::kI8TokenShared;
+}
+
+template <int MT, bool FP16>
+int32_t launch_token(const bsg::I8TokenParams& p, cudaStream_t s, int sms, int dev) {
+  static SmemOnce once;
+  auto kernel = bsg::bsg_i8_token_kernel<MT, FP16>;
+  int32_t rc = once.set(reinterpret_cast<const void*>(kernel), bsg::kI8TokenShared, dev);
+  if (rc != BSG_OK) return rc;
+  const int groups = int((int64_t(p.N) * p.parts + 15) / 16), grid = groups < 2 * sms ? groups : 2 * sms;      // two CTAs fit an SM
+  kernel<<<grid, bsg::kI8TokenThreads, MT * ((p.K + 15) / 16 * 16), s>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
+  return BSG_OK;
+}
+template <bool FP16>
+int32_t pick_token(const bsg::I8TokenParams& p, cudaStream_t s, int sms, int dev) {
+  if (p.M <= 1) return launch_token<1, FP16>(p, s, sms, dev);
+  if (p.M <= 2) return launch_token<2, FP16>(p, s, sms, dev);
+  return launch_token<4, FP16>(p, s, sms, dev);
+}
+int32_t token_product(const bsg_int8_args& a, cudaStream_t s, int sms, int dev) {
+  bsg::I8TokenParams p;
+  p.X = static_cast<const uint16_t*>(a.X); p.W = static_cast<const int8_t*>(a.W); p.sb = a.w_scale; p.bias = a.bias; p.D = a.D;
+  p.ldx = a.ldx; p.ldw = a.ldw; p.ldd = a.ldd; p.M = int32_t(a.rows); p.N = int32_t(a.N); p.K = int32_t(a.K);
+  p.wide = host_aligned(a.X, 16) && a.ldx % 8 == 0;
+  p.out_kind = a.out_kind; p.activation = a.activation;
+  // Warps share two channels where there would be fewer CTAs than SMs otherwise (every CTA quantises the tokens for itself, so
+  // more of them than that cost more than they bring: one token, 4096 x 4096: 6.4 us unshared, 8.5 shared by two; 512 x 16384:
+  // 14.3 unshared, 7.0 shared by eight).
+  p.parts = 1;
+  while (p.parts < 8 && a.N * p.parts < 16 * int64_t(sms) && a.K > p.parts * 512) p.parts *= 2;
+  return a.in_kind == BSG_OUT_F16 ? pick_token<true>(p, s, sms, dev) : pick_token<false>(p, s, sms, dev);
 }
 
 int32_t product(const bsg_int8_args& a, const I8Plan& plan, void* workspace, cudaStream_t s, int sms, int dev, bool pdl) {
@@ -196,10 +280,10 @@ int32_t product(const bsg_int8_args& a, const I8Plan& plan, void* workspace, cud
   p.status = static_cast<uint32_t*>(workspace);
   if (plan.few) {
     switch (plan.tile) {
-      case 16: return launch_few<16>(a, p, plan.split, s, sms, dev, pdl);
-      case 32: return launch_few<32>(a, p, plan.split, s, sms, dev, pdl);
-      case 64: return launch_few<64>(a, p, plan.split, s, sms, dev, pdl);
-      default: return launch_few<128>(a, p, plan.split, s, sms, dev, pdl);
+      case 16: return launch_few_split<16>(a, p, plan.split, s, sms, dev, pdl);
+      case 32: return launch_few_split<32>(a, p, plan.split, s, sms, dev, pdl);
+      case 64: return launch_few_split<64>(a, p, plan.split, s, sms, dev, pdl);
+      default: return launch_few<128, 1>(a, p, s, sms, dev, pdl);
     }
   }
   return plan.tile == 128 ? launch_rows<2, 128>(a, p, s, sms, dev, pdl) : launch_rows<2, 256>(a, p, s, sms, dev, pdl);
@@ -218,7 +302,7 @@ extern "C" {
 int32_t bsg_int8_query(const bsg_int8_args* args, bsg_caps* caps) {
   if (!args) return host_fail(BSG_ERR_INVALID_PROBLEM, "args is null");
   I8Plan plan;
-  int32_t rc = check_product(*args, &plan);
+  int32_t rc = check_product(*args, true, &plan);
   if (rc != BSG_OK) return rc;
   if (caps) {
     memset(caps, 0, sizeof(*caps));
@@ -233,7 +317,7 @@ int32_t bsg_int8_query(const bsg_int8_args* args, bsg_caps* caps) {
 
 int32_t bsg_int8_quantize(const bsg_int8_args* args, void* cuda_stream) {
   if (!args) return host_fail(BSG_ERR_INVALID_PROBLEM, "args is null");
-  int32_t rc = check_quantise(*args);
+  int32_t rc = check_quantise(*args, true);
   int dev = 0, sms = 0;
   if (rc == BSG_OK && args->rows > 0) rc = bsg::host_device(BSG_ERR_ARCH_MISMATCH, BSG_ERR_CUDA, &dev, &sms);
   return rc != BSG_OK ? rc : quantise(*args, static_cast<cudaStream_t>(cuda_stream));
@@ -243,7 +327,7 @@ int32_t bsg_int8_gemm_run(const bsg_int8_args* args, void* workspace, size_t wor
   if (!args) return host_fail(BSG_ERR_INVALID_PROBLEM, "args is null");
   I8Plan plan;
   int dev = 0, sms = 0;
-  int32_t rc = check_product(*args, &plan);
+  int32_t rc = check_product(*args, true, &plan);
   if (rc == BSG_OK) rc = check_workspace(workspace, workspace_bytes);
   if (rc != BSG_OK || args->rows == 0) return rc;
   if ((rc = bsg::host_device(BSG_ERR_ARCH_MISMATCH, BSG_ERR_CUDA, &dev, &sms)) != BSG_OK) return rc;
@@ -254,12 +338,14 @@ int32_t bsg_int8_linear_run(const bsg_int8_args* args, void* workspace, size_t w
   if (!args) return host_fail(BSG_ERR_INVALID_PROBLEM, "args is null");
   I8Plan plan;
   int dev = 0, sms = 0;
-  int32_t rc = check_quantise(*args);
-  if (rc == BSG_OK) rc = check_product(*args, &plan);
+  const bool token = !args->Q && !args->q_scale && args->kernel == 0 && fits_token_kernel(*args);
+  int32_t rc = check_quantise(*args, !token);
+  if (rc == BSG_OK) rc = check_product(*args, !token, &plan);
   if (rc == BSG_OK) rc = check_workspace(workspace, workspace_bytes);
   if (rc != BSG_OK || args->rows == 0) return rc;
   if ((rc = bsg::host_device(BSG_ERR_ARCH_MISMATCH, BSG_ERR_CUDA, &dev, &sms)) != BSG_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
+  if (token) return token_product(*args, s, sms, dev);
   if ((rc = quantise(*args, s)) != BSG_OK) return rc;
   return product(*args, plan, workspace, s, sms, dev, true);
 }

@@ -4,12 +4,13 @@
 //   D[m,n] = act(sa[m] * sb[n] * sum_k q[m,k] w[n,k] + bias[n])
 //
 // The sum is a 32-bit integer and exact (K <= 131071: 127 * 127 * K < 2^31), so neither the order of the additions nor
-// a split of K changes a result.  Three kernels:
+// a split of K changes a result.  The kernels:
 //
 //   bsg_i8_quant_kernel   tokens -> 8 bits; bound by HBM
 //   bsg_i8_rows_kernel    many rows: tokens are the M side of the MMA; bound by the tensor pipe
-//   bsg_i8_few_kernel     few rows (one token to a few hundred): the output channels are the M side of the MMA and the
-//                         tokens its N side, so that the tile carries no padding rows; bound by reading the weights
+//   bsg_i8_few_kernel     few rows: the output channels are the M side of the MMA and the tokens its N side, so that the
+//                         tile carries no padding rows; bound by reading the weights
+//   bsg_i8_token_kernel   up to four tokens, quantised on the way; bound by reading the weights
 //
 // The two products are dense (one group of rows) or grouped (ragged rows per group, end rows on the device).
 #pragma once
@@ -597,24 +598,30 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   }
 }
 
-// ---- few rows: D^T tile = 128 channels x BT tokens.  The CTAs of a cluster (`split` of them) take consecutive parts of K of
-// one tile; each sends the columns that another one finishes into that CTA's shared memory, and each finishes BT / split.
-template <int BT>
+// ---- few rows: D^T tile = 128 channels x BT tokens.  The CTAs of a cluster (SPLIT of them) take consecutive parts of K of
+// one tile; each sends the columns that another one finishes into that CTA's shared memory, and each finishes BT / SPLIT.
+template <int BT, int SPLIT>
 struct I8FewCfg {
+  static_assert(SPLIT == 1 || BT <= 64, "wide tiles do not split");
   static constexpr int kWBytes = 128 * 128;
   static constexpr int kTBytes = BT * 128;
   static constexpr int kStageBytes = kWBytes + kTBytes;
-  static constexpr int kRedBytes = BT <= 64 ? BT * 512 : 0;           // [split][BT / split][128] int32; wider tiles do not split
-  static constexpr int kStagesRaw = (115712 - 1024 - kI8CtlBytes - kRedBytes) / kStageBytes;     // two CTAs per SM
+  static constexpr int kRedBytes = SPLIT > 1 ? BT * 512 : 0;          // [SPLIT][BT / SPLIT][128] int32
+  static constexpr int kSaBytes = 2 * BT * 4;                         // token scales of two tiles
+  static constexpr int kStagesRaw = (115712 - 1024 - kI8CtlBytes - kRedBytes - kSaBytes) / kStageBytes;     // two CTAs per SM
   static constexpr int kStages = kStagesRaw > 6 ? 6 : kStagesRaw;
-  static constexpr int kSmemBytes = kStages * kStageBytes + kRedBytes + kI8CtlBytes + 1024;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kRedBytes + kSaBytes + kI8CtlBytes + 1024;
   static constexpr int kTmemCols = 2 * BT;
   static_assert(kStages >= 3, "stages");
 };
 
-// Column of N values (tokens) of one channel; consecutive lanes hold consecutive channels.
+// Columns (tokens) of one channel, finished and stored; consecutive lanes hold consecutive channels.
 template <int N>
-__device__ __forceinline__ void i8_put(const I8GemmParams& p, const float (&x)[N], int n_here, int64_t at) {
+__device__ __forceinline__ void i8_put(const I8GemmParams& p, const uint32_t (&v)[N], const float* sa, int n_here, float sb, float bias, int64_t at) {
+  float x[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) x[j] = i8_finish(v[j], sa[j], sb, bias);
+  i8_activate(x, p.activation);
   if (p.out_kind == kOutBf16) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -633,59 +640,72 @@ __device__ __forceinline__ void i8_put(const I8GemmParams& p, const float (&x)[N
   }
 }
 
-template <int BT>
+template <int BT, int SPLIT>
 __global__ void __launch_bounds__(192, 2)
-bsg_i8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const I8GemmParams p, const int32_t split) {
-  using C = I8FewCfg<BT>;
+bsg_i8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const I8GemmParams p) {
+  using C = I8FewCfg<BT, SPLIT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sW = smem;
   uint8_t* sT = sW + C::kStages * C::kWBytes;
   uint8_t* sRed = sT + C::kStages * C::kTBytes;
-  I8Ctl* ctl = reinterpret_cast<I8Ctl*>(sRed + C::kRedBytes);
+  float* sSa = reinterpret_cast<float*>(sRed + C::kRedBytes);
+  I8Ctl* ctl = reinterpret_cast<I8Ctl*>(sRed + C::kRedBytes + C::kSaBytes);
 
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
-  const int32_t rank = split > 1 ? int32_t(ptx::cluster_ctarank()) : 0;
-  const int32_t worker = int32_t(blockIdx.x) / split, workers = int32_t(gridDim.x) / split;
+  const int32_t rank = SPLIT > 1 ? int32_t(ptx::cluster_ctarank()) : 0;
+  const int32_t worker = int32_t(blockIdx.x) / SPLIT, workers = int32_t(gridDim.x) / SPLIT;
+  const int32_t k_all = (p.K + 127) / 128;
+  const int32_t kt0 = k_all * rank / SPLIT, kt1 = k_all * (rank + 1) / SPLIT;
+  const int32_t early_tiles = min(kt1 - kt0, C::kStages);
+  const bool dense = p.offsets == nullptr;
 
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < C::kStages; ++s) {
-      ptx::mbar_init(ptx::smem_u32(&ctl->full[s]), 1);
-      ptx::mbar_init(ptx::smem_u32(&ctl->empty[s]), 1);
+  // The weights do not depend on the quantiser in front of this kernel: those of the first stages are asked for before
+  // anything else (dense: the first tile is known without the group table), and before its results are waited for.
+  auto fetch_early = [&](int32_t tn, int32_t g) {
+    const uint32_t full0 = ptx::smem_u32(&ctl->full[0]), sW0 = ptx::smem_u32(sW);
+    for (int32_t i = 0; i < early_tiles; ++i) {
+      ptx::mbar_arrive_expect_tx(full0 + i * 8, C::kStageBytes);
+      ptx::tma_load_3d<1>(sW0 + i * C::kWBytes, &tmW, full0 + i * 8, (kt0 + i) * 128, tn * 128, g);
     }
-    for (int s = 0; s < 2; ++s) {
-      ptx::mbar_init(ptx::smem_u32(&ctl->tmem_full[s]), 1);
-      ptx::mbar_init(ptx::smem_u32(&ctl->tmem_empty[s]), 4);
+  };
+  const int32_t dense_tiles_m = (p.total_rows + BT - 1) / BT;
+  if (warp == 5) {
+    if (ptx::elect_one_sync()) {
+      for (int s = 0; s < C::kStages; ++s) {
+        ptx::mbar_init(ptx::smem_u32(&ctl->full[s]), 1);
+        ptx::mbar_init(ptx::smem_u32(&ctl->empty[s]), 1);
+      }
+      for (int s = 0; s < 2; ++s) {
+        ptx::mbar_init(ptx::smem_u32(&ctl->tmem_full[s]), 1);
+        ptx::mbar_init(ptx::smem_u32(&ctl->tmem_empty[s]), 4);
+      }
+      ctl->abort = 0;
+      ptx::fence_mbar_init();
+      ptx::fence_proxy_async();
+      if (dense) fetch_early(worker / dense_tiles_m, 0);       // one band: the token tiles of a channel tile follow one another
+      ptx::prefetch_tmap(&tmX);
     }
-    ctl->abort = 0;
-    ptx::fence_mbar_init();
-    ptx::fence_proxy_async();
-  }
-  if (warp == 5 && lane == 0) {
-    ptx::prefetch_tmap(&tmW);
-    ptx::prefetch_tmap(&tmX);
-  }
-  if (warp == 4) {
+    __syncwarp();
+  } else if (warp == 4) {
     ptx::tmem_alloc<1>(ptx::smem_u32(&ctl->tmem_base), C::kTmemCols);
     ptx::tmem_relinquish<1>();
+  } else if (warp == 0) {
+    // needs the end rows only, which are older than the quantiser this kernel may overlap with
+    i8_build_groups(ctl, p, BT);
   }
-  // The group table needs the end rows only, which are older than the quantiser this kernel may overlap with.
-  if (warp == 0) i8_build_groups(ctl, p, BT);
   __syncwarp();
   ptx::tc_fence_before();
-  if (split > 1) { ptx::cluster_arrive(); ptx::cluster_wait(); } else { __syncthreads(); }
+  if constexpr (SPLIT > 1) { ptx::cluster_arrive(); ptx::cluster_wait(); } else { __syncthreads(); }
   ptx::tc_fence_after();
 
   const uint32_t tmem_base = bcast(ctl->tmem_base);
   const int32_t total_tiles = bcast(ctl->total_tiles);
-  const int32_t k_all = (p.K + 127) / 128;
-  const int32_t kt0 = int32_t(int64_t(k_all) * rank / split), kt1 = int32_t(int64_t(k_all) * (rank + 1) / split);
   uint32_t dead = 0;
 
   if (warp == 5) {
     // ---------------------------------------------------------------- TMA producer
-    // The weights do not depend on the quantiser in front: the first stages' weights are asked for before waiting for it.
     const uint32_t elected = ptx::elect_one_sync();
     const uint32_t sW0 = ptx::smem_u32(sW), sT0 = ptx::smem_u32(sT);
     const uint32_t full0 = ptx::smem_u32(&ctl->full[0]), empty0 = ptx::smem_u32(&ctl->empty[0]);
@@ -693,14 +713,10 @@ bsg_i8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     uint32_t phase = 0;
     int32_t early = 0;
     if (worker < total_tiles) {
-      const I8Tile ti = i8_decode(ctl, p, worker, BT);
-      early = bcast(min(kt1 - kt0, C::kStages));
-      const int32_t w_row = bcast(ti.tn * 128), g = bcast(ti.g);
-      if (elected) {
-        for (int32_t i = 0; i < early; ++i) {
-          ptx::mbar_arrive_expect_tx(full0 + i * 8, C::kStageBytes);
-          ptx::tma_load_3d<1>(sW0 + i * C::kWBytes, &tmW, full0 + i * 8, (kt0 + i) * 128, w_row, g);
-        }
+      early = early_tiles;
+      if (!dense) {
+        const I8Tile ti = i8_decode(ctl, p, worker, BT);
+        if (elected) fetch_early(ti.tn, ti.g);
       }
     }
     ptx::grid_dependency_wait();
@@ -760,8 +776,9 @@ bsg_i8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     if (dead) atomicOr(p.status, kStTimeoutFull | kStTimeoutTmemEmpty);
   } else {
     // ---------------------------------------------------------------- epilogue: a lane is an output channel
+    constexpr int kPer = BT / SPLIT;             // columns that this CTA finishes
+    constexpr int kChunk = BT < 32 ? BT : 32;
     const uint32_t tfull0 = ptx::smem_u32(&ctl->tmem_full[0]), tempty0 = ptx::smem_u32(&ctl->tmem_empty[0]);
-    const int act = p.activation;
     const bool has_bias = p.bias != nullptr;
     ptx::grid_dependency_wait();          // the token scales come from the quantiser, and D may still be read by what ran before
     int32_t it = 0;
@@ -773,36 +790,33 @@ bsg_i8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
       const int64_t at = int64_t(ti.g) * p.N + n;
       const float sb = n_ok ? __ldg(p.sb + at) : 0.0f;
       const float bias = n_ok && has_bias ? __ldg(p.bias + at) : 0.0f;
+      const int32_t cols = min(BT, ti.row_end - ti.row0);
+      float* sa = sSa + acc * BT;
+      if (threadIdx.x < BT) sa[threadIdx.x] = int32_t(threadIdx.x) < cols ? __ldcg(p.sa + ti.row0 + threadIdx.x) : 0.0f;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
       i8_wait(tfull0 + acc * 8, uint32_t(it >> 1) & 1u, ctl, dead);
       __syncwarp();
       ptx::tc_fence_after();
       const uint32_t lane_addr = tmem_base + (uint32_t(warp * 32) << 16) + uint32_t(acc) * BT;
-      const int32_t cols = min(BT, ti.row_end - ti.row0);
 #pragma unroll 1
-      for (int c0 = 0; c0 < BT; c0 += 16) {
-        uint32_t v[16];
-        i8_tmem_ld_x16(lane_addr + c0, v);
+      for (int c0 = 0; c0 < BT; c0 += kChunk) {
+        uint32_t v[kChunk];
+        if constexpr (kChunk == 32) ptx::tmem_ld_32x32b_x32(lane_addr + c0, v);
+        else i8_tmem_ld_x16(lane_addr + c0, v);
         ptx::tmem_ld_wait();
-        if (c0 + 16 == BT) {
+        if (c0 + kChunk == BT) {
           ptx::tc_fence_before();
           __syncwarp();
           if (lane == 0) ptx::mbar_arrive_relaxed(tempty0 + acc * 8);
         }
-        if (split == 1) {
-          if (n_ok && c0 < cols) {
-            float x[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = i8_finish(v[j], c0 + j < cols ? __ldcg(p.sa + ti.row0 + c0 + j) : 0.0f, sb, bias);
-            i8_activate(x, act);
-            i8_put(p, x, min(16, cols - c0), int64_t(ti.row0 + c0) * p.ldd + n);
-          }
+        if constexpr (SPLIT == 1) {
+          if (n_ok && c0 < cols) i8_put(p, v, sa + c0, min(kChunk, cols - c0), sb, bias, int64_t(ti.row0 + c0) * p.ldd + n);
         } else {
-          const int per = BT / split;
+          const uint32_t mine = ptx::smem_u32(sRed) + uint32_t((rank * kPer * 128 + warp * 32 + lane) * 4);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int c = c0 + j, owner = c / per;
-            if (c < cols)
-              ptx::st_shared_cluster_u32(ptx::mapa(ptx::smem_u32(sRed) + uint32_t(((rank * per + c - owner * per) * 128 + warp * 32 + lane) * 4), uint32_t(owner)), v[j]);
+          for (int j = 0; j < kChunk; ++j) {
+            const int c = c0 + j;
+            if (c < cols) ptx::st_shared_cluster_u32(ptx::mapa(mine + uint32_t((c % kPer) * 512), uint32_t(c / kPer)), v[j]);
           }
         }
       }
@@ -810,34 +824,30 @@ bsg_i8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
     if (dead) atomicOr(p.status, kStTimeoutTmemFull);
   }
 
-  if (split > 1) {
+  if constexpr (SPLIT > 1) {
     // One tile per cluster: every part of it has been sent once all CTAs are here.
     __syncwarp();
     ptx::cluster_arrive();
     ptx::cluster_wait();
-    if (warp < 4 && worker < total_tiles) {
+    if (warp < 4) {
+      constexpr int kPer = BT / SPLIT, kStep = kPer < 8 ? kPer : 8;
       const I8Tile ti = i8_decode(ctl, p, worker, BT);
       const int32_t n = ti.tn * 128 + warp * 32 + lane;
-      const int per = BT / split;
+      const int32_t left = ti.row_end - (ti.row0 + rank * kPer);
       if (n < p.N) {
-        const int64_t at = int64_t(ti.g) * p.N + n;
-        const bool has_bias = p.bias != nullptr;
-        const float sb = __ldg(p.sb + at), bias = has_bias ? __ldg(p.bias + at) : 0.0f;
+        const float sb = __ldg(p.sb + n), bias = p.bias ? __ldg(p.bias + n) : 0.0f;
         const int32_t* red = reinterpret_cast<const int32_t*>(sRed) + warp * 32 + lane;
-        const int32_t left = ti.row_end - (ti.row0 + rank * per);
-        for (int c0 = 0; c0 < per && c0 < left; c0 += 4) {
-          const int n_here = min(4, min(per, left) - c0);
-          float x[4];
+#pragma unroll 1
+        for (int c0 = 0; c0 < kPer && c0 < left; c0 += kStep) {
+          uint32_t v[kStep];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < kStep; ++j) {      // columns behind the last token hold nothing and are not stored
             int32_t sum = 0;
-            if (j < n_here) {
-              for (int s = 0; s < split; ++s) sum += red[(s * per + c0 + j) * 128];
-            }
-            x[j] = i8_finish(uint32_t(sum), j < n_here ? __ldcg(p.sa + ti.row0 + rank * per + c0 + j) : 0.0f, sb, bias);
+#pragma unroll
+            for (int s = 0; s < SPLIT; ++s) sum += red[(s * kPer + c0 + j) * 128];
+            v[j] = uint32_t(sum);
           }
-          i8_activate(x, p.activation);
-          i8_put(p, x, n_here, int64_t(ti.row0 + rank * per + c0) * p.ldd + n);
+          i8_put(p, v, sSa + rank * kPer + c0, min(kStep, left - c0), sb, bias, int64_t(ti.row0 + rank * kPer + c0) * p.ldd + n);
         }
       }
     }
@@ -852,6 +862,165 @@ bsg_i8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
   if (warp == 4) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc<1>(tmem_base, C::kTmemCols);
+  }
+}
+
+// ---- up to four tokens, quantised in the kernel itself: one launch, no tensor memory, no tensor maps.
+// Every CTA quantises the tokens into its shared memory (they are few and come from L2) while its first weights are already on
+// their way.  A warp owns two channels, or, where there are few channels, `parts` warps share two and take every parts-th
+// piece of K; lanes stride over K with 16-byte loads and __dp4a, and one integer warp reduction per sum ends it.
+constexpr int kI8TokenThreads = 256;
+constexpr int kI8TokenMost = 4;
+constexpr int kI8TokenShared = 65536;         // bytes of tokens in shared memory, at most
+struct I8TokenParams {
+  const uint16_t* X;
+  const int8_t* W;
+  const float* sb;
+  const float* bias;
+  void* D;
+  int64_t ldx, ldw, ldd;
+  int32_t M, N, K, wide;
+  int32_t out_kind, activation;
+  int32_t parts;            // 1, 2, 4 or 8
+};
+
+// Sixteen weights of a row, zeros past its end (nothing past K is read).
+__device__ __forceinline__ uint4 i8_weights16(const int8_t* row, int32_t k, int32_t K) {
+  if (k + 16 <= K) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(row + k));
+    return v;
+  }
+  uint32_t w[4] = {0, 0, 0, 0};
+  for (int j = 0; j < 16 && k + j < K; ++j) w[j >> 2] |= uint32_t(uint8_t(row[k + j])) << (8 * (j & 3));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int MT, bool FP16>
+__global__ void __launch_bounds__(kI8TokenThreads, 2) bsg_i8_token_kernel(const I8TokenParams p) {
+  constexpr int kWarps = kI8TokenThreads / 32, kChan = 2, kUnroll = 4;
+  constexpr int kPerToken = kI8TokenThreads / MT;            // threads that quantise one token: whole warps
+  extern __shared__ __align__(16) uint8_t s_tok[];           // [MT][K rounded up to 16]
+  __shared__ float s_max[kWarps], s_scale[MT];
+  __shared__ int32_t s_part[2][kWarps][kChan * MT];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int32_t pitch = (p.K + 15) & ~15;
+  const int32_t k_first = (warp % p.parts) * 512 + lane * 16, k_step = p.parts * 512;
+  const int32_t batches = (pitch + kUnroll * k_step - 1) / (kUnroll * k_step);       // per group, the same for every warp
+  const int32_t per_group = kChan * (kWarps / p.parts);                               // channels of a CTA's group
+  const int32_t groups = (p.N + per_group - 1) / per_group;
+  const int32_t n_warp = (warp / p.parts) * kChan;
+
+  uint4 w[kUnroll][kChan], ahead[kUnroll][kChan];
+  auto fetch = [&](uint4 (&to)[kUnroll][kChan], int32_t grp, int32_t batch) {
+    const int32_t n0 = grp * per_group + n_warp, k0 = k_first + batch * kUnroll * k_step;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+      for (int c = 0; c < kChan; ++c) {
+        const int32_t k = k0 + u * k_step;
+        to[u][c] = n0 + c < p.N && k < p.K ? i8_weights16(p.W + int64_t(n0 + c) * p.ldw, k, p.K) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+  fetch(w, blockIdx.x, 0);      // the weights are read-only for this kernel's whole life
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+
+  {
+    const int m = threadIdx.x / kPerToken, t = threadIdx.x % kPerToken;
+    const uint16_t* row = p.X + int64_t(m < p.M ? m : 0) * p.ldx;
+    const bool wide = p.wide != 0;
+    uint32_t mx = 0;
+    for (int32_t k = t * 8; k < p.K; k += kPerToken * 8) {
+      const uint4 u = i8_load8(row, k, p.K, wide);
+      mx = i8_maxabs2<FP16>(mx, i8_maxabs2<FP16>(i8_maxabs2<FP16>(u.x, u.y), i8_maxabs2<FP16>(u.z, u.w)));
+    }
+    mx &= 0x7FFF7FFFu;
+    float amax = ptx::fmax_nan(i8_unpack(mx & 0xFFFFu, FP16), i8_unpack(mx >> 16, FP16));
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) amax = ptx::fmax_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (lane == 0) s_max[warp] = amax;
+    __syncthreads();
+    const int w0 = m * (kPerToken / 32);
+    amax = s_max[w0];
+#pragma unroll
+    for (int i = 1; i < kPerToken / 32; ++i) amax = ptx::fmax_nan(amax, s_max[w0 + i]);
+    const I8Scale s = i8_scale(amax);
+    if (t == 0) s_scale[m] = s.scale;
+    for (int32_t k = t * 8; k < pitch; k += kPerToken * 8)
+      *reinterpret_cast<uint2*>(s_tok + m * pitch + k) = i8_levels8<FP16>(i8_load8(row, k, p.K, wide), s);
+    __syncthreads();
+  }
+
+  int32_t acc[kChan][MT];
+#pragma unroll
+  for (int c = 0; c < kChan; ++c) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[c][m] = 0;
+  }
+  int32_t grp = blockIdx.x, batch = 0, turn = 0;
+  while (grp < groups) {
+    // the next batch, of this group or the CTA's next one, is fetched while this one is multiplied
+    const bool last = batch + 1 == batches;
+    const int32_t next_grp = last ? grp + int32_t(gridDim.x) : grp, next_batch = last ? 0 : batch + 1;
+    if (next_grp < groups) fetch(ahead, next_grp, next_batch);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int32_t k = k_first + (batch * kUnroll + u) * k_step;
+      if (k < pitch) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const int4 x = *reinterpret_cast<const int4*>(s_tok + m * pitch + k);
+#pragma unroll
+          for (int c = 0; c < kChan; ++c) {
+            acc[c][m] = __dp4a(x.x, int(w[u][c].x), acc[c][m]);
+            acc[c][m] = __dp4a(x.y, int(w[u][c].y), acc[c][m]);
+            acc[c][m] = __dp4a(x.z, int(w[u][c].z), acc[c][m]);
+            acc[c][m] = __dp4a(x.w, int(w[u][c].w), acc[c][m]);
+          }
+        }
+      }
+    }
+    if (last) {
+      // lane m of the warp holds token m of the first channel, lane MT + m that of the second
+      int32_t mine = 0;
+#pragma unroll
+      for (int c = 0; c < kChan; ++c) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const int32_t sum = __reduce_add_sync(0xffffffffu, acc[c][m]);
+          if (lane == c * MT + m) mine = sum;
+          acc[c][m] = 0;
+        }
+      }
+      bool finish = lane < kChan * MT;
+      if (p.parts > 1) {
+        if (finish) s_part[turn][warp][lane] = mine;
+        __syncthreads();      // two turns of s_part: a warp is at most one group ahead of another
+        finish = finish && warp % p.parts == 0;
+        if (finish) {
+          for (int i = 1; i < p.parts; ++i) mine += s_part[turn][warp + i][lane];
+        }
+        turn ^= 1;
+      }
+      const int32_t n = grp * per_group + n_warp + lane / MT, m = lane % MT;
+      if (finish && n < p.N && m < p.M) {
+        float x[1] = {i8_finish(uint32_t(mine), s_scale[m], __ldg(p.sb + n), p.bias ? __ldg(p.bias + n) : 0.0f)};
+        i8_activate(x, p.activation);
+        const int64_t at = int64_t(m) * p.ldd + n;
+        if (p.out_kind == kOutBf16) reinterpret_cast<__nv_bfloat16*>(p.D)[at] = __float2bfloat16_rn(x[0]);
+        else if (p.out_kind == kOutF16) reinterpret_cast<__half*>(p.D)[at] = __float2half_rn(x[0]);
+        else reinterpret_cast<float*>(p.D)[at] = x[0];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+      for (int c = 0; c < kChan; ++c) w[u][c] = ahead[u][c];
+    }
+    grp = next_grp;
+    batch = next_batch;
   }
 }
 

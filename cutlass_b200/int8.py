@@ -17,6 +17,7 @@ from .operator import MAX_INT8_K, _default_workspace, _default_workspaces, to_cu
 
 _IN_KINDS = {torch.bfloat16: L.OUT_BF16, torch.float16: L.OUT_F16}
 _OUT_KINDS = {torch.bfloat16: L.OUT_BF16, torch.float16: L.OUT_F16, torch.float32: L.OUT_F32}
+_POWER = (1, 1, 2, 4, 4)       # number of tokens -> the next power of two
 _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
@@ -143,27 +144,32 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r}: one of {sorted(ACTIVATIONS)}")
-    scratch = x.new_empty(R * (pitch + 4), dtype=torch.int8)        # 8-bit tokens, then their scales
+    made = []
     if out is None:
-        out = x.new_empty((R, N), dtype=out_dtype)
-        made, ldd = (scratch, out), N
+        out, ldd = x.new_empty((R, N), dtype=out_dtype), N
+        made.append(out)
         out_kind = _OUT_KINDS.get(out.dtype)
     else:
         out_kind, out_device, out_rows, out_cols, ldd = _matrix("out", out, _OUT_KINDS)
-        made = (scratch,)
         if (out_rows, out_cols, out_device) != (R, N, device) or (out_dtype is not None and out.dtype != out_dtype):
             raise ValueError(f"out must be a {out_dtype or ''} tensor of shape {(R, N)} on CUDA device {device}")
     if out_kind is None:
         raise ValueError(f"out dtype {out.dtype} is not supported (bf16, fp16 or fp32)")
     if R == 0:
         return out
-    q = scratch.data_ptr()
+    if offsets is None and R <= 4 and _POWER[R] * pitch <= 65536:      # quantised inside the product's kernel
+        q = q_scale = 0
+    else:
+        scratch = x.new_empty(R * (pitch + 4), dtype=torch.int8)       # 8-bit tokens, then their scales
+        made.append(scratch)
+        q = scratch.data_ptr()
+        q_scale = q + R * pitch
     status = _default_workspaces.get(device)
     if status is None:
         status = _default_workspace(x.device)
     pack, call = L.direct("bsg_int8_linear_run", L.INT8_LAYOUT)
     args = pack(in_kind, out_kind, experts, act, R, M, N, K, x.data_ptr(), ldx, 0 if rows is None else rows.data_ptr(), q, pitch,
-                q + R * pitch, w, ldw, group_stride, weight_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
+                q_scale, w, ldw, group_stride, weight_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
                 0 if offsets is None else offsets.data_ptr(), out.data_ptr(), ldd, 0, 0, 0, 0)
     _launch(device, stream, made, call, args, status.data_ptr(), 16)
     return out

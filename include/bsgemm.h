@@ -339,7 +339,9 @@ int32_t bsg_int8_query(const bsg_int8_args* args, bsg_caps* caps);
 int32_t bsg_int8_quantize(const bsg_int8_args* args, void* cuda_stream);
 /* Q, q_scale, W, ... -> D.  Workspace and device status as in bsg_gemm_run. */
 int32_t bsg_int8_gemm_run(const bsg_int8_args* args, void* workspace, size_t workspace_bytes, void* cuda_stream);
-/* Both steps; the product's set-up and its first weights overlap the quantiser. */
+/* Both steps; the product's set-up and its first weights overlap the quantiser.  With Q and q_scale NULL the tokens are
+ * quantised inside the product's kernel: dense, without an index, at most 4 rows, which in 8 bits (their number rounded up to
+ * a power of two times K rounded up to 16) take at most 64 KB. */
 int32_t bsg_int8_linear_run(const bsg_int8_args* args, void* workspace, size_t workspace_bytes, void* cuda_stream);
 
 /*

@@ -145,6 +145,20 @@ def test_dense_product(cuda_lib, M, N, K, out_dtype):
     status_ok()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("M,N,K,pitch", [(1, 33, 8192, None), (2, 17, 515, 517), (3, 100, 16384, None), (4, 16, 2064, None), (3, 50, 1000, 1001), (4, 5000, 512, None), (5, 64, 512, None),
+                                         (4, 40, 16384, None), (4, 40, 16385, None), (1, 9, 65536, None), (1, 9, 65537, None)])
+def test_a_few_tokens(cuda_lib, M, N, K, pitch, dtype):
+    """Around the limits of the kernel that quantises on the way; its bits are those of the two-step form."""
+    x = tokens(M, K, dtype, seed=M + N, pitch=pitch)
+    w, ws = weights((N,), K, seed=N)
+    bias = torch.randn(N, device="cuda")
+    got = ops.int8_linear(x, w, ws, bias, activation="silu", out_dtype=F32)
+    check(got, x, w, ws, bias, "silu")
+    one = torch.tensor([M], dtype=torch.int32, device="cuda")
+    assert torch.equal(got, ops.int8_linear(x, w[None], ws[None], bias[None], activation="silu", out_dtype=F32, offsets=one))
+
+
 @pytest.mark.parametrize("M,N,K", [(5, 200, 2000), (40, 1030, 1024), (130, 264, 256), (260, 515, 130)])
 @pytest.mark.parametrize("activation", ["identity", "relu", "gelu", "silu"])
 def test_bias_and_activation(cuda_lib, M, N, K, activation):
