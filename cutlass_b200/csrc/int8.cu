@@ -73,7 +73,7 @@ int32_t choose(const bsg_int8_args& a, I8Plan* plan) {
       if (waves * slots < tiles * split) waves += 1.0;
       double t = waves * double((k_tiles + split - 1) / split) * v.per_k_tile;
       if (t < weights) t = weights;
-      t += v.fixed + 0.1 * split;
+      t += v.fixed + (split > 1 ? 0.8 + 0.02 * v.tile : 0.0);      // the cluster's barrier and the exchange of partial sums
       if (t < best) {
         best = t;
         found = true;
@@ -145,6 +145,24 @@ int32_t quantise(const bsg_int8_args& a, cudaStream_t s) {
   p.fp16 = a.in_kind == BSG_OUT_F16;
   p.wide = host_aligned(a.X, 16) && a.ldx % 8 == 0;
   return p.fp16 ? launch_quantise<true>(p, s) : launch_quantise<false>(p, s);
+}
+
+// Where tokens are used by several rows each, and there is enough of them to pay for one more kernel, they are quantised once
+// and copied into order (32768 rows of 4096 tokens x 7168: 60 us instead of 117).
+bool copies_rows(const bsg_int8_args& a) { return a.index && a.rows >= 2 * a.tokens && a.rows * a.K >= (int64_t(1) << 24); }
+
+int32_t copy_rows(const bsg_int8_args& a, const void* q, const float* scale, cudaStream_t s) {
+  bsg::I8CopyParams p;
+  p.Q = static_cast<const int8_t*>(q); p.scale = scale; p.index = a.index; p.out = static_cast<int8_t*>(a.Q); p.out_scale = a.q_scale;
+  p.rows = int32_t(a.rows); p.tokens = int32_t(a.tokens); p.pitch = int32_t(a.ldq);
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(unsigned((a.rows + 7) / 8), 1, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = s;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, bsg::bsg_i8_copy_rows_kernel, p);
+  if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
+  return BSG_OK;
 }
 
 int32_t launch_ex(cudaLaunchConfig_t& cfg, int clusters, bool pdl, cudaLaunchAttribute* attr) {
@@ -346,8 +364,24 @@ int32_t bsg_int8_linear_run(const bsg_int8_args* args, void* workspace, size_t w
   if ((rc = bsg::host_device(BSG_ERR_ARCH_MISMATCH, BSG_ERR_CUDA, &dev, &sms)) != BSG_OK) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   if (token) return token_product(*args, s, sms, dev);
-  if ((rc = quantise(*args, s)) != BSG_OK) return rc;
+  if (copies_rows(*args)) {
+    // the tokens' 8-bit rows and scales lie behind those of the product's rows, with the same pitch
+    bsg_int8_args t = *args;
+    t.index = nullptr;
+    t.rows = args->tokens;
+    t.Q = static_cast<int8_t*>(args->Q) + args->rows * args->ldq;
+    t.q_scale = args->q_scale + args->rows;
+    if ((rc = quantise(t, s)) != BSG_OK || (rc = copy_rows(*args, t.Q, t.q_scale, s)) != BSG_OK) return rc;
+  } else if ((rc = quantise(*args, s)) != BSG_OK) {
+    return rc;
+  }
   return product(*args, plan, workspace, s, sms, dev, true);
+}
+
+int32_t bsg_int8_scratch_rows(const bsg_int8_args* args, int64_t* rows) {
+  if (!args || !rows) return host_fail(BSG_ERR_INVALID_PROBLEM, "args and rows must not be null");
+  *rows = args->rows + (copies_rows(*args) ? args->tokens : 0);
+  return BSG_OK;
 }
 
 }  // extern "C"

@@ -83,9 +83,30 @@ __device__ __forceinline__ uint32_t i8_pack4(int a, int b, int c, int d) {
   return (uint32_t(a) & 0xFFu) | ((uint32_t(b) & 0xFFu) << 8) | ((uint32_t(c) & 0xFFu) << 16) | (uint32_t(d) << 24);
 }
 
-// Eight consecutive values of a row, zeros past its end.
+// 32 bytes that start on a 16-byte boundary -> the 16 of them that start `skip` bytes in (skip even, below 16).
+__device__ __forceinline__ uint4 i8_shift16(const uint4& lo, const uint4& hi, uint32_t skip) {
+  uint32_t w[7] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z}, last = hi.w;
+  const bool two = skip & 8u, one = skip & 4u;
+  uint32_t v[6];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) v[j] = two ? w[j + 2] : w[j];
+  v[5] = two ? last : w[5];
+  uint32_t u[5];
+#pragma unroll
+  for (int j = 0; j < 5; ++j) u[j] = one ? v[j + 1] : v[j];
+  const uint32_t bits = (skip & 2u) * 8u;
+  return make_uint4(__funnelshift_r(u[0], u[1], bits), __funnelshift_r(u[1], u[2], bits), __funnelshift_r(u[2], u[3], bits), __funnelshift_r(u[3], u[4], bits));
+}
+
+// Eight consecutive values of a row, zeros past its end.  Rows that do not start on 16 bytes are read in aligned pairs of
+// 16-byte words where both lie inside the row, value by value at its ends.
 __device__ __forceinline__ uint4 i8_load8(const uint16_t* row, int32_t k, int32_t K, bool wide) {
   if (wide && k + 8 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  if (!wide && k > 0 && k + 16 <= K) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(row + k);
+    const uint4* at = reinterpret_cast<const uint4*>(a & ~uintptr_t(15));
+    return i8_shift16(__ldg(at), __ldg(at + 1), uint32_t(a) & 15u);
+  }
   uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -173,6 +194,42 @@ __global__ void __launch_bounds__(TPR > kI8QuantThreads ? TPR : kI8QuantThreads)
     if (k < p.K) store(k, v[c]);
   }
   for (int32_t k = (kI8Chunks * TPR + t) * 8; k < p.K; k += TPR * 8) store(k, i8_load8(row, k, K, wide));
+}
+
+// Rows of quantised tokens, and their scales, copied into the order of an index: one warp per row, so that a token that
+// several rows use is quantised once.  Entries that name no token: zeros with the scale NaN.
+struct I8CopyParams {
+  const int8_t* Q;
+  const float* scale;
+  const int32_t* index;
+  int8_t* out;
+  float* out_scale;
+  int32_t rows, tokens, pitch;      // bytes per row, a multiple of 16
+};
+static __global__ void __launch_bounds__(256) bsg_i8_copy_rows_kernel(const I8CopyParams p) {
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
+  const int32_t r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (r >= p.rows) return;
+  const int32_t at = __ldg(p.index + r);
+  const bool ok = at >= 0 && at < p.tokens;
+  const uint4* src = reinterpret_cast<const uint4*>(p.Q + (ok ? int64_t(at) * p.pitch : 0));
+  uint4* dst = reinterpret_cast<uint4*>(p.out + int64_t(r) * p.pitch);
+  const int32_t n = p.pitch / 16;
+  for (int32_t i0 = 0; i0 < n; i0 += 32 * 8) {
+    uint4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int32_t i = i0 + u * 32 + lane;
+      v[u] = ok && i < n ? __ldcg(src + i) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int32_t i = i0 + u * 32 + lane;
+      if (i < n) dst[i] = v[u];
+    }
+  }
+  if (lane == 0) p.out_scale[r] = ok ? __ldcg(p.scale + at) : __uint_as_float(0x7FC00000u);
 }
 
 // ------------------------------------------------------------------------------------------------ products

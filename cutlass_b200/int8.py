@@ -9,6 +9,8 @@ experts.  Operands that are already quantised go through ``GemmArguments`` / ``G
 """
 from __future__ import annotations
 
+import ctypes as C
+
 import torch
 
 from . import lib as L
@@ -160,10 +162,15 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
     if offsets is None and R <= 4 and _POWER[R] * pitch <= 65536:      # quantised inside the product's kernel
         q = q_scale = 0
     else:
-        scratch = x.new_empty(R * (pitch + 4), dtype=torch.int8)       # 8-bit tokens, then their scales
+        held = R
+        if rows is not None:      # tokens that several rows use may be held twice: as they come, and in the order of the rows
+            count = C.c_int64()
+            L.check(L.load().bsg_int8_scratch_rows(C.byref(L.Int8Args(rows=R, tokens=M, K=K, index=rows.data_ptr())), C.byref(count)))
+            held = count.value
+        scratch = x.new_empty(held * (pitch + 4), dtype=torch.int8)       # 8-bit tokens, then their scales
         made.append(scratch)
         q = scratch.data_ptr()
-        q_scale = q + R * pitch
+        q_scale = q + held * pitch
     status = _default_workspaces.get(device)
     if status is None:
         status = _default_workspace(x.device)

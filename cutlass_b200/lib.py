@@ -161,6 +161,7 @@ SYMBOLS = {
     "bsg_ptr_array_run": (C.c_int32, [C.POINTER(PtrArrayArgs), C.c_void_p, C.c_size_t, C.c_void_p]),
     "bsg_quantize": (C.c_int32, [C.POINTER(QuantArgs), C.c_void_p]),
     "bsg_int8_query": (C.c_int32, [C.POINTER(Int8Args), C.POINTER(Caps)]),
+    "bsg_int8_scratch_rows": (C.c_int32, [C.POINTER(Int8Args), C.POINTER(C.c_int64)]),
     "bsg_int8_quantize": (C.c_int32, [C.POINTER(Int8Args), C.c_void_p]),
     "bsg_int8_gemm_run": (C.c_int32, [C.POINTER(Int8Args), C.c_void_p, C.c_size_t, C.c_void_p]),
     "bsg_int8_linear_run": (C.c_int32, [C.POINTER(Int8Args), C.c_void_p, C.c_size_t, C.c_void_p]),

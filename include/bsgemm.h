@@ -335,6 +335,9 @@ typedef struct bsg_int8_args {
 } bsg_int8_args;
 
 int32_t bsg_int8_query(const bsg_int8_args* args, bsg_caps* caps);
+/* Rows that Q and q_scale must have for bsg_int8_linear_run: `rows`, and `tokens` more where the tokens are quantised before
+ * they are copied into the order of the index (depends on rows, tokens, K and whether there is an index). */
+int32_t bsg_int8_scratch_rows(const bsg_int8_args* args, int64_t* rows);
 /* X -> Q, q_scale. */
 int32_t bsg_int8_quantize(const bsg_int8_args* args, void* cuda_stream);
 /* Q, q_scale, W, ... -> D.  Workspace and device status as in bsg_gemm_run. */

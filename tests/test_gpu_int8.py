@@ -252,6 +252,68 @@ def test_grouped_product(cuda_lib, sizes, N, K, dtype):
     status_ok()
 
 
+@pytest.mark.parametrize("kernel,tile", [(1, 16), (1, 32), (1, 64), (1, 128), (2, 128), (2, 256), (0, 0)])
+@pytest.mark.parametrize("sizes,N,K", [([3, 0, 130, 257, 1], 264, 400), ([700, 0, 300], 515, 130), ([0, 0], 64, 64)])
+def test_every_kernel_takes_an_index(cuda_lib, kernel, tile, sizes, N, K):
+    """Quantise + product with indexed rows, in each kernel.  Entries that name no token give NaN rows; unused rows are left
+    alone."""
+    import ctypes as C
+    E, T, total = len(sizes), 41, sum(sizes)
+    x = tokens(T, K, BF16, seed=1)
+    w, ws = weights((E, N), K, seed=2)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    rows = torch.randint(0, T, (total + 9,), device="cuda", generator=g, dtype=torch.int32)
+    if total:
+        rows[2], rows[total - 1] = T, -1
+    offsets = torch.tensor(sizes, device="cuda").cumsum(0).to(torch.int32)
+    out = torch.full((total + 9, N), 3.0, dtype=torch.float32, device="cuda")
+    pitch = -(-K // 16) * 16
+    a = L.Int8Args(L.OUT_BF16, L.OUT_F32, E, 0, total + 9, T, N, K, x.data_ptr(), x.stride(0), rows.data_ptr(), None, pitch, None, w.data_ptr(),
+                   w.stride(1), w.stride(0), ws.data_ptr(), None, offsets.data_ptr(), out.data_ptr(), N, kernel, tile)
+    held = C.c_int64()
+    L.check(L.load().bsg_int8_scratch_rows(C.byref(a), C.byref(held)))
+    assert held.value == total + 9
+    q, s = torch.empty((held.value, pitch), dtype=torch.int8, device="cuda"), torch.empty(held.value, device="cuda")
+    a.Q, a.q_scale = q.data_ptr(), s.data_ptr()
+    workspace = torch.zeros(16, dtype=torch.uint8, device="cuda")
+    L.check(L.load().bsg_int8_linear_run(C.byref(a), workspace.data_ptr(), 16, torch.cuda.current_stream().cuda_stream))
+    L.check(L.load().bsg_read_device_status(workspace.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    assert bool((out[total:] == 3).all())
+    if not total:
+        return
+    for bad in (2, total - 1):
+        assert bool(torch.isnan(out[bad]).all())
+    out[2] = out[total - 1] = 0
+    begin = 0
+    for e, n in enumerate(sizes):
+        part = [i for i in range(begin, begin + n) if i not in (2, total - 1)]
+        if part:
+            check(out[part], x[rows[part].long()], w[e], ws[e])
+        begin += n
+
+
+def test_tokens_that_many_rows_use(cuda_lib):
+    """Enough rows per token that they are quantised once and copied; the result is that of rows given one by one."""
+    E, T, N, K, per = 5, 600, 72, 3001, 11
+    x = tokens(T, K, F16, seed=1)
+    w, ws = weights((E, N), K, seed=2)
+    ws = ws * 0.01
+    total = T * per
+    rows = torch.randperm(total, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)).to(torch.int32) % T
+    rows[7], rows[total - 3] = -5, T
+    offsets = torch.tensor([1000, 1000, 4000, 6100, total - 20], dtype=torch.int32, device="cuda")
+    buf = torch.full((total, N), 3.0, dtype=F16, device="cuda")
+    out = ops.int8_linear(x, w, ws, offsets=offsets, rows=rows, out=buf)
+    safe = rows.long().clamp(0, T - 1)
+    want = ops.int8_linear(x[safe], w, ws, offsets=offsets)
+    used = torch.arange(total, device="cuda") < total - 20
+    assert bool(torch.isnan(out[7]).all()) and bool((out[~used] == 3).all())
+    used[7] = False
+    assert torch.equal(out[used], want[used])
+    check(out[6100:6400], x[safe[6100:6400]], w[4], ws[4])
+    status_ok()
+
+
 def test_grouped_without_an_index_and_through_the_operator(cuda_lib):
     sizes, N, K = [5, 0, 130, 9], 264, 144
     x = tokens(sum(sizes), K, BF16, seed=2)
