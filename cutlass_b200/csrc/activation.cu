@@ -30,16 +30,20 @@ int32_t check(const bsg_act_args* a, bool forward) {
   return BSG_OK;
 }
 
-template <int ACT, bool GATED, bool FP16>
+template <int ACT, bool GATED, bool FP16, bool WIDE>
 void launch(const bsg::ActParams& p, bool forward, cudaStream_t s) {
   const unsigned grid = (p.items + bsg::kActThreads / 16 - 1) / (bsg::kActThreads / 16);
-  if (forward) bsg::bsg_act_forward_kernel<ACT, GATED, FP16><<<grid, bsg::kActThreads, 0, s>>>(p);
-  else bsg::bsg_act_backward_kernel<ACT, GATED, FP16><<<grid, bsg::kActThreads, 0, s>>>(p);
+  if (forward) bsg::bsg_act_forward_kernel<ACT, GATED, FP16, WIDE><<<grid, bsg::kActThreads, 0, s>>>(p);
+  else bsg::bsg_act_backward_kernel<ACT, GATED, FP16, WIDE><<<grid, bsg::kActThreads, 0, s>>>(p);
+}
+template <int ACT, bool GATED, bool FP16>
+void pick_wide(const bsg::ActParams& p, bool wide, bool forward, cudaStream_t s) {
+  wide ? launch<ACT, GATED, FP16, true>(p, forward, s) : launch<ACT, GATED, FP16, false>(p, forward, s);
 }
 template <int ACT>
-void pick(const bsg::ActParams& p, bool gated, bool fp16, bool forward, cudaStream_t s) {
-  if (gated) fp16 ? launch<ACT, true, true>(p, forward, s) : launch<ACT, true, false>(p, forward, s);
-  else fp16 ? launch<ACT, false, true>(p, forward, s) : launch<ACT, false, false>(p, forward, s);
+void pick(const bsg::ActParams& p, bool gated, bool fp16, bool wide, bool forward, cudaStream_t s) {
+  if (gated) fp16 ? pick_wide<ACT, true, true>(p, wide, forward, s) : pick_wide<ACT, true, false>(p, wide, forward, s);
+  else fp16 ? pick_wide<ACT, false, true>(p, wide, forward, s) : pick_wide<ACT, false, false>(p, wide, forward, s);
 }
 
 int32_t run(const bsg_act_args* a, bool forward, void* stream) {
@@ -53,21 +57,19 @@ int32_t run(const bsg_act_args* a, bool forward, void* stream) {
   p.blocks = int32_t((a->width + bsg::kActBlock - 1) / bsg::kActBlock);
   p.pitch = int32_t((a->width + 15) / 16 * 16);
   p.items = uint32_t(a->rows * p.blocks);
-  p.Q = static_cast<int8_t*>(a->kept); p.scale = a->kept_scale; p.act = a->activation;
+  p.Q = static_cast<int8_t*>(a->kept); p.scale = a->kept_scale;
   p.Y = static_cast<uint16_t*>(a->out); p.ldy = a->ld_out;
   if (forward) { p.X = static_cast<const uint16_t*>(a->in); p.ldx = a->ld_in; }
   else { p.G = static_cast<const uint16_t*>(a->in); p.ldg = a->ld_in; }
-  // the second half of a gated row starts at column `width`
-  const bool half_ok = !a->gated || a->width % 8 == 0;
-  p.wide_in = host_aligned(a->in, 16) && a->ld_in % 8 == 0 && (!forward || half_ok);
-  p.wide_out = host_aligned(a->out, 16) && a->ld_out % 8 == 0 && (forward || half_ok);
+  // every group of 8 values of the input and of the output starts on a 16-byte boundary
+  const bool wide = a->width % 8 == 0 && host_aligned(a->in, 16) && a->ld_in % 8 == 0 && host_aligned(a->out, 16) && a->ld_out % 8 == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool fp16 = a->type == BSG_OUT_F16;
   switch (a->activation) {
-    case BSG_ACT_RELU: pick<bsg::kActRelu>(p, a->gated, fp16, forward, s); break;
-    case BSG_ACT_GELU: pick<bsg::kActGelu>(p, a->gated, fp16, forward, s); break;
-    case BSG_ACT_SILU: pick<bsg::kActSilu>(p, a->gated, fp16, forward, s); break;
-    default: pick<bsg::kActIdentity>(p, a->gated, fp16, forward, s); break;
+    case BSG_ACT_RELU: pick<bsg::kActRelu>(p, a->gated, fp16, wide, forward, s); break;
+    case BSG_ACT_GELU: pick<bsg::kActGelu>(p, a->gated, fp16, wide, forward, s); break;
+    case BSG_ACT_SILU: pick<bsg::kActSilu>(p, a->gated, fp16, wide, forward, s); break;
+    default: pick<bsg::kActIdentity>(p, a->gated, fp16, wide, forward, s); break;
   }
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "activation launch: %s", cudaGetErrorString(e));

@@ -51,37 +51,34 @@ __device__ __forceinline__ uint32_t i8_maxabs2(uint32_t a, uint32_t b) {
   return d;
 }
 
-// Level of one value.  `inv` is 127 / amax, enlarged by 2^-21: the distance of 127 |x| / amax from the next half
-// k + 1/2 is 0 or, for 16-bit x and amax, at least 2^-19 of its size (254 |x| - (2k + 1) amax is a multiple of the
-// smaller operand's last place), so the enlarged product, whose own roundings amount to 2^-23, lies above every half
-// that the exact ratio reaches and below every half that it does not: rounding to nearest gives
-// floor(127 |x| / amax + 1/2) without a division per value.
-__device__ __forceinline__ int i8_level(float x, float pre, float inv) { return __float2int_rn(__fmul_rn(__fmul_rn(x, pre), inv)); }
-
+// Levels.  `inv` is 127 / amax, enlarged by 2^-21: the distance of 127 |x| / amax from the next half k + 1/2 is 0 or, for 16-bit
+// x and amax, at least 2^-19 of its size (254 |x| - (2k + 1) amax is a multiple of the smaller operand's last place), so the
+// enlarged ratio, in which `inv` is off by at most 2^-22, lies above every half that the exact ratio reaches and below every
+// half that it does not: rounding to nearest gives floor(127 |x| / amax + 1/2) without a division per value.  The rounding is
+// that of one fused multiply-add with 1.5 * 2^23, whose last byte is then the level in two's complement.
 struct I8Scale {
-  float scale;     // amax / 127; NaN for a row that holds a NaN or an infinity, 0 for a row of zeros
-  float pre, inv;  // levels are rn(x * pre * inv); both 0 where the scale is 0 or NaN
+  float inv;       // 127 / (amax * pre), enlarged; 0 for a row of zeros
+  float pre;       // 2^64 for rows so small that 127 / amax leaves fp32's range, else 1
+  uint32_t keep;   // all ones; 0 for a row that holds a NaN or an infinity, whose levels are 0
 };
+__device__ __forceinline__ float i8_rcp(float x) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));      // off by at most 2^-23 between 2^-64 and 2^128
+  return r;
+}
 __device__ __forceinline__ I8Scale i8_scale(float amax) {
   I8Scale s;
-  s.scale = __fdiv_rn(amax, 127.0f);
-  s.pre = 1.0f;
-  if (!(amax < __uint_as_float(0x7F800000u))) {
-    s.scale = __uint_as_float(0x7FC00000u);
-    s.pre = s.inv = 0.0f;
-  } else if (amax == 0.0f) {
-    s.pre = s.inv = 0.0f;
-  } else {
-    // 127 / amax leaves fp32's range below 2^-121: such rows are scaled by 2^64 first (exact)
-    if (amax < 0x1p-64f) s.pre = 0x1p64f;
-    s.inv = __fmul_rn(__fdiv_rn(127.0f, __fmul_rn(amax, s.pre)), 1.0f + 0x1p-21f);
-  }
+  const bool finite = amax < __uint_as_float(0x7F800000u);
+  s.keep = finite ? 0xFFFFFFFFu : 0u;
+  s.pre = amax < 0x1p-64f ? 0x1p64f : 1.0f;
+  s.inv = amax > 0.0f && finite ? __fmul_rn(i8_rcp(__fmul_rn(amax, s.pre)), 127.0f * (1.0f + 0x1p-21f)) : 0.0f;
   return s;
 }
-
-__device__ __forceinline__ uint32_t i8_pack4(int a, int b, int c, int d) {
-  return (uint32_t(a) & 0xFFu) | ((uint32_t(b) & 0xFFu) << 8) | ((uint32_t(c) & 0xFFu) << 16) | (uint32_t(d) << 24);
+// amax / 127; NaN for a row that holds a NaN or an infinity.
+__device__ __forceinline__ float i8_step(float amax) {
+  return amax < __uint_as_float(0x7F800000u) ? __fdiv_rn(amax, 127.0f) : __uint_as_float(0x7FC00000u);
 }
+__device__ __forceinline__ uint32_t i8_level_bits(float x, float inv) { return __float_as_uint(__fmaf_rn(x, inv, 12582912.0f)); }
 
 // 32 bytes that start on a 16-byte boundary -> the 16 of them that start `skip` bytes in (skip even, below 16).
 __device__ __forceinline__ uint4 i8_shift16(const uint4& lo, const uint4& hi, uint32_t skip) {
@@ -117,17 +114,32 @@ __device__ __forceinline__ uint4 i8_load8(const uint16_t* row, int32_t k, int32_
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Two packed 16-bit values to fp32.
+template <bool FP16>
+__device__ __forceinline__ void i8_unpack2(uint32_t w, float& lo, float& hi) {
+  if constexpr (FP16) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    lo = f.x; hi = f.y;
+  } else {
+    lo = __uint_as_float(w << 16); hi = __uint_as_float(w & 0xFFFF0000u);
+  }
+}
 template <bool FP16>
 __device__ __forceinline__ uint2 i8_levels8(const uint4& v, const I8Scale& s) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  int q[8];
+  float x[8];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    q[2 * j] = i8_level(i8_unpack(w[j] & 0xFFFFu, FP16), s.pre, s.inv);
-    q[2 * j + 1] = i8_level(i8_unpack(w[j] >> 16, FP16), s.pre, s.inv);
+  for (int j = 0; j < 4; ++j) i8_unpack2<FP16>(w[j], x[2 * j], x[2 * j + 1]);
+  if (!FP16 && s.pre != 1.0f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(x[j], s.pre);
   }
-  // A NaN or infinity times 0 is NaN, which converts to 0.
-  return make_uint2(i8_pack4(q[0], q[1], q[2], q[3]), i8_pack4(q[4], q[5], q[6], q[7]));
+  uint32_t q[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) q[j] = i8_level_bits(x[j], s.inv);
+  const uint32_t lo = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+  const uint32_t hi = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+  return make_uint2(lo & s.keep, hi & s.keep);
 }
 
 // TPR threads own a row; a thread holds kI8Chunks groups of 8 values in registers between the maximum and the rounding, so
@@ -175,10 +187,9 @@ __global__ void __launch_bounds__(TPR > kI8QuantThreads ? TPR : kI8QuantThreads)
     for (int w = 1; w < TPR / 32; ++w) amax = ptx::fmax_nan(amax, s_max[w0 + w]);
   }
   if (!row_ok) return;
-  I8Scale s = i8_scale(amax);
+  const I8Scale s = i8_scale(amax);
   // a row whose index names no token: zeros with a NaN scale, so that a product that uses it shows it
-  if (!src_ok) s.scale = __uint_as_float(0x7FC00000u);
-  if (t == 0) p.scale[r] = s.scale;
+  if (t == 0) p.scale[r] = src_ok ? i8_step(amax) : __uint_as_float(0x7FC00000u);
   int8_t* out = p.Q + int64_t(r) * p.ldq;
   auto store = [&](int32_t k, const uint4& u) {
     const uint2 q = i8_levels8<FP16>(u, s);
@@ -1004,7 +1015,7 @@ __global__ void __launch_bounds__(kI8TokenThreads, 2) bsg_i8_token_kernel(const 
 #pragma unroll
     for (int i = 1; i < kPerToken / 32; ++i) amax = ptx::fmax_nan(amax, s_max[w0 + i]);
     const I8Scale s = i8_scale(amax);
-    if (t == 0) s_scale[m] = s.scale;
+    if (t == 0) s_scale[m] = i8_step(amax);
     for (int32_t k = t * 8; k < pitch; k += kPerToken * 8)
       *reinterpret_cast<uint2*>(s_tok + m * pitch + k) = i8_levels8<FP16>(i8_load8(row, k, p.K, wide), s);
     __syncthreads();
