@@ -32,7 +32,8 @@ int32_t check(const bsg_act_args* a, bool forward) {
 
 template <int ACT, bool GATED, bool FP16, bool WIDE>
 void launch(const bsg::ActParams& p, bool forward, cudaStream_t s) {
-  const unsigned grid = (p.items + bsg::kActThreads / 16 - 1) / (bsg::kActThreads / 16);
+  const unsigned per_cta = bsg::kActThreads / (forward ? bsg::kActForwardLanes : bsg::kActBackwardLanes);
+  const unsigned grid = (p.items + per_cta - 1) / per_cta;
   if (forward) bsg::bsg_act_forward_kernel<ACT, GATED, FP16, WIDE><<<grid, bsg::kActThreads, 0, s>>>(p);
   else bsg::bsg_act_backward_kernel<ACT, GATED, FP16, WIDE><<<grid, bsg::kActThreads, 0, s>>>(p);
 }
@@ -57,6 +58,14 @@ int32_t run(const bsg_act_args* a, bool forward, void* stream) {
   p.blocks = int32_t((a->width + bsg::kActBlock - 1) / bsg::kActBlock);
   p.pitch = int32_t((a->width + 15) / 16 * 16);
   p.items = uint32_t(a->rows * p.blocks);
+  // division of items below 2^31 by the number of blocks d: with l = ceil(log2 d), floor(2^(31 + l) / d) + 1 fits 32 bits and
+  // (item * that) >> (31 + l) is exact
+  if (p.blocks > 1) {
+    int l = 0;
+    while ((int64_t(1) << l) < p.blocks) ++l;
+    p.div_mul = uint32_t((uint64_t(1) << (31 + l)) / uint64_t(p.blocks) + 1);
+    p.div_shift = uint32_t(l - 1);
+  }
   p.Q = static_cast<int8_t*>(a->kept); p.scale = a->kept_scale;
   p.Y = static_cast<uint16_t*>(a->out); p.ldy = a->ld_out;
   if (forward) { p.X = static_cast<const uint16_t*>(a->in); p.ldx = a->ld_in; }

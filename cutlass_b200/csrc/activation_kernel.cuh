@@ -4,8 +4,11 @@
 //   kept, per block of 128 columns of a row:     s = max|.| / 127,  q = sign(.) floor(127 |.| / max|.| + 1/2)
 //   backward, with g^ = s q and u^ likewise:     dg = dh u^ act'(g^),  du = dh act(g^)      (or dg = dh act'(g^))
 //
-// Both passes are bound by HBM.  Sixteen lanes own a block: eight consecutive values of g and of u per lane (16-byte loads),
-// so the two maxima travel together as one packed pair through four shuffles, and everything else stays in registers.
+// Both passes are bound by HBM, and nearly by the issue of instructions.  Forward, eight lanes own a block, sixteen values of g
+// and of u per lane in two groups of eight (16-byte loads), so that what a block costs besides its values is spread over many
+// of them (8192 x 14336 gated silu: 147 us, 175 with sixteen lanes); the two maxima travel together as one packed pair through
+// three shuffles, and everything else stays in registers.  Backward there is no such cost, and sixteen lanes with eight values
+// each, whose rows leave 256 bytes at a time, are faster (152 us, 182 with eight lanes).
 // h is computed from x itself, not from what is kept.
 #pragma once
 #include <cuda_bf16.h>
@@ -18,6 +21,7 @@ namespace bsg {
 
 constexpr int kActBlock = 128;        // columns per scale
 constexpr int kActThreads = 256;
+constexpr int kActForwardLanes = 8, kActBackwardLanes = 16;      // threads per block of columns
 
 struct ActParams {
   const uint16_t* X;      // forward: input
@@ -28,6 +32,7 @@ struct ActParams {
   int64_t ldx, ldg, ldy;  // elements
   int32_t F, blocks, pitch;
   uint32_t items;         // rows * blocks
+  uint32_t div_mul, div_shift;      // item / blocks == umulhi(item, div_mul) >> div_shift  (blocks > 1)
 };
 
 template <bool FP16>
@@ -43,25 +48,23 @@ __device__ __forceinline__ uint4 act_pack(const float (&x)[8]) {
   else return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
 
-// Stores the eight values of every lane of a block; executed by whole warps.  Rows that do not start on 16 bytes leave as
-// aligned 16-byte words all the same, each made of a lane's values and its left neighbour's; the two ends of the block go value
-// by value.  `live`: the lane has values (k < K).
+// Stores eight values of a row.  Rows that do not start on 16 bytes leave as aligned 16-byte words all the same, each made of
+// a lane's values and the eight in front of them; the two ends of the block go value by value.
+// `left`: the eight values in front of them, where `has_left`; `last`: no other lane of the block takes this lane's last values.
 template <bool WIDE>
-__device__ __forceinline__ void act_store8(uint16_t* row, int32_t k, int32_t K, const uint4& v, int sub, bool live) {
+__device__ __forceinline__ void act_store8(uint16_t* row, int32_t k, int32_t K, const uint4& v, const uint4& left, bool has_left, bool last, bool live) {
+  if (!live) return;
   if constexpr (WIDE) {
-    if (live) *reinterpret_cast<uint4*>(row + k) = v;       // K is a multiple of 8
+    *reinterpret_cast<uint4*>(row + k) = v;       // K is a multiple of 8
   } else {
-    const uint4 left = make_uint4(__shfl_up_sync(0xffffffffu, v.x, 1, 16), __shfl_up_sync(0xffffffffu, v.y, 1, 16),
-                                  __shfl_up_sync(0xffffffffu, v.z, 1, 16), __shfl_up_sync(0xffffffffu, v.w, 1, 16));
-    if (!live) return;
     const uint32_t skip = uint32_t(reinterpret_cast<uintptr_t>(row + k)) & 15u;      // bytes from the boundary to this lane's values
     const int32_t moved = int32_t(skip >> 1);                                          // values of the left neighbour in this lane's word
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    if (sub > 0 && k + 8 - moved <= K) {
+    if (has_left && k + 8 - moved <= K) {
       *reinterpret_cast<uint4*>(row + k - moved) = skip ? i8_shift16(left, v, 16u - skip) : v;
     } else {
       const uint32_t l[4] = {left.x, left.y, left.z, left.w};
-      if (sub > 0) {
+      if (has_left) {
 #pragma unroll
         for (int j = 1; j < 8; ++j) {
           if (j >= 8 - moved) row[k - 8 + j] = uint16_t(l[j >> 1] >> (16 * (j & 1)));
@@ -72,7 +75,7 @@ __device__ __forceinline__ void act_store8(uint16_t* row, int32_t k, int32_t K, 
         if (j < 8 - moved && k + j < K) row[k + j] = uint16_t(w[j >> 1] >> (16 * (j & 1)));
       }
     }
-    if (sub == 15 || k + 8 >= K) {      // nobody to the right takes this lane's last values
+    if (last || k + 8 >= K) {
 #pragma unroll
       for (int j = 1; j < 8; ++j) {
         if (j >= 8 - moved && k + j < K) row[k + j] = uint16_t(w[j >> 1] >> (16 * (j & 1)));
@@ -83,8 +86,8 @@ __device__ __forceinline__ void act_store8(uint16_t* row, int32_t k, int32_t K, 
 
 // act(x), and its slope.  The results are rounded to 16 bits, so the fast exponential and quotient (errors near 2^-21) do.
 // gelu: erfc(z) = t (a1 + t (a2 + ... a5)) exp(-z^2), t = 1 / (1 + 0.3275911 z), z >= 0 (Abramowitz and Stegun, Handbook of
-// Mathematical Functions, 7.1.26: off by at most 1.5e-7); its exponential is also that of the slope.  CUDA's erfc takes
-// twice as long: 343 us instead of 160 for the forward pass of 8192 x 14336 gated values.
+// Mathematical Functions, 7.1.26: off by at most 1.5e-7); its exponential is also that of the slope.  CUDA's erfc took
+// the forward pass of 8192 x 14336 gated values from 223 to 343 us.
 __device__ __forceinline__ void act_normal(float x, float& cdf, float& gauss) {      // Phi(x), exp(-x^2 / 2)
   gauss = __expf(-0.5f * x * x);
   const float t = i8_rcp(1.0f + 0.23164189f * fabsf(x));      // 0.3275911 / sqrt(2)
@@ -129,46 +132,98 @@ __device__ __forceinline__ uint32_t act_max_of(const uint4& v) {
   return i8_maxabs2<FP16>(m, m >> 16);
 }
 
+// The two groups of a lane: columns 8 sub ... and 64 + 8 sub ... of its block.
+template <bool WIDE>
+__device__ __forceinline__ void act_store16(uint16_t* row, int32_t k, int32_t K, const uint4 (&v)[2], int sub, bool ok) {
+  uint4 left[2] = {v[0], v[1]};
+  if constexpr (!WIDE) {
+    auto up = [](const uint4& a) {
+      return make_uint4(__shfl_up_sync(0xffffffffu, a.x, 1, 8), __shfl_up_sync(0xffffffffu, a.y, 1, 8), __shfl_up_sync(0xffffffffu, a.z, 1, 8), __shfl_up_sync(0xffffffffu, a.w, 1, 8));
+    };
+    // in front of the first lane's second group lies the last lane's first one
+    const uint4 end = make_uint4(__shfl_sync(0xffffffffu, v[0].x, 7, 8), __shfl_sync(0xffffffffu, v[0].y, 7, 8), __shfl_sync(0xffffffffu, v[0].z, 7, 8), __shfl_sync(0xffffffffu, v[0].w, 7, 8));
+    left[0] = up(v[0]);
+    left[1] = up(v[1]);
+    if (sub == 0) left[1] = end;
+  }
+  act_store8<WIDE>(row, k, K, v[0], left[0], sub > 0, false, ok && k < K);
+  act_store8<WIDE>(row, k + 64, K, v[1], left[1], true, sub == 7, ok && k + 64 < K);
+}
+
+template <bool WIDE>
+__device__ __forceinline__ void act_store16lanes(uint16_t* row, int32_t k, int32_t K, const uint4& v, int sub, bool live) {
+  uint4 left = v;
+  if constexpr (!WIDE)
+    left = make_uint4(__shfl_up_sync(0xffffffffu, v.x, 1, 16), __shfl_up_sync(0xffffffffu, v.y, 1, 16), __shfl_up_sync(0xffffffffu, v.z, 1, 16), __shfl_up_sync(0xffffffffu, v.w, 1, 16));
+  act_store8<WIDE>(row, k, K, v, left, sub > 0, sub == 15, live);
+}
+
+// LANES threads own a block.
+template <int LANES>
+struct ActItem {
+  uint32_t row;
+  int32_t block, k;      // k: first column of the lane's first group
+  bool ok;
+};
+template <int LANES>
+__device__ __forceinline__ ActItem<LANES> act_item(const ActParams& p) {
+  ActItem<LANES> it;
+  const uint32_t item = blockIdx.x * (kActThreads / LANES) + threadIdx.x / LANES;
+  it.ok = item < p.items;
+  it.row = !it.ok ? 0u : p.blocks == 1 ? item : __umulhi(item, p.div_mul) >> p.div_shift;
+  it.block = it.ok ? int32_t(item - it.row * uint32_t(p.blocks)) : 0;
+  it.k = it.block * kActBlock + int(threadIdx.x % LANES) * 8;
+  return it;
+}
+
 template <int ACT, bool GATED, bool FP16, bool WIDE>
 __global__ void __launch_bounds__(kActThreads) bsg_act_forward_kernel(const ActParams p) {
-  const uint32_t item = blockIdx.x * (kActThreads / 16) + threadIdx.x / 16;
-  const int sub = threadIdx.x & 15;
-  const bool ok = item < p.items;
-  const uint32_t row = ok ? item / uint32_t(p.blocks) : 0u;
-  const int32_t block = ok ? int32_t(item - row * uint32_t(p.blocks)) : 0;
-  const int32_t k = block * kActBlock + sub * 8;
-  const bool live = ok && k < p.F;
-  const int32_t F = live ? p.F : 0;
-  const uint16_t* x = p.X + int64_t(row) * p.ldx;
-  const uint4 gv = i8_load8(x, k, F, WIDE);
-  uint4 uv = make_uint4(0, 0, 0, 0);
-  if constexpr (GATED) uv = i8_load8(x + p.F, k, F, WIDE);
-  uint32_t m = act_max_of<FP16>(gv) & 0xFFFFu;
-  if constexpr (GATED) m |= act_max_of<FP16>(uv) << 16;
-#pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) m = i8_maxabs2<FP16>(m, __shfl_xor_sync(0xffffffffu, m, o));
-  m &= 0x7FFF7FFFu;
   constexpr int kParts = GATED ? 2 : 1;
+  const ActItem<kActForwardLanes> it = act_item<kActForwardLanes>(p);
+  const int sub = threadIdx.x % kActForwardLanes;
+  const int32_t F = it.ok ? p.F : 0;
+  const uint16_t* x = p.X + int64_t(it.row) * p.ldx;
+  uint4 gv[2], uv[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int32_t k = it.k + 64 * c;
+    gv[c] = uv[c] = make_uint4(0, 0, 0, 0);
+    if (k < F) {
+      gv[c] = i8_load8(x, k, F, WIDE);
+      if constexpr (GATED) uv[c] = i8_load8(x + p.F, k, F, WIDE);
+    }
+  }
+  uint32_t m = i8_maxabs2<FP16>(act_max_of<FP16>(gv[0]), act_max_of<FP16>(gv[1])) & 0xFFFFu;
+  if constexpr (GATED) m |= i8_maxabs2<FP16>(act_max_of<FP16>(uv[0]), act_max_of<FP16>(uv[1])) << 16;
+#pragma unroll
+  for (int o = 4; o >= 1; o >>= 1) m = i8_maxabs2<FP16>(m, __shfl_xor_sync(0xffffffffu, m, o));
+  m &= 0x7FFF7FFFu;
   const float mg = i8_unpack(m & 0xFFFFu, FP16), mu = i8_unpack(m >> 16, FP16);
-  int8_t* q = p.Q + int64_t(row) * kParts * p.pitch + k;
-  // the first lane stores the scale of g, the second that of u; kept rows are padded to 16 values: a group of 8 is stored whole
+  // the first lane stores the scale of g, the second that of u
   const float step = i8_step(GATED && sub == 1 ? mu : mg);
-  if (live || (GATED && ok && sub == 1)) {
-    if (sub < kParts) p.scale[(int64_t(row) * kParts + sub) * p.blocks + block] = step;
-  }
-  if (live) *reinterpret_cast<uint2*>(q) = i8_levels8<FP16>(gv, i8_scale(mg));
-  float g[8], h[8];
-  act_unpack<FP16>(gv, g);
+  if (it.ok && sub < kParts) p.scale[(int64_t(it.row) * kParts + sub) * p.blocks + it.block] = step;
+  int8_t* q = p.Q + int64_t(it.row) * kParts * p.pitch + it.k;
+  const I8Scale sg = i8_scale(mg), su = i8_scale(mu);
+  uint4 out[2];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) h[j] = act_value<ACT>(g[j]);
-  if constexpr (GATED) {
-    if (live) *reinterpret_cast<uint2*>(q + p.pitch) = i8_levels8<FP16>(uv, i8_scale(mu));
-    float u[8];
-    act_unpack<FP16>(uv, u);
+  for (int c = 0; c < 2; ++c) {
+    if (it.k + 64 * c < F) {      // kept rows are padded to 16 values: a group of 8 is stored whole
+      *reinterpret_cast<uint2*>(q + 64 * c) = i8_levels8<FP16>(gv[c], sg);
+      if constexpr (GATED) *reinterpret_cast<uint2*>(q + p.pitch + 64 * c) = i8_levels8<FP16>(uv[c], su);
+    }
+    float g[8], h[8];
+    act_unpack<FP16>(gv[c], g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[j] *= u[j];
+    for (int j = 0; j < 8; ++j) h[j] = act_value<ACT>(g[j]);
+    if constexpr (GATED) {
+      float u[8];
+      act_unpack<FP16>(uv[c], u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) h[j] *= u[j];
+    }
+    out[c] = act_pack<FP16>(h);
   }
-  act_store8<WIDE>(p.Y + int64_t(row) * p.ldy, k, p.F, act_pack<FP16>(h), sub, live);
+  act_store16<WIDE>(p.Y + int64_t(it.row) * p.ldy, it.k, p.F, out, sub, it.ok);
 }
 
 // s * q for four levels: a byte becomes fp32 as the last byte of 2^23 (exact), without the conversion unit.
@@ -180,18 +235,15 @@ __device__ __forceinline__ void act_dequant4(uint32_t q, float s, float* x) {
 
 template <int ACT, bool GATED, bool FP16, bool WIDE>
 __global__ void __launch_bounds__(kActThreads) bsg_act_backward_kernel(const ActParams p) {
-  const uint32_t item = blockIdx.x * (kActThreads / 16) + threadIdx.x / 16;
-  const int sub = threadIdx.x & 15;
-  const bool ok = item < p.items;
-  const uint32_t row = ok ? item / uint32_t(p.blocks) : 0u;
-  const int32_t block = ok ? int32_t(item - row * uint32_t(p.blocks)) : 0;
-  const int32_t k = block * kActBlock + sub * 8;
-  const bool live = ok && k < p.F;
-  if (WIDE && !live) return;
   constexpr int kParts = GATED ? 2 : 1;
-  const uint4 dv = i8_load8(p.G + int64_t(row) * p.ldg, k, live ? p.F : 0, WIDE);
-  const int8_t* q = p.Q + int64_t(row) * kParts * p.pitch + (live ? k : 0);
-  const float* scale = p.scale + int64_t(row) * kParts * p.blocks + block;
+  const ActItem<kActBackwardLanes> it = act_item<kActBackwardLanes>(p);
+  const int sub = threadIdx.x % kActBackwardLanes;
+  const bool live = it.ok && it.k < p.F;
+  if (WIDE && !live) return;
+  const int32_t k = live ? it.k : 0;
+  const uint4 dv = i8_load8(p.G + int64_t(it.row) * p.ldg, k, live ? p.F : 0, WIDE);
+  const int8_t* q = p.Q + int64_t(it.row) * kParts * p.pitch + k;
+  const float* scale = p.scale + int64_t(it.row) * kParts * p.blocks + it.block;
   const uint2 qg = __ldg(reinterpret_cast<const uint2*>(q));
   const float sg = __ldg(scale);
   uint2 qu = make_uint2(0, 0);
@@ -215,9 +267,9 @@ __global__ void __launch_bounds__(kActThreads) bsg_act_backward_kernel(const Act
     dg[j] = GATED ? d[j] * u[j] * slope : d[j] * slope;
     du[j] = d[j] * value;
   }
-  uint16_t* y = p.Y + int64_t(row) * p.ldy;
-  act_store8<WIDE>(y, k, p.F, act_pack<FP16>(dg), sub, live);
-  if constexpr (GATED) act_store8<WIDE>(y + p.F, k, p.F, act_pack<FP16>(du), sub, live);
+  uint16_t* y = p.Y + int64_t(it.row) * p.ldy;
+  act_store16lanes<WIDE>(y, k, p.F, act_pack<FP16>(dg), sub, live);
+  if constexpr (GATED) act_store16lanes<WIDE>(y + p.F, k, p.F, act_pack<FP16>(du), sub, live);
 }
 
 }  // namespace bsg
