@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <cstring>
+#include <mutex>
 
 #include "../../include/bsgemm.h"
 #include "gemm_kernel.cuh"
@@ -14,12 +15,12 @@ namespace {
 using bsg::host_aligned;
 using bsg::host_fail;
 
-constexpr int64_t kBlocksMax = 4 * 148;
-
 int64_t route_blocks(int64_t tokens) {
-  const int64_t b = (tokens + 31) / 32;      // at least four tokens a warp
-  return b < 1 ? 1 : b > kBlocksMax ? kBlocksMax : b;
+  if (tokens <= bsg::kRouteOneTokens) return 1;
+  const int64_t b = (tokens + 15) / 16;      // at least two tokens a warp
+  return b > bsg::kRouteBlocksMax ? bsg::kRouteBlocksMax : b;
 }
+int64_t route_pitch(int64_t tokens) { return (route_blocks(tokens) + 3) / 4 * 4; }
 
 int32_t check(const bsg_route_args* a, bool forward) {
   if (!a) return host_fail(BSG_ERR_INVALID_PROBLEM, "args is null");
@@ -30,7 +31,8 @@ int32_t check(const bsg_route_args* a, bool forward) {
   if (a->normalize != 0 && a->normalize != 1) return host_fail(BSG_ERR_INVALID_PROBLEM, "normalize must be 0 or 1");
   if (!a->counts || !a->live || (forward && (!a->offsets || !a->loss))) return host_fail(BSG_ERR_INVALID_PROBLEM, "per-expert tensors and the loss must not be null");
   if (a->tokens > 0) {
-    if (!a->logits || !a->chosen || !a->weights) return host_fail(BSG_ERR_INVALID_PROBLEM, "logits, chosen and weights must not be null");
+    if (!a->logits || !a->chosen || !a->weights || !a->softmax) return host_fail(BSG_ERR_INVALID_PROBLEM, "logits, chosen, weights and softmax must not be null");
+    if (!host_aligned(a->softmax, 8)) return host_fail(BSG_ERR_MISALIGNED_OPERAND, "softmax must be 8-byte aligned");
     if (forward && (!a->rows || !a->positions)) return host_fail(BSG_ERR_INVALID_PROBLEM, "rows and positions must not be null");
     if (!forward && !a->grad_logits) return host_fail(BSG_ERR_INVALID_PROBLEM, "grad_logits must not be null");
     if (a->ld < a->experts || (!forward && a->ld_grad < a->experts)) return host_fail(BSG_ERR_INVALID_PROBLEM, "a row pitch is smaller than the %d experts", a->experts);
@@ -41,8 +43,8 @@ int32_t check(const bsg_route_args* a, bool forward) {
 }
 
 int64_t scratch_words(const bsg_route_args* a) {
-  const int64_t b = route_blocks(a->tokens);
-  return b * (a->experts + 1) + b * a->experts + a->experts;
+  if (a->tokens <= bsg::kRouteOneTokens) return 0;
+  return route_pitch(a->tokens) * (2 * a->experts + 1) + a->experts;
 }
 
 bsg::RouteParams params(const bsg_route_args* a, void* scratch) {
@@ -60,33 +62,90 @@ bsg::RouteParams params(const bsg_route_args* a, void* scratch) {
   p.blocks = int32_t(p.per_block > 0 ? (a->tokens + p.per_block - 1) / p.per_block : 1);
   if (p.blocks < 1) p.blocks = 1;
   int32_t* w = static_cast<int32_t*>(scratch);
+  p.pitch = int32_t(route_pitch(a->tokens));
   p.block_counts = w;
-  p.block_sums = reinterpret_cast<float*>(w + b * (a->experts + 1));
-  p.sums = p.block_sums + b * a->experts;
+  p.block_sums = reinterpret_cast<float*>(w + int64_t(p.pitch) * (a->experts + 1));
+  p.sums = p.block_sums + int64_t(p.pitch) * a->experts;
+  p.softmax = reinterpret_cast<float2*>(a->softmax);
   return p;
 }
 
+// Kernels that use more than 48 KB of shared memory (more than 768 or 384 experts) are allowed to once per device.
+struct SmemOnce {
+  std::mutex mu;
+  bool done[64] = {};
+  int32_t set(const void* kernel, int bytes, int dev) {
+    if (bytes <= 48 * 1024) return BSG_OK;
+    if (dev < 0 || dev >= 64) return host_fail(BSG_ERR_NOT_SUPPORTED, "device ordinal %d is outside [0, 64)", dev);
+    std::lock_guard<std::mutex> lock(mu);
+    if (done[dev]) return BSG_OK;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * bsg::kRouteOneWarps * bsg::kRouteMaxExperts * 4);
+    if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    done[dev] = true;
+    return BSG_OK;
+  }
+};
+
+template <class... Args>
+cudaError_t launch_behind(void (*kernel)(Args...), unsigned grid, unsigned threads, cudaStream_t s, const bsg::RouteParams& p) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 template <int TYPE, int V>
-int32_t forward_v(const bsg::RouteParams& p, cudaStream_t s) {
-  const size_t shared1 = size_t(p.experts + 1 + bsg::kRouteWarps * p.experts) * 4;
-  bsg::bsg_route_tokens_kernel<TYPE, V><<<p.blocks, bsg::kRouteThreads, shared1, s>>>(p);
-  bsg::bsg_route_scan_kernel<<<(p.experts + 1 + bsg::kRouteWarps - 1) / bsg::kRouteWarps, bsg::kRouteThreads, 0, s>>>(p);
-  bsg::bsg_route_order_kernel<<<p.blocks, bsg::kRouteThreads, size_t(1 + bsg::kRouteWarps) * p.experts * 4, s>>>(p);
-  cudaError_t e = cudaGetLastError();
+int32_t forward_v(const bsg::RouteParams& p, int dev, cudaStream_t s) {
+  cudaError_t e;
+  if (p.tokens <= bsg::kRouteOneTokens) {
+    static SmemOnce once;
+    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteOneWarps, true>;
+    const int shared = 2 * bsg::kRouteOneWarps * p.experts * 4;
+    int32_t rc = once.set(reinterpret_cast<const void*>(kernel), shared, dev);
+    if (rc != BSG_OK) return rc;
+    kernel<<<1, bsg::kRouteOneWarps * 32, shared, s>>>(p);
+    e = cudaGetLastError();
+  } else {
+    static SmemOnce once;
+    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteWarps, false>;
+    const int shared = 2 * bsg::kRouteWarps * p.experts * 4;
+    int32_t rc = once.set(reinterpret_cast<const void*>(kernel), shared, dev);
+    if (rc != BSG_OK) return rc;
+    kernel<<<p.blocks, bsg::kRouteThreads, shared, s>>>(p);
+    e = cudaGetLastError();
+    if (e == cudaSuccess) e = launch_behind(bsg::bsg_route_scan_kernel, (p.experts + 1 + 3) / 4, 128, s, p);
+    if (e == cudaSuccess) e = launch_behind(bsg::bsg_route_order_kernel, p.blocks, bsg::kRouteThreads, s, p);
+  }
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "router launch: %s", cudaGetErrorString(e));
   return BSG_OK;
 }
 template <int TYPE, int V>
 int32_t backward_v(const bsg::RouteParams& p, int sms, cudaStream_t s) {
-  const int64_t want = (int64_t(p.tokens) + bsg::kRouteWarps - 1) / bsg::kRouteWarps, most = 8 * int64_t(sms);
-  bsg::bsg_route_backward_kernel<TYPE, V><<<unsigned(want < most ? want : most), bsg::kRouteThreads, size_t(bsg::kRouteWarps) * 32 * V * 4, s>>>(p);
+  // one wave of what fits the SMs: a block goes on to its next tokens with their data already asked for
+  static int per_sm = 0;      // the same for every device of this architecture
+  auto kernel = bsg::bsg_route_backward_kernel<TYPE, V>;
+  const size_t shared = size_t(bsg::kRouteWarps) * 32 * V * 4;
+  if (per_sm == 0) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, bsg::kRouteThreads, shared) != cudaSuccess || n < 1) n = 4;
+    per_sm = n;
+  }
+  const int64_t want = (int64_t(p.tokens) + bsg::kRouteWarps - 1) / bsg::kRouteWarps, most = int64_t(per_sm) * sms;
+  kernel<<<unsigned(want < most ? want : most), bsg::kRouteThreads, shared, s>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "router launch: %s", cudaGetErrorString(e));
   return BSG_OK;
 }
 template <int TYPE>
-int32_t pick(const bsg::RouteParams& p, bool forward, int sms, cudaStream_t s) {
-#define BSG_ROUTE_V(V) return forward ? forward_v<TYPE, V>(p, s) : backward_v<TYPE, V>(p, sms, s)
+int32_t pick(const bsg::RouteParams& p, bool forward, int dev, int sms, cudaStream_t s) {
+#define BSG_ROUTE_V(V) return forward ? forward_v<TYPE, V>(p, dev, s) : backward_v<TYPE, V>(p, sms, s)
   if (p.experts <= 32) BSG_ROUTE_V(1);
   if (p.experts <= 64) BSG_ROUTE_V(2);
   if (p.experts <= 128) BSG_ROUTE_V(4);
@@ -95,10 +154,10 @@ int32_t pick(const bsg::RouteParams& p, bool forward, int sms, cudaStream_t s) {
   BSG_ROUTE_V(32);
 #undef BSG_ROUTE_V
 }
-int32_t run(const bsg::RouteParams& p, int32_t type, bool forward, int sms, cudaStream_t s) {
-  if (type == BSG_OUT_BF16) return pick<bsg::kRouteBf16>(p, forward, sms, s);
-  if (type == BSG_OUT_F16) return pick<bsg::kRouteF16>(p, forward, sms, s);
-  return pick<bsg::kRouteF32>(p, forward, sms, s);
+int32_t run(const bsg::RouteParams& p, int32_t type, bool forward, int dev, int sms, cudaStream_t s) {
+  if (type == BSG_OUT_BF16) return pick<bsg::kRouteBf16>(p, forward, dev, sms, s);
+  if (type == BSG_OUT_F16) return pick<bsg::kRouteF16>(p, forward, dev, sms, s);
+  return pick<bsg::kRouteF32>(p, forward, dev, sms, s);
 }
 
 }  // namespace
@@ -115,11 +174,11 @@ int32_t bsg_route_scratch_size(const bsg_route_args* args, size_t* bytes) {
 int32_t bsg_route_forward(const bsg_route_args* args, void* scratch, size_t scratch_bytes, void* cuda_stream) {
   int32_t rc = check(args, true);
   if (rc != BSG_OK) return rc;
-  if (!scratch || scratch_bytes < size_t(scratch_words(args)) * 4) return host_fail(BSG_ERR_WORKSPACE_NULL, "the router needs %lld bytes of scratch", (long long)scratch_words(args) * 4);
-  if (!host_aligned(scratch, 4)) return host_fail(BSG_ERR_MISALIGNED_OPERAND, "scratch must be 4-byte aligned");
+  if (scratch_words(args) > 0 && (!scratch || scratch_bytes < size_t(scratch_words(args)) * 4)) return host_fail(BSG_ERR_WORKSPACE_NULL, "the router needs %lld bytes of scratch", (long long)scratch_words(args) * 4);
+  if (!host_aligned(scratch, 16)) return host_fail(BSG_ERR_MISALIGNED_OPERAND, "scratch must be 16-byte aligned");
   int dev = 0, sms = 0;
   if ((rc = bsg::host_device(BSG_ERR_ARCH_MISMATCH, BSG_ERR_CUDA, &dev, &sms)) != BSG_OK) return rc;
-  return run(params(args, scratch), args->type, true, sms, static_cast<cudaStream_t>(cuda_stream));
+  return run(params(args, scratch), args->type, true, dev, sms, static_cast<cudaStream_t>(cuda_stream));
 }
 
 int32_t bsg_route_backward(const bsg_route_args* args, void* cuda_stream) {
@@ -127,7 +186,7 @@ int32_t bsg_route_backward(const bsg_route_args* args, void* cuda_stream) {
   if (rc != BSG_OK || args->tokens == 0) return rc;
   int dev = 0, sms = 0;
   if ((rc = bsg::host_device(BSG_ERR_ARCH_MISMATCH, BSG_ERR_CUDA, &dev, &sms)) != BSG_OK) return rc;
-  return run(params(args, nullptr), args->type, false, sms, static_cast<cudaStream_t>(cuda_stream));
+  return run(params(args, nullptr), args->type, false, dev, sms, static_cast<cudaStream_t>(cuda_stream));
 }
 
 }  // extern "C"

@@ -109,7 +109,7 @@ class QuantArgs(C.Structure):
 
 INT8_LAYOUT = "4i4qPqPPqPPqqPPPPq4i"      # Int8Args, ActArgs and RouteArgs below as struct formats
 ACT_LAYOUT = "4i2qPqPqPP"
-ROUTE_LAYOUT = "4iqPq12Pq"
+ROUTE_LAYOUT = "4iqPq13Pq"
 
 
 class Int8Args(C.Structure):
@@ -137,7 +137,7 @@ class RouteArgs(C.Structure):
     _fields_ = [
         ("type", C.c_int32), ("experts", C.c_int32), ("k", C.c_int32), ("normalize", C.c_int32), ("tokens", C.c_int64),
         ("logits", C.c_void_p), ("ld", C.c_int64), ("mask", C.c_void_p),
-        ("chosen", C.c_void_p), ("weights", C.c_void_p), ("counts", C.c_void_p), ("live", C.c_void_p),
+        ("chosen", C.c_void_p), ("weights", C.c_void_p), ("counts", C.c_void_p), ("live", C.c_void_p), ("softmax", C.c_void_p),
         ("offsets", C.c_void_p), ("rows", C.c_void_p), ("positions", C.c_void_p), ("loss", C.c_void_p),
         ("grad_weights", C.c_void_p), ("grad_loss", C.c_void_p), ("grad_logits", C.c_void_p), ("ld_grad", C.c_int64),
     ]

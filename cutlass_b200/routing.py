@@ -32,12 +32,14 @@ class Routing(NamedTuple):
     positions: torch.Tensor       # (T, k) int32: row of every slot
     balance_loss: torch.Tensor    # () fp32
     num_tokens: torch.Tensor      # (1,) int32: tokens that count
+    softmax: torch.Tensor         # (T, 2) fp32, for the backward pass: largest logit, 1 / sum of exp(logit - largest)
     normalize: bool
 
 
-def _scratch_words(T: int, E: int) -> int:
-    blocks = min(max(-(-T // 32), 1), 592)
-    return blocks * (2 * E + 1) + E
+def _scratch_words(T: int, E: int) -> int:      # what bsg_route_scratch_size says
+    if T <= 128:
+        return 0
+    return ((min((T + 15) // 16, 592) + 3) & ~3) * (2 * E + 1) + E
 
 
 def _check_logits(logits, top_k):
@@ -61,14 +63,21 @@ def _forward(logits, top_k, token_mask, normalize, stream) -> Routing:
     whole = logits.new_empty(3 * n + 2 * E + 1, dtype=torch.int32)
     weights = logits.new_empty((T, top_k), dtype=torch.float32)
     loss = logits.new_empty((), dtype=torch.float32)
-    scratch = logits.new_empty(_scratch_words(T, E), dtype=torch.int32)
+    softmax = logits.new_empty((T, 2), dtype=torch.float32)
+    words = _scratch_words(T, E)
+    scratch = logits.new_empty(words, dtype=torch.int32) if words else None
     w = whole.data_ptr()
     pack, call = L.direct("bsg_route_forward", L.ROUTE_LAYOUT)
     args = pack(kind, E, top_k, normalize, T, logits.data_ptr(), ld, 0 if token_mask is None else token_mask.data_ptr(),
-                w, weights.data_ptr(), w + 12 * n, w + 12 * n + 8 * E, w + 12 * n + 4 * E, w + 4 * n, w + 8 * n, loss.data_ptr(), 0, 0, 0, 0)
-    _launch(device, stream, (whole, weights, loss, scratch), call, args, scratch.data_ptr(), 4 * scratch.numel())
+                w, weights.data_ptr(), w + 12 * n, w + 12 * n + 8 * E, softmax.data_ptr(),
+                w + 12 * n + 4 * E, w + 4 * n, w + 8 * n, loss.data_ptr(), 0, 0, 0, 0)
+    made = (whole, weights, loss, softmax)
+    if words:
+        _launch(device, stream, made + (scratch,), call, args, scratch.data_ptr(), 4 * words)
+    else:
+        _launch(device, stream, made, call, args, 0, 0)
     experts, rows, positions, counts, offsets, live = whole.split_with_sizes([n, n, n, E, E, 1])
-    return Routing(experts.view(T, top_k), weights, counts, offsets, rows, positions.view(T, top_k), loss, live, normalize)
+    return Routing(experts.view(T, top_k), weights, counts, offsets, rows, positions.view(T, top_k), loss, live, softmax, normalize)
 
 
 def route_tokens_backward(logits, routing: Routing, grad_weights=None, grad_balance_loss=None, *, stream=None) -> torch.Tensor:
@@ -88,7 +97,7 @@ def route_tokens_backward(logits, routing: Routing, grad_weights=None, grad_bala
     out = logits.new_empty((T, E))
     pack, call = L.direct("bsg_route_backward", L.ROUTE_LAYOUT)
     args = pack(kind, E, k, routing.normalize, T, logits.data_ptr(), ld, 0, experts.data_ptr(), routing.weights.data_ptr(),
-                counts.data_ptr(), routing.num_tokens.data_ptr(), 0, 0, 0, 0, 0 if grad_weights is None else grad_weights.data_ptr(),
+                counts.data_ptr(), routing.num_tokens.data_ptr(), routing.softmax.data_ptr(), 0, 0, 0, 0, 0 if grad_weights is None else grad_weights.data_ptr(),
                 0 if grad_balance_loss is None else grad_balance_loss.data_ptr(), out.data_ptr(), E)
     _launch(device, stream, (out,), call, args)
     return out
@@ -98,9 +107,9 @@ class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, top_k, token_mask, normalize, stream):
         r = _forward(logits, top_k, token_mask, normalize, stream)
-        ctx.save_for_backward(logits, r.experts, r.weights, r.counts, r.num_tokens)
+        ctx.save_for_backward(logits, r.experts, r.weights, r.counts, r.num_tokens, r.softmax)
         ctx.normalize = r.normalize
-        whole = (r.experts, r.counts, r.offsets, r.rows, r.positions, r.num_tokens)
+        whole = (r.experts, r.counts, r.offsets, r.rows, r.positions, r.num_tokens, r.softmax)
         ctx.mark_non_differentiable(*whole)
         ctx.set_materialize_grads(False)
         return (r.weights, r.balance_loss) + whole
@@ -108,10 +117,10 @@ class _Route(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_weights, grad_loss, *_):
-        logits, experts, weights, counts, live = ctx.saved_tensors
+        logits, experts, weights, counts, live, softmax = ctx.saved_tensors
         if grad_weights is None and grad_loss is None:
             return None, None, None, None, None
-        r = Routing(experts, weights, counts, None, None, None, None, live, ctx.normalize)
+        r = Routing(experts, weights, counts, None, None, None, None, live, softmax, ctx.normalize)
         grad = route_tokens_backward(logits, r, grad_weights.contiguous() if grad_weights is not None else None, grad_loss)
         return grad, None, None, None, None
 
@@ -129,5 +138,5 @@ def route_tokens(logits, top_k: int, *, token_mask=None, normalize: bool = True,
     (None: torch's current stream); the backward pass runs on the stream that autograd makes current."""
     if not (torch.is_grad_enabled() and logits.requires_grad):
         return _forward(logits, top_k, token_mask, normalize, stream)
-    weights, loss, experts, counts, offsets, rows, positions, live = _Route.apply(logits, top_k, token_mask, normalize, stream)
-    return Routing(experts, weights, counts, offsets, rows, positions, loss, live, bool(normalize))
+    weights, loss, experts, counts, offsets, rows, positions, live, softmax = _Route.apply(logits, top_k, token_mask, normalize, stream)
+    return Routing(experts, weights, counts, offsets, rows, positions, loss, live, softmax, bool(normalize))

@@ -392,6 +392,7 @@ typedef struct bsg_route_args {
   float* weights;           /* (tokens, k) */
   int32_t* counts;          /* [experts] */
   int32_t* live;            /* [1]: n */
+  float* softmax;           /* (tokens, 2): largest logit, 1 / sum of exp(logit - largest); 8-byte aligned */
   /* written by forward */
   int32_t* offsets;         /* [experts] */
   int32_t* rows;            /* [tokens * k]: token of every row */
