@@ -8,8 +8,6 @@ What is kept is one byte per value of ``x`` and one fp32 scale per 128 of them, 
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
-
 import torch
 
 from . import lib as L
@@ -19,20 +17,29 @@ from .int8 import _IN_KINDS, _launch, _matrix, _no_gradient
 BLOCK = 128      # columns of a row that share one scale
 
 
-@dataclass
 class ActivationCheckpoint:
     """Input of an activation in 8 bits: ``quantized`` (T, parts, F rounded up to 16) int8 and ``scale`` (T, parts, F / 128
-    rounded up) fp32, with parts = 2 (gate, up) when ``gated``, else 1; its value is ``scale * quantized`` per block."""
+    rounded up) fp32, with parts = 2 (gate, up) when ``gated``, else 1; its value is ``scale * quantized`` per block.  Both lie
+    in one buffer, ``data``."""
 
-    quantized: torch.Tensor
-    scale: torch.Tensor
-    activation: str
-    gated: bool
-    width: int
-    dtype: torch.dtype
+    __slots__ = ("data", "activation", "gated", "rows", "width", "dtype")
+
+    def __init__(self, data: torch.Tensor, activation: str, gated: bool, rows: int, width: int, dtype: torch.dtype):
+        self.data, self.activation, self.gated, self.rows, self.width, self.dtype = data, activation, gated, rows, width, dtype
+
+    def _split(self) -> int:
+        return self.rows * (2 if self.gated else 1) * ((self.width + 15) & ~15)
+
+    @property
+    def quantized(self) -> torch.Tensor:
+        return self.data[:self._split()].view(self.rows, 2 if self.gated else 1, (self.width + 15) & ~15)
+
+    @property
+    def scale(self) -> torch.Tensor:
+        return self.data[self._split():].view(torch.float32).view(self.rows, 2 if self.gated else 1, -(-self.width // BLOCK))
 
     def nbytes(self) -> int:
-        return self.quantized.numel() + 4 * self.scale.numel()
+        return self.data.numel()
 
 
 def _given(name, t, kind, device, rows, cols) -> int:
@@ -57,24 +64,25 @@ def checkpoint_activation(x, activation: str = "silu", *, gated: bool = True, ou
     if gated and cols % 2 != 0:
         raise ValueError(f"a gated activation needs an even number of columns (gate | up), got {cols}")
     parts, F = (2, cols // 2) if gated else (1, cols)
-    q = x.new_empty((T, parts, (F + 15) & ~15), dtype=torch.int8)
-    scale = x.new_empty((T, parts, (F + BLOCK - 1) // BLOCK), dtype=torch.float32)
+    split = T * parts * ((F + 15) & ~15)
+    data = x.new_empty(split + 4 * T * parts * ((F + BLOCK - 1) // BLOCK), dtype=torch.int8)
     if out is None:
         out, ldh = x.new_empty((T, F)), F
-        made = (q, scale, out)
+        made = (data, out)
     else:
         ldh = _given("out", out, kind, device, T, F)
-        made = (q, scale)
+        made = (data,)
+    q = data.data_ptr()
     pack, call = L.direct("bsg_act_forward", L.ACT_LAYOUT)
-    _launch(device, stream, made, call, pack(kind, act, parts - 1, 0, T, F, x.data_ptr(), ldx, out.data_ptr(), ldh, q.data_ptr(), scale.data_ptr()))
-    return out, ActivationCheckpoint(q, scale, activation, gated, F, x.dtype)
+    _launch(device, stream, made, call, pack(kind, act, parts - 1, 0, T, F, x.data_ptr(), ldx, out.data_ptr(), ldh, q, q + split))
+    return out, ActivationCheckpoint(data, activation, gated, T, F, x.dtype)
 
 
 def checkpoint_activation_backward(grad, kept: ActivationCheckpoint, *, out=None, stream=None) -> torch.Tensor:
     """Gradient of ``x`` for the gradient ``grad`` (T, F) of ``h``, from what ``checkpoint_activation`` kept: (T, 2F) or (T, F)
     in the type of ``x``.  ``out`` may be given.  Asynchronous on ``stream`` (None: torch's current stream)."""
-    q, F = kept.quantized, kept.width
-    kind, device, (T, parts, _) = _IN_KINDS[kept.dtype], q.get_device(), q.shape
+    data, T, F, parts = kept.data, kept.rows, kept.width, 2 if kept.gated else 1
+    kind, device, q = _IN_KINDS[kept.dtype], data.get_device(), data.data_ptr()
     ldg = _given("grad", grad, kind, device, T, F)
     _no_gradient("checkpoint_activation_backward", grad)
     if out is None:
@@ -84,7 +92,7 @@ def checkpoint_activation_backward(grad, kept: ActivationCheckpoint, *, out=None
         ldx, made = _given("out", out, kind, device, T, parts * F), ()
     pack, call = L.direct("bsg_act_backward", L.ACT_LAYOUT)
     _launch(device, stream, made, call, pack(kind, ACTIVATIONS[kept.activation], parts - 1, 0, T, F, grad.data_ptr(), ldg, out.data_ptr(), ldx,
-                                             q.data_ptr(), kept.scale.data_ptr()))
+                                             q, q + kept._split()))
     return out
 
 
@@ -92,8 +100,8 @@ class _CheckpointedActivation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, activation, gated):
         h, kept = checkpoint_activation(x, activation, gated=gated)
-        ctx.save_for_backward(kept.quantized, kept.scale)
-        ctx.how = (activation, kept.gated, kept.width, kept.dtype)
+        ctx.save_for_backward(kept.data)
+        ctx.how = (activation, kept.gated, kept.rows, kept.width, kept.dtype)
         return h
 
     @staticmethod

@@ -84,13 +84,26 @@ __device__ __forceinline__ void act_store8(uint16_t* row, int32_t k, int32_t K, 
   }
 }
 
-// act(x), and its slope.  The results are rounded to 16 bits, so the fast exponential and quotient (errors near 2^-21) do.
+// exp(x) and 1 / x of the special-function unit, off by about 2^-22 (the exponential by |x| 2^-24 more); results below 2^-126 are 0.
+// All that they feed is rounded to 16 bits, and 1 / x is only taken of 1 and more.
+__device__ __forceinline__ float act_exp(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+__device__ __forceinline__ float act_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// act(x), and its slope.
 // gelu: erfc(z) = t (a1 + t (a2 + ... a5)) exp(-z^2), t = 1 / (1 + 0.3275911 z), z >= 0 (Abramowitz and Stegun, Handbook of
 // Mathematical Functions, 7.1.26: off by at most 1.5e-7); its exponential is also that of the slope.  CUDA's erfc took
 // the forward pass of 8192 x 14336 gated values from 223 to 343 us.
 __device__ __forceinline__ void act_normal(float x, float& cdf, float& gauss) {      // Phi(x), exp(-x^2 / 2)
-  gauss = __expf(-0.5f * x * x);
-  const float t = i8_rcp(1.0f + 0.23164189f * fabsf(x));      // 0.3275911 / sqrt(2)
+  gauss = act_exp(-0.5f * x * x);
+  const float t = act_rcp(1.0f + 0.23164189f * fabsf(x));      // 0.3275911 / sqrt(2)
   const float poly = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
   const float tail = 0.5f * poly * gauss;
   cdf = x < 0.0f ? tail : 1.0f - tail;
@@ -98,7 +111,7 @@ __device__ __forceinline__ void act_normal(float x, float& cdf, float& gauss) { 
 template <int ACT>
 __device__ __forceinline__ float act_value(float x) {
   if constexpr (ACT == kActRelu) return x != x ? x : fmaxf(x, 0.0f);
-  else if constexpr (ACT == kActSilu) return __fdividef(x, 1.0f + __expf(-x));
+  else if constexpr (ACT == kActSilu) return x * act_rcp(1.0f + act_exp(-x));
   else if constexpr (ACT == kActGelu) {
     float cdf, gauss;
     act_normal(x, cdf, gauss);
@@ -111,7 +124,7 @@ __device__ __forceinline__ void act_value_slope(float x, float& value, float& sl
     value = x != x ? x : fmaxf(x, 0.0f);
     slope = x != x ? x : (x > 0.0f ? 1.0f : 0.0f);
   } else if constexpr (ACT == kActSilu) {
-    const float s = i8_rcp(1.0f + __expf(-x));
+    const float s = act_rcp(1.0f + act_exp(-x));
     value = x * s;
     slope = s * (1.0f + x * (1.0f - s));
   } else if constexpr (ACT == kActGelu) {

@@ -32,7 +32,7 @@ class Routing(NamedTuple):
     positions: torch.Tensor       # (T, k) int32: row of every slot
     balance_loss: torch.Tensor    # () fp32
     num_tokens: torch.Tensor      # (1,) int32: tokens that count
-    softmax: torch.Tensor         # (T, 2) fp32, for the backward pass: largest logit, 1 / sum of exp(logit - largest)
+    softmax: torch.Tensor         # (2 T,) bits of fp32, for the backward pass: largest logit, 1 / sum of exp(logit - largest)
     normalize: bool
 
 
@@ -59,24 +59,23 @@ def _forward(logits, top_k, token_mask, normalize, stream) -> Routing:
         _check_array("token_mask", token_mask, torch.bool, (T,), device)
     normalize = bool(normalize)
     n = T * top_k
-    # what is whole comes from one allocation; the two results that carry gradients are tensors of their own
-    whole = logits.new_empty(3 * n + 2 * E + 1, dtype=torch.int32)
+    # What carries no gradient comes from one allocation (int32: softmax, as bits, first, since it is read eight bytes at a time);
+    # the two results that carry one are tensors of their own.
+    whole = logits.new_empty(2 * T + 3 * n + 2 * E + 1, dtype=torch.int32)
     weights = logits.new_empty((T, top_k), dtype=torch.float32)
     loss = logits.new_empty((), dtype=torch.float32)
-    softmax = logits.new_empty((T, 2), dtype=torch.float32)
-    words = _scratch_words(T, E)
-    scratch = logits.new_empty(words, dtype=torch.int32) if words else None
-    w = whole.data_ptr()
+    soft = whole.data_ptr()
+    w = soft + 8 * T
     pack, call = L.direct("bsg_route_forward", L.ROUTE_LAYOUT)
     args = pack(kind, E, top_k, normalize, T, logits.data_ptr(), ld, 0 if token_mask is None else token_mask.data_ptr(),
-                w, weights.data_ptr(), w + 12 * n, w + 12 * n + 8 * E, softmax.data_ptr(),
-                w + 12 * n + 4 * E, w + 4 * n, w + 8 * n, loss.data_ptr(), 0, 0, 0, 0)
-    made = (whole, weights, loss, softmax)
+                w, weights.data_ptr(), w + 12 * n, w + 12 * n + 8 * E, soft, w + 12 * n + 4 * E, w + 4 * n, w + 8 * n, loss.data_ptr(), 0, 0, 0, 0)
+    words = _scratch_words(T, E)
     if words:
-        _launch(device, stream, made + (scratch,), call, args, scratch.data_ptr(), 4 * words)
+        scratch = logits.new_empty(words, dtype=torch.int32)
+        _launch(device, stream, (whole, weights, loss, scratch), call, args, scratch.data_ptr(), 4 * words)
     else:
-        _launch(device, stream, made, call, args, 0, 0)
-    experts, rows, positions, counts, offsets, live = whole.split_with_sizes([n, n, n, E, E, 1])
+        _launch(device, stream, (whole, weights, loss), call, args, 0, 0)
+    softmax, experts, rows, positions, counts, offsets, live = whole.split_with_sizes((2 * T, n, n, n, E, E, 1))
     return Routing(experts.view(T, top_k), weights, counts, offsets, rows, positions.view(T, top_k), loss, live, softmax, normalize)
 
 
