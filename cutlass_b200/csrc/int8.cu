@@ -70,7 +70,8 @@ int32_t choose(const bsg_int8_args& a, I8Plan* plan) {
       if (a.split ? a.split != split : split > 1 && (tiles * split > 296 || k_tiles < split * 2)) continue;
       const double slots = v.few ? 296.0 : 74.0;
       double waves = double(int64_t(tiles * split / slots));
-      if (waves * slots < tiles * split) waves += 1.0;
+      const double tail = tiles * split - waves * slots;
+      if (tail > 0.0) waves += !v.few && v.tile == 256 && waves > 0.0 && 2.0 * tail <= slots ? 0.6 : 1.0;      // a thin last wave is split
       double t = waves * double((k_tiles + split - 1) / split) * v.per_k_tile;
       if (t < weights) t = weights;
       t += v.fixed + (split > 1 ? 0.8 + 0.02 * v.tile : 0.0);      // the cluster's barrier and the exchange of partial sums

@@ -476,6 +476,13 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   const int32_t total_tiles = bcast(ctl->total_tiles);
   const int32_t k_tiles = (p.K + 127) / 128;
   uint32_t dead = 0;
+  // The tiles of a last wave that is at most half full are computed as two halves of their columns each, by twice as many pairs.
+  int32_t split_from = total_tiles;
+  if (BN == 256 && total_tiles > num_clusters) {
+    const int32_t tail = total_tiles % num_clusters;
+    if (2 * tail <= num_clusters) split_from = total_tiles - tail;
+  }
+  const int32_t total_work = split_from + 2 * (total_tiles - split_from);
 
   if (warp == 5) {
     // ---------------------------------------------------------------- TMA producer
@@ -485,10 +492,12 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     const uint32_t full0_leader = CG == 2 ? ptx::mapa(full0, 0) : full0;
     int stage = 0;
     uint32_t phase = 0;
-    for (int32_t t = cluster_idx; t < total_tiles; t += num_clusters) {
-      const I8Tile ti = i8_decode(ctl, p, t, C::kTileM);
+    for (int32_t t = cluster_idx; t < total_work; t += num_clusters) {
+      const WorkItem wi = decode_work(t, split_from);
+      const I8Tile ti = i8_decode(ctl, p, wi.t, C::kTileM);
       const int32_t a_row = bcast(ti.row0 + int32_t(cta_rank) * 128);
-      const int32_t b_row = bcast(ti.tn * BN + int32_t(cta_rank) * C::kBRows);
+      // (the box of a half tile brings kBRows rows as well, of which the MMA reads the first half)
+      const int32_t b_row = bcast(ti.tn * BN + (wi.split ? wi.half * (BN / 2) + int32_t(cta_rank) * (C::kBRows / 2) : int32_t(cta_rank) * C::kBRows));
       const int32_t g = bcast(ti.g);
       for (int32_t kt = 0; kt < k_tiles; ++kt) {
         i8_wait(empty0 + stage * 8, phase ^ 1u, ctl, dead);
@@ -510,7 +519,7 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   } else if (warp == 4) {
     // ---------------------------------------------------------------- MMA issue
     if (is_leader) {
-      constexpr uint32_t idesc = i8_idesc(C::kTileM, BN);
+      constexpr uint32_t idesc_full = i8_idesc(C::kTileM, BN), idesc_half = i8_idesc(C::kTileM, BN / 2);
       const uint32_t elected = ptx::elect_one_sync();
       const uint32_t sA0 = ptx::smem_u32(sA), sB0 = ptx::smem_u32(sB);
       const uint32_t full0 = ptx::smem_u32(&ctl->full[0]), empty0 = ptx::smem_u32(&ctl->empty[0]);
@@ -518,7 +527,8 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       int stage = 0;
       uint32_t phase = 0, ready = 0;
       int32_t it = 0;
-      for (int32_t t = cluster_idx; t < total_tiles; t += num_clusters, ++it) {
+      for (int32_t t = cluster_idx; t < total_work; t += num_clusters, ++it) {
+        const uint32_t idesc = t >= split_from ? idesc_half : idesc_full;
         const int acc = it & 1;
         const uint32_t d_tmem = tmem_base + uint32_t(acc) * BN;
         i8_wait(tempty0 + acc * 8, (uint32_t(it >> 1) & 1u) ^ 1u, ctl, dead);
@@ -551,13 +561,14 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     const int out_kind = p.out_kind, act = p.activation;
     const bool f32 = out_kind == kOutF32, has_bias = p.bias != nullptr;
     int32_t it = 0;
-    for (int32_t t = cluster_idx; t < total_tiles; t += num_clusters, ++it) {
-      const I8Tile ti = i8_decode(ctl, p, t, C::kTileM);
+    for (int32_t t = cluster_idx; t < total_work; t += num_clusters, ++it) {
+      const WorkItem wi = decode_work(t, split_from);
+      const I8Tile ti = i8_decode(ctl, p, wi.t, C::kTileM);
       const int acc = it & 1;
-      const int32_t col0 = ti.tn * BN;
+      const int32_t col0 = ti.tn * BN + wi.half * (BN / 2), cols = wi.split ? BN / 2 : BN;
       // scales and bias of the tile's columns, while its products are still being summed
       float* cs = sCol + acc * 2 * BN;
-      for (int c = threadIdx.x; c < BN; c += 128) {
+      for (int c = threadIdx.x; c < cols; c += 128) {
         const bool in = col0 + c < p.N;
         const int64_t at = int64_t(ti.g) * p.N + col0 + c;
         cs[c] = in ? __ldg(p.sb + at) : 0.0f;
@@ -575,11 +586,11 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       // on 16 bytes, are copied row by row from the same staging tile.
       const bool tma = p.tma_out != 0 && rows_here == 32;
 #pragma unroll 1
-      for (int c0 = 0; c0 < BN; c0 += 32) {
+      for (int c0 = 0; c0 < cols; c0 += 32) {
         uint32_t v[32];
         ptx::tmem_ld_32x32b_x32(lane_addr + c0, v);
         ptx::tmem_ld_wait();
-        if (c0 + 32 == BN) {
+        if (c0 + 32 == cols) {
           ptx::tc_fence_before();
           __syncwarp();
           if (lane == 0) {       // relaxed: what is handed back is tensor memory, whose reads have completed
@@ -633,10 +644,10 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           }
         } else {
           __syncwarp();
-          const int32_t cols = min(f32 ? 32 : 64, p.N - out_col);
+          const int32_t left = min(f32 ? 32 : 64, p.N - out_col);
           for (int r = 0; r < rows_here; ++r) {
             const uint8_t* srow = stage_buf + r * 128;
-            for (int c = lane; c < cols; c += 32) {
+            for (int c = lane; c < left; c += 32) {
               if (f32)
                 reinterpret_cast<float*>(p.D)[int64_t(warp_row0 + r) * p.ldd + out_col + c] =
                     *reinterpret_cast<const float*>(srow + (((c >> 2) ^ (r & 7)) * 16) + (c & 3) * 4);

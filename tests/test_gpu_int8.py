@@ -193,6 +193,25 @@ def test_every_kernel_gives_the_same_bits(cuda_lib, kernel, tile, split, M, N, K
     check(out, x, w, ws)
 
 
+@pytest.mark.parametrize("M,N,dtype", [(2560, 2048, BF16), (2560, 1928, F32), (2300, 2051, F16)])
+def test_more_tiles_than_pairs_of_sms(cuda_lib, M, N, dtype):
+    """80 tiles of 256 x 256: a whole wave and a thin one, whose tiles are computed in halves, on any number of SMs up to 158."""
+    import ctypes as C
+    K = 200
+    x = tokens(M, K, BF16, seed=1)
+    w, ws = weights((N,), K, seed=2)
+    ws = ws * 0.001
+    A = ops.quantize_int8(x)
+    out = torch.full((M, N), math.nan, dtype=dtype, device="cuda")
+    op = ops.Int8GemmOperator(ops.get_operators(metadata_filter=lambda m: m.kind == L.KIND_INT8)[0].metadata)
+    a = op.build_args(ops.GemmArguments(A, ops.ScaledOperand(w.t(), ws, (1, 1, K), ops.ScaleSwizzleMode.SwizzleNone), out, torch.int32))
+    a.kernel, a.tile = 2, 256
+    workspace = torch.zeros(16, dtype=torch.uint8, device="cuda")
+    L.check(L.load().bsg_int8_gemm_run(C.byref(a), workspace.data_ptr(), 16, None))
+    L.check(L.load().bsg_read_device_status(workspace.data_ptr(), None))
+    check(out, x, w, ws)
+
+
 def test_the_longest_sum_is_exact(cuda_lib):
     """All products 127 * 127 at the largest K: the sum comes within 2^-9 of the 32-bit range."""
     K = 131071
