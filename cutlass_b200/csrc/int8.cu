@@ -190,7 +190,7 @@ int32_t launch_rows(const bsg_int8_args& a, bsg::I8GemmParams& p, cudaStream_t s
   p.tma_out = host_aligned(a.D, 16) && (a.ldd * esz) % 16 == 0;
   p.tma_edge = (a.N * esz) % 16 == 0;
   tmD = tmA;
-  if (p.tma_out && (rc = bsg::host_out_map(&tmD, a.D, a.out_kind, a.N, a.rows, a.ldd)) != BSG_OK) return rc;
+  if (p.tma_out && (rc = bsg::host_out64_map(&tmD, a.D, a.out_kind, a.N, a.rows, a.ldd)) != BSG_OK) return rc;
   p.tiles_n = int32_t((a.N + BN - 1) / BN);
   p.band = 16;
   int64_t clusters = sms / CG;
@@ -201,7 +201,7 @@ int32_t launch_rows(const bsg_int8_args& a, bsg::I8GemmParams& p, cudaStream_t s
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(unsigned(clusters * CG), 1, 1);
-  cfg.blockDim = dim3(192, 1, 1);
+  cfg.blockDim = dim3(bsg::kI8RowsThreads, 1, 1);
   cfg.dynamicSmemBytes = C::kSmemBytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];

@@ -404,7 +404,11 @@ __device__ __forceinline__ void i8_activate(float (&x)[N], int act) {
   }
 }
 
-// ---- many rows: D tile = (128 * CG rows) x BN columns, persistent, two accumulators of BN columns in tensor memory
+// ---- many rows: D tile = (128 * CG rows) x BN columns, persistent, two accumulators of BN columns in tensor memory.
+// Eight epilogue warps, two for every quarter of the rows with half of the columns each: with four, a tile took 6 us to finish
+// (latencies of tensor-memory loads, conversions and staged stores, one after the other), more than its products up to K = 2500.
+constexpr int kI8EpiWarps = 8;
+constexpr int kI8RowsThreads = 32 * (2 + kI8EpiWarps);      // warps 0-3 and 6-9 epilogue, 4 MMA, 5 TMA
 template <int CG, int BN>
 struct I8RowsCfg {
   static constexpr int kTileM = 128 * CG;
@@ -412,7 +416,7 @@ struct I8RowsCfg {
   static constexpr int kBRows = BN / CG;
   static constexpr int kBBytes = kBRows * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kEpiBytes = 4 * 4096;
+  static constexpr int kEpiBytes = kI8EpiWarps * 2048;    // per warp 32 rows of 64 bytes
   static constexpr int kColBytes = 2 * 2 * BN * 4;        // scale and bias of the tile's columns, two tiles
   static constexpr int kStagesRaw = (232448 - 1024 - kI8CtlBytes - kEpiBytes - kColBytes) / kStageBytes;
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
@@ -422,7 +426,7 @@ struct I8RowsCfg {
 };
 
 template <int CG, int BN>
-__global__ void __launch_bounds__(192, 1)
+__global__ void __launch_bounds__(kI8RowsThreads, 1)
 bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmD, const I8GemmParams p) {
   using C = I8RowsCfg<CG, BN>;
@@ -448,7 +452,7 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     }
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(ptx::smem_u32(&ctl->tmem_full[s]), 1);
-      ptx::mbar_init(ptx::smem_u32(&ctl->tmem_empty[s]), 4 * CG);
+      ptx::mbar_init(ptx::smem_u32(&ctl->tmem_empty[s]), kI8EpiWarps * CG);
     }
     ctl->abort = 0;
     ptx::fence_mbar_init();
@@ -555,11 +559,14 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       if (dead) atomicOr(p.status, kStTimeoutFull | kStTimeoutTmemEmpty);
     }
   } else {
-    // ---------------------------------------------------------------- epilogue (warps 0-3: one quarter of the rows each)
+    // ---------------------------------------------------------------- epilogue
+    const int quarter = warp & 3, half = warp >= 6 ? 1 : 0;      // (a warp reaches the tensor-memory lanes of its number mod 4)
+    const int epi = half * 4 + quarter;
     const uint32_t tfull0 = ptx::smem_u32(&ctl->tmem_full[0]), tempty0 = ptx::smem_u32(&ctl->tmem_empty[0]);
-    uint8_t* stage_buf = sEpi + warp * 4096;
+    uint8_t* stage_buf = sEpi + epi * 2048;
     const int out_kind = p.out_kind, act = p.activation;
     const bool f32 = out_kind == kOutF32, has_bias = p.bias != nullptr;
+    const int swizzle = (lane >> 1) & 3;                         // staging: 16-byte chunk c of row r at chunk c ^ ((r >> 1) & 3)
     int32_t it = 0;
     for (int32_t t = cluster_idx; t < total_work; t += num_clusters, ++it) {
       const WorkItem wi = decode_work(t, split_from);
@@ -568,29 +575,30 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const int32_t col0 = ti.tn * BN + wi.half * (BN / 2), cols = wi.split ? BN / 2 : BN;
       // scales and bias of the tile's columns, while its products are still being summed
       float* cs = sCol + acc * 2 * BN;
-      for (int c = threadIdx.x; c < cols; c += 128) {
+      for (int c = epi * 32 + lane; c < cols; c += 32 * kI8EpiWarps) {
         const bool in = col0 + c < p.N;
         const int64_t at = int64_t(ti.g) * p.N + col0 + c;
         cs[c] = in ? __ldg(p.sb + at) : 0.0f;
         cs[BN + c] = in && has_bias ? __ldg(p.bias + at) : 0.0f;
       }
-      const int32_t warp_row0 = ti.row0 + int32_t(cta_rank) * 128 + warp * 32;
+      const int32_t warp_row0 = ti.row0 + int32_t(cta_rank) * 128 + quarter * 32;
       const int32_t rows_here = min(32, ti.row_end - warp_row0);
       const float sa = lane < rows_here ? __ldcg(p.sa + warp_row0 + lane) : 0.0f;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      asm volatile("bar.sync 1, 256;" ::: "memory");
       i8_wait(tfull0 + acc * 8, uint32_t(it >> 1) & 1u, ctl, dead);
       __syncwarp();
       ptx::tc_fence_after();
-      const uint32_t lane_addr = tmem_base + (uint32_t(warp * 32) << 16) + uint32_t(acc) * BN;
+      const uint32_t lane_addr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(acc) * BN;
       // Whole warps of rows leave by TMA; the warp that holds a group's last rows, and outputs whose rows do not start
       // on 16 bytes, are copied row by row from the same staging tile.
       const bool tma = p.tma_out != 0 && rows_here == 32;
+      const int32_t c_end = (half + 1) * (cols / 2);
 #pragma unroll 1
-      for (int c0 = 0; c0 < cols; c0 += 32) {
+      for (int c0 = half * (cols / 2); c0 < c_end; c0 += 32) {
         uint32_t v[32];
         ptx::tmem_ld_32x32b_x32(lane_addr + c0, v);
         ptx::tmem_ld_wait();
-        if (c0 + 32 == cols) {
+        if (c0 + 32 == c_end) {
           ptx::tc_fence_before();
           __syncwarp();
           if (lane == 0) {       // relaxed: what is handed back is tensor memory, whose reads have completed
@@ -610,53 +618,57 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           x[j + 3] = i8_finish(v[j + 3], sa, s4.w, b4.w);
         }
         i8_activate(x, act);
-        // Staging tile: 32 rows of 128 bytes (64 columns of 16 bits or 32 of 32 bits), 16-byte chunk c of row r at chunk c ^ (r & 7).
-        const int half = f32 ? 0 : (c0 >> 5) & 1;
-        if (half == 0) {
+        // 64 bytes of a row at a time: 32 columns of 16 bits, or twice 16 of 32 bits
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int32_t out_col = col0 + c0 + 16 * h;
+          if (h == 1 && (!f32 || out_col >= p.N)) break;
           if (tma && lane == 0) ptx::bulk_wait_group_read<0>();
           __syncwarp();
-        }
-        if (f32) {
+          uint4 o[4];
+          if (f32) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            *reinterpret_cast<float4*>(stage_buf + lane * 128 + ((q ^ (lane & 7)) * 16)) = make_float4(x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]);
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint4 o;
-            if (out_kind == kOutBf16)
-              o = make_uint4(pack_bf16x2(x[q * 8], x[q * 8 + 1]), pack_bf16x2(x[q * 8 + 2], x[q * 8 + 3]), pack_bf16x2(x[q * 8 + 4], x[q * 8 + 5]), pack_bf16x2(x[q * 8 + 6], x[q * 8 + 7]));
-            else
-              o = make_uint4(pack_f16x2(x[q * 8], x[q * 8 + 1]), pack_f16x2(x[q * 8 + 2], x[q * 8 + 3]), pack_f16x2(x[q * 8 + 4], x[q * 8 + 5]), pack_f16x2(x[q * 8 + 6], x[q * 8 + 7]));
-            *reinterpret_cast<uint4*>(stage_buf + lane * 128 + (((half * 4 + q) ^ (lane & 7)) * 16)) = o;
-          }
-        }
-        // 16-bit output: the tile is full after two steps, or at the last columns of the matrix
-        const bool full = f32 || half == 1 || col0 + c0 + 32 >= p.N;
-        if (!full) continue;
-        const int32_t out_col = col0 + c0 - 32 * half;
-        if (tma && (p.tma_edge || out_col + (f32 ? 32 : 64) <= p.N)) {
-          ptx::fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) {
-            ptx::tma_store_3d(&tmD, ptx::smem_u32(stage_buf), out_col, warp_row0, 0);
-            ptx::bulk_commit_group();
-          }
-        } else {
-          __syncwarp();
-          const int32_t left = min(f32 ? 32 : 64, p.N - out_col);
-          for (int r = 0; r < rows_here; ++r) {
-            const uint8_t* srow = stage_buf + r * 128;
-            for (int c = lane; c < left; c += 32) {
-              if (f32)
-                reinterpret_cast<float*>(p.D)[int64_t(warp_row0 + r) * p.ldd + out_col + c] =
-                    *reinterpret_cast<const float*>(srow + (((c >> 2) ^ (r & 7)) * 16) + (c & 3) * 4);
-              else
-                reinterpret_cast<uint16_t*>(p.D)[int64_t(warp_row0 + r) * p.ldd + out_col + c] =
-                    *reinterpret_cast<const uint16_t*>(srow + (((c >> 3) ^ (r & 7)) * 16) + (c & 7) * 2);
+            for (int q = 0; q < 4; ++q) {
+              const float* y = x + 16 * h + 4 * q;
+              o[q] = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
             }
+          } else if (out_kind == kOutBf16) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              o[q] = make_uint4(pack_bf16x2(x[q * 8], x[q * 8 + 1]), pack_bf16x2(x[q * 8 + 2], x[q * 8 + 3]), pack_bf16x2(x[q * 8 + 4], x[q * 8 + 5]), pack_bf16x2(x[q * 8 + 6], x[q * 8 + 7]));
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              o[q] = make_uint4(pack_f16x2(x[q * 8], x[q * 8 + 1]), pack_f16x2(x[q * 8 + 2], x[q * 8 + 3]), pack_f16x2(x[q * 8 + 4], x[q * 8 + 5]), pack_f16x2(x[q * 8 + 6], x[q * 8 + 7]));
           }
-          __syncwarp();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(stage_buf + lane * 64 + ((q ^ swizzle) * 16)) = o[q];
+          const int32_t width = f32 ? 16 : 32;
+          if (tma && (p.tma_edge || out_col + width <= p.N)) {
+            ptx::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+              ptx::tma_store_3d(&tmD, ptx::smem_u32(stage_buf), out_col, warp_row0, 0);
+              ptx::bulk_commit_group();
+            }
+          } else {
+            __syncwarp();
+            const int32_t left = min(width, p.N - out_col);
+            if (f32) {      // two rows of 16 columns per step
+              const int c = lane & 15;
+              for (int r = lane >> 4; r < rows_here; r += 2) {
+                if (c < left)
+                  reinterpret_cast<float*>(p.D)[int64_t(warp_row0 + r) * p.ldd + out_col + c] =
+                      *reinterpret_cast<const float*>(stage_buf + r * 64 + (((c >> 2) ^ ((r >> 1) & 3)) * 16) + (c & 3) * 4);
+              }
+            } else if (lane < left) {
+#pragma unroll 4
+              for (int r = 0; r < rows_here; ++r)
+                reinterpret_cast<uint16_t*>(p.D)[int64_t(warp_row0 + r) * p.ldd + out_col + lane] =
+                    *reinterpret_cast<const uint16_t*>(stage_buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16) + (lane & 7) * 2);
+            }
+            __syncwarp();
+          }
         }
       }
     }
