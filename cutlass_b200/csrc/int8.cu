@@ -35,18 +35,19 @@ struct I8Plan {
 };
 
 // Kernel, tile and split, by a model of the time.  A CTA (or pair) streams its part of K through a pipeline that is bound by the
-// latency of a TMA round trip, so a k-tile of 128 values takes a time that depends on the tile alone; two CTAs of the kernel
-// for few rows are resident on an SM, one pair of the other kernel on two SMs; a grid runs in whole waves.  The constants were
-// fitted to 60 problems from 16 x 512 x 512 to 777 x 14336 x 8192 (rows x N x K), where the choice is within 10 % of the best
-// of all variants in all but six: e.g. 777 x 5000 x 8192: 128-token tiles 34.5 us, 64-token tiles 43.7, 256 x 128 44.5,
-// 256 x 256 48.8; 256 x 5000 x 8192: 256 x 128 20.7 us, 64-token tiles 25.2, 256 x 256 27.2, 128-token tiles 30.7.
+// latency of a TMA round trip, so a k-tile of 128 values takes a time that depends on the tile alone, and a tile takes at least
+// as long as its epilogue; two CTAs of the kernel for few rows are resident on an SM, one pair of the other kernel on two SMs; a
+// grid runs in whole waves.  The constants were fitted to 80 problems from 16 x 512 x 512 to 5000 x 14336 x 8192 (rows x N x K).
+// Both sides of some choices: 777 x 5000 x 8192: 128-token tiles 34.3 us, 256 x 256 40.4, 64-token tiles 43.9; 2000 x 5000 x
+// 8192: 256 x 256 60.3, 256 x 128 68.8, 128-token tiles 78.8; 777 x 512 x 512: 32-token tiles 4.6, 16 4.9, 64 6.2, 128 8.1.  Over
+// 45 other problems, drawn at random, the choice took 1.03 times the time of the best variant in the geometric mean, 1.14 at most.
 struct Variant {
   bool few;
   int32_t tile;
-  double per_k_tile, fixed;      // microseconds
+  double per_k_tile, least, fixed;      // microseconds: of a k-tile, of a tile's epilogue, of the launch
 };
-constexpr Variant kVariants[] = {{true, 16, 0.20, 4.5}, {true, 32, 0.235, 4.5}, {true, 64, 0.29, 4.6}, {true, 128, 0.40, 4.8},
-                                 {false, 128, 0.19, 7.0}, {false, 256, 0.30, 8.0}};
+constexpr Variant kVariants[] = {{true, 16, 0.20, 1.3, 4.0}, {true, 32, 0.24, 1.6, 3.7}, {true, 64, 0.31, 2.8, 4.6}, {true, 128, 0.45, 5.0, 6.0},
+                                 {false, 128, 0.225, 2.4, 5.5}, {false, 256, 0.33, 3.7, 6.8}};
 constexpr double kHbmBytesPerUs = 6.5e6;
 
 int32_t choose(const bsg_int8_args& a, I8Plan* plan) {
@@ -72,7 +73,9 @@ int32_t choose(const bsg_int8_args& a, I8Plan* plan) {
       double waves = double(int64_t(tiles * split / slots));
       const double tail = tiles * split - waves * slots;
       if (tail > 0.0) waves += !v.few && v.tile == 256 && waves > 0.0 && 2.0 * tail <= slots ? 0.6 : 1.0;      // a thin last wave is split
-      double t = waves * double((k_tiles + split - 1) / split) * v.per_k_tile;
+      double tile_time = double((k_tiles + split - 1) / split) * v.per_k_tile;
+      if (waves > 1.0 && tile_time < v.least) tile_time = v.least;      // (the first tile's epilogue is in `fixed`)
+      double t = waves * tile_time;
       if (t < weights) t = weights;
       t += v.fixed + (split > 1 ? 0.8 + 0.02 * v.tile : 0.0);      // the cluster's barrier and the exchange of partial sums
       if (t < best) {
