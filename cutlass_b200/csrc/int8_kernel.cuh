@@ -385,7 +385,7 @@ __device__ __forceinline__ I8Tile i8_decode(const I8Ctl* ctl, const I8GemmParams
 
 // The bias is 0 where there is none: adding it then changes nothing (a sum of -0 becomes +0).
 __device__ __forceinline__ float i8_finish(uint32_t acc, float sa, float sb, float bias) {
-  return __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(int32_t(acc)), sa), sb), bias);
+  return __fmaf_rn(__fmul_rn(__int2float_rn(int32_t(acc)), sa), sb, bias);
 }
 // Activation of a register tile, behind one branch and in a loop that is not unrolled: inlined at every value, its code was
 // larger than the instruction caches and a 256-column epilogue took 28 us instead of 2.
@@ -567,23 +567,39 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     const int out_kind = p.out_kind, act = p.activation;
     const bool f32 = out_kind == kOutF32, has_bias = p.bias != nullptr;
     const int swizzle = (lane >> 1) & 3;                         // staging: 16-byte chunk c of row r at chunk c ^ ((r >> 1) & 3)
-    int32_t it = 0;
-    for (int32_t t = cluster_idx; t < total_work; t += num_clusters, ++it) {
+    // What a tile needs besides its sums: its place, the scale and the bias of one of its columns per thread, the scale of this
+    // lane's row.  Asked for one tile ahead.
+    struct Need { int32_t g, col0, cols, row0, rows; float sb, bias, sa; };
+    auto need_of = [&](int32_t t) {
       const WorkItem wi = decode_work(t, split_from);
       const I8Tile ti = i8_decode(ctl, p, wi.t, C::kTileM);
+      Need n;
+      n.g = ti.g;
+      n.col0 = ti.tn * BN + wi.half * (BN / 2);
+      n.cols = wi.split ? BN / 2 : BN;
+      n.row0 = ti.row0 + int32_t(cta_rank) * 128 + quarter * 32;
+      n.rows = min(32, ti.row_end - n.row0);
+      const int32_t c = n.col0 + epi * 32 + lane;
+      const bool in = epi * 32 + lane < n.cols && c < p.N;
+      n.sb = in ? __ldg(p.sb + int64_t(n.g) * p.N + c) : 0.0f;
+      n.bias = in && has_bias ? __ldg(p.bias + int64_t(n.g) * p.N + c) : 0.0f;
+      n.sa = lane < n.rows ? __ldcg(p.sa + n.row0 + lane) : 0.0f;
+      return n;
+    };
+    static_assert(BN <= 32 * kI8EpiWarps, "one column per thread");
+    int32_t it = 0;
+    Need need{};
+    if (cluster_idx < total_work) need = need_of(cluster_idx);
+    for (int32_t t = cluster_idx; t < total_work; t += num_clusters, ++it) {
       const int acc = it & 1;
-      const int32_t col0 = ti.tn * BN + wi.half * (BN / 2), cols = wi.split ? BN / 2 : BN;
-      // scales and bias of the tile's columns, while its products are still being summed
+      const int32_t col0 = need.col0, cols = need.cols, warp_row0 = need.row0, rows_here = need.rows;
+      const float sa = need.sa;
       float* cs = sCol + acc * 2 * BN;
-      for (int c = epi * 32 + lane; c < cols; c += 32 * kI8EpiWarps) {
-        const bool in = col0 + c < p.N;
-        const int64_t at = int64_t(ti.g) * p.N + col0 + c;
-        cs[c] = in ? __ldg(p.sb + at) : 0.0f;
-        cs[BN + c] = in && has_bias ? __ldg(p.bias + at) : 0.0f;
+      if (epi * 32 + lane < cols) {
+        cs[epi * 32 + lane] = need.sb;
+        cs[BN + epi * 32 + lane] = need.bias;
       }
-      const int32_t warp_row0 = ti.row0 + int32_t(cta_rank) * 128 + quarter * 32;
-      const int32_t rows_here = min(32, ti.row_end - warp_row0);
-      const float sa = lane < rows_here ? __ldcg(p.sa + warp_row0 + lane) : 0.0f;
+      if (t + num_clusters < total_work) need = need_of(t + num_clusters);
       asm volatile("bar.sync 1, 256;" ::: "memory");
       i8_wait(tfull0 + acc * 8, uint32_t(it >> 1) & 1u, ctl, dead);
       __syncwarp();
