@@ -906,11 +906,8 @@ int32_t host_operand_map(CUtensorMap* map, const void* base, uint64_t row_bytes,
                          uint64_t batch_stride_bytes, uint32_t box_rows) {
   return make_operand_map(map, base, row_bytes, rows, batches, pitch_bytes, batch_stride_bytes, box_rows);
 }
-int32_t host_out64_map(CUtensorMap* map, const void* base, int32_t out_kind, uint64_t cols, uint64_t rows, uint64_t pitch_elems) {
-  const int type = out_kind == BSG_OUT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : out_kind == BSG_OUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const uint64_t size = out_kind == BSG_OUT_F32 ? 4 : 2;
-  return g_maps.get(make_key(base, type, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, cols, rows, 1, pitch_elems * size,
-                             rows * pitch_elems * size, uint32_t(64 / size), 32, 1), map);
+int32_t host_out_map(CUtensorMap* map, const void* base, int32_t out_kind, uint64_t cols, uint64_t rows, uint64_t pitch_elems) {
+  return make_out_map(map, base, out_kind, cols, rows, 1, pitch_elems, rows * pitch_elems);
 }
 int32_t host_device(int32_t not_sm100, int32_t cuda_error, int* dev, int* sms) {
   static std::mutex mu;

@@ -13,8 +13,8 @@ BSG_HIDDEN int32_t host_fail(int32_t code, const char* fmt, ...);
 // Tensor map of K-major byte matrices (batches x rows x row_bytes), box = 128 bytes x box_rows, 128-byte swizzle.
 BSG_HIDDEN int32_t host_operand_map(CUtensorMap* map, const void* base, uint64_t row_bytes, uint64_t rows, uint64_t batches,
                                     uint64_t pitch_bytes, uint64_t batch_stride_bytes, uint32_t box_rows);
-// Tensor map of a row-major bf16, fp16 or fp32 output matrix, box = 32 rows x 64 bytes, 64-byte swizzle.
-BSG_HIDDEN int32_t host_out64_map(CUtensorMap* map, const void* base, int32_t out_kind, uint64_t cols, uint64_t rows, uint64_t pitch_elems);
+// Tensor map of a row-major bf16, fp16 or fp32 output matrix, box = 32 rows x 128 bytes, 128-byte swizzle.
+BSG_HIDDEN int32_t host_out_map(CUtensorMap* map, const void* base, int32_t out_kind, uint64_t cols, uint64_t rows, uint64_t pitch_elems);
 
 inline bool host_aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 

@@ -40,14 +40,14 @@ struct I8Plan {
 // grid runs in whole waves.  The constants were fitted to 80 problems from 16 x 512 x 512 to 5000 x 14336 x 8192 (rows x N x K).
 // Both sides of some choices: 777 x 5000 x 8192: 128-token tiles 34.3 us, 256 x 256 40.4, 64-token tiles 43.9; 2000 x 5000 x
 // 8192: 256 x 256 60.3, 256 x 128 68.8, 128-token tiles 78.8; 777 x 512 x 512: 32-token tiles 4.6, 16 4.9, 64 6.2, 128 8.1.  Over
-// 45 other problems, drawn at random, the choice took 1.03 times the time of the best variant in the geometric mean, 1.14 at most.
+// 85 other problems, drawn at random, the choice took 1.04 times the time of the best variant in the geometric mean, 1.21 at most.
 struct Variant {
   bool few;
   int32_t tile;
   double per_k_tile, least, fixed;      // microseconds: of a k-tile, of a tile's epilogue, of the launch
 };
-constexpr Variant kVariants[] = {{true, 16, 0.20, 1.3, 4.0}, {true, 32, 0.24, 1.6, 3.7}, {true, 64, 0.31, 2.8, 4.6}, {true, 128, 0.45, 5.0, 6.0},
-                                 {false, 128, 0.225, 2.4, 5.5}, {false, 256, 0.33, 3.7, 6.8}};
+constexpr Variant kVariants[] = {{true, 16, 0.20, 1.3, 3.6}, {true, 32, 0.24, 1.6, 3.8}, {true, 64, 0.31, 2.8, 4.6}, {true, 128, 0.45, 5.0, 6.0},
+                                 {false, 128, 0.225, 2.2, 5.5}, {false, 256, 0.33, 3.3, 6.8}};
 constexpr double kHbmBytesPerUs = 6.5e6;
 
 int32_t choose(const bsg_int8_args& a, I8Plan* plan) {
@@ -68,7 +68,7 @@ int32_t choose(const bsg_int8_args& a, I8Plan* plan) {
     const double tiles = tiles_m * double((a.N + tile_n - 1) / tile_n);
     for (int split = 1; split <= 8; split *= 2) {
       if (split > 1 && (!v.few || v.tile > 64 || a.offsets || split > k_tiles)) break;
-      if (a.split ? a.split != split : split > 1 && (tiles * split > 296 || k_tiles < split * 2)) continue;
+      if (a.split ? a.split != split : split > 1 && (tiles * split > 296 || k_tiles < split)) continue;
       const double slots = v.few ? 296.0 : 74.0;
       double waves = double(int64_t(tiles * split / slots));
       const double tail = tiles * split - waves * slots;
@@ -193,7 +193,7 @@ int32_t launch_rows(const bsg_int8_args& a, bsg::I8GemmParams& p, cudaStream_t s
   p.tma_out = host_aligned(a.D, 16) && (a.ldd * esz) % 16 == 0;
   p.tma_edge = (a.N * esz) % 16 == 0;
   tmD = tmA;
-  if (p.tma_out && (rc = bsg::host_out64_map(&tmD, a.D, a.out_kind, a.N, a.rows, a.ldd)) != BSG_OK) return rc;
+  if (p.tma_out && (rc = bsg::host_out_map(&tmD, a.D, a.out_kind, a.N, a.rows, a.ldd)) != BSG_OK) return rc;
   p.tiles_n = int32_t((a.N + BN - 1) / BN);
   p.band = 16;
   int64_t clusters = sms / CG;

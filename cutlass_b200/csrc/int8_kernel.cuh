@@ -407,6 +407,8 @@ __device__ __forceinline__ void i8_activate(float (&x)[N], int act) {
 // ---- many rows: D tile = (128 * CG rows) x BN columns, persistent, two accumulators of BN columns in tensor memory.
 // Eight epilogue warps, two for every quarter of the rows with half of the columns each: with four, a tile took 6 us to finish
 // (latencies of tensor-memory loads, conversions and staged stores, one after the other), more than its products up to K = 2500.
+// The staging of eight warps leaves room for five stages of 256 columns: 2 % slower than six at K = 4096, 8 % faster at K = 512
+// than six with half of the staging.
 constexpr int kI8EpiWarps = 8;
 constexpr int kI8RowsThreads = 32 * (2 + kI8EpiWarps);      // warps 0-3 and 6-9 epilogue, 4 MMA, 5 TMA
 template <int CG, int BN>
@@ -416,7 +418,7 @@ struct I8RowsCfg {
   static constexpr int kBRows = BN / CG;
   static constexpr int kBBytes = kBRows * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kEpiBytes = kI8EpiWarps * 2048;    // per warp 32 rows of 64 bytes
+  static constexpr int kEpiBytes = kI8EpiWarps * 4096;    // per warp 32 rows of 128 bytes
   static constexpr int kColBytes = 2 * 2 * BN * 4;        // scale and bias of the tile's columns, two tiles
   static constexpr int kStagesRaw = (232448 - 1024 - kI8CtlBytes - kEpiBytes - kColBytes) / kStageBytes;
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
@@ -563,10 +565,9 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     const int quarter = warp & 3, half = warp >= 6 ? 1 : 0;      // (a warp reaches the tensor-memory lanes of its number mod 4)
     const int epi = half * 4 + quarter;
     const uint32_t tfull0 = ptx::smem_u32(&ctl->tmem_full[0]), tempty0 = ptx::smem_u32(&ctl->tmem_empty[0]);
-    uint8_t* stage_buf = sEpi + epi * 2048;
+    uint8_t* stage_buf = sEpi + epi * 4096;
     const int out_kind = p.out_kind, act = p.activation;
     const bool f32 = out_kind == kOutF32, has_bias = p.bias != nullptr;
-    const int swizzle = (lane >> 1) & 3;                         // staging: 16-byte chunk c of row r at chunk c ^ ((r >> 1) & 3)
     // What a tile needs besides its sums: its place, the scale and the bias of one of its columns per thread, the scale of this
     // lane's row.  Asked for one tile ahead.
     struct Need { int32_t g, col0, cols, row0, rows; float sb, bias, sa; };
@@ -634,57 +635,54 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           x[j + 3] = i8_finish(v[j + 3], sa, s4.w, b4.w);
         }
         i8_activate(x, act);
-        // 64 bytes of a row at a time: 32 columns of 16 bits, or twice 16 of 32 bits
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int32_t out_col = col0 + c0 + 16 * h;
-          if (h == 1 && (!f32 || out_col >= p.N)) break;
+        // 128 bytes of a row at a time: 32 columns of 32 bits, or two steps of 32 columns of 16 bits (TMA moves a row of a box in
+        // about seven cycles, whatever its length).  Staging: 16-byte piece c of row r at piece c ^ (r & 7).
+        const int second = f32 ? 0 : (c0 >> 5) & 1;
+        if (second == 0) {
           if (tma && lane == 0) ptx::bulk_wait_group_read<0>();
           __syncwarp();
-          uint4 o[4];
-          if (f32) {
+        }
+        if (f32) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float* y = x + 16 * h + 4 * q;
-              o[q] = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
-            }
-          } else if (out_kind == kOutBf16) {
+          for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<float4*>(stage_buf + lane * 128 + ((q ^ (lane & 7)) * 16)) = make_float4(x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]);
+        } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              o[q] = make_uint4(pack_bf16x2(x[q * 8], x[q * 8 + 1]), pack_bf16x2(x[q * 8 + 2], x[q * 8 + 3]), pack_bf16x2(x[q * 8 + 4], x[q * 8 + 5]), pack_bf16x2(x[q * 8 + 6], x[q * 8 + 7]));
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              o[q] = make_uint4(pack_f16x2(x[q * 8], x[q * 8 + 1]), pack_f16x2(x[q * 8 + 2], x[q * 8 + 3]), pack_f16x2(x[q * 8 + 4], x[q * 8 + 5]), pack_f16x2(x[q * 8 + 6], x[q * 8 + 7]));
+          for (int q = 0; q < 4; ++q) {
+            uint4 o;
+            if (out_kind == kOutBf16)
+              o = make_uint4(pack_bf16x2(x[q * 8], x[q * 8 + 1]), pack_bf16x2(x[q * 8 + 2], x[q * 8 + 3]), pack_bf16x2(x[q * 8 + 4], x[q * 8 + 5]), pack_bf16x2(x[q * 8 + 6], x[q * 8 + 7]));
+            else
+              o = make_uint4(pack_f16x2(x[q * 8], x[q * 8 + 1]), pack_f16x2(x[q * 8 + 2], x[q * 8 + 3]), pack_f16x2(x[q * 8 + 4], x[q * 8 + 5]), pack_f16x2(x[q * 8 + 6], x[q * 8 + 7]));
+            *reinterpret_cast<uint4*>(stage_buf + lane * 128 + (((second * 4 + q) ^ (lane & 7)) * 16)) = o;
           }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(stage_buf + lane * 64 + ((q ^ swizzle) * 16)) = o[q];
-          const int32_t width = f32 ? 16 : 32;
-          if (tma && (p.tma_edge || out_col + width <= p.N)) {
-            ptx::fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-              ptx::tma_store_3d(&tmD, ptx::smem_u32(stage_buf), out_col, warp_row0, 0);
-              ptx::bulk_commit_group();
-            }
-          } else {
-            __syncwarp();
-            const int32_t left = min(width, p.N - out_col);
-            if (f32) {      // two rows of 16 columns per step
-              const int c = lane & 15;
-              for (int r = lane >> 4; r < rows_here; r += 2) {
-                if (c < left)
-                  reinterpret_cast<float*>(p.D)[int64_t(warp_row0 + r) * p.ldd + out_col + c] =
-                      *reinterpret_cast<const float*>(stage_buf + r * 64 + (((c >> 2) ^ ((r >> 1) & 3)) * 16) + (c & 3) * 4);
-              }
-            } else if (lane < left) {
+        }
+        if (!f32 && second == 0 && col0 + c0 + 32 < p.N) continue;      // the tile fills up in the next step
+        const int32_t out_col = col0 + c0 - 32 * second, width = f32 ? 32 : 64;
+        if (tma && (p.tma_edge || out_col + width <= p.N)) {
+          ptx::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) {
+            ptx::tma_store_3d(&tmD, ptx::smem_u32(stage_buf), out_col, warp_row0, 0);
+            ptx::bulk_commit_group();
+          }
+        } else {
+          __syncwarp();
+          const int32_t left = min(width, p.N - out_col);
+          for (int c = lane; c < left; c += 32) {
+            if (f32) {
 #pragma unroll 4
               for (int r = 0; r < rows_here; ++r)
-                reinterpret_cast<uint16_t*>(p.D)[int64_t(warp_row0 + r) * p.ldd + out_col + lane] =
-                    *reinterpret_cast<const uint16_t*>(stage_buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16) + (lane & 7) * 2);
+                reinterpret_cast<float*>(p.D)[int64_t(warp_row0 + r) * p.ldd + out_col + c] =
+                    *reinterpret_cast<const float*>(stage_buf + r * 128 + (((c >> 2) ^ (r & 7)) * 16) + (c & 3) * 4);
+            } else {      // (32-bit words, shifted for rows that start on an odd column, took 1.7 times as long)
+#pragma unroll 4
+              for (int r = 0; r < rows_here; ++r)
+                reinterpret_cast<uint16_t*>(p.D)[int64_t(warp_row0 + r) * p.ldd + out_col + c] =
+                    *reinterpret_cast<const uint16_t*>(stage_buf + r * 128 + (((c >> 3) ^ (r & 7)) * 16) + (c & 7) * 2);
             }
-            __syncwarp();
           }
+          __syncwarp();
         }
       }
     }
