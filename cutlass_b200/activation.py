@@ -55,12 +55,17 @@ def checkpoint_activation(x, activation: str = "silu", *, gated: bool = True, ou
     itself, and the ``ActivationCheckpoint`` that ``checkpoint_activation_backward`` takes.  ``x`` is (T, 2F) or (T, F) bf16 /
     fp16; ``activation``: "identity", "relu", "gelu" (erf form) or "silu"; ``out`` (T, F) may be given.  A block of 128 values
     with a NaN or an infinity is kept as NaN.  Asynchronous on ``stream`` (None: torch's current stream)."""
+    gated = bool(gated)
+    if out is None and stream is None and x.is_cuda:
+        done = L.binding().act_forward(x, ACTIVATIONS.get(activation, -1), gated)
+        if done is not None:
+            h, data, T, F = done
+            return h, ActivationCheckpoint(data, activation, gated, T, F, x.dtype)
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r}: one of {sorted(ACTIVATIONS)}")
     kind, device, T, cols, ldx = _matrix("x", x, _IN_KINDS)
     _no_gradient("checkpoint_activation", x)
-    gated = bool(gated)
     if gated and cols % 2 != 0:
         raise ValueError(f"a gated activation needs an even number of columns (gate | up), got {cols}")
     parts, F = (2, cols // 2) if gated else (1, cols)
@@ -81,6 +86,10 @@ def checkpoint_activation(x, activation: str = "silu", *, gated: bool = True, ou
 def checkpoint_activation_backward(grad, kept: ActivationCheckpoint, *, out=None, stream=None) -> torch.Tensor:
     """Gradient of ``x`` for the gradient ``grad`` (T, F) of ``h``, from what ``checkpoint_activation`` kept: (T, 2F) or (T, F)
     in the type of ``x``.  ``out`` may be given.  Asynchronous on ``stream`` (None: torch's current stream)."""
+    if out is None and stream is None and grad.is_cuda:
+        dx = L.binding().act_backward(grad, kept.data, ACTIVATIONS[kept.activation], kept.gated, kept.rows, kept.width, kept.dtype)
+        if dx is not None:
+            return dx
     data, T, F, parts = kept.data, kept.rows, kept.width, 2 if kept.gated else 1
     kind, device, q = _IN_KINDS[kept.dtype], data.get_device(), data.data_ptr()
     ldg = _given("grad", grad, kind, device, T, F)

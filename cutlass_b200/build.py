@@ -19,6 +19,7 @@ def lib_name(profile: bool) -> str:
 
 
 OUT = os.path.join(_HERE, "lib", lib_name(PROFILE))
+BINDING = os.path.join(_HERE, "lib", "_binding.so")
 SOURCES = {      # translation unit -> the headers it includes
     "bsgemm.cu": ["gemm_kernel.cuh", "quant_kernel.cuh", "ptx.cuh", "host.h"],
     "int8.cu": ["int8_kernel.cuh", "gemm_kernel.cuh", "ptx.cuh", "host.h"],
@@ -57,17 +58,39 @@ def _nvcc(args: list[str]) -> str:
     return proc.stderr
 
 
+def _build_binding(force: bool) -> None:
+    """The Python module of csrc/binding.cpp (host code; needs torch's headers)."""
+    src = os.path.join(CSRC, "binding.cpp")
+    if not force and os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in (src, os.path.join(CSRC, ABI_HEADER))):
+        return
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem" + os.path.join(root, "include"), "-isystem" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-isystem" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], src, "-o", BINDING,
+           "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError("the compiler failed:\n" + proc.stdout + proc.stderr)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the CUDA library if it is missing or older than its sources; return its path.  Translation units are
-    compiled side by side, and only those whose sources changed."""
+    """Compile the CUDA library, and the Python binding of its short calls, if they are missing or older than their sources;
+    return the library's path.  Translation units are compiled side by side, and only those whose sources changed."""
+    os.makedirs(os.path.dirname(OUT), exist_ok=True)
     if not force and not _stale():
+        _build_binding(False)
         return OUT
     units = _objects()
-    os.makedirs(os.path.dirname(OUT), exist_ok=True)
     os.makedirs(os.path.join(_HERE, "build"), exist_ok=True)
     extra = (["-DBSG_PROFILE"] if PROFILE else []) + (["-Xptxas", "-v"] if verbose else [])
     with ThreadPoolExecutor() as pool:
+        binding = pool.submit(_build_binding, force)
         logs = list(pool.map(lambda u: _nvcc(extra + ["-c", "-o", u[1], u[0]]), [u for u in units if force or u[2]]))
+        binding.result()
     _nvcc(["--shared", "-o", OUT] + [u[1] for u in units])
     if verbose:
         sys.stderr.write("".join(logs))

@@ -1,0 +1,289 @@
+// Python calls of the operators whose kernels take a few microseconds, without the interpreter's share of the work: a call
+// through ctypes with its checks in Python takes 10 to 15 microseconds of host time, which such kernels do not hide.
+//
+// Every function here either makes the whole call (checks, outputs, launch on torch's current stream) and returns its
+// results, or returns None without having done anything: for whatever is not the plain case -- wrong types and shapes, other
+// devices than the current one, tensors that want a gradient -- the caller goes on in Python, which says what is wrong or does
+// it step by step.  The library's C entry points are handed over by address (bind), so that there is one copy of the library.
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <exception>
+
+#include "../../include/bsgemm.h"
+
+namespace {
+
+struct {
+  decltype(&bsg_int8_linear_run) int8_linear_run;
+  decltype(&bsg_int8_scratch_rows) int8_scratch_rows;
+  decltype(&bsg_act_forward) act_forward;
+  decltype(&bsg_act_backward) act_backward;
+  decltype(&bsg_route_forward) route_forward;
+  decltype(&bsg_route_backward) route_backward;
+  decltype(&bsg_route_scratch_size) route_scratch_size;
+  decltype(&bsg_last_error_string) last_error_string;
+} g;
+PyObject* g_raise = nullptr;      // called with the status code of a call that failed
+
+constexpr int64_t kMaxExperts = 1024, kMaxTopK = 32;
+
+int kind_of(at::ScalarType t, bool with_f32) {
+  if (t == at::kBFloat16) return BSG_OUT_BF16;
+  if (t == at::kHalf) return BSG_OUT_F16;
+  return with_f32 && t == at::kFloat ? BSG_OUT_F32 : -1;
+}
+
+// The tensor of an argument that is a plain torch.Tensor (or Parameter) on CUDA device `device`; null otherwise.
+const at::Tensor* tensor(PyObject* o) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  return t.defined() && t.layout() == at::kStrided && t.is_cuda() && !t.is_neg() ? &t : nullptr;
+}
+const at::Tensor* array(PyObject* o, at::ScalarType type, at::IntArrayRef shape, int device) {
+  const at::Tensor* t = tensor(o);
+  return t && t->scalar_type() == type && t->get_device() == device && t->sizes() == shape && t->is_contiguous() ? t : nullptr;
+}
+struct Matrix {
+  const at::Tensor* t;
+  int kind, device;
+  int64_t rows, cols, pitch;
+};
+bool matrix(PyObject* o, bool with_f32, Matrix* m) {
+  m->t = tensor(o);
+  if (!m->t || m->t->dim() != 2) return false;
+  m->kind = kind_of(m->t->scalar_type(), with_f32);
+  m->device = m->t->get_device();
+  m->rows = m->t->size(0);
+  m->cols = m->t->size(1);
+  m->pitch = m->rows > 1 ? m->t->stride(0) : m->cols;
+  return m->kind >= 0 && m->device == c10::cuda::current_device() && m->cols >= 1 && (m->cols == 1 || m->t->stride(1) == 1) && m->pitch >= m->cols;
+}
+bool wants_gradient(const at::Tensor* t) { return t && t->requires_grad() && at::GradMode::is_enabled(); }
+
+at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) { return at::empty(shape, at::TensorOptions().dtype(type).device(like.device())); }
+
+// Part of a buffer as a tensor of its own (contiguous, `offset` in elements of `type`); not a view for autograd.
+at::Tensor part(const at::Tensor& buffer, at::ScalarType type, int64_t offset, at::IntArrayRef shape) {
+  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), c10::scalarTypeToTypeMeta(type));
+  impl->set_storage_offset(offset);
+  impl->set_sizes_contiguous(shape);
+  return at::Tensor(std::move(impl));
+}
+
+void* current_stream(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
+
+PyObject* failed(int32_t code) { return PyObject_CallFunction(g_raise, "i", int(code)); }      // raises
+
+template <class F>
+PyObject* guarded(F body) {
+  try {
+    return body();
+  } catch (const c10::OutOfMemoryError& e) {
+    PyErr_SetString(PyExc_MemoryError, e.what_without_backtrace());
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+  }
+  return nullptr;
+}
+
+// int8_linear(x, weight, weight_scale, bias, activation, offsets, rows, out_dtype, status) -> y
+PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Matrix x;
+    if (n != 9 || !matrix(a[0], false, &x)) Py_RETURN_NONE;
+    const int dev = x.device;
+    const bool grouped = a[5] != Py_None;
+    const at::Tensor *w = tensor(a[1]), *status = tensor(a[8]);
+    if (!w || !status || w->scalar_type() != at::kChar || w->get_device() != dev || w->dim() != (grouped ? 3 : 2)) Py_RETURN_NONE;
+    const int64_t K = x.cols, N = w->size(-2), groups = grouped ? w->size(0) : 1, pitch = (K + 15) & ~int64_t(15);
+    const int64_t ldw = N > 1 ? w->stride(-2) : pitch, group_stride = groups > 1 ? w->stride(0) : 0;
+    if (w->size(-1) != K || N < 1 || groups < 1 || groups > BSG_MAX_GROUPS || (K > 1 && w->stride(-1) != 1) || ldw < K || ((ldw | group_stride) & 15) != 0 || K > 131071 ||
+        (reinterpret_cast<uintptr_t>(w->const_data_ptr()) & 15) != 0)
+      Py_RETURN_NONE;
+    const auto per_channel = w->sizes().slice(0, grouped ? 2 : 1);
+    const at::Tensor* ws = array(a[2], at::kFloat, per_channel, dev);
+    const at::Tensor* bias = a[3] == Py_None ? nullptr : array(a[3], at::kFloat, per_channel, dev);
+    const at::Tensor* offsets = grouped ? array(a[5], at::kInt, w->sizes().slice(0, 1), dev) : nullptr;
+    const at::Tensor* rows = a[6] == Py_None ? nullptr : tensor(a[6]);
+    if (!ws || (a[3] != Py_None && !bias) || (grouped && !offsets)) Py_RETURN_NONE;
+    if (a[6] != Py_None && (!grouped || !rows || rows->scalar_type() != at::kInt || rows->dim() != 1 || rows->get_device() != dev || !rows->is_contiguous())) Py_RETURN_NONE;
+    if (wants_gradient(x.t) || wants_gradient(ws) || wants_gradient(bias)) Py_RETURN_NONE;
+    at::ScalarType out_type = x.t->scalar_type();
+    if (a[7] != Py_None) {
+      if (!THPDtype_Check(a[7])) Py_RETURN_NONE;
+      out_type = reinterpret_cast<THPDtype*>(a[7])->scalar_type;
+    }
+    const int out_kind = kind_of(out_type, true);
+    const long act = PyLong_AsLong(a[4]);
+    const int64_t R = rows ? rows->size(0) : x.rows;
+    if (out_kind < 0 || act < BSG_ACT_IDENTITY || act > BSG_ACT_SILU || R == 0) Py_RETURN_NONE;
+    bsg_int8_args c{};
+    c.in_kind = x.kind; c.out_kind = out_kind; c.num_groups = int32_t(groups); c.activation = int32_t(act);
+    c.rows = R; c.tokens = x.rows; c.N = N; c.K = K;
+    c.X = x.t->const_data_ptr(); c.ldx = x.pitch; c.index = rows ? rows->const_data_ptr<int32_t>() : nullptr; c.ldq = pitch;
+    c.W = w->const_data_ptr(); c.ldw = ldw; c.group_stride_w = group_stride; c.w_scale = ws->const_data_ptr<float>();
+    c.bias = bias ? bias->const_data_ptr<float>() : nullptr; c.offsets = offsets ? offsets->const_data_ptr<int32_t>() : nullptr;
+    c.ldd = N;
+    at::Tensor scratch;
+    if (grouped || R > 4 || (R <= 2 ? R : 4) * pitch > 65536) {      // else the tokens are quantised inside the product's kernel
+      int64_t held = R;
+      if (rows && g.int8_scratch_rows(&c, &held) != BSG_OK) Py_RETURN_NONE;
+      scratch = empty({held * (pitch + 4)}, at::kChar, *x.t);        // 8-bit tokens, then their scales
+      c.Q = scratch.mutable_data_ptr();
+      c.q_scale = reinterpret_cast<float*>(static_cast<char*>(c.Q) + held * pitch);
+    }
+    at::Tensor y = empty({R, N}, out_type, *x.t);
+    c.D = y.mutable_data_ptr();
+    const int32_t code = g.int8_linear_run(&c, status->mutable_data_ptr(), 16, current_stream(dev));
+    return code ? failed(code) : THPVariable_Wrap(std::move(y));
+  });
+}
+
+// act_forward(x, activation, gated) -> (h, data, rows, width)
+PyObject* act_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Matrix x;
+    if (n != 3 || !matrix(a[0], false, &x) || wants_gradient(x.t)) Py_RETURN_NONE;
+    const long act = PyLong_AsLong(a[1]);
+    const bool gated = a[2] == Py_True;
+    if (act < BSG_ACT_IDENTITY || act > BSG_ACT_SILU || (gated && x.cols % 2 != 0)) Py_RETURN_NONE;
+    const int64_t parts = gated ? 2 : 1, T = x.rows, F = x.cols / parts, split = T * parts * ((F + 15) & ~int64_t(15));
+    at::Tensor data = empty({split + 4 * T * parts * ((F + 127) / 128)}, at::kChar, *x.t);
+    at::Tensor h = empty({T, F}, x.t->scalar_type(), *x.t);
+    bsg_act_args c{};
+    c.type = x.kind; c.activation = int32_t(act); c.gated = gated; c.rows = T; c.width = F;
+    c.in = x.t->const_data_ptr(); c.ld_in = x.pitch; c.out = h.mutable_data_ptr(); c.ld_out = F;
+    c.kept = data.mutable_data_ptr(); c.kept_scale = reinterpret_cast<float*>(static_cast<char*>(c.kept) + split);
+    const int32_t code = g.act_forward(&c, current_stream(x.device));
+    if (code) return failed(code);
+    return Py_BuildValue("(NNLL)", THPVariable_Wrap(std::move(h)), THPVariable_Wrap(std::move(data)), (long long)T, (long long)F);
+  });
+}
+
+// act_backward(grad, data, activation, gated, rows, width, dtype) -> dx
+PyObject* act_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Matrix d;
+    if (n != 7 || !matrix(a[0], false, &d) || wants_gradient(d.t) || !THPDtype_Check(a[6])) Py_RETURN_NONE;
+    const long act = PyLong_AsLong(a[2]);
+    const bool gated = a[3] == Py_True;
+    const int64_t T = PyLong_AsLongLong(a[4]), F = PyLong_AsLongLong(a[5]), parts = gated ? 2 : 1, split = T * parts * ((F + 15) & ~int64_t(15));
+    const at::Tensor* data = array(a[1], at::kChar, {split + 4 * T * parts * ((F + 127) / 128)}, d.device);
+    if (!data || d.rows != T || d.cols != F || reinterpret_cast<THPDtype*>(a[6])->scalar_type != d.t->scalar_type()) Py_RETURN_NONE;
+    at::Tensor dx = empty({T, parts * F}, d.t->scalar_type(), *d.t);
+    bsg_act_args c{};
+    c.type = d.kind; c.activation = int32_t(act); c.gated = gated; c.rows = T; c.width = F;
+    c.in = d.t->const_data_ptr(); c.ld_in = d.pitch; c.out = dx.mutable_data_ptr(); c.ld_out = parts * F;
+    c.kept = const_cast<void*>(data->const_data_ptr());
+    c.kept_scale = reinterpret_cast<float*>(static_cast<char*>(c.kept) + split);
+    const int32_t code = g.act_backward(&c, current_stream(d.device));
+    return code ? failed(code) : THPVariable_Wrap(std::move(dx));
+  });
+}
+
+bool routable(const Matrix& l, int64_t k) { return l.cols <= kMaxExperts && k >= 1 && k <= kMaxTopK && k <= l.cols && l.rows * k <= 0x7FFFFFFFll; }
+
+// route_forward(logits, top_k, token_mask, normalize) -> (experts, weights, counts, offsets, rows, positions, loss, live, softmax)
+PyObject* route_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Matrix l;
+    if (n != 4 || !matrix(a[0], true, &l) || !PyLong_CheckExact(a[1])) Py_RETURN_NONE;
+    const int64_t T = l.rows, E = l.cols, k = PyLong_AsLongLong(a[1]);
+    if (k < 1 || !routable(l, k)) { PyErr_Clear(); Py_RETURN_NONE; }
+    const at::Tensor* mask = a[2] == Py_None ? nullptr : array(a[2], at::kBool, {T}, l.device);
+    if (a[2] != Py_None && !mask) Py_RETURN_NONE;
+    const int64_t slots = T * k;
+    // one allocation: softmax (2 T), experts, rows, positions, weights (slots each), counts, offsets (E each), live, loss
+    at::Tensor all = empty({2 * T + 4 * slots + 2 * E + 2}, at::kInt, *l.t);
+    int32_t* p = static_cast<int32_t*>(all.mutable_data_ptr());
+    int64_t at_ = 0;
+    auto take = [&](int64_t count) { const int64_t o = at_; at_ += count; return o; };
+    const int64_t soft = take(2 * T), experts = take(slots), rows = take(slots), positions = take(slots), weights = take(slots), counts = take(E), offsets = take(E),
+                  live = take(1), loss = take(1);
+    bsg_route_args c{};
+    c.type = l.kind; c.experts = int32_t(E); c.k = int32_t(k); c.normalize = a[3] == Py_True; c.tokens = T;
+    c.logits = l.t->const_data_ptr(); c.ld = l.pitch; c.mask = mask ? static_cast<const uint8_t*>(mask->const_data_ptr()) : nullptr;
+    c.chosen = p + experts; c.weights = reinterpret_cast<float*>(p + weights); c.counts = p + counts; c.live = p + live;
+    c.softmax = reinterpret_cast<float*>(p + soft); c.offsets = p + offsets; c.rows = p + rows; c.positions = p + positions;
+    c.loss = reinterpret_cast<float*>(p + loss);
+    size_t bytes = 0;
+    if (g.route_scratch_size(&c, &bytes) != BSG_OK) Py_RETURN_NONE;
+    at::Tensor scratch;
+    if (bytes) scratch = empty({int64_t(bytes)}, at::kByte, *l.t);
+    const int32_t code = g.route_forward(&c, bytes ? scratch.mutable_data_ptr() : nullptr, bytes, current_stream(l.device));
+    if (code) return failed(code);
+    auto ints = [&](int64_t o, at::IntArrayRef s) { return THPVariable_Wrap(part(all, at::kInt, o, s)); };
+    auto reals = [&](int64_t o, at::IntArrayRef s) { return THPVariable_Wrap(part(all, at::kFloat, o, s)); };
+    return Py_BuildValue("(NNNNNNNNN)", ints(experts, {T, k}), reals(weights, {T, k}), ints(counts, {E}), ints(offsets, {E}), ints(rows, {slots}),
+                         ints(positions, {T, k}), reals(loss, {}), ints(live, {1}), ints(soft, {2 * T}));
+  });
+}
+
+// route_backward(logits, experts, weights, counts, live, softmax, normalize, grad_weights, grad_loss) -> grad_logits
+PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Matrix l;
+    if (n != 9 || !matrix(a[0], true, &l)) Py_RETURN_NONE;
+    const at::Tensor* experts = tensor(a[1]);
+    if (!experts || experts->dim() != 2) Py_RETURN_NONE;
+    const int64_t T = l.rows, E = l.cols, k = experts->size(1);
+    if (!routable(l, k)) Py_RETURN_NONE;
+    experts = array(a[1], at::kInt, {T, k}, l.device);
+    const at::Tensor *weights = array(a[2], at::kFloat, {T, k}, l.device), *counts = array(a[3], at::kInt, {E}, l.device), *live = array(a[4], at::kInt, {1}, l.device),
+                     *soft = array(a[5], at::kInt, {2 * T}, l.device);
+    const at::Tensor* gw = a[7] == Py_None ? nullptr : array(a[7], at::kFloat, {T, k}, l.device);
+    const at::Tensor* gl = a[8] == Py_None ? nullptr : tensor(a[8]);
+    if (!experts || !weights || !counts || !live || !soft || (a[7] != Py_None && !gw)) Py_RETURN_NONE;
+    if (a[8] != Py_None && (!gl || gl->scalar_type() != at::kFloat || gl->numel() != 1 || gl->get_device() != l.device)) Py_RETURN_NONE;
+    at::Tensor d = empty({T, E}, l.t->scalar_type(), *l.t);
+    bsg_route_args c{};
+    c.type = l.kind; c.experts = int32_t(E); c.k = int32_t(k); c.normalize = a[6] == Py_True; c.tokens = T;
+    c.logits = l.t->const_data_ptr(); c.ld = l.pitch;
+    c.chosen = const_cast<int32_t*>(experts->const_data_ptr<int32_t>()); c.weights = const_cast<float*>(weights->const_data_ptr<float>());
+    c.counts = const_cast<int32_t*>(counts->const_data_ptr<int32_t>()); c.live = const_cast<int32_t*>(live->const_data_ptr<int32_t>());
+    c.softmax = reinterpret_cast<float*>(const_cast<int32_t*>(soft->const_data_ptr<int32_t>()));
+    c.grad_weights = gw ? gw->const_data_ptr<float>() : nullptr; c.grad_loss = gl ? gl->const_data_ptr<float>() : nullptr;
+    c.grad_logits = d.mutable_data_ptr(); c.ld_grad = E;
+    const int32_t code = g.route_backward(&c, current_stream(l.device));
+    return code ? failed(code) : THPVariable_Wrap(std::move(d));
+  });
+}
+
+// bind(raise, address, ...): the entry points in the order of `g`.
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  void** slots = reinterpret_cast<void**>(&g);
+  constexpr Py_ssize_t kSlots = Py_ssize_t(sizeof(g) / sizeof(void*));
+  if (n != kSlots + 1) {
+    PyErr_Format(PyExc_TypeError, "bind takes %zd addresses", kSlots);
+    return nullptr;
+  }
+  for (Py_ssize_t i = 0; i < kSlots; ++i) {
+    slots[i] = PyLong_AsVoidPtr(a[i + 1]);
+    if (PyErr_Occurred()) return nullptr;
+  }
+  Py_INCREF(a[0]);
+  g_raise = a[0];
+  Py_RETURN_NONE;
+}
+
+PyMethodDef methods[] = {
+    {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(bind)), METH_FASTCALL, nullptr},
+    {"int8_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(int8_linear)), METH_FASTCALL, nullptr},
+    {"act_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(act_forward)), METH_FASTCALL, nullptr},
+    {"act_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(act_backward)), METH_FASTCALL, nullptr},
+    {"route_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(route_forward)), METH_FASTCALL, nullptr},
+    {"route_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(route_backward)), METH_FASTCALL, nullptr},
+    {nullptr, nullptr, 0, nullptr},
+};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__binding() { return PyModule_Create(&module); }

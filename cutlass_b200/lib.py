@@ -7,6 +7,8 @@ is missing, loading raises.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 import struct
 
@@ -185,6 +187,27 @@ SYMBOLS = {
 
 _lib = None
 _direct: dict = {}
+BINDING_PATH = os.path.join(_HERE, "lib", "_binding.so")
+# What csrc/binding.cpp calls, in the order of its table.
+BOUND = ("bsg_int8_linear_run", "bsg_int8_scratch_rows", "bsg_act_forward", "bsg_act_backward", "bsg_route_forward", "bsg_route_backward",
+         "bsg_route_scratch_size", "bsg_last_error_string")
+_binding = None
+
+
+def binding():
+    """The module of ``csrc/binding.cpp``: whole calls with little host time.  Each of its functions returns None, having done
+    nothing, for a call that is not the plain case; the Python around it then does the work or says what is wrong."""
+    global _binding
+    if _binding is None:
+        if not os.path.exists(BINDING_PATH):
+            raise FileNotFoundError(f"{BINDING_PATH} is missing: build it with `python -m cutlass_b200.build`")
+        lib = load()
+        loader = importlib.machinery.ExtensionFileLoader("_binding", BINDING_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
+        loader.exec_module(module)
+        module.bind(check, *(C.cast(getattr(lib, name), C.c_void_p).value for name in BOUND))
+        _binding = module
+    return _binding
 
 
 def direct(name: str, layout: str):

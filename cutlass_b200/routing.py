@@ -54,6 +54,10 @@ def _check_logits(logits, top_k):
 
 
 def _forward(logits, top_k, token_mask, normalize, stream) -> Routing:
+    if stream is None and logits.is_cuda:
+        done = L.binding().route_forward(logits, top_k, token_mask, bool(normalize))
+        if done is not None:
+            return tuple.__new__(Routing, done + (bool(normalize),))
     kind, device, T, E, ld = _check_logits(logits, top_k)
     if token_mask is not None:
         _check_array("token_mask", token_mask, torch.bool, (T,), device)
@@ -83,6 +87,11 @@ def route_tokens_backward(logits, routing: Routing, grad_weights=None, grad_bala
     """Gradient of ``logits`` (in their type) for the gradients of ``routing.weights`` (T, k) fp32 and ``routing.balance_loss``
     () fp32, either of which may be None (zero).  The counts are constants.  Asynchronous on ``stream`` (None: torch's current
     stream)."""
+    if stream is None and logits.is_cuda:
+        d = L.binding().route_backward(logits, routing.experts, routing.weights, routing.counts, routing.num_tokens, routing.softmax,
+                                       routing.normalize, grad_weights, grad_balance_loss)
+        if d is not None:
+            return d
     experts, counts = routing.experts, routing.counts
     k = experts.shape[1]
     kind, device, T, E, ld = _check_logits(logits, k)

@@ -1,0 +1,77 @@
+"""The binding of the short calls: what is not its plain case it leaves to the Python around it, which says what is wrong; and
+the sizes that both sides compute are the library's."""
+import ctypes as C
+
+import pytest
+import torch
+
+import cutlass_b200 as ops
+from cutlass_b200 import lib as L
+from cutlass_b200.routing import _scratch_words
+
+
+def test_anything_but_cuda_tensors_is_left_alone():
+    b = L.binding()
+    x = torch.zeros((4, 32), dtype=torch.bfloat16)
+    assert b.int8_linear(x, x, x, None, 0, None, None, None, x) is None
+    assert b.act_forward(x, 3, True) is None
+    assert b.act_backward(x, x, 3, True, 4, 16, torch.bfloat16) is None
+    assert b.route_forward(x, 2, None, True) is None
+    assert b.route_backward(x, x, x, x, x, x, True, None, None) is None
+    assert b.act_forward(3, 3, True) is None and b.act_forward(x) is None
+
+
+def test_scratch_of_the_router_is_what_the_library_asks_for():
+    for T in (0, 1, 127, 128, 129, 130, 592 * 16, 592 * 16 + 1, 100000, 1 << 20):
+        for E in (1, 7, 256, 1024):
+            a, size = L.RouteArgs(experts=E, k=1, tokens=T), C.c_size_t()
+            L.check(L.load().bsg_route_scratch_size(C.byref(a), C.byref(size)))
+            assert size.value == 4 * _scratch_words(T, E)
+
+
+def test_the_bound_entry_points_exist():
+    assert set(L.BOUND) <= set(L.SYMBOLS)
+
+
+@pytest.mark.gpu
+def test_both_ways_give_the_same_bits(cuda_lib):
+    """A call with its stream or output given goes through Python; without, through the binding."""
+    stream = torch.cuda.current_stream()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn((50, 130), device="cuda", generator=g).to(torch.bfloat16)
+    w = ops.quantize_int8(torch.randn((70, 130), device="cuda", generator=g).to(torch.bfloat16))
+    W, S = w.quantized.tensor, w.scale.tensor
+    for rows in (50, 3):
+        assert torch.equal(ops.int8_linear(x[:rows], W, S, out_dtype=torch.float32), ops.int8_linear(x[:rows], W, S, out_dtype=torch.float32, stream=stream))
+    index = torch.randint(0, 50, (90,), device="cuda", generator=g, dtype=torch.int32)
+    ends = torch.tensor([30, 90], dtype=torch.int32, device="cuda")
+    W2, S2 = torch.zeros((2, 70, 144), dtype=torch.int8, device="cuda")[..., :130], S.expand(2, 70).contiguous()
+    W2.copy_(W)
+    assert torch.equal(ops.int8_linear(x, W2, S2, offsets=ends, rows=index), ops.int8_linear(x, W2, S2, offsets=ends, rows=index, stream=stream))
+    (h, kept), (h2, kept2) = ops.checkpoint_activation(x), ops.checkpoint_activation(x, stream=stream)
+    assert torch.equal(h, h2) and torch.equal(kept.quantized[..., :65], kept2.quantized[..., :65]) and torch.equal(kept.scale, kept2.scale)
+    assert torch.equal(ops.checkpoint_activation_backward(h, kept), ops.checkpoint_activation_backward(h, kept2, stream=stream))
+    for T in (50, 300):
+        l = torch.randn((T, 33), device="cuda", generator=g)
+        r, r2 = ops.route_tokens(l, 4), ops.route_tokens(l, 4, stream=stream)
+        for a, b in zip(r, r2):
+            assert a is b or torch.equal(a, b)
+        gl = torch.ones((), device="cuda")
+        assert torch.equal(ops.route_tokens_backward(l, r, r.weights, gl), ops.route_tokens_backward(l, r2, r.weights, gl, stream=stream))
+
+
+@pytest.mark.gpu
+def test_results_are_tensors_of_their_own(cuda_lib):
+    """The router's results lie in one buffer: changing one in place neither changes another nor what the backward pass reads."""
+    l = torch.randn((9, 8), device="cuda", requires_grad=True)
+    r = ops.route_tokens(l, 2)
+    keep = [t.clone() for t in (r.experts, r.weights, r.rows, r.positions)]
+    r.offsets.zero_()
+    r.rows.fill_(7)
+    with torch.no_grad():
+        r.balance_loss.add_(1)
+    assert torch.equal(r.experts, keep[0]) and torch.equal(r.weights, keep[1]) and torch.equal(r.positions, keep[3])
+    (r.weights.sum() + r.balance_loss).backward()
+    again = ops.route_tokens(l.detach(), 2)
+    want = ops.route_tokens_backward(l.detach(), again, torch.ones_like(again.weights), torch.ones((), device="cuda"))
+    assert torch.equal(l.grad, want)
