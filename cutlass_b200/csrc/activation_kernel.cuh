@@ -197,13 +197,18 @@ __global__ void __launch_bounds__(kActThreads) bsg_act_forward_kernel(const ActP
   const int32_t F = it.ok ? p.F : 0;
   const uint16_t* x = p.X + int64_t(it.row) * p.ldx;
   uint4 gv[2], uv[2];
+  {
+    I8Raw rg[2], ru[2];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int32_t k = it.k + 64 * c;
-    gv[c] = uv[c] = make_uint4(0, 0, 0, 0);
-    if (k < F) {
-      gv[c] = i8_load8(x, k, F, WIDE);
-      if constexpr (GATED) uv[c] = i8_load8(x + p.F, k, F, WIDE);
+    for (int c = 0; c < 2; ++c) {
+      rg[c] = i8_raw8<WIDE>(x, it.k + 64 * c, F);
+      if constexpr (GATED) ru[c] = i8_raw8<WIDE>(x + p.F, it.k + 64 * c, F);
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      gv[c] = i8_fix8<WIDE>(rg[c], x, it.k + 64 * c, F);
+      uv[c] = make_uint4(0, 0, 0, 0);
+      if constexpr (GATED) uv[c] = i8_fix8<WIDE>(ru[c], x + p.F, it.k + 64 * c, F);
     }
   }
   uint32_t m = i8_maxabs2<FP16>(act_max_of<FP16>(gv[0]), act_max_of<FP16>(gv[1])) & 0xFFFFu;
@@ -254,7 +259,8 @@ __global__ void __launch_bounds__(kActThreads) bsg_act_backward_kernel(const Act
   const bool live = it.ok && it.k < p.F;
   if (WIDE && !live) return;
   const int32_t k = live ? it.k : 0;
-  const uint4 dv = i8_load8(p.G + int64_t(it.row) * p.ldg, k, live ? p.F : 0, WIDE);
+  const uint16_t* grad = p.G + int64_t(it.row) * p.ldg;
+  const I8Raw rd = i8_raw8<WIDE>(grad, k, live ? p.F : 0);
   const int8_t* q = p.Q + int64_t(it.row) * kParts * p.pitch + k;
   const float* scale = p.scale + int64_t(it.row) * kParts * p.blocks + it.block;
   const uint2 qg = __ldg(reinterpret_cast<const uint2*>(q));
@@ -266,7 +272,7 @@ __global__ void __launch_bounds__(kActThreads) bsg_act_backward_kernel(const Act
     su = __ldg(scale + p.blocks);
   }
   float d[8], g[8], u[8], dg[8], du[8];
-  act_unpack<FP16>(dv, d);
+  act_unpack<FP16>(i8_fix8<WIDE>(rd, grad, k, live ? p.F : 0), d);
   act_dequant4(qg.x, sg, g);
   act_dequant4(qg.y, sg, g + 4);
   if constexpr (GATED) {

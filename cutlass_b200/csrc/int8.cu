@@ -130,25 +130,28 @@ struct SmemOnce {
   }
 };
 
-template <bool FP16>
+template <bool FP16, bool WIDE>
 int32_t launch_quantise(const bsg::I8QuantParams& p, cudaStream_t s) {
   // A thread keeps up to 64 values, so these rows are read once; one warp per row needs no shared memory.
-  if (p.K <= 32 * 64) bsg::bsg_i8_quant_kernel<32, FP16><<<(p.rows + 7) / 8, 256, 0, s>>>(p);
-  else if (p.K <= 128 * 64) bsg::bsg_i8_quant_kernel<128, FP16><<<(p.rows + 1) / 2, 256, 0, s>>>(p);
-  else bsg::bsg_i8_quant_kernel<512, FP16><<<p.rows, 512, 0, s>>>(p);
+  if (p.K <= 32 * 64) bsg::bsg_i8_quant_kernel<32, FP16, WIDE><<<(p.rows + 7) / 8, 256, 0, s>>>(p);
+  else if (p.K <= 64 * 64) bsg::bsg_i8_quant_kernel<64, FP16, WIDE><<<(p.rows + 3) / 4, 256, 0, s>>>(p);
+  else if (p.K <= 128 * 64) bsg::bsg_i8_quant_kernel<128, FP16, WIDE><<<(p.rows + 1) / 2, 256, 0, s>>>(p);
+  else bsg::bsg_i8_quant_kernel<512, FP16, WIDE><<<p.rows, 512, 0, s>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "quantiser launch: %s", cudaGetErrorString(e));
   return BSG_OK;
 }
+
+// Whether rows of 16-bit values can be read in groups of eight with single 16-byte loads.
+bool wide_rows(const bsg_int8_args& a) { return host_aligned(a.X, 16) && a.K % 8 == 0 && (a.ldx % 8 == 0 || a.tokens <= 1); }
 
 int32_t quantise(const bsg_int8_args& a, cudaStream_t s) {
   if (a.rows == 0) return BSG_OK;
   bsg::I8QuantParams p;
   p.X = static_cast<const uint16_t*>(a.X); p.index = a.index; p.Q = static_cast<int8_t*>(a.Q); p.scale = a.q_scale;
   p.ldx = a.ldx; p.ldq = a.ldq; p.rows = int32_t(a.rows); p.tokens = int32_t(a.tokens); p.K = int32_t(a.K);
-  p.fp16 = a.in_kind == BSG_OUT_F16;
-  p.wide = host_aligned(a.X, 16) && a.ldx % 8 == 0;
-  return p.fp16 ? launch_quantise<true>(p, s) : launch_quantise<false>(p, s);
+  if (wide_rows(a)) return a.in_kind == BSG_OUT_F16 ? launch_quantise<true, true>(p, s) : launch_quantise<false, true>(p, s);
+  return a.in_kind == BSG_OUT_F16 ? launch_quantise<true, false>(p, s) : launch_quantise<false, false>(p, s);
 }
 
 // Where tokens are used by several rows each, and there is enough of them to pay for one more kernel, they are quantised once
@@ -261,10 +264,10 @@ bool fits_token_kernel(const bsg_int8_args& a) {
          int64_t(a.rows <= 1 ? 1 : a.rows <= 2 ? 2 : 4) * ((a.K + 15) / 16 * 16) <= bsg::kI8TokenShared;
 }
 
-template <int MT, bool FP16>
+template <int MT, bool FP16, bool WIDE>
 int32_t launch_token(const bsg::I8TokenParams& p, cudaStream_t s, int sms, int dev) {
   static SmemOnce once;
-  auto kernel = bsg::bsg_i8_token_kernel<MT, FP16>;
+  auto kernel = bsg::bsg_i8_token_kernel<MT, FP16, WIDE>;
   int32_t rc = once.set(reinterpret_cast<const void*>(kernel), bsg::kI8TokenShared, dev);
   if (rc != BSG_OK) return rc;
   const int groups = int((int64_t(p.N) * p.parts + 15) / 16), grid = groups < 2 * sms ? groups : 2 * sms;      // two CTAs fit an SM
@@ -273,24 +276,24 @@ int32_t launch_token(const bsg::I8TokenParams& p, cudaStream_t s, int sms, int d
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   return BSG_OK;
 }
-template <bool FP16>
+template <bool FP16, bool WIDE>
 int32_t pick_token(const bsg::I8TokenParams& p, cudaStream_t s, int sms, int dev) {
-  if (p.M <= 1) return launch_token<1, FP16>(p, s, sms, dev);
-  if (p.M <= 2) return launch_token<2, FP16>(p, s, sms, dev);
-  return launch_token<4, FP16>(p, s, sms, dev);
+  if (p.M <= 1) return launch_token<1, FP16, WIDE>(p, s, sms, dev);
+  if (p.M <= 2) return launch_token<2, FP16, WIDE>(p, s, sms, dev);
+  return launch_token<4, FP16, WIDE>(p, s, sms, dev);
 }
 int32_t token_product(const bsg_int8_args& a, cudaStream_t s, int sms, int dev) {
   bsg::I8TokenParams p;
   p.X = static_cast<const uint16_t*>(a.X); p.W = static_cast<const int8_t*>(a.W); p.sb = a.w_scale; p.bias = a.bias; p.D = a.D;
   p.ldx = a.ldx; p.ldw = a.ldw; p.ldd = a.ldd; p.M = int32_t(a.rows); p.N = int32_t(a.N); p.K = int32_t(a.K);
-  p.wide = host_aligned(a.X, 16) && a.ldx % 8 == 0;
   p.out_kind = a.out_kind; p.activation = a.activation;
   // Warps share two channels where there would be fewer CTAs than SMs otherwise (every CTA quantises the tokens for itself, so
   // more of them than that cost more than they bring: one token, 4096 x 4096: 6.4 us unshared, 8.5 shared by two; 512 x 16384:
   // 14.3 unshared, 7.0 shared by eight).
   p.parts = 1;
   while (p.parts < 8 && a.N * p.parts < 16 * int64_t(sms) && a.K > p.parts * 512) p.parts *= 2;
-  return a.in_kind == BSG_OUT_F16 ? pick_token<true>(p, s, sms, dev) : pick_token<false>(p, s, sms, dev);
+  if (wide_rows(a)) return a.in_kind == BSG_OUT_F16 ? pick_token<true, true>(p, s, sms, dev) : pick_token<false, true>(p, s, sms, dev);
+  return a.in_kind == BSG_OUT_F16 ? pick_token<true, false>(p, s, sms, dev) : pick_token<false, false>(p, s, sms, dev);
 }
 
 int32_t product(const bsg_int8_args& a, const I8Plan& plan, void* workspace, cudaStream_t s, int sms, int dev, bool pdl) {

@@ -34,8 +34,6 @@ struct I8QuantParams {
   float* scale;
   int64_t ldx, ldq;          // elements
   int32_t rows, tokens, K;
-  int32_t fp16;
-  int32_t wide;              // rows of X and Q start on 16- / 8-byte boundaries
 };
 
 __device__ __forceinline__ float i8_unpack(uint32_t bits16, bool fp16) {
@@ -95,24 +93,39 @@ __device__ __forceinline__ uint4 i8_shift16(const uint4& lo, const uint4& hi, ui
   return make_uint4(__funnelshift_r(u[0], u[1], bits), __funnelshift_r(u[1], u[2], bits), __funnelshift_r(u[2], u[3], bits), __funnelshift_r(u[3], u[4], bits));
 }
 
-// Eight consecutive values of a row, zeros past its end.  Rows that do not start on 16 bytes are read in aligned pairs of
-// 16-byte words where both lie inside the row, value by value at its ends.
-__device__ __forceinline__ uint4 i8_load8(const uint16_t* row, int32_t k, int32_t K, bool wide) {
-  if (wide && k + 8 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
-  if (!wide && k > 0 && k + 16 <= K) {
+// Eight consecutive values of a row, zeros past its end, in two steps, so that many loads are under way before the first is
+// looked at.  WIDE: rows start on 16 bytes and K is a multiple of 8 where it ends inside a group.  Otherwise the one or two
+// aligned 16-byte words that hold the values are read whole: a word with at least one value of the row lies in the row's
+// allocation (and on its page), whose bounds are multiples of 16.
+struct I8Raw { uint4 lo, hi; };
+template <bool WIDE>
+__device__ __forceinline__ I8Raw i8_raw8(const uint16_t* row, int32_t k, int32_t K) {
+  I8Raw r;
+  r.lo = r.hi = make_uint4(0, 0, 0, 0);
+  if constexpr (WIDE) {
+    if (k < K) r.lo = __ldg(reinterpret_cast<const uint4*>(row + k));
+  } else {
     const uintptr_t a = reinterpret_cast<uintptr_t>(row + k);
     const uint4* at = reinterpret_cast<const uint4*>(a & ~uintptr_t(15));
-    return i8_shift16(__ldg(at), __ldg(at + 1), uint32_t(a) & 15u);
+    if (k < K) r.lo = __ldg(at);
+    if (k < K && reinterpret_cast<const uint16_t*>(at + 1) < row + K) r.hi = __ldg(at + 1);
   }
-  uint32_t w[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t lo = k + 2 * j < K ? uint32_t(__ldg(row + k + 2 * j)) : 0u;
-    const uint32_t hi = k + 2 * j + 1 < K ? uint32_t(__ldg(row + k + 2 * j + 1)) : 0u;
-    w[j] = lo | (hi << 16);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return r;
 }
+template <bool WIDE>
+__device__ __forceinline__ uint4 i8_fix8(const I8Raw& r, const uint16_t* row, int32_t k, int32_t K) {
+  if constexpr (WIDE) return r.lo;
+  uint4 v = i8_shift16(r.lo, r.hi, uint32_t(reinterpret_cast<uintptr_t>(row + k)) & 15u);
+  if (k + 8 > K) {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] &= (k + 2 * j < K ? 0xFFFFu : 0u) | (k + 2 * j + 1 < K ? 0xFFFF0000u : 0u);
+    v = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return v;
+}
+template <bool WIDE>
+__device__ __forceinline__ uint4 i8_load8(const uint16_t* row, int32_t k, int32_t K) { return i8_fix8<WIDE>(i8_raw8<WIDE>(row, k, K), row, k, K); }
 
 // Two packed 16-bit values to fp32.
 template <bool FP16>
@@ -146,7 +159,7 @@ __device__ __forceinline__ uint2 i8_levels8(const uint4& v, const I8Scale& s) {
 // a row of up to TPR * 64 values is read once.  Longer rows are read a second time (from L2).
 constexpr int kI8Chunks = 8;
 constexpr int kI8QuantThreads = 256;
-template <int TPR, bool FP16>
+template <int TPR, bool FP16, bool WIDE>
 __global__ void __launch_bounds__(TPR > kI8QuantThreads ? TPR : kI8QuantThreads) bsg_i8_quant_kernel(const I8QuantParams p) {
   constexpr int kThreads = TPR > kI8QuantThreads ? TPR : kI8QuantThreads;
   constexpr int kRows = kThreads / TPR;
@@ -162,16 +175,21 @@ __global__ void __launch_bounds__(TPR > kI8QuantThreads ? TPR : kI8QuantThreads)
   const bool src_ok = row_ok && src >= 0 && src < p.tokens;
   const uint16_t* row = p.X + (src_ok ? int64_t(src) * p.ldx : 0);
   const int32_t K = src_ok ? p.K : 0;
-  const bool wide = p.wide != 0;
   uint4 v[kI8Chunks];
   uint32_t m = 0;
+  {
+    I8Raw raw[kI8Chunks];
 #pragma unroll
-  for (int c = 0; c < kI8Chunks; ++c) v[c] = i8_load8(row, (c * TPR + t) * 8, K, wide);
+    for (int c = 0; c < kI8Chunks; ++c) raw[c] = i8_raw8<WIDE>(row, (c * TPR + t) * 8, K);
 #pragma unroll
-  for (int c = 0; c < kI8Chunks; ++c)
-    m = i8_maxabs2<FP16>(m, i8_maxabs2<FP16>(i8_maxabs2<FP16>(v[c].x, v[c].y), i8_maxabs2<FP16>(v[c].z, v[c].w)));
+    for (int c = 0; c < kI8Chunks; ++c) v[c] = i8_fix8<WIDE>(raw[c], row, (c * TPR + t) * 8, K);
+  }
+#pragma unroll
+  for (int c = 0; c < kI8Chunks; ++c) {
+    if (c * TPR * 8 < K) m = i8_maxabs2<FP16>(m, i8_maxabs2<FP16>(i8_maxabs2<FP16>(v[c].x, v[c].y), i8_maxabs2<FP16>(v[c].z, v[c].w)));
+  }
   for (int32_t k = (kI8Chunks * TPR + t) * 8; k < K; k += TPR * 8) {
-    const uint4 u = i8_load8(row, k, K, wide);
+    const uint4 u = i8_load8<WIDE>(row, k, K);
     m = i8_maxabs2<FP16>(m, i8_maxabs2<FP16>(i8_maxabs2<FP16>(u.x, u.y), i8_maxabs2<FP16>(u.z, u.w)));
   }
   m &= 0x7FFF7FFFu;
@@ -193,7 +211,7 @@ __global__ void __launch_bounds__(TPR > kI8QuantThreads ? TPR : kI8QuantThreads)
   int8_t* out = p.Q + int64_t(r) * p.ldq;
   auto store = [&](int32_t k, const uint4& u) {
     const uint2 q = i8_levels8<FP16>(u, s);
-    if (wide && k + 8 <= p.K) {
+    if (k + 8 <= p.K) {      // (rows of Q start on 16 bytes)
       *reinterpret_cast<uint2*>(out + k) = q;
     } else {
       for (int j = 0; j < 8 && k + j < p.K; ++j) out[k + j] = int8_t((j < 4 ? q.x : q.y) >> (8 * (j & 3)));
@@ -204,7 +222,7 @@ __global__ void __launch_bounds__(TPR > kI8QuantThreads ? TPR : kI8QuantThreads)
     const int32_t k = (c * TPR + t) * 8;
     if (k < p.K) store(k, v[c]);
   }
-  for (int32_t k = (kI8Chunks * TPR + t) * 8; k < p.K; k += TPR * 8) store(k, i8_load8(row, k, K, wide));
+  for (int32_t k = (kI8Chunks * TPR + t) * 8; k < p.K; k += TPR * 8) store(k, i8_load8<WIDE>(row, k, K));
 }
 
 // Rows of quantised tokens, and their scales, copied into the order of an index: one warp per row, so that a token that
@@ -984,7 +1002,7 @@ struct I8TokenParams {
   const float* bias;
   void* D;
   int64_t ldx, ldw, ldd;
-  int32_t M, N, K, wide;
+  int32_t M, N, K;
   int32_t out_kind, activation;
   int32_t parts;            // 1, 2, 4 or 8
 };
@@ -1001,7 +1019,7 @@ __device__ __forceinline__ uint4 i8_weights16(const int8_t* row, int32_t k, int3
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int MT, bool FP16>
+template <int MT, bool FP16, bool WIDE>
 __global__ void __launch_bounds__(kI8TokenThreads, 2) bsg_i8_token_kernel(const I8TokenParams p) {
   constexpr int kWarps = kI8TokenThreads / 32, kChan = 2, kUnroll = 4;
   constexpr int kPerToken = kI8TokenThreads / MT;            // threads that quantise one token: whole warps
@@ -1035,10 +1053,9 @@ __global__ void __launch_bounds__(kI8TokenThreads, 2) bsg_i8_token_kernel(const 
   {
     const int m = threadIdx.x / kPerToken, t = threadIdx.x % kPerToken;
     const uint16_t* row = p.X + int64_t(m < p.M ? m : 0) * p.ldx;
-    const bool wide = p.wide != 0;
     uint32_t mx = 0;
     for (int32_t k = t * 8; k < p.K; k += kPerToken * 8) {
-      const uint4 u = i8_load8(row, k, p.K, wide);
+      const uint4 u = i8_load8<WIDE>(row, k, p.K);
       mx = i8_maxabs2<FP16>(mx, i8_maxabs2<FP16>(i8_maxabs2<FP16>(u.x, u.y), i8_maxabs2<FP16>(u.z, u.w)));
     }
     mx &= 0x7FFF7FFFu;
@@ -1054,7 +1071,7 @@ __global__ void __launch_bounds__(kI8TokenThreads, 2) bsg_i8_token_kernel(const 
     const I8Scale s = i8_scale(amax);
     if (t == 0) s_scale[m] = i8_step(amax);
     for (int32_t k = t * 8; k < pitch; k += kPerToken * 8)
-      *reinterpret_cast<uint2*>(s_tok + m * pitch + k) = i8_levels8<FP16>(i8_load8(row, k, p.K, wide), s);
+      *reinterpret_cast<uint2*>(s_tok + m * pitch + k) = i8_levels8<FP16>(i8_load8<WIDE>(row, k, p.K), s);
     __syncthreads();
   }
 

@@ -27,7 +27,7 @@ constexpr int kRouteThreads = 256;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kRouteOneWarps = 16;           // warps of the block that does a small batch alone
 constexpr int kRouteOneTokens = 128;
-constexpr int kRouteBlocksMax = 592;         // four blocks for each of 148 SMs
+constexpr int kRouteBlocksMax = 740;         // five blocks for each of 148 SMs
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxK = 32;
 
@@ -237,6 +237,7 @@ __device__ __forceinline__ void route_choose(const RouteRow<TYPE, V>& r, int lan
       if (v + 1 < V) key[v + 1] = (two & 0xFFFF0000u) | uint32_t(kRouteMaxExperts - 1 - RouteMap<V>::expert(lane, v + 1 < V ? v + 1 : v));
     }
     if constexpr (kSorted) route_sort<V>(key);
+#pragma unroll 2
     for (int j = 0; j < K; ++j) {
       uint32_t m = key[0];
       if constexpr (!kSorted) {
@@ -244,7 +245,6 @@ __device__ __forceinline__ void route_choose(const RouteRow<TYPE, V>& r, int lan
         for (int v = 1; v < V; ++v) m = max(m, key[v]);
       }
       m = __reduce_max_sync(0xffffffffu, m);
-      if ((m | 0xFFFFu) <= route_lowest<TYPE>()) break;
       if (lane == j) won = m;
       if constexpr (kSorted) {
         if (key[0] == m) {
@@ -257,6 +257,7 @@ __device__ __forceinline__ void route_choose(const RouteRow<TYPE, V>& r, int lan
         for (int v = 0; v < V; ++v) key[v] = key[v] == m ? 0u : key[v];
       }
     }
+    if ((won | 0xFFFFu) <= route_lowest<TYPE>()) won = 0u;
     won_at = kRouteMaxExperts - 1 - (won & 0xFFFFu);
   } else {
     uint32_t key[V], at[V];
@@ -273,7 +274,6 @@ __device__ __forceinline__ void route_choose(const RouteRow<TYPE, V>& r, int lan
         for (int v = 1; v < V; ++v) m = max(m, key[v]);
       }
       m = __reduce_max_sync(0xffffffffu, m);
-      if (m <= route_lowest<TYPE>()) break;
       uint32_t e = 0xFFFFFFFFu;
       if constexpr (kSorted) {
         e = __reduce_min_sync(0xffffffffu, key[0] == m ? at[0] : e);
@@ -298,6 +298,7 @@ __device__ __forceinline__ void route_choose(const RouteRow<TYPE, V>& r, int lan
       }
     }
   }
+  if (TYPE == kRouteF32 && won <= route_lowest<TYPE>()) won = 0u;
   my_expert = won ? int32_t(won_at) : -1;
   my_logit = won ? route_value_of<TYPE>(won) : -INFINITY;
 }

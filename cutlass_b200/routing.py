@@ -39,7 +39,7 @@ class Routing(NamedTuple):
 def _scratch_words(T: int, E: int) -> int:      # what bsg_route_scratch_size says
     if T <= 128:
         return 0
-    return ((min((T + 15) // 16, 592) + 3) & ~3) * (2 * E + 1) + E
+    return ((min((T + 15) // 16, 740) + 3) & ~3) * (2 * E + 1) + E
 
 
 def _check_logits(logits, top_k):
