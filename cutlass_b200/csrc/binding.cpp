@@ -104,7 +104,7 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!w || !status || w->scalar_type() != at::kChar || w->get_device() != dev || w->dim() != (grouped ? 3 : 2)) Py_RETURN_NONE;
     const int64_t K = x.cols, N = w->size(-2), groups = grouped ? w->size(0) : 1, pitch = (K + 15) & ~int64_t(15);
     const int64_t ldw = N > 1 ? w->stride(-2) : pitch, group_stride = groups > 1 ? w->stride(0) : 0;
-    if (w->size(-1) != K || N < 1 || groups < 1 || groups > BSG_MAX_GROUPS || (K > 1 && w->stride(-1) != 1) || ldw < K || ((ldw | group_stride) & 15) != 0 || K > 131071 ||
+    if (w->size(-1) != K || N < 1 || groups < 1 || groups > BSG_MAX_GROUPS || (K > 1 && w->stride(-1) != 1) || ldw < K || ((ldw | group_stride) & 15) != 0 || (groups > 1 && group_stride < K) || K > 131071 ||
         (reinterpret_cast<uintptr_t>(w->const_data_ptr()) & 15) != 0)
       Py_RETURN_NONE;
     const auto per_channel = w->sizes().slice(0, grouped ? 2 : 1);

@@ -108,7 +108,8 @@ int32_t check_product(const bsg_int8_args& a, bool own_q, I8Plan* plan) {
   if (!host_aligned(a.W, 16) || a.ldw % 16 != 0 || (own_q && (!host_aligned(a.Q, 16) || a.ldq % 16 != 0)))
     return host_fail(BSG_ERR_MISALIGNED_OPERAND, "rows of Q and W must start on 16-byte boundaries (ldq=%lld, ldw=%lld)", (long long)a.ldq, (long long)a.ldw);
   if (a.ldw < a.K || (own_q && a.ldq < a.K) || a.ldd < a.N) return host_fail(BSG_ERR_INVALID_PROBLEM, "ldq, ldw or ldd is smaller than a row");
-  if (a.num_groups > 1 && (a.group_stride_w % 16 != 0 || a.group_stride_w < 0)) return host_fail(BSG_ERR_MISALIGNED_OPERAND, "group_stride_w must be a multiple of 16");
+  if (a.num_groups > 1 && a.group_stride_w % 16 != 0) return host_fail(BSG_ERR_MISALIGNED_OPERAND, "group_stride_w must be a multiple of 16");
+  if (a.num_groups > 1 && a.group_stride_w < a.K) return host_fail(BSG_ERR_INVALID_PROBLEM, "the groups of W overlap (group_stride_w=%lld)", (long long)a.group_stride_w);
   const int esz = a.out_kind == BSG_OUT_F32 ? 4 : 2;
   if (!host_aligned(a.D, esz) || !host_aligned(a.w_scale, 4) || !host_aligned(a.q_scale, 4) || !host_aligned(a.bias, 4) || !host_aligned(a.offsets, 4))
     return host_fail(BSG_ERR_MISALIGNED_OPERAND, "tensors must be aligned to their elements");
@@ -199,6 +200,7 @@ int32_t launch_rows(const bsg_int8_args& a, bsg::I8GemmParams& p, cudaStream_t s
   if (p.tma_out && (rc = bsg::host_out_map(&tmD, a.D, a.out_kind, a.N, a.rows, a.ldd)) != BSG_OK) return rc;
   p.tiles_n = int32_t((a.N + BN - 1) / BN);
   p.band = 16;
+  if (a.rows / C::kTileM + a.num_groups > 0x3FFFFFFF / p.tiles_n) return host_fail(BSG_ERR_INVALID_PROBLEM, "too many tiles for one launch");
   int64_t clusters = sms / CG;
   if (!a.offsets) {
     const int64_t tiles = ((a.rows + C::kTileM - 1) / C::kTileM) * p.tiles_n;
@@ -230,7 +232,7 @@ int32_t launch_few(const bsg_int8_args& a, bsg::I8GemmParams& p, cudaStream_t s,
   if ((rc = bsg::host_operand_map(&tmX, a.Q, a.K, a.rows, 1, a.ldq, a.rows * a.ldq, BT)) != BSG_OK) return rc;
   p.tiles_n = int32_t((a.N + 127) / 128);
   p.band = int32_t((a.rows + BT - 1) / BT);      // all token tiles of a channel tile in a row: its weights are then in L2
-  if (p.band > 0x7FFFFFFF / p.tiles_n) return host_fail(BSG_ERR_INVALID_PROBLEM, "too many tiles for one launch");
+  if (a.rows / BT + a.num_groups > 0x3FFFFFFF / split / p.tiles_n) return host_fail(BSG_ERR_INVALID_PROBLEM, "too many tiles for one launch");
   p.tma_out = 0;
   int64_t workers = int64_t(2) * sms;
   const int64_t tiles = a.offsets ? (a.rows / BT + a.num_groups) * p.tiles_n : ((a.rows + BT - 1) / BT) * p.tiles_n;

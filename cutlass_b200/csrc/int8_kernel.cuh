@@ -292,8 +292,7 @@ struct alignas(16) I8Ctl {
   int32_t tile_start[kMaxGroups + 1];
   int32_t end[kMaxGroups];
 };
-constexpr int kI8CtlBytes = 3072;
-static_assert(sizeof(I8Ctl) <= kI8CtlBytes, "control block");
+constexpr int kI8CtlBytes = (int(sizeof(I8Ctl)) + 127) / 128 * 128;
 
 static __device__ __noinline__ uint32_t i8_slow_wait(uint32_t bar, uint32_t parity, I8Ctl* ctl) {
   const long long t0 = clock64();

@@ -2,6 +2,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstring>
 #include <mutex>
 
@@ -129,15 +130,15 @@ int32_t forward_v(const bsg::RouteParams& p, int dev, cudaStream_t s) {
 template <int TYPE, int V>
 int32_t backward_v(const bsg::RouteParams& p, int sms, cudaStream_t s) {
   // one wave of what fits the SMs: a block goes on to its next tokens with their data already asked for
-  static int per_sm = 0;      // the same for every device of this architecture
+  static std::atomic<int> per_sm{0};      // the same for every device of this architecture
   auto kernel = bsg::bsg_route_backward_kernel<TYPE, V>;
   const size_t shared = size_t(bsg::kRouteWarps) * 32 * V * 4;
-  if (per_sm == 0) {
-    int n = 0;
+  int n = per_sm.load(std::memory_order_relaxed);
+  if (n == 0) {
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, bsg::kRouteThreads, shared) != cudaSuccess || n < 1) n = 4;
-    per_sm = n;
+    per_sm.store(n, std::memory_order_relaxed);
   }
-  const int64_t want = (int64_t(p.tokens) + bsg::kRouteWarps - 1) / bsg::kRouteWarps, most = int64_t(per_sm) * sms;
+  const int64_t want = (int64_t(p.tokens) + bsg::kRouteWarps - 1) / bsg::kRouteWarps, most = int64_t(n) * sms;
   kernel<<<unsigned(want < most ? want : most), bsg::kRouteThreads, shared, s>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "router launch: %s", cudaGetErrorString(e));

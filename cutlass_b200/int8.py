@@ -143,8 +143,8 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
     ldw = strides[-2] if N > 1 else pitch
     if weight.dtype != torch.int8 or weight.get_device() != device or shape[-1] != K or N < 1:
         raise ValueError(f"weight must be an int8 tensor on CUDA device {device} whose last extent is K = {K}, got {weight.dtype} {tuple(shape)} on {weight.device}")
-    if (strides[-1] != 1 and K > 1) or ldw < K or ldw & 15 or w & 15 or group_stride & 15:
-        raise ValueError("the rows of weight must have unit stride along K and start on 16-byte boundaries (quantize_int8 lays them out so)")
+    if (strides[-1] != 1 and K > 1) or ldw < K or ldw & 15 or w & 15 or group_stride & 15 or (experts > 1 and group_stride < K):
+        raise ValueError("the rows of weight must have unit stride along K, start on 16-byte boundaries (quantize_int8 lays them out so) and not overlap")
     _check_array("weight_scale", weight_scale, torch.float32, per_channel, device)
     if bias is not None:
         _check_array("bias", bias, torch.float32, per_channel, device)

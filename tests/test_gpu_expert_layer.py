@@ -1,0 +1,219 @@
+"""Router, 8-bit products and the activation with an 8-bit checkpoint together: a layer of experts, forward and backward; and
+tensors of more than 2^31 elements."""
+import pytest
+import torch
+
+import cutlass_b200 as ops
+import test_gpu_activation as activation_tests
+import test_gpu_int8 as product_tests
+import test_gpu_routing as routing_tests
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+class Layer:
+    """Tokens of D columns, E experts with F hidden columns, k of them per token."""
+
+    def __init__(self, T, D, F, E, k, dtype, seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.k, self.x = k, torch.randn((T, D), device="cuda", generator=g).to(dtype)
+        self.mask = torch.rand(T, device="cuda", generator=g) >= 0.2
+        self.logits = (2 * torch.randn((T, E), device="cuda", generator=g)).to(dtype)
+        self.logits[:, E // 2] = -float("inf")           # an expert that nobody may choose
+        made = [ops.quantize_int8(torch.randn((E * n, c), device="cuda", generator=g).to(dtype)) for n, c in ((2 * F, D), (D, F))]
+        (self.w1, self.s1), (self.w2, self.s2) = [(W.quantized.tensor.unflatten(0, (E, -1)), W.scale.tensor.view(E, -1)) for W in made]
+        self.up = torch.zeros((T * k, 2 * F), dtype=dtype, device="cuda")      # rows behind the last end row stay zero
+        self.down = torch.zeros((T * k, D), dtype=dtype, device="cuda")
+        self.grad = torch.randn((T, D), device="cuda", generator=g)
+        self.grad_h = torch.randn((T * k, F), device="cuda", generator=g).to(dtype)
+
+    def run(self):
+        """Everything on the way, and the gradients of the logits and of the first product's result."""
+        logits = self.logits.detach().requires_grad_(True)
+        r = ops.route_tokens(logits, self.k, token_mask=self.mask)
+        up = ops.int8_linear(self.x, self.w1, self.s1, offsets=r.offsets, rows=r.rows, out=self.up).detach().requires_grad_(True)
+        h = ops.checkpointed_activation(up, "silu")
+        down = ops.int8_linear(h.detach(), self.w2, self.s2, offsets=r.offsets, out=self.down)
+        mine = down[r.positions.clamp_min(0).long()].float() * (r.positions >= 0)[..., None]      # (T, k, D)
+        y = (r.weights[..., None] * mine).sum(1)
+        ((y * self.grad).sum() + 0.01 * r.balance_loss).backward()
+        h.backward(self.grad_h)
+        return r, up, h, down, y, logits.grad, up.grad, (mine * self.grad[:, None]).sum(2)
+
+    def check(self, result):
+        r, up, h, down, y, d_logits, d_up, d_weights = [t.detach() if torch.is_tensor(t) else t for t in result]
+        want = routing_tests.check(self.logits, self.k, self.mask, True, type(r)(*[t.detach() if torch.is_tensor(t) else t for t in r]))
+        total, begin = int(r.offsets[-1]), 0
+        assert total == int(self.mask.sum()) * self.k
+        for e, end in enumerate(r.offsets.tolist()):
+            if end > begin:
+                token = r.rows[begin:end].long()
+                product_tests.check(up[begin:end], self.x[token], self.w1[e], self.s1[e])
+                product_tests.check(down[begin:end], h[begin:end], self.w2[e], self.s2[e])
+                begin = end
+        assert bool((up[total:] == 0).all()) and bool((down[total:] == 0).all())
+        kept = ops.checkpoint_activation(up, "silu")[1]
+        activation_tests.check(up, self.grad_h, "silu", True, h, d_up, kept)
+        # the weighted sum is torch's, in fp32: k products and k - 1 sums
+        parts = r.weights.double()[..., None] * down.double()[r.positions.clamp_min(0).long()] * (r.positions >= 0)[..., None]
+        assert bool(((y.double() - parts.sum(1)).abs() <= (self.k + 1) * 2.0 ** -24 * parts.abs().sum(1)).all())
+        routing_tests.check_grad(d_logits, want, self.k, True, d_weights, 0.01, self.logits.dtype)
+
+
+@pytest.mark.parametrize("T,D,F,E,k,dtype", [(1, 64, 32, 4, 1, BF16), (16, 200, 136, 8, 2, F16), (77, 256, 130, 5, 4, BF16), (300, 136, 264, 16, 2, BF16)])
+def test_a_layer_forward_and_backward(cuda_lib, T, D, F, E, k, dtype):
+    layer = Layer(T, D, F, E, k, dtype, seed=T)
+    layer.mask[0] = True
+    layer.check(layer.run())
+    product_tests.status_ok()
+
+
+def test_a_layer_whose_tokens_are_all_padding(cuda_lib):
+    layer = Layer(40, 64, 32, 4, 2, BF16, seed=1)
+    layer.mask.zero_()
+    r, up, h, down, y, d_logits, d_up, _ = layer.run()
+    assert int(r.offsets[-1]) == 0 and bool((r.rows == -1).all()) and float(r.balance_loss.detach()) == 0.0
+    for t in (up, h, down, y, d_logits, d_up):
+        assert not bool(t.detach().any())
+
+
+def test_a_captured_layer_follows_its_inputs(cuda_lib):
+    """Forward and backward in one graph; replays with other tokens, logits and masks, on the stream of the replay."""
+    layer, other = Layer(50, 128, 72, 8, 2, BF16, seed=3), Layer(50, 128, 72, 8, 2, BF16, seed=4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer.run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        result = layer.run()
+    for source in (other, Layer(50, 128, 72, 8, 2, BF16, seed=5)):
+        for name in ("x", "mask", "logits", "grad", "grad_h"):
+            getattr(layer, name).copy_(getattr(source, name))
+        layer.up.zero_()
+        layer.down.zero_()
+        graph.replay()
+        layer.check(result)
+
+
+# ------------------------------------------------------------------------------------------------ more than 2^31 elements
+def test_a_product_with_more_outputs_than_31_bits(cuda_lib):
+    M, N, K = 66000, 33000, 32
+    x = product_tests.tokens(M, K, BF16, seed=1)
+    w, ws = product_tests.weights((N,), K, seed=2)
+    y = ops.int8_linear(x, w, ws)
+    for part in (slice(0, 300), slice(31000, 31300), slice(M - 300, M)):
+        product_tests.check(y[part], x[part], w, ws)
+
+
+def test_tokens_with_more_values_than_31_bits(cuda_lib):
+    M, N, K = 70000, 24, 32768
+    x = torch.zeros((M, K), dtype=F16, device="cuda")
+    x[-200:] = product_tests.tokens(200, K, F16, seed=3)
+    x[:200] = x[-200:].flip(0)
+    w, ws = product_tests.weights((N,), K, seed=4)
+    y = ops.int8_linear(x, w, ws)
+    assert not bool(y[200:-200].any())
+    product_tests.check(y[-200:], x[-200:], w, ws)
+    product_tests.check(y[:200], x[:200], w, ws)
+    rows = torch.arange(M - 1, M - 201, -1, dtype=torch.int32, device="cuda")
+    assert torch.equal(ops.int8_linear(x, w[None], ws[None], offsets=torch.tensor([200], dtype=torch.int32, device="cuda"), rows=rows), y[-200:].flip(0))
+
+
+def test_experts_with_more_weights_than_31_bits(cuda_lib):
+    E, N, K = 136, 4096, 4096
+    w = torch.zeros((E, N, K), dtype=torch.int8, device="cuda")
+    last, ws = product_tests.weights((N,), K, seed=5)
+    w[-1], w[0] = last, last
+    x = product_tests.tokens(9, K, BF16, seed=6)
+    offsets = torch.full((E,), 4, dtype=torch.int32, device="cuda")
+    offsets[-1] = 9
+    y = ops.int8_linear(x, w, ws.expand(E, N).contiguous(), offsets=offsets)
+    product_tests.check(y, x, last, ws)
+
+
+@pytest.mark.parametrize("gated", [True, False])
+def test_an_activation_of_more_values_than_31_bits(cuda_lib, gated):
+    T, F = 140000, 16000 if not gated else 8000
+    x = torch.zeros((T, 16000), dtype=BF16, device="cuda")
+    some, dh_some = activation_tests.make(300, F, BF16, gated, seed=7)
+    dh = torch.zeros((T, F), dtype=BF16, device="cuda")
+    x[-300:], dh[-300:] = some, dh_some
+    h, kept = ops.checkpoint_activation(x, "silu", gated=gated)
+    dx = ops.checkpoint_activation_backward(dh, kept)
+    assert not bool(h[:-300].any()) and not bool(dx[:-300].any())
+
+    class Last:
+        quantized, scale = kept.quantized[-300:], kept.scale[-300:]
+    activation_tests.check(some, dh_some, "silu", gated, h[-300:], dx[-300:], Last)
+
+
+def test_logits_of_more_values_than_31_bits(cuda_lib):
+    """All tokens but the last 300 are padding, so the definition is that of the last ones, with their numbers shifted."""
+    T, E, k, n = 2_200_000, 1024, 4, 300
+    logits = torch.zeros((T, E), dtype=BF16, device="cuda")
+    logits[-n:], _ = routing_tests.make(n, E, BF16, seed=8)
+    mask = torch.zeros(T, dtype=torch.bool, device="cuda")
+    mask[-n:] = True
+    r = ops.route_tokens(logits, k, token_mask=mask)
+    assert bool((r.experts[:-n] == -1).all()) and not bool(r.weights[:-n].any()) and bool((r.positions[:-n] == -1).all()) and bool((r.rows[n * k:] == -1).all())
+    part = r._replace(experts=r.experts[-n:], weights=r.weights[-n:], positions=r.positions[-n:], rows=r.rows[:n * k] - (T - n))
+    want = routing_tests.check(logits[-n:], k, None, True, part)
+    gw, gl = torch.zeros((T, k), device="cuda"), torch.tensor(0.3, device="cuda")
+    gw[-n:] = torch.randn((n, k), device="cuda", generator=torch.Generator(device="cuda").manual_seed(9))
+    d = ops.route_tokens_backward(logits, r, gw, gl)
+    assert not bool(d[:-n].any())
+    routing_tests.check_grad(d[-n:], want, k, True, gw[-n:], 0.3, BF16)
+
+
+# --------------------------------------------------------------------------------------------------- refusals of CUDA tensors
+def test_refusals(cuda_lib):
+    x = torch.zeros((6, 40), dtype=BF16, device="cuda")
+    w, ws = product_tests.weights((24,), 40, seed=1)
+    end = torch.tensor([3, 6], dtype=torch.int32, device="cuda")
+    w2, ws2 = product_tests.weights((2, 24), 40, seed=1)
+    linear = [
+        dict(x=x.t()), dict(x=x[0]), dict(x=x.float()), dict(x=x[:1].expand(6, 40)), dict(x=x.cpu()), dict(weight=w.float()), dict(weight=w[:, :32]), dict(weight=w.contiguous()),
+        dict(weight=w.cpu()), dict(weight=w[:1].expand(24, 40)), dict(weight=w[0]), dict(weight_scale=ws[:5]), dict(weight_scale=ws.double()), dict(weight_scale=ws.cpu()),
+        dict(bias=ws[:1]), dict(bias=ws.half()), dict(activation="tanh"), dict(rows=end), dict(out=torch.empty((6, 23), dtype=BF16, device="cuda")),
+        dict(out=torch.empty((24, 6), dtype=BF16, device="cuda").t()), dict(out=torch.empty((6, 24), dtype=torch.float64, device="cuda")), dict(out_dtype=torch.int32),
+        dict(out=torch.empty((6, 24), dtype=BF16, device="cuda"), out_dtype=F32), dict(out=torch.empty((1, 24), dtype=BF16, device="cuda").expand(6, 24)), dict(offsets=end),
+        dict(x=x.detach().requires_grad_()), dict(bias=torch.zeros(24, device="cuda", requires_grad=True))]
+    grouped = [dict(weight=w), dict(offsets=end.long()), dict(offsets=end[:1]), dict(offsets=end.cpu()), dict(weight_scale=ws), dict(bias=ws), dict(rows=end.long()), dict(rows=end[None]),
+               dict(rows=end.cpu()), dict(weight=w2[:1].expand(2, 24, 40))]
+    for base, cases in ((dict(x=x, weight=w, weight_scale=ws), linear), (dict(x=x, weight=w2, weight_scale=ws2, offsets=end), grouped)):
+        ops.int8_linear(**base)
+        for case in cases:
+            with pytest.raises(ValueError):
+                ops.int8_linear(**{**base, **case})
+    long = torch.zeros((1, 131072), dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="131071"):
+        ops.int8_linear(long, torch.zeros((4, 131072), dtype=torch.int8, device="cuda"), ws[:4].contiguous())
+    for case in (dict(x=x.float()), dict(x=x, out=torch.empty((6, 40), dtype=torch.int8, device="cuda")), dict(x=x, scale_out=ws), dict(x=x, rows=end.long()),
+                 dict(x=x.detach().requires_grad_())):
+        with pytest.raises(ValueError):
+            ops.quantize_int8(**case)
+
+    for case in (dict(x=x.float()), dict(x=x[:, :39]), dict(x=x, activation="tanh"), dict(x=x.t()), dict(x=x, out=x), dict(x=x, out=torch.empty((6, 20), dtype=F16, device="cuda")),
+                 dict(x=x.detach().requires_grad_()), dict(x=x[:1].expand(6, 40))):
+        with pytest.raises(ValueError):
+            ops.checkpoint_activation(**case)
+    h, kept = ops.checkpoint_activation(x)
+    for case in (dict(grad=x), dict(grad=h.half()), dict(grad=h[:5]), dict(grad=h.cpu()), dict(grad=h, out=h), dict(grad=h[:1].expand(6, 20)), dict(grad=h.detach().requires_grad_())):
+        with pytest.raises(ValueError):
+            ops.checkpoint_activation_backward(kept=kept, **case)
+
+    logits = torch.zeros((6, 8), device="cuda")
+    for case in (dict(top_k=0), dict(top_k=9), dict(top_k=2.0), dict(logits=logits.double()), dict(logits=logits.t()), dict(logits=logits[0]), dict(logits=torch.zeros((2, 1025), device="cuda")),
+                 dict(logits=torch.zeros((2, 64), device="cuda"), top_k=33), dict(token_mask=torch.ones(5, dtype=torch.bool, device="cuda")), dict(token_mask=torch.ones(6, device="cuda")),
+                 dict(token_mask=torch.ones(6, dtype=torch.bool))):
+        with pytest.raises(ValueError):
+            ops.route_tokens(**{**dict(logits=logits, top_k=2), **case})
+    r = ops.route_tokens(logits, 2)
+    for case in (dict(logits=logits[:5]), dict(logits=logits[:, :7]), dict(grad_weights=torch.zeros((6, 3), device="cuda")), dict(grad_weights=torch.zeros((6, 2), device="cuda").half()),
+                 dict(grad_balance_loss=torch.zeros(2, device="cuda")), dict(grad_balance_loss=torch.zeros(()))):
+        with pytest.raises(ValueError):
+            ops.route_tokens_backward(**{**dict(logits=logits, routing=r, grad_weights=None, grad_balance_loss=None), **case})
