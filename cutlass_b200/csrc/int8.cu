@@ -48,6 +48,9 @@ struct Variant {
 };
 constexpr Variant kVariants[] = {{true, 16, 0.20, 1.3, 3.6}, {true, 32, 0.24, 1.6, 3.8}, {true, 64, 0.31, 2.8, 4.6}, {true, 128, 0.45, 5.0, 6.0},
                                  {false, 128, 0.225, 2.2, 5.5}, {false, 256, 0.33, 3.3, 6.8}};
+// Grouped, 256 channels: tiles of 256 channels by up to 256 tokens, whose results leave by plain stores.  13818 rows in 16 groups,
+// 7168 x 512: 147 us, in tiles of 256 rows x 128 columns 110; 7971 rows in 16 groups, 7168 x 4096: 198 and 250.
+constexpr Variant kTurned = {false, 256, 0.40, 6.0, 6.8};
 constexpr double kHbmBytesPerUs = 6.5e6;
 
 int32_t choose(const bsg_int8_args& a, I8Plan* plan) {
@@ -56,7 +59,8 @@ int32_t choose(const bsg_int8_args& a, I8Plan* plan) {
   const double weights = double(a.N) * double(a.K) * double(active > 0 ? active : 1) / kHbmBytesPerUs;
   double best = 1e300;
   bool found = false;
-  for (const Variant& v : kVariants) {
+  for (const Variant& of : kVariants) {
+    const Variant& v = a.offsets && !of.few && of.tile == 256 ? kTurned : of;
     if ((a.kernel == 1 && !v.few) || (a.kernel == 2 && v.few) || (a.tile && a.tile != v.tile)) continue;
     const int64_t tile_m = v.few ? v.tile : 256, tile_n = v.few ? 128 : v.tile;
     // row tiles: grouped, half of a group's last tile is empty on average
@@ -183,11 +187,11 @@ int32_t launch_ex(cudaLaunchConfig_t& cfg, int clusters, bool pdl, cudaLaunchAtt
   return BSG_OK;
 }
 
-template <int CG, int BN>
+template <int CG, int BN, bool TURN>
 int32_t launch_rows(const bsg_int8_args& a, bsg::I8GemmParams& p, cudaStream_t s, int sms, int dev, bool pdl) {
   using C = bsg::I8RowsCfg<CG, BN>;
   static SmemOnce once;
-  auto kernel = bsg::bsg_i8_rows_kernel<CG, BN>;
+  auto kernel = bsg::bsg_i8_rows_kernel<CG, BN, TURN>;
   int32_t rc = once.set(reinterpret_cast<const void*>(kernel), C::kSmemBytes, dev);
   if (rc != BSG_OK) return rc;
   CUtensorMap tmA, tmB, tmD;
@@ -313,7 +317,8 @@ int32_t product(const bsg_int8_args& a, const I8Plan& plan, void* workspace, cud
       default: return launch_few<128, 1>(a, p, s, sms, dev, pdl);
     }
   }
-  return plan.tile == 128 ? launch_rows<2, 128>(a, p, s, sms, dev, pdl) : launch_rows<2, 256>(a, p, s, sms, dev, pdl);
+  if (plan.tile == 128) return launch_rows<2, 128, false>(a, p, s, sms, dev, pdl);
+  return a.offsets ? launch_rows<2, 256, true>(a, p, s, sms, dev, pdl) : launch_rows<2, 256, false>(a, p, s, sms, dev, pdl);
 }
 
 int32_t check_workspace(const void* workspace, size_t bytes) {

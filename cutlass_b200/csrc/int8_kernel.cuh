@@ -291,6 +291,7 @@ struct alignas(16) I8Ctl {
   int32_t pad;
   int32_t tile_start[kMaxGroups + 1];
   int32_t end[kMaxGroups];
+  uint16_t order[kMaxGroups];      // sorted walk: the group at every place
 };
 constexpr int kI8CtlBytes = (int(sizeof(I8Ctl)) + 127) / 128 * 128;
 
@@ -378,6 +379,75 @@ __device__ __forceinline__ void i8_build_groups(I8Ctl* ctl, const I8GemmParams& 
 struct I8Tile {
   int32_t g, tm, tn, row0, row_end;
 };
+
+// Tokens of a tile of a group with r rows, when tiles take any multiple of 32 tokens up to 256: its tiles are of one height.
+__device__ __forceinline__ int32_t i8_height(int32_t r) {
+  if (r <= 0) return 0;
+  const int32_t m = (r + 255) / 256;
+  return ((r + m - 1) / m + 31) & ~31;
+}
+// The group table of a walk over the groups by falling height of their tiles: a walk in steps of the number of CTA pairs then
+// gives every pair the same sum of heights, but for one tile.  i8_build_groups has left the end rows.  One whole warp.
+__device__ __forceinline__ void i8_sort_groups(I8Ctl* ctl, const I8GemmParams& p) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  int32_t place = 0, tiles = 0;
+  for (int32_t height = 256; height >= 0; height -= 32) {
+    for (int base = 0; base < p.num_groups; base += 32) {
+      const int g = base + lane;
+      const int32_t r = g < p.num_groups ? ctl->end[g] - (g ? ctl->end[g - 1] : 0) : 0;
+      const bool mine = g < p.num_groups && i8_height(r) == height;
+      const uint32_t all = __ballot_sync(0xffffffffu, mine);
+      if (all == 0) continue;
+      const int32_t n = mine && height ? (r + height - 1) / height * p.tiles_n : 0;
+      int32_t upto = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int32_t up = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += up;
+      }
+      if (mine) {
+        const int32_t at = place + __popc(all & ((1u << lane) - 1u));
+        ctl->order[at] = uint16_t(g);
+        ctl->tile_start[at] = tiles + upto - n;
+      }
+      place += __popc(all);
+      tiles += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  if (lane == 0) {
+    ctl->tile_start[p.num_groups] = tiles;
+    ctl->total_tiles = tiles;
+  }
+}
+// Tile t of that walk; `height` is its number of MMA columns.
+__device__ __forceinline__ I8Tile i8_decode_sorted(const I8Ctl* ctl, const I8GemmParams& p, const WorkItem& wi, int32_t* height) {
+  int lo = 0, hi = p.num_groups;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (ctl->tile_start[mid] <= wi.t) lo = mid; else hi = mid;
+  }
+  I8Tile ti;
+  ti.g = ctl->order[lo];
+  const int32_t begin = ti.g ? ctl->end[ti.g - 1] : 0, end = ctl->end[ti.g];
+  const int32_t h = i8_height(end - begin);
+  const int32_t local = wi.t - ctl->tile_start[lo];
+  const int32_t tiles_m = (end - begin + h - 1) / h;
+  const int32_t per_band = p.band * p.tiles_n;
+  const int32_t b = local / per_band, rem = local - b * per_band;
+  const int32_t bh = min(p.band, tiles_m - b * p.band);
+  ti.tm = b * p.band + rem % bh;
+  ti.tn = rem / bh;
+  ti.row0 = begin + ti.tm * h;
+  ti.row_end = min(ti.row0 + h, end);
+  *height = h;
+  if (wi.split) {      // a half of the tokens; of 32 all are in the first half
+    const int32_t first = ((h >> 1) + 31) & ~31;
+    if (wi.half) ti.row0 += first; else ti.row_end = min(ti.row_end, ti.row0 + first);
+    *height = wi.half ? max(h - first, 32) : first;
+  }
+  return ti;
+}
 // Tile t of the walk: groups in order; inside a group bands of `band` row tiles, rows fastest.
 __device__ __forceinline__ I8Tile i8_decode(const I8Ctl* ctl, const I8GemmParams& p, int32_t t, int32_t tile_rows) {
   int lo = 0, hi = p.num_groups;
@@ -421,6 +491,31 @@ __device__ __forceinline__ void i8_activate(float (&x)[N], int act) {
   }
 }
 
+// Columns (tokens) of one channel, finished and stored; consecutive lanes hold consecutive channels.
+template <int N>
+__device__ __forceinline__ void i8_put(const I8GemmParams& p, const uint32_t (&v)[N], const float* sa, int n_here, float sb, float bias, int64_t at) {
+  float x[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) x[j] = i8_finish(v[j], sa[j], sb, bias);
+  i8_activate(x, p.activation);
+  if (p.out_kind == kOutBf16) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j < n_here) reinterpret_cast<__nv_bfloat16*>(p.D)[at + j * p.ldd] = __float2bfloat16_rn(x[j]);
+    }
+  } else if (p.out_kind == kOutF16) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j < n_here) reinterpret_cast<__half*>(p.D)[at + j * p.ldd] = __float2half_rn(x[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j < n_here) reinterpret_cast<float*>(p.D)[at + j * p.ldd] = x[j];
+    }
+  }
+}
+
 // ---- many rows: D tile = (128 * CG rows) x BN columns, persistent, two accumulators of BN columns in tensor memory.
 // Eight epilogue warps, two for every quarter of the rows with half of the columns each: with four, a tile took 6 us to finish
 // (latencies of tensor-memory loads, conversions and staged stores, one after the other), more than its products up to K = 2500.
@@ -444,7 +539,7 @@ struct I8RowsCfg {
   static_assert(kTmemCols == 64 || kTmemCols == 128 || kTmemCols == 256 || kTmemCols == 512, "tensor-memory columns");
 };
 
-template <int CG, int BN>
+template <int CG, int BN, bool TURN>
 __global__ void __launch_bounds__(kI8RowsThreads, 1)
 bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmD, const I8GemmParams p) {
@@ -489,7 +584,10 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   // Launched behind the quantiser with programmatic stream serialisation: from here on its results are read.
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
-  if (warp == 0) i8_build_groups(ctl, p, C::kTileM);
+  if (warp == 0) {
+    i8_build_groups(ctl, p, C::kTileM);
+    if constexpr (TURN) i8_sort_groups(ctl, p);
+  }
   __syncwarp();
   ptx::tc_fence_before();
   if constexpr (CG == 2) { ptx::cluster_arrive(); ptx::cluster_wait(); } else { __syncthreads(); }
@@ -517,18 +615,27 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     uint32_t phase = 0;
     for (int32_t t = cluster_idx; t < total_work; t += num_clusters) {
       const WorkItem wi = decode_work(t, split_from);
-      const I8Tile ti = i8_decode(ctl, p, wi.t, C::kTileM);
-      const int32_t a_row = bcast(ti.row0 + int32_t(cta_rank) * 128);
-      // (the box of a half tile brings kBRows rows as well, of which the MMA reads the first half)
-      const int32_t b_row = bcast(ti.tn * BN + (wi.split ? wi.half * (BN / 2) + int32_t(cta_rank) * (C::kBRows / 2) : int32_t(cta_rank) * C::kBRows));
-      const int32_t g = bcast(ti.g);
+      int32_t a_row, b_row, g;
+      // (boxes always bring kBRows rows of B, of which the MMA may read fewer)
+      if constexpr (TURN) {
+        int32_t height;
+        const I8Tile ti = i8_decode_sorted(ctl, p, wi, &height);
+        a_row = bcast(ti.tn * 256 + int32_t(cta_rank) * 128);
+        b_row = bcast(ti.row0 + int32_t(cta_rank) * (height >> 1));
+        g = bcast(ti.g);
+      } else {
+        const I8Tile ti = i8_decode(ctl, p, wi.t, C::kTileM);
+        a_row = bcast(ti.row0 + int32_t(cta_rank) * 128);
+        b_row = bcast(ti.tn * BN + (wi.split ? wi.half * (BN / 2) + int32_t(cta_rank) * (C::kBRows / 2) : int32_t(cta_rank) * C::kBRows));
+        g = bcast(ti.g);
+      }
       for (int32_t kt = 0; kt < k_tiles; ++kt) {
         i8_wait(empty0 + stage * 8, phase ^ 1u, ctl, dead);
         if (elected && !dead) {
           if (is_leader) ptx::mbar_arrive_expect_tx(full0 + stage * 8, uint32_t(C::kStageBytes) * CG);
           const uint32_t bar = full0_leader + stage * 8;
-          ptx::tma_load_3d<CG>(sA0 + stage * C::kABytes, &tmA, bar, kt * 128, a_row, 0);
-          ptx::tma_load_3d<CG>(sB0 + stage * C::kBBytes, &tmB, bar, kt * 128, b_row, g);
+          ptx::tma_load_3d<CG>(sA0 + stage * C::kABytes, TURN ? &tmB : &tmA, bar, kt * 128, a_row, TURN ? g : 0);
+          ptx::tma_load_3d<CG>(sB0 + stage * C::kBBytes, TURN ? &tmA : &tmB, bar, kt * 128, b_row, TURN ? 0 : g);
         }
         if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
       }
@@ -551,7 +658,12 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       uint32_t phase = 0, ready = 0;
       int32_t it = 0;
       for (int32_t t = cluster_idx; t < total_work; t += num_clusters, ++it) {
-        const uint32_t idesc = t >= split_from ? idesc_half : idesc_full;
+        uint32_t idesc = t >= split_from ? idesc_half : idesc_full;
+        if constexpr (TURN) {
+          int32_t height;
+          i8_decode_sorted(ctl, p, decode_work(t, split_from), &height);
+          idesc = i8_idesc(256, uint32_t(bcast(height)));
+        }
         const int acc = it & 1;
         const uint32_t d_tmem = tmem_base + uint32_t(acc) * BN;
         i8_wait(tempty0 + acc * 8, (uint32_t(it >> 1) & 1u) ^ 1u, ctl, dead);
@@ -577,6 +689,51 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       }
       if (dead) atomicOr(p.status, kStTimeoutFull | kStTimeoutTmemEmpty);
     }
+  } else if constexpr (TURN) {
+    // ---------------------------------------------------------------- epilogue: a lane is an output channel
+    const int quarter = warp & 3, half = warp >= 6 ? 1 : 0;      // every second step of 32 tokens
+    const int epi = half * 4 + quarter;
+    const uint32_t tfull0 = ptx::smem_u32(&ctl->tmem_full[0]), tempty0 = ptx::smem_u32(&ctl->tmem_empty[0]);
+    const bool has_bias = p.bias != nullptr;
+    struct Need { int32_t n, row0, rows, height; float sb, bias, sa; };
+    auto need_of = [&](int32_t t) {
+      Need d;
+      const I8Tile ti = i8_decode_sorted(ctl, p, decode_work(t, split_from), &d.height);
+      d.n = ti.tn * 256 + int32_t(cta_rank) * 128 + quarter * 32 + lane;
+      d.row0 = ti.row0;
+      d.rows = ti.row_end - ti.row0;
+      const int64_t at = int64_t(ti.g) * p.N + d.n;
+      d.sb = d.n < p.N ? __ldg(p.sb + at) : 0.0f;
+      d.bias = d.n < p.N && has_bias ? __ldg(p.bias + at) : 0.0f;
+      d.sa = epi * 32 + lane < d.rows ? __ldcg(p.sa + ti.row0 + epi * 32 + lane) : 0.0f;
+      return d;
+    };
+    int32_t it = 0;
+    Need need{};
+    if (cluster_idx < total_work) need = need_of(cluster_idx);
+    for (int32_t t = cluster_idx; t < total_work; t += num_clusters, ++it) {
+      const int acc = it & 1;
+      const Need d = need;
+      float* sa = sCol + acc * 256;
+      sa[epi * 32 + lane] = d.sa;
+      if (t + num_clusters < total_work) need = need_of(t + num_clusters);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      i8_wait(tfull0 + acc * 8, uint32_t(it >> 1) & 1u, ctl, dead);
+      __syncwarp();
+      ptx::tc_fence_after();
+      const uint32_t lane_addr = tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(acc) * BN;
+#pragma unroll 1
+      for (int c0 = half * 32; c0 < d.height; c0 += 64) {
+        uint32_t v[32];
+        ptx::tmem_ld_32x32b_x32(lane_addr + c0, v);
+        ptx::tmem_ld_wait();
+        if (d.n < p.N && c0 < d.rows) i8_put(p, v, sa + c0, min(32, d.rows - c0), d.sb, d.bias, int64_t(d.row0 + c0) * p.ldd + d.n);
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_remote_relaxed(ptx::mapa(tempty0 + acc * 8, 0));
+    }
+    if (dead) atomicOr(p.status, kStTimeoutTmemFull);
   } else {
     // ---------------------------------------------------------------- epilogue
     const int quarter = warp & 3, half = warp >= 6 ? 1 : 0;      // (a warp reaches the tensor-memory lanes of its number mod 4)
@@ -736,31 +893,6 @@ struct I8FewCfg {
   static constexpr int kTmemCols = 2 * BT;
   static_assert(kStages >= 3, "stages");
 };
-
-// Columns (tokens) of one channel, finished and stored; consecutive lanes hold consecutive channels.
-template <int N>
-__device__ __forceinline__ void i8_put(const I8GemmParams& p, const uint32_t (&v)[N], const float* sa, int n_here, float sb, float bias, int64_t at) {
-  float x[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) x[j] = i8_finish(v[j], sa[j], sb, bias);
-  i8_activate(x, p.activation);
-  if (p.out_kind == kOutBf16) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (j < n_here) reinterpret_cast<__nv_bfloat16*>(p.D)[at + j * p.ldd] = __float2bfloat16_rn(x[j]);
-    }
-  } else if (p.out_kind == kOutF16) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (j < n_here) reinterpret_cast<__half*>(p.D)[at + j * p.ldd] = __float2half_rn(x[j]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (j < n_here) reinterpret_cast<float*>(p.D)[at + j * p.ldd] = x[j];
-    }
-  }
-}
 
 template <int BT, int SPLIT>
 __global__ void __launch_bounds__(192, 2)
