@@ -8,6 +8,8 @@ What is kept is one byte per value of ``x`` and one fp32 scale per 128 of them, 
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from . import lib as L
@@ -17,15 +19,17 @@ from .int8 import _IN_KINDS, _launch, _matrix, _no_gradient
 BLOCK = 128      # columns of a row that share one scale
 
 
-class ActivationCheckpoint:
+class ActivationCheckpoint(NamedTuple):
     """Input of an activation in 8 bits: ``quantized`` (T, parts, F rounded up to 16) int8 and ``scale`` (T, parts, F / 128
     rounded up) fp32, with parts = 2 (gate, up) when ``gated``, else 1; its value is ``scale * quantized`` per block.  Both lie
     in one buffer, ``data``."""
 
-    __slots__ = ("data", "activation", "gated", "rows", "width", "dtype")
-
-    def __init__(self, data: torch.Tensor, activation: str, gated: bool, rows: int, width: int, dtype: torch.dtype):
-        self.data, self.activation, self.gated, self.rows, self.width, self.dtype = data, activation, gated, rows, width, dtype
+    data: torch.Tensor
+    activation: str
+    gated: bool
+    rows: int
+    width: int
+    dtype: torch.dtype
 
     def _split(self) -> int:
         return self.rows * (2 if self.gated else 1) * ((self.width + 15) & ~15)
@@ -55,12 +59,11 @@ def checkpoint_activation(x, activation: str = "silu", *, gated: bool = True, ou
     itself, and the ``ActivationCheckpoint`` that ``checkpoint_activation_backward`` takes.  ``x`` is (T, 2F) or (T, F) bf16 /
     fp16; ``activation``: "identity", "relu", "gelu" (erf form) or "silu"; ``out`` (T, F) may be given.  A block of 128 values
     with a NaN or an infinity is kept as NaN.  Asynchronous on ``stream`` (None: torch's current stream)."""
-    gated = bool(gated)
     if out is None and stream is None and x.is_cuda:
-        done = L.binding().act_forward(x, ACTIVATIONS.get(activation, -1), gated)
+        done = L.binding().act_forward(x, activation, gated)
         if done is not None:
-            h, data, T, F = done
-            return h, ActivationCheckpoint(data, activation, gated, T, F, x.dtype)
+            return done
+    gated = bool(gated)
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r}: one of {sorted(ACTIVATIONS)}")
@@ -87,7 +90,7 @@ def checkpoint_activation_backward(grad, kept: ActivationCheckpoint, *, out=None
     """Gradient of ``x`` for the gradient ``grad`` (T, F) of ``h``, from what ``checkpoint_activation`` kept: (T, 2F) or (T, F)
     in the type of ``x``.  ``out`` may be given.  Asynchronous on ``stream`` (None: torch's current stream)."""
     if out is None and stream is None and grad.is_cuda:
-        dx = L.binding().act_backward(grad, kept.data, ACTIVATIONS[kept.activation], kept.gated, kept.rows, kept.width, kept.dtype)
+        dx = L.binding().act_backward(grad, kept)
         if dx is not None:
             return dx
     data, T, F, parts = kept.data, kept.rows, kept.width, 2 if kept.gated else 1

@@ -71,7 +71,7 @@ def _build_binding(force: bool) -> None:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-isystem" + os.path.join(root, "include"), "-isystem" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-isystem" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], src, "-o", BINDING,
-           "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+           "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError("the compiler failed:\n" + proc.stdout + proc.stderr)

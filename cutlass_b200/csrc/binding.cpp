@@ -8,13 +8,16 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <exception>
+#include <initializer_list>
 
 #include "../../include/bsgemm.h"
 
@@ -30,7 +33,11 @@ struct {
   decltype(&bsg_route_scratch_size) route_scratch_size;
   decltype(&bsg_last_error_string) last_error_string;
 } g;
-PyObject* g_raise = nullptr;      // called with the status code of a call that failed
+// Objects of the Python side: what is called with the status code of a call that failed; activation name -> code; device -> status
+// words; the named tuples that the operators return.
+struct {
+  PyObject *raise, *activations, *workspaces, *checkpoint, *routing;
+} g_py;
 
 constexpr int64_t kMaxExperts = 1024, kMaxTopK = 32;
 
@@ -67,7 +74,7 @@ bool matrix(PyObject* o, bool with_f32, Matrix* m) {
 }
 bool wants_gradient(const at::Tensor* t) { return t && t->requires_grad() && at::GradMode::is_enabled(); }
 
-at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) { return at::empty(shape, at::TensorOptions().dtype(type).device(like.device())); }
+at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) { return at::Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt)); }
 
 // Part of a buffer as a tensor of its own (contiguous, `offset` in elements of `type`); not a view for autograd.
 at::Tensor part(const at::Tensor& buffer, at::ScalarType type, int64_t offset, at::IntArrayRef shape) {
@@ -79,7 +86,26 @@ at::Tensor part(const at::Tensor& buffer, at::ScalarType type, int64_t offset, a
 
 void* current_stream(int device) { return c10::cuda::getCurrentCUDAStream(device).stream(); }
 
-PyObject* failed(int32_t code) { return PyObject_CallFunction(g_raise, "i", int(code)); }      // raises
+PyObject* failed(int32_t code) { return PyObject_CallFunction(g_py.raise, "i", int(code)); }      // raises
+
+// A tuple of the (named) tuple type `type`; takes the items over.
+PyObject* tuple_of(PyObject* type, std::initializer_list<PyObject*> items) {
+  PyTypeObject* t = reinterpret_cast<PyTypeObject*>(type);
+  PyObject* made = t->tp_alloc(t, Py_ssize_t(items.size()));
+  bool whole = made != nullptr;
+  Py_ssize_t i = 0;
+  for (PyObject* o : items) {
+    whole = whole && o;
+    if (made) PyTuple_SET_ITEM(made, i++, o); else Py_XDECREF(o);
+  }
+  if (!whole) Py_CLEAR(made);
+  return made;
+}
+// Activation code of a name; -1 where there is none.
+int32_t activation_of(PyObject* name) {
+  PyObject* code = PyUnicode_Check(name) ? PyDict_GetItem(g_py.activations, name) : nullptr;
+  return code ? int32_t(PyLong_AsLong(code)) : -1;
+}
 
 template <class F>
 PyObject* guarded(F body) {
@@ -93,14 +119,17 @@ PyObject* guarded(F body) {
   return nullptr;
 }
 
-// int8_linear(x, weight, weight_scale, bias, activation, offsets, rows, out_dtype, status) -> y
+// int8_linear(x, weight, weight_scale, bias, activation, offsets, rows, out_dtype) -> y
 PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Matrix x;
-    if (n != 9 || !matrix(a[0], false, &x)) Py_RETURN_NONE;
+    if (n != 8 || !matrix(a[0], false, &x)) Py_RETURN_NONE;
     const int dev = x.device;
     const bool grouped = a[5] != Py_None;
-    const at::Tensor *w = tensor(a[1]), *status = tensor(a[8]);
+    PyObject* device_key = PyLong_FromLong(dev);
+    PyObject* words = device_key ? PyDict_GetItem(g_py.workspaces, device_key) : nullptr;      // borrowed
+    Py_XDECREF(device_key);
+    const at::Tensor *w = tensor(a[1]), *status = words ? tensor(words) : nullptr;
     if (!w || !status || w->scalar_type() != at::kChar || w->get_device() != dev || w->dim() != (grouped ? 3 : 2)) Py_RETURN_NONE;
     const int64_t K = x.cols, N = w->size(-2), groups = grouped ? w->size(0) : 1, pitch = (K + 15) & ~int64_t(15);
     const int64_t ldw = N > 1 ? w->stride(-2) : pitch, group_stride = groups > 1 ? w->stride(0) : 0;
@@ -121,11 +150,11 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
       out_type = reinterpret_cast<THPDtype*>(a[7])->scalar_type;
     }
     const int out_kind = kind_of(out_type, true);
-    const long act = PyLong_AsLong(a[4]);
+    const int32_t act = activation_of(a[4]);
     const int64_t R = rows ? rows->size(0) : x.rows;
-    if (out_kind < 0 || act < BSG_ACT_IDENTITY || act > BSG_ACT_SILU || R == 0) Py_RETURN_NONE;
+    if (out_kind < 0 || act < 0 || R == 0) Py_RETURN_NONE;
     bsg_int8_args c{};
-    c.in_kind = x.kind; c.out_kind = out_kind; c.num_groups = int32_t(groups); c.activation = int32_t(act);
+    c.in_kind = x.kind; c.out_kind = out_kind; c.num_groups = int32_t(groups); c.activation = act;
     c.rows = R; c.tokens = x.rows; c.N = N; c.K = K;
     c.X = x.t->const_data_ptr(); c.ldx = x.pitch; c.index = rows ? rows->const_data_ptr<int32_t>() : nullptr; c.ldq = pitch;
     c.W = w->const_data_ptr(); c.ldw = ldw; c.group_stride_w = group_stride; c.w_scale = ws->const_data_ptr<float>();
@@ -146,40 +175,51 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// act_forward(x, activation, gated) -> (h, data, rows, width)
+// act_forward(x, activation, gated) -> (h, ActivationCheckpoint)
 PyObject* act_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Matrix x;
     if (n != 3 || !matrix(a[0], false, &x) || wants_gradient(x.t)) Py_RETURN_NONE;
-    const long act = PyLong_AsLong(a[1]);
+    const int32_t act = activation_of(a[1]);
     const bool gated = a[2] == Py_True;
-    if (act < BSG_ACT_IDENTITY || act > BSG_ACT_SILU || (gated && x.cols % 2 != 0)) Py_RETURN_NONE;
+    if (act < 0 || (!gated && a[2] != Py_False) || (gated && x.cols % 2 != 0)) Py_RETURN_NONE;
     const int64_t parts = gated ? 2 : 1, T = x.rows, F = x.cols / parts, split = T * parts * ((F + 15) & ~int64_t(15));
     at::Tensor data = empty({split + 4 * T * parts * ((F + 127) / 128)}, at::kChar, *x.t);
     at::Tensor h = empty({T, F}, x.t->scalar_type(), *x.t);
     bsg_act_args c{};
-    c.type = x.kind; c.activation = int32_t(act); c.gated = gated; c.rows = T; c.width = F;
+    c.type = x.kind; c.activation = act; c.gated = gated; c.rows = T; c.width = F;
     c.in = x.t->const_data_ptr(); c.ld_in = x.pitch; c.out = h.mutable_data_ptr(); c.ld_out = F;
     c.kept = data.mutable_data_ptr(); c.kept_scale = reinterpret_cast<float*>(static_cast<char*>(c.kept) + split);
     const int32_t code = g.act_forward(&c, current_stream(x.device));
     if (code) return failed(code);
-    return Py_BuildValue("(NNLL)", THPVariable_Wrap(std::move(h)), THPVariable_Wrap(std::move(data)), (long long)T, (long long)F);
+    PyObject* dtype = reinterpret_cast<PyObject*>(torch::getTHPDtype(x.t->scalar_type()));
+    Py_INCREF(a[1]);
+    Py_INCREF(a[2]);
+    Py_INCREF(dtype);
+    PyObject* kept = tuple_of(g_py.checkpoint, {THPVariable_Wrap(std::move(data)), a[1], a[2], PyLong_FromLongLong(T), PyLong_FromLongLong(F), dtype});
+    return kept ? tuple_of(reinterpret_cast<PyObject*>(&PyTuple_Type), {THPVariable_Wrap(std::move(h)), kept}) : nullptr;
   });
 }
 
-// act_backward(grad, data, activation, gated, rows, width, dtype) -> dx
+// act_backward(grad, kept) -> dx
 PyObject* act_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Matrix d;
-    if (n != 7 || !matrix(a[0], false, &d) || wants_gradient(d.t) || !THPDtype_Check(a[6])) Py_RETURN_NONE;
-    const long act = PyLong_AsLong(a[2]);
-    const bool gated = a[3] == Py_True;
-    const int64_t T = PyLong_AsLongLong(a[4]), F = PyLong_AsLongLong(a[5]), parts = gated ? 2 : 1, split = T * parts * ((F + 15) & ~int64_t(15));
-    const at::Tensor* data = array(a[1], at::kChar, {split + 4 * T * parts * ((F + 127) / 128)}, d.device);
-    if (!data || d.rows != T || d.cols != F || reinterpret_cast<THPDtype*>(a[6])->scalar_type != d.t->scalar_type()) Py_RETURN_NONE;
+    if (n != 2 || !matrix(a[0], false, &d) || wants_gradient(d.t) || reinterpret_cast<PyObject*>(Py_TYPE(a[1])) != g_py.checkpoint || PyTuple_GET_SIZE(a[1]) != 6) Py_RETURN_NONE;
+    PyObject* const* kept = &PyTuple_GET_ITEM(a[1], 0);      // data, activation, gated, rows, width, dtype
+    const int32_t act = activation_of(kept[1]);
+    const bool gated = kept[2] == Py_True;
+    if (act < 0 || !PyLong_Check(kept[3]) || !PyLong_Check(kept[4]) || !THPDtype_Check(kept[5])) Py_RETURN_NONE;
+    const int64_t T = d.rows, F = d.cols, parts = gated ? 2 : 1, split = T * parts * ((F + 15) & ~int64_t(15));
+    if (PyLong_AsLongLong(kept[3]) != T || PyLong_AsLongLong(kept[4]) != F || reinterpret_cast<THPDtype*>(kept[5])->scalar_type != d.t->scalar_type()) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    const at::Tensor* data = array(kept[0], at::kChar, {split + 4 * T * parts * ((F + 127) / 128)}, d.device);
+    if (!data) Py_RETURN_NONE;
     at::Tensor dx = empty({T, parts * F}, d.t->scalar_type(), *d.t);
     bsg_act_args c{};
-    c.type = d.kind; c.activation = int32_t(act); c.gated = gated; c.rows = T; c.width = F;
+    c.type = d.kind; c.activation = act; c.gated = gated; c.rows = T; c.width = F;
     c.in = d.t->const_data_ptr(); c.ld_in = d.pitch; c.out = dx.mutable_data_ptr(); c.ld_out = parts * F;
     c.kept = const_cast<void*>(data->const_data_ptr());
     c.kept_scale = reinterpret_cast<float*>(static_cast<char*>(c.kept) + split);
@@ -190,11 +230,11 @@ PyObject* act_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 bool routable(const Matrix& l, int64_t k) { return l.cols <= kMaxExperts && k >= 1 && k <= kMaxTopK && k <= l.cols && l.rows * k <= 0x7FFFFFFFll; }
 
-// route_forward(logits, top_k, token_mask, normalize) -> (experts, weights, counts, offsets, rows, positions, loss, live, softmax)
+// route_forward(logits, top_k, token_mask, normalize) -> Routing
 PyObject* route_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Matrix l;
-    if (n != 4 || !matrix(a[0], true, &l) || !PyLong_CheckExact(a[1])) Py_RETURN_NONE;
+    if (n != 4 || !matrix(a[0], true, &l) || !PyLong_CheckExact(a[1]) || (a[3] != Py_True && a[3] != Py_False) || wants_gradient(l.t)) Py_RETURN_NONE;
     const int64_t T = l.rows, E = l.cols, k = PyLong_AsLongLong(a[1]);
     if (k < 1 || !routable(l, k)) { PyErr_Clear(); Py_RETURN_NONE; }
     const at::Tensor* mask = a[2] == Py_None ? nullptr : array(a[2], at::kBool, {T}, l.device);
@@ -221,30 +261,33 @@ PyObject* route_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (code) return failed(code);
     auto ints = [&](int64_t o, at::IntArrayRef s) { return THPVariable_Wrap(part(all, at::kInt, o, s)); };
     auto reals = [&](int64_t o, at::IntArrayRef s) { return THPVariable_Wrap(part(all, at::kFloat, o, s)); };
-    return Py_BuildValue("(NNNNNNNNN)", ints(experts, {T, k}), reals(weights, {T, k}), ints(counts, {E}), ints(offsets, {E}), ints(rows, {slots}),
-                         ints(positions, {T, k}), reals(loss, {}), ints(live, {1}), ints(soft, {2 * T}));
+    Py_INCREF(a[3]);
+    return tuple_of(g_py.routing, {ints(experts, {T, k}), reals(weights, {T, k}), ints(counts, {E}), ints(offsets, {E}), ints(rows, {slots}),
+                                   ints(positions, {T, k}), reals(loss, {}), ints(live, {1}), ints(soft, {2 * T}), a[3]});
   });
 }
 
-// route_backward(logits, experts, weights, counts, live, softmax, normalize, grad_weights, grad_loss) -> grad_logits
+// route_backward(logits, routing, grad_weights, grad_loss) -> grad_logits
 PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Matrix l;
-    if (n != 9 || !matrix(a[0], true, &l)) Py_RETURN_NONE;
-    const at::Tensor* experts = tensor(a[1]);
+    if (n != 4 || !matrix(a[0], true, &l) || reinterpret_cast<PyObject*>(Py_TYPE(a[1])) != g_py.routing || PyTuple_GET_SIZE(a[1]) != 10) Py_RETURN_NONE;
+    // experts, weights, counts, offsets, rows, positions, balance_loss, num_tokens, softmax, normalize
+    PyObject* const* r = &PyTuple_GET_ITEM(a[1], 0);
+    const at::Tensor* experts = tensor(r[0]);
     if (!experts || experts->dim() != 2) Py_RETURN_NONE;
     const int64_t T = l.rows, E = l.cols, k = experts->size(1);
     if (!routable(l, k)) Py_RETURN_NONE;
-    experts = array(a[1], at::kInt, {T, k}, l.device);
-    const at::Tensor *weights = array(a[2], at::kFloat, {T, k}, l.device), *counts = array(a[3], at::kInt, {E}, l.device), *live = array(a[4], at::kInt, {1}, l.device),
-                     *soft = array(a[5], at::kInt, {2 * T}, l.device);
-    const at::Tensor* gw = a[7] == Py_None ? nullptr : array(a[7], at::kFloat, {T, k}, l.device);
-    const at::Tensor* gl = a[8] == Py_None ? nullptr : tensor(a[8]);
-    if (!experts || !weights || !counts || !live || !soft || (a[7] != Py_None && !gw)) Py_RETURN_NONE;
-    if (a[8] != Py_None && (!gl || gl->scalar_type() != at::kFloat || gl->numel() != 1 || gl->get_device() != l.device)) Py_RETURN_NONE;
+    experts = array(r[0], at::kInt, {T, k}, l.device);
+    const at::Tensor *weights = array(r[1], at::kFloat, {T, k}, l.device), *counts = array(r[2], at::kInt, {E}, l.device), *live = array(r[7], at::kInt, {1}, l.device),
+                     *soft = array(r[8], at::kInt, {2 * T}, l.device);
+    const at::Tensor* gw = a[2] == Py_None ? nullptr : array(a[2], at::kFloat, {T, k}, l.device);
+    const at::Tensor* gl = a[3] == Py_None ? nullptr : tensor(a[3]);
+    if (!experts || !weights || !counts || !live || !soft || (a[2] != Py_None && !gw)) Py_RETURN_NONE;
+    if (a[3] != Py_None && (!gl || gl->scalar_type() != at::kFloat || gl->numel() != 1 || gl->get_device() != l.device)) Py_RETURN_NONE;
     at::Tensor d = empty({T, E}, l.t->scalar_type(), *l.t);
     bsg_route_args c{};
-    c.type = l.kind; c.experts = int32_t(E); c.k = int32_t(k); c.normalize = a[6] == Py_True; c.tokens = T;
+    c.type = l.kind; c.experts = int32_t(E); c.k = int32_t(k); c.normalize = r[9] == Py_True; c.tokens = T;
     c.logits = l.t->const_data_ptr(); c.ld = l.pitch;
     c.chosen = const_cast<int32_t*>(experts->const_data_ptr<int32_t>()); c.weights = const_cast<float*>(weights->const_data_ptr<float>());
     c.counts = const_cast<int32_t*>(counts->const_data_ptr<int32_t>()); c.live = const_cast<int32_t*>(live->const_data_ptr<int32_t>());
@@ -256,20 +299,24 @@ PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// bind(raise, address, ...): the entry points in the order of `g`.
+// bind(raise, activations, workspaces, checkpoint, routing, address, ...): the objects of `g_py`, then the entry points in the
+// order of `g`.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  PyObject** objects = reinterpret_cast<PyObject**>(&g_py);
   void** slots = reinterpret_cast<void**>(&g);
-  constexpr Py_ssize_t kSlots = Py_ssize_t(sizeof(g) / sizeof(void*));
-  if (n != kSlots + 1) {
-    PyErr_Format(PyExc_TypeError, "bind takes %zd addresses", kSlots);
+  constexpr Py_ssize_t kObjects = Py_ssize_t(sizeof(g_py) / sizeof(PyObject*)), kSlots = Py_ssize_t(sizeof(g) / sizeof(void*));
+  if (n != kObjects + kSlots || !PyDict_Check(a[1]) || !PyDict_Check(a[2]) || !PyType_Check(a[3]) || !PyType_Check(a[4])) {
+    PyErr_Format(PyExc_TypeError, "bind takes a function, two dicts, two tuple types and %zd addresses", kSlots);
     return nullptr;
   }
   for (Py_ssize_t i = 0; i < kSlots; ++i) {
-    slots[i] = PyLong_AsVoidPtr(a[i + 1]);
+    slots[i] = PyLong_AsVoidPtr(a[kObjects + i]);
     if (PyErr_Occurred()) return nullptr;
   }
-  Py_INCREF(a[0]);
-  g_raise = a[0];
+  for (Py_ssize_t i = 0; i < kObjects; ++i) {
+    Py_INCREF(a[i]);
+    objects[i] = a[i];
+  }
   Py_RETURN_NONE;
 }
 

@@ -117,10 +117,7 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
 
     No gradient is kept.  Asynchronous on ``stream`` (None: torch's current stream)."""
     if out is None and stream is None and x.is_cuda:
-        status = _default_workspaces.get(x.get_device())
-        if status is None:
-            status = _default_workspace(x.device)
-        y = L.binding().int8_linear(x, weight, weight_scale, bias, ACTIVATIONS.get(activation, -1), offsets, rows, out_dtype, status)
+        y = L.binding().int8_linear(x, weight, weight_scale, bias, activation, offsets, rows, out_dtype)
         if y is not None:
             return y
     in_kind, device, M, K, ldx = _matrix("x", x, _IN_KINDS)

@@ -205,7 +205,11 @@ def binding():
         loader = importlib.machinery.ExtensionFileLoader("_binding", BINDING_PATH)
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
         loader.exec_module(module)
-        module.bind(check, *(C.cast(getattr(lib, name), C.c_void_p).value for name in BOUND))
+        from .activation import ActivationCheckpoint
+        from .arguments import ACTIVATIONS
+        from .operator import _default_workspaces
+        from .routing import Routing
+        module.bind(check, ACTIVATIONS, _default_workspaces, ActivationCheckpoint, Routing, *(C.cast(getattr(lib, name), C.c_void_p).value for name in BOUND))
         _binding = module
     return _binding
 

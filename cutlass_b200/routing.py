@@ -55,9 +55,9 @@ def _check_logits(logits, top_k):
 
 def _forward(logits, top_k, token_mask, normalize, stream) -> Routing:
     if stream is None and logits.is_cuda:
-        done = L.binding().route_forward(logits, top_k, token_mask, bool(normalize))
-        if done is not None:
-            return tuple.__new__(Routing, done + (bool(normalize),))
+        r = L.binding().route_forward(logits, top_k, token_mask, bool(normalize))
+        if r is not None:
+            return r
     kind, device, T, E, ld = _check_logits(logits, top_k)
     if token_mask is not None:
         _check_array("token_mask", token_mask, torch.bool, (T,), device)
@@ -88,8 +88,7 @@ def route_tokens_backward(logits, routing: Routing, grad_weights=None, grad_bala
     () fp32, either of which may be None (zero).  The counts are constants.  Asynchronous on ``stream`` (None: torch's current
     stream)."""
     if stream is None and logits.is_cuda:
-        d = L.binding().route_backward(logits, routing.experts, routing.weights, routing.counts, routing.num_tokens, routing.softmax,
-                                       routing.normalize, grad_weights, grad_balance_loss)
+        d = L.binding().route_backward(logits, routing, grad_weights, grad_balance_loss)
         if d is not None:
             return d
     experts, counts = routing.experts, routing.counts
@@ -144,6 +143,10 @@ def route_tokens(logits, top_k: int, *, token_mask=None, normalize: bool = True,
 
     E is at most 1024 and k at most 32.  Results do not depend on the order in which anything runs.  Asynchronous on ``stream``
     (None: torch's current stream); the backward pass runs on the stream that autograd makes current."""
+    if stream is None and logits.is_cuda:      # (None for logits that want a gradient, too)
+        r = L.binding().route_forward(logits, top_k, token_mask, normalize)
+        if r is not None:
+            return r
     if not (torch.is_grad_enabled() and logits.requires_grad):
         return _forward(logits, top_k, token_mask, normalize, stream)
     weights, loss, experts, counts, offsets, rows, positions, live, softmax = _Route.apply(logits, top_k, token_mask, normalize, stream)

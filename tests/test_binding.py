@@ -13,16 +13,16 @@ from cutlass_b200.routing import _scratch_words
 def test_anything_but_cuda_tensors_is_left_alone():
     b = L.binding()
     x = torch.zeros((4, 32), dtype=torch.bfloat16)
-    assert b.int8_linear(x, x, x, None, 0, None, None, None, x) is None
-    assert b.act_forward(x, 3, True) is None
-    assert b.act_backward(x, x, 3, True, 4, 16, torch.bfloat16) is None
+    assert b.int8_linear(x, x, x, None, "relu", None, None, None) is None
+    assert b.act_forward(x, "relu", True) is None
+    assert b.act_backward(x, ops.ActivationCheckpoint(x, "relu", True, 4, 16, torch.bfloat16)) is None
     assert b.route_forward(x, 2, None, True) is None
-    assert b.route_backward(x, x, x, x, x, x, True, None, None) is None
+    assert b.route_backward(x, ops.Routing(x, x, x, x, x, x, x, x, x, True), None, None) is None
     assert b.act_forward(3, 3, True) is None and b.act_forward(x) is None
 
 
 def test_scratch_of_the_router_is_what_the_library_asks_for():
-    for T in (0, 1, 127, 128, 129, 130, 592 * 16, 592 * 16 + 1, 100000, 1 << 20):
+    for T in (0, 1, 127, 128, 129, 130, 592 * 16, 740 * 16, 740 * 16 + 1, 100000, 1 << 20):
         for E in (1, 7, 256, 1024):
             a, size = L.RouteArgs(experts=E, k=1, tokens=T), C.c_size_t()
             L.check(L.load().bsg_route_scratch_size(C.byref(a), C.byref(size)))
