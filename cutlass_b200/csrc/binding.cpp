@@ -131,8 +131,9 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_XDECREF(device_key);
     const at::Tensor *w = tensor(a[1]), *status = words ? tensor(words) : nullptr;
     if (!w || !status || w->scalar_type() != at::kChar || w->get_device() != dev || w->dim() != (grouped ? 3 : 2)) Py_RETURN_NONE;
-    const int64_t K = x.cols, N = w->size(-2), groups = grouped ? w->size(0) : 1, pitch = (K + 15) & ~int64_t(15);
-    const int64_t ldw = N > 1 ? w->stride(-2) : pitch, group_stride = groups > 1 ? w->stride(0) : 0;
+    const int64_t K = x.cols, N = w->size(-2), groups = grouped ? w->size(0) : 1, whole = (K + 15) & ~int64_t(15);
+    const int64_t pitch = K <= 128 ? whole : (K + 127) & ~int64_t(127);      // of the scratch
+    const int64_t ldw = N > 1 ? w->stride(-2) : whole, group_stride = groups > 1 ? w->stride(0) : 0;
     if (w->size(-1) != K || N < 1 || groups < 1 || groups > BSG_MAX_GROUPS || (K > 1 && w->stride(-1) != 1) || ldw < K || ((ldw | group_stride) & 15) != 0 || (groups > 1 && group_stride < K) || K > 131071 ||
         (reinterpret_cast<uintptr_t>(w->const_data_ptr()) & 15) != 0)
       Py_RETURN_NONE;
@@ -161,7 +162,7 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     c.bias = bias ? bias->const_data_ptr<float>() : nullptr; c.offsets = offsets ? offsets->const_data_ptr<int32_t>() : nullptr;
     c.ldd = N;
     at::Tensor scratch;
-    if (grouped || R > 4 || (R <= 2 ? R : 4) * pitch > 65536) {      // else the tokens are quantised inside the product's kernel
+    if (grouped || R > 4 || (R <= 2 ? R : 4) * whole > 65536) {      // else the tokens are quantised inside the product's kernel
       int64_t held = R;
       if (rows && g.int8_scratch_rows(&c, &held) != BSG_OK) Py_RETURN_NONE;
       scratch = empty({held * (pitch + 4)}, at::kChar, *x.t);        // 8-bit tokens, then their scales

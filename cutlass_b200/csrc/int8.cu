@@ -166,7 +166,7 @@ bool copies_rows(const bsg_int8_args& a) { return a.index && a.rows >= 2 * a.tok
 int32_t copy_rows(const bsg_int8_args& a, const void* q, const float* scale, cudaStream_t s) {
   bsg::I8CopyParams p;
   p.Q = static_cast<const int8_t*>(q); p.scale = scale; p.index = a.index; p.out = static_cast<int8_t*>(a.Q); p.out_scale = a.q_scale;
-  p.rows = int32_t(a.rows); p.tokens = int32_t(a.tokens); p.pitch = int32_t(a.ldq);
+  p.rows = int32_t(a.rows); p.tokens = int32_t(a.tokens); p.pitch = int32_t(a.ldq); p.words = int32_t((a.K + 15) / 16);
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(unsigned((a.rows + 7) / 8), 1, 1);
@@ -189,7 +189,7 @@ int32_t launch_ex(cudaLaunchConfig_t& cfg, int clusters, bool pdl, cudaLaunchAtt
 
 template <int CG, int BN, bool TURN>
 int32_t launch_rows(const bsg_int8_args& a, bsg::I8GemmParams& p, cudaStream_t s, int sms, int dev, bool pdl) {
-  using C = bsg::I8RowsCfg<CG, BN>;
+  using C = bsg::I8RowsCfg<CG, BN, TURN>;
   static SmemOnce once;
   auto kernel = bsg::bsg_i8_rows_kernel<CG, BN, TURN>;
   int32_t rc = once.set(reinterpret_cast<const void*>(kernel), C::kSmemBytes, dev);

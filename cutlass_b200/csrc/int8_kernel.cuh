@@ -233,7 +233,7 @@ struct I8CopyParams {
   const int32_t* index;
   int8_t* out;
   float* out_scale;
-  int32_t rows, tokens, pitch;      // bytes per row, a multiple of 16
+  int32_t rows, tokens, pitch, words;      // bytes between rows, a multiple of 16; 16-byte words of a row
 };
 static __global__ void __launch_bounds__(256) bsg_i8_copy_rows_kernel(const I8CopyParams p) {
   ptx::grid_dependency_wait();
@@ -244,7 +244,7 @@ static __global__ void __launch_bounds__(256) bsg_i8_copy_rows_kernel(const I8Co
   const bool ok = at >= 0 && at < p.tokens;
   const uint4* src = reinterpret_cast<const uint4*>(p.Q + (ok ? int64_t(at) * p.pitch : 0));
   uint4* dst = reinterpret_cast<uint4*>(p.out + int64_t(r) * p.pitch);
-  const int32_t n = p.pitch / 16;
+  const int32_t n = p.words;
   for (int32_t i0 = 0; i0 < n; i0 += 32 * 8) {
     uint4 v[8];
 #pragma unroll
@@ -517,20 +517,27 @@ __device__ __forceinline__ void i8_put(const I8GemmParams& p, const uint32_t (&v
 }
 
 // ---- many rows: D tile = (128 * CG rows) x BN columns, persistent, two accumulators of BN columns in tensor memory.
+// Bound by the tensor cores (8192^3: 316 us, 3.5 P op/s, the pipe 92 % active) and, in a long run, by the power that they take.
 // Eight epilogue warps, two for every quarter of the rows with half of the columns each: with four, a tile took 6 us to finish
 // (latencies of tensor-memory loads, conversions and staged stores, one after the other), more than its products up to K = 2500.
 // The staging of eight warps leaves room for five stages of 256 columns: 2 % slower than six at K = 4096, 8 % faster at K = 512
 // than six with half of the staging.
+// TURN, for groups: the weights are the MMA's rows and the tokens its columns, of which there may be any multiple of 32; the
+// tiles of a group then carry at most 31 tokens too many each, where tiles of 256 rows are on average half empty at a group's
+// end.  A lane of the epilogue holds a channel, and 32 of them a 64-byte piece of a result row, which goes to memory as it is: no
+// staging, and a stage more.  32768 rows in 64 groups of uneven size, 2048 x 7168: 380 us, 397 with five stages, 406 with tiles of
+// 256 rows (what is left to bound it is power: 327 us on weights and tokens of zeros, 390 in tiles of 256 rows).  Asking L2 for weights ahead of their copies made it
+// slower (16 k-tiles ahead 402, 32 ahead 440).
 constexpr int kI8EpiWarps = 8;
 constexpr int kI8RowsThreads = 32 * (2 + kI8EpiWarps);      // warps 0-3 and 6-9 epilogue, 4 MMA, 5 TMA
-template <int CG, int BN>
+template <int CG, int BN, bool TURN>
 struct I8RowsCfg {
   static constexpr int kTileM = 128 * CG;
   static constexpr int kABytes = 128 * 128;
   static constexpr int kBRows = BN / CG;
   static constexpr int kBBytes = kBRows * 128;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kEpiBytes = kI8EpiWarps * 4096;    // per warp 32 rows of 128 bytes
+  static constexpr int kEpiBytes = TURN ? 0 : kI8EpiWarps * 4096;    // per warp 32 rows of 128 bytes
   static constexpr int kColBytes = 2 * 2 * BN * 4;        // scale and bias of the tile's columns, two tiles
   static constexpr int kStagesRaw = (232448 - 1024 - kI8CtlBytes - kEpiBytes - kColBytes) / kStageBytes;
   static constexpr int kStages = kStagesRaw > 8 ? 8 : kStagesRaw;
@@ -543,7 +550,7 @@ template <int CG, int BN, bool TURN>
 __global__ void __launch_bounds__(kI8RowsThreads, 1)
 bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ CUtensorMap tmD, const I8GemmParams p) {
-  using C = I8RowsCfg<CG, BN>;
+  using C = I8RowsCfg<CG, BN, TURN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;

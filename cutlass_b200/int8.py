@@ -43,6 +43,13 @@ def _launch(device: int, stream, made, call, *args) -> None:
         L.check(code)
 
 
+def _pitch(K: int) -> int:
+    """Bytes between 8-bit rows.  Rows on 128-byte boundaries, where they are longer: a copy of 128 of a row's bytes by TMA then
+    takes one line of L2 instead of two (777 x 5000 x 2050, tokens and weights: 15.0 us, on 16-byte boundaries 20.2; only the
+    tokens 17.4)."""
+    return (K + 15) & ~15 if K <= 128 else (K + 127) & ~127
+
+
 def _no_gradient(name, *tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -79,15 +86,15 @@ def quantize_int8(x, *, rows=None, out=None, scale_out=None, stream=None) -> Sca
     ``quantized = sign(x) floor(127 |x| / max|x| + 1/2)``.  A row with a NaN or an infinity gets scale NaN and zeros.
 
     ``rows`` (int32, R entries): row r of the result is made from ``x[rows[r]]`` (an entry outside ``x`` gives zeros with
-    scale NaN), as a grouped product wants its tokens.  The result's rows start on 16-byte boundaries, whatever K is.
-    ``out`` (R, K) int8 with such rows and ``scale_out`` (R,) fp32 may be given.  Asynchronous on ``stream`` (None: torch's
+    scale NaN), as a grouped product wants its tokens.  The result's rows start on 128-byte boundaries (up to K = 128: 16-byte).
+    ``out`` (R, K) int8 with rows on 16-byte boundaries and ``scale_out`` (R,) fp32 may be given.  Asynchronous on ``stream`` (None: torch's
     current stream)."""
     kind, device, M, K, ldx = _matrix("x", x, _IN_KINDS)
     _no_gradient("quantize_int8", x)
     R = M if rows is None else _check_rows(rows, device)
     made = []
     if out is None:
-        made.append(torch.empty((R, -(-K // 16) * 16), dtype=torch.int8, device=x.device))
+        made.append(torch.empty((R, _pitch(K)), dtype=torch.int8, device=x.device))
         out = made[-1][:, :K]
     elif tuple(out.shape) != (R, K) or out.dtype != torch.int8 or out.device != x.device or (K > 1 and out.stride(1) != 1) \
             or (R > 1 and (out.stride(0) < K or out.stride(0) % 16 != 0)) or out.data_ptr() % 16 != 0:
@@ -98,7 +105,7 @@ def quantize_int8(x, *, rows=None, out=None, scale_out=None, stream=None) -> Sca
     _check_array("scale_out", scale_out, torch.float32, (R,), device)
     pack, call = L.direct("bsg_int8_quantize", L.INT8_LAYOUT)
     args = pack(kind, 0, 1, 0, R, M, 1, K, x.data_ptr(), ldx, 0 if rows is None else rows.data_ptr(), out.data_ptr(),
-                out.stride(0) if R > 1 else -(-K // 16) * 16, scale_out.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+                out.stride(0) if R > 1 else _pitch(K), scale_out.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
     _launch(device, stream, made, call, args)
     return ScaledOperand(out, scale_out, (1, 1, K), ScaleSwizzleMode.SwizzleNone)
 
@@ -136,8 +143,8 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
         group_stride = strides[0] if experts > 1 else 0
         _check_array("offsets", offsets, torch.int32, shape[:1], device)
         R = M if rows is None else _check_rows(rows, device)
-    N, pitch = shape[-2], (K + 15) & ~15
-    ldw = strides[-2] if N > 1 else pitch
+    N, whole, pitch = shape[-2], (K + 15) & ~15, _pitch(K)
+    ldw = strides[-2] if N > 1 else whole
     if weight.dtype != torch.int8 or weight.get_device() != device or shape[-1] != K or N < 1:
         raise ValueError(f"weight must be an int8 tensor on CUDA device {device} whose last extent is K = {K}, got {weight.dtype} {tuple(shape)} on {weight.device}")
     if (strides[-1] != 1 and K > 1) or ldw < K or ldw & 15 or w & 15 or group_stride & 15 or (experts > 1 and group_stride < K):
@@ -163,7 +170,7 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
         raise ValueError(f"out dtype {out.dtype} is not supported (bf16, fp16 or fp32)")
     if R == 0:
         return out
-    if offsets is None and R <= 4 and _POWER[R] * pitch <= 65536:      # quantised inside the product's kernel
+    if offsets is None and R <= 4 and _POWER[R] * whole <= 65536:      # quantised inside the product's kernel
         q = q_scale = 0
     else:
         held = R
