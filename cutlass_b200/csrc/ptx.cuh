@@ -94,6 +94,11 @@ __device__ __forceinline__ uint32_t clc_query_first_ctaid_x(uint32_t response) {
       : "memory");
   return ok ? x : 0xFFFFFFFFu;
 }
+__device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t cluster_addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
 // 32-bit store into the shared memory of another CTA of the cluster (address from mapa).
 __device__ __forceinline__ void st_shared_cluster_u32(uint32_t cluster_addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");

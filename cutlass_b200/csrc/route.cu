@@ -18,6 +18,7 @@ using bsg::host_fail;
 
 int64_t route_blocks(int64_t tokens) {
   if (tokens <= bsg::kRouteOneTokens) return 1;
+  if (tokens <= bsg::kRouteClusterTokens) return bsg::kRouteClusterCtas;
   const int64_t b = (tokens + 15) / 16;      // at least two tokens a warp
   return b > bsg::kRouteBlocksMax ? bsg::kRouteBlocksMax : b;
 }
@@ -44,7 +45,7 @@ int32_t check(const bsg_route_args* a, bool forward) {
 }
 
 int64_t scratch_words(const bsg_route_args* a) {
-  if (a->tokens <= bsg::kRouteOneTokens) return 0;
+  if (a->tokens <= bsg::kRouteClusterTokens) return 0;
   return route_pitch(a->tokens) * (2 * a->experts + 1) + a->experts;
 }
 
@@ -107,15 +108,33 @@ int32_t forward_v(const bsg::RouteParams& p, int dev, cudaStream_t s) {
   cudaError_t e;
   if (p.tokens <= bsg::kRouteOneTokens) {
     static SmemOnce once;
-    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteOneWarps, true>;
+    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteOneWarps, 1>;
     const int shared = 2 * bsg::kRouteOneWarps * p.experts * 4;
     int32_t rc = once.set(reinterpret_cast<const void*>(kernel), shared, dev);
     if (rc != BSG_OK) return rc;
     kernel<<<1, bsg::kRouteOneWarps * 32, shared, s>>>(p);
     e = cudaGetLastError();
+  } else if (p.tokens <= bsg::kRouteClusterTokens) {
+    static SmemOnce once;
+    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteOneWarps, bsg::kRouteClusterCtas>;
+    const int shared = 2 * bsg::kRouteOneWarps * p.experts * 4;
+    int32_t rc = once.set(reinterpret_cast<const void*>(kernel), shared, dev);
+    if (rc != BSG_OK) return rc;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(bsg::kRouteClusterCtas, 1, 1);
+    cfg.blockDim = dim3(bsg::kRouteOneWarps * 32, 1, 1);
+    cfg.dynamicSmemBytes = size_t(shared);
+    cfg.stream = s;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = bsg::kRouteClusterCtas; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, p);
   } else {
     static SmemOnce once;
-    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteWarps, false>;
+    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteWarps, 0>;
     const int shared = 2 * bsg::kRouteWarps * p.experts * 4;
     int32_t rc = once.set(reinterpret_cast<const void*>(kernel), shared, dev);
     if (rc != BSG_OK) return rc;

@@ -37,7 +37,7 @@ class Routing(NamedTuple):
 
 
 def _scratch_words(T: int, E: int) -> int:      # what bsg_route_scratch_size says
-    if T <= 128:
+    if T <= 512:
         return 0
     return ((min((T + 15) // 16, 740) + 3) & ~3) * (2 * E + 1) + E
 

@@ -22,7 +22,7 @@ def test_anything_but_cuda_tensors_is_left_alone():
 
 
 def test_scratch_of_the_router_is_what_the_library_asks_for():
-    for T in (0, 1, 127, 128, 129, 130, 592 * 16, 740 * 16, 740 * 16 + 1, 100000, 1 << 20):
+    for T in (0, 1, 128, 16, 17, 512, 513, 520, 1024, 592 * 16, 740 * 16, 740 * 16 + 1, 100000, 1 << 20):
         for E in (1, 7, 256, 1024):
             a, size = L.RouteArgs(experts=E, k=1, tokens=T), C.c_size_t()
             L.check(L.load().bsg_route_scratch_size(C.byref(a), C.byref(size)))

@@ -116,8 +116,8 @@ def test_the_router_refuses_one_way(lib):
     for kw, code in ((dict(offsets=None), 2), (dict(loss=None), 2), (dict(rows=None), 2), (dict(positions=None), 2)):
         assert lib.bsg_route_forward(C.byref(route_args(**kw)), None, 0, None) == code
     assert lib.bsg_route_backward(C.byref(route_args(grad_logits=None)), None) == 2 and lib.bsg_route_backward(C.byref(route_args(ld_grad=15)), None) == 2
-    assert lib.bsg_route_forward(C.byref(route_args(tokens=1000)), None, 0, None) == 4 and lib.bsg_route_forward(C.byref(route_args(tokens=1000)), 0x100, 16, None) == 4
-    assert lib.bsg_route_forward(C.byref(route_args(tokens=1000)), 0x104, 1 << 20, None) == 1
+    assert lib.bsg_route_forward(C.byref(route_args(tokens=2000)), None, 0, None) == 4 and lib.bsg_route_forward(C.byref(route_args(tokens=2000)), 0x100, 16, None) == 4
+    assert lib.bsg_route_forward(C.byref(route_args(tokens=2000)), 0x104, 1 << 20, None) == 1
 
 
 # --------------------------------------------------------------------------------------------------------- Python
