@@ -217,3 +217,77 @@ def test_refusals(cuda_lib):
                  dict(grad_balance_loss=torch.zeros(2, device="cuda")), dict(grad_balance_loss=torch.zeros(()))):
         with pytest.raises(ValueError):
             ops.route_tokens_backward(**{**dict(logits=logits, routing=r, grad_weights=None, grad_balance_loss=None), **case})
+
+
+# ------------------------------------------------------------------------------------- calls that the documentation allows
+def test_no_tokens_at_all(cuda_lib):
+    logits = torch.empty((0, 8), device="cuda", requires_grad=True)
+    r = ops.route_tokens(logits, 2)
+    assert r.experts.shape == (0, 2) and not bool(r.counts.any()) and not bool(r.offsets.any()) and int(r.num_tokens) == 0 and float(r.balance_loss.detach()) == 0.0
+    (r.weights.sum() + r.balance_loss).backward()
+    assert logits.grad.shape == (0, 8)
+    w, ws = product_tests.weights((3, 24), 40, seed=1)
+    end = torch.zeros(3, dtype=torch.int32, device="cuda")
+    none = torch.empty((0, 40), dtype=BF16, device="cuda")
+    assert ops.int8_linear(none, w, ws, offsets=end, rows=torch.empty(0, dtype=torch.int32, device="cuda")).shape == (0, 24)
+    x = torch.empty((0, 48), dtype=BF16, device="cuda", requires_grad=True)
+    ops.checkpointed_activation(x).sum().backward()
+    assert x.grad.shape == (0, 48)
+
+
+def test_rows_of_tokens_that_do_not_exist_are_not_numbers(cuda_lib):
+    w, ws = product_tests.weights((2, 24), 40, seed=1)
+    end = torch.tensor([1, 3], dtype=torch.int32, device="cuda")
+    index = torch.tensor([0, 5, -1], dtype=torch.int32, device="cuda")
+    for tokens in (0, 1):
+        x = product_tests.tokens(1, 40, BF16, seed=2)[:tokens]
+        y = ops.int8_linear(x, w, ws, offsets=end, rows=index)
+        assert bool(torch.isnan(y[tokens:]).all())
+        if tokens:
+            product_tests.check(y[:1], x, w[0], ws[0])
+
+
+def test_the_lowest_weight_and_one_channel(cuda_lib):
+    for M in (1, 40, 600):
+        x = torch.full((M, 131071), -3.0, dtype=BF16, device="cuda")
+        w = torch.full((1, 131072), -128, dtype=torch.int8, device="cuda")[:, :131071]
+        y = ops.int8_linear(x, w, torch.ones(1, device="cuda"), out_dtype=F32)
+        product_tests.check(y, x, w, torch.ones(1, device="cuda"))
+
+
+def test_in_inference_mode_and_with_results_as_leaves(cuda_lib):
+    layer = Layer(30, 64, 32, 4, 2, BF16, seed=6)
+    with torch.inference_mode():
+        r = ops.route_tokens(layer.logits, 2, token_mask=layer.mask)
+        up = ops.int8_linear(layer.x, layer.w1, layer.s1, offsets=r.offsets, rows=r.rows)
+        h, kept = ops.checkpoint_activation(up)
+        down = ops.int8_linear(h, layer.w2, layer.s2, offsets=r.offsets)
+    live = int(r.offsets[-1])
+    again = ops.route_tokens(layer.logits, 2, token_mask=layer.mask)
+    assert torch.equal(r.experts, again.experts) and torch.equal(r.weights, again.weights)
+    up2 = ops.int8_linear(layer.x, layer.w1, layer.s1, offsets=again.offsets, rows=again.rows)
+    assert torch.equal(up[:live], up2[:live])
+    leaf = up2[:live].requires_grad_(True)
+    h2 = ops.checkpointed_activation(leaf)
+    assert torch.equal(h[:live], h2.detach())
+    h2.sum().backward()
+    assert bool(torch.isfinite(leaf.grad).all())
+    assert torch.equal(down[:live], ops.int8_linear(h2.detach(), layer.w2, layer.s2, offsets=again.offsets)[:live])
+
+
+def test_two_streams_at_once(cuda_lib):
+    """The same layer on two streams, many times without waiting: the shared status words are all that they share."""
+    layers = [Layer(200, 128, 72, 8, 2, BF16, seed=s) for s in (7, 8)]
+    want = [[t.clone() for t in layer.run()[1:5]] for layer in layers]
+    streams = [torch.cuda.Stream() for _ in layers]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [None, None]
+    for _ in range(10):
+        for i, (s, layer) in enumerate(zip(streams, layers)):
+            with torch.cuda.stream(s):
+                got[i] = layer.run()[1:5]
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
