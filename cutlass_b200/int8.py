@@ -64,7 +64,7 @@ def _matrix(name, t, kinds):
         raise ValueError(f"{name} must be a 2-D CUDA tensor of type {', '.join(str(k) for k in kinds)}, got {t.dtype} {tuple(shape)} on {t.device}")
     rows, cols = shape
     pitch, step = t.stride()
-    if cols < 1 or (step != 1 and cols > 1) or (rows > 1 and pitch < cols):
+    if cols < 1 or (step != 1 and cols > 1 and rows > 0) or (rows > 1 and pitch < cols):
         raise ValueError(f"{name} must have at least one column, unit stride along its columns and rows that do not overlap")
     return kind, device, rows, cols, (pitch if rows > 1 else cols)
 
