@@ -103,12 +103,12 @@ cudaError_t launch_behind(void (*kernel)(Args...), unsigned grid, unsigned threa
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-template <int TYPE, int V>
+template <int TYPE, int V, int ROUNDS>
 int32_t forward_v(const bsg::RouteParams& p, int dev, cudaStream_t s) {
   cudaError_t e;
   if (p.tokens <= bsg::kRouteOneTokens) {
     static SmemOnce once;
-    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteOneWarps, 1>;
+    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteOneWarps, 1, ROUNDS>;
     const int shared = 2 * bsg::kRouteOneWarps * p.experts * 4;
     int32_t rc = once.set(reinterpret_cast<const void*>(kernel), shared, dev);
     if (rc != BSG_OK) return rc;
@@ -116,7 +116,7 @@ int32_t forward_v(const bsg::RouteParams& p, int dev, cudaStream_t s) {
     e = cudaGetLastError();
   } else if (p.tokens <= bsg::kRouteClusterTokens) {
     static SmemOnce once;
-    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteOneWarps, bsg::kRouteClusterCtas>;
+    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteOneWarps, bsg::kRouteClusterCtas, ROUNDS>;
     const int shared = 2 * bsg::kRouteOneWarps * p.experts * 4;
     int32_t rc = once.set(reinterpret_cast<const void*>(kernel), shared, dev);
     if (rc != BSG_OK) return rc;
@@ -134,7 +134,7 @@ int32_t forward_v(const bsg::RouteParams& p, int dev, cudaStream_t s) {
     e = cudaLaunchKernelEx(&cfg, kernel, p);
   } else {
     static SmemOnce once;
-    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteWarps, 0>;
+    auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteWarps, 0, ROUNDS>;
     const int shared = 2 * bsg::kRouteWarps * p.experts * 4;
     int32_t rc = once.set(reinterpret_cast<const void*>(kernel), shared, dev);
     if (rc != BSG_OK) return rc;
@@ -145,6 +145,16 @@ int32_t forward_v(const bsg::RouteParams& p, int dev, cudaStream_t s) {
   }
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "router launch: %s", cudaGetErrorString(e));
   return BSG_OK;
+}
+// Up to 256 experts (sorted lanes) and k = 8 the rounds are unrolled.
+template <int TYPE, int V>
+int32_t forward_k(const bsg::RouteParams& p, int dev, cudaStream_t s) {
+  if constexpr (V <= 8) {
+    if (p.k <= 2) return forward_v<TYPE, V, 2>(p, dev, s);
+    if (p.k <= 4) return forward_v<TYPE, V, 4>(p, dev, s);
+    if (p.k <= 8) return forward_v<TYPE, V, 8>(p, dev, s);
+  }
+  return forward_v<TYPE, V, 0>(p, dev, s);
 }
 template <int TYPE, int V>
 int32_t backward_v(const bsg::RouteParams& p, int sms, cudaStream_t s) {
@@ -165,7 +175,7 @@ int32_t backward_v(const bsg::RouteParams& p, int sms, cudaStream_t s) {
 }
 template <int TYPE>
 int32_t pick(const bsg::RouteParams& p, bool forward, int dev, int sms, cudaStream_t s) {
-#define BSG_ROUTE_V(V) return forward ? forward_v<TYPE, V>(p, dev, s) : backward_v<TYPE, V>(p, sms, s)
+#define BSG_ROUTE_V(V) return forward ? forward_k<TYPE, V>(p, dev, s) : backward_v<TYPE, V>(p, sms, s)
   if (p.experts <= 32) BSG_ROUTE_V(1);
   if (p.experts <= 64) BSG_ROUTE_V(2);
   if (p.experts <= 128) BSG_ROUTE_V(4);

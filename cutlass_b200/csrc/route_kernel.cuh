@@ -14,8 +14,8 @@
 // a token differ, so a warp counts its rows per expert without atomics and knows the rank of each at once; (1) ranks inside a
 // block and counts per block and expert, (2) prefix over blocks, (3) rows.  A batch of up to 128 tokens is one block, which
 // does all three in one launch.
-// 65536 tokens, 256 experts, k = 8, bf16: (1) 42 us (74 % of the issue slots taken; 34 MB are read, 5 us), (2) and (3), which start
-// while it ends, 9 more; the gradient 23 us (67 MB, 10 us).  16 tokens, 64 experts: 4.2 and 2.9 us.
+// 65536 tokens, 256 experts, k = 8, bf16: (1) 32 us (bound by issue; 34 MB are read, 5 us), (2) and (3), which start while it ends,
+// 9 more; the gradient 23 us (67 MB, 10 us).  16 tokens, 64 experts: 3.6 and 2.5 us.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -221,17 +221,28 @@ __device__ __forceinline__ void route_sort_pairs(uint32_t (&key)[N], uint32_t (&
   });
 }
 
-// The k largest of a warp's values, one per round, until nothing above -inf is left: lane j gets the j-th largest (its value and
-// the lowest expert that has it; expert -1 where there is none).  Up to eight values a lane are sorted first: a lane then shows
-// its largest only, and where that is taken the others move up; more of them are searched in every round.
+// The k largest of a warp's values, one per round: lane j gets the j-th largest (its value and the lowest expert that has it;
+// expert -1 where there is nothing above -inf left).  Up to eight values a lane are sorted first: a lane then shows its largest
+// only, and where that is taken the others move up; more of them are searched in every round.
 // 16-bit logits: the upper half of a 32-bit word takes the key and the lower half the expert (the lower one larger), so that one
-// warp maximum gives both; fp32 logits take a second one, for the expert.  The integer unit, which compares and selects, is what
-// bounds all of this: 65536 tokens, 256 experts, k = 8: 87 us for the kernel when every round searched, took two reductions and
-// turned its result back into a value; 72 with packed keys of fp32 width; 42 sorted, with both halves of a word made at a time.
-template <int TYPE, int V>
+// warp maximum gives both; fp32 logits take a second one, for the expert.  ROUNDS: 2, 4 or 8, at least k, or 0 for k of them;
+// known, the rounds are free of branches, and in each only as many values move up as can still be taken.  The integer unit, which
+// compares and selects, is what bounds all of this: 65536 tokens, 256 experts, k = 8: 87 us for the kernel when every round
+// searched, took two reductions and turned its result back into a value; 72 with packed keys of fp32 width; 42 sorted, with both
+// halves of a word made at a time; 32 with known rounds.
+template <int TYPE, int V, int ROUNDS>
 __device__ __forceinline__ void route_choose(const RouteRow<TYPE, V>& r, int lane, int K, int32_t& my_expert, float& my_logit) {
   constexpr bool kSorted = V <= 8;
   uint32_t won = 0, won_at = 0;
+  auto rounds = [&](auto body) {
+    if constexpr (ROUNDS > 0) {
+#pragma unroll
+      for (int j = 0; j < ROUNDS; ++j) body(j, ROUNDS - 1 - j);
+    } else {
+#pragma unroll 2
+      for (int j = 0; j < K; ++j) body(j, V);
+    }
+  };
   if constexpr (TYPE != kRouteF32) {
     uint32_t key[V];
 #pragma unroll
@@ -241,8 +252,7 @@ __device__ __forceinline__ void route_choose(const RouteRow<TYPE, V>& r, int lan
       if (v + 1 < V) key[v + 1] = (two & 0xFFFF0000u) | uint32_t(kRouteMaxExperts - 1 - RouteMap<V>::expert(lane, v + 1 < V ? v + 1 : v));
     }
     if constexpr (kSorted) route_sort<V>(key);
-#pragma unroll 2
-    for (int j = 0; j < K; ++j) {
+    rounds([&](int j, int left) {      // `left` rounds follow
       uint32_t m = key[0];
       if constexpr (!kSorted) {
 #pragma unroll
@@ -253,14 +263,15 @@ __device__ __forceinline__ void route_choose(const RouteRow<TYPE, V>& r, int lan
       if constexpr (kSorted) {
         if (key[0] == m) {
 #pragma unroll
-          for (int v = 0; v + 1 < V; ++v) key[v] = key[v + 1];
-          key[V - 1] = 0u;
+          for (int v = 0; v < V; ++v) {
+            if (v < left) key[v] = v + 1 < V ? key[v + 1 < V ? v + 1 : v] : 0u;
+          }
         }
       } else {
 #pragma unroll
         for (int v = 0; v < V; ++v) key[v] = key[v] == m ? 0u : key[v];
       }
-    }
+    });
     if ((won | 0xFFFFu) <= route_lowest<TYPE>()) won = 0u;
     won_at = kRouteMaxExperts - 1 - (won & 0xFFFFu);
   } else {
@@ -271,7 +282,7 @@ __device__ __forceinline__ void route_choose(const RouteRow<TYPE, V>& r, int lan
       at[v] = uint32_t(RouteMap<V>::expert(lane, v));
     }
     if constexpr (kSorted) route_sort_pairs<V>(key, at);
-    for (int j = 0; j < K; ++j) {
+    rounds([&](int j, int left) {
       uint32_t m = key[0];
       if constexpr (!kSorted) {
 #pragma unroll
@@ -283,11 +294,12 @@ __device__ __forceinline__ void route_choose(const RouteRow<TYPE, V>& r, int lan
         e = __reduce_min_sync(0xffffffffu, key[0] == m ? at[0] : e);
         if (key[0] == m && at[0] == e) {
 #pragma unroll
-          for (int v = 0; v + 1 < V; ++v) {
-            key[v] = key[v + 1];
-            at[v] = at[v + 1];
+          for (int v = 0; v < V; ++v) {
+            if (v < left) {
+              key[v] = v + 1 < V ? key[v + 1 < V ? v + 1 : v] : 0u;
+              at[v] = at[v + 1 < V ? v + 1 : v];
+            }
           }
-          key[V - 1] = 0u;
         }
       } else {
 #pragma unroll
@@ -300,9 +312,10 @@ __device__ __forceinline__ void route_choose(const RouteRow<TYPE, V>& r, int lan
         won = m;
         won_at = e;
       }
-    }
+    });
+    if (won <= route_lowest<TYPE>()) won = 0u;
   }
-  if (TYPE == kRouteF32 && won <= route_lowest<TYPE>()) won = 0u;
+  if (ROUNDS > 0 && lane >= K) won = 0u;
   my_expert = won ? int32_t(won_at) : -1;
   my_logit = won ? route_value_of<TYPE>(won) : -INFINITY;
 }
@@ -355,7 +368,7 @@ __device__ __forceinline__ float route_loss(float* s_part, int E, int K, int32_t
 // (1) one warp per token: choice, weights, rank of every row among those of its expert in the block, counts and sums of p per
 // block.  CTAS: 0, or that many blocks, one cluster, are all there is and finish everything; they see one another's counts and sums
 // through distributed shared memory.
-template <int TYPE, int V, int WARPS, int CTAS>
+template <int TYPE, int V, int WARPS, int CTAS, int ROUNDS>
 __global__ void __launch_bounds__(WARPS * 32) bsg_route_tokens_kernel(const RouteParams p) {
   constexpr bool ONE = CTAS > 0;
   extern __shared__ uint32_t s_route[];
@@ -380,8 +393,10 @@ __global__ void __launch_bounds__(WARPS * 32) bsg_route_tokens_kernel(const Rout
   const int per_warp = (t1 - t0 + WARPS - 1) / WARPS;
   const int a = min(t0 + warp * per_warp, t1), b = min(a + per_warp, t1);
   constexpr bool kAhead = V <= 8;             // the next token's logits are asked for before this one's are used
-  int k_lanes = 1;
-  while (k_lanes < K) k_lanes <<= 1;
+  int k_lanes = ROUNDS > 0 ? ROUNDS : 1;       // a power of two, at least k
+  if constexpr (ROUNDS == 0) {
+    while (k_lanes < K) k_lanes <<= 1;
+  }
   RouteRow<TYPE, V> raw, next;
   int32_t live_tokens = 0;
   if (a < b) route_load<TYPE, V>(raw, p.logits, int64_t(a) * p.ld, lane, E, p.wide != 0);
@@ -391,7 +406,7 @@ __global__ void __launch_bounds__(WARPS * 32) bsg_route_tokens_kernel(const Rout
     }
     int32_t my_expert = -1;
     float my_logit = -INFINITY;
-    if (!p.mask || p.mask[t] != 0) route_choose<TYPE, V>(raw, lane, K, my_expert, my_logit);
+    if (!p.mask || p.mask[t] != 0) route_choose<TYPE, V, ROUNDS>(raw, lane, K, my_expert, my_logit);
     const float top = __shfl_sync(0xffffffffu, my_logit, 0);
     const bool live = __shfl_sync(0xffffffffu, my_expert, 0) >= 0;
     float x[V];
