@@ -122,7 +122,8 @@ def check_grad(got, want, k, normalize, gw, gl, dtype):
     (70, 33, 4, 0, 0.5, 40), (257, 160, 6, 0.1, 0.2, None), (300, 256, 8, 0, 0, 264), (129, 257, 3, 0.9, 0, None), (64, 513, 8, 0, 0, None),
     (40, 1024, 8, 0.97, 0, None), (1000, 60, 8, 0.05, 0.1, 61), (2500, 17, 2, 0, 0.3, None),
     (512, 16, 4, 0, 0, None), (513, 513, 8, 0.2, 0.1, None), (1100, 160, 6, 0.1, 0.2, 168), (540, 257, 32, 0.5, 0, None), (136, 1000, 2, 0, 0.1, None),
-    (16, 300, 5, 0.1, 0.2, None), (17, 300, 5, 0.1, 0.2, None)])
+    (16, 300, 5, 0.1, 0.2, None), (17, 300, 5, 0.1, 0.2, None),
+    (60, 200, 12, 0.1, 0, None), (700, 128, 7, 0.9, 0.1, None), (90, 256, 32, 0.8, 0, None)])
 def test_routing_and_its_gradient(cuda_lib, T, E, k, masked, padded, pitch, normalize, dtype):
     logits, mask = make(T, E, dtype, seed=T + E, masked=masked, padded=padded, pitch=pitch)
     r = ops.route_tokens(logits, k, token_mask=mask, normalize=normalize)
