@@ -31,20 +31,20 @@ int32_t check(const bsg_act_args* a, bool forward) {
 }
 
 template <int ACT, bool GATED, bool FP16, bool WIDE>
-void launch(const bsg::ActParams& p, bool forward, cudaStream_t s) {
+cudaError_t launch(const bsg::ActParams& p, bool forward, cudaStream_t s) {
   const unsigned per_cta = bsg::kActThreads / (forward ? bsg::kActForwardLanes : bsg::kActBackwardLanes);
   const unsigned grid = (p.items + per_cta - 1) / per_cta;
-  if (forward) bsg::bsg_act_forward_kernel<ACT, GATED, FP16, WIDE><<<grid, bsg::kActThreads, 0, s>>>(p);
-  else bsg::bsg_act_backward_kernel<ACT, GATED, FP16, WIDE><<<grid, bsg::kActThreads, 0, s>>>(p);
+  return bsg::host_launch(forward ? bsg::bsg_act_forward_kernel<ACT, GATED, FP16, WIDE> : bsg::bsg_act_backward_kernel<ACT, GATED, FP16, WIDE>, grid,
+                          bsg::kActThreads, 0, s, p);
 }
 template <int ACT, bool GATED, bool FP16>
-void pick_wide(const bsg::ActParams& p, bool wide, bool forward, cudaStream_t s) {
-  wide ? launch<ACT, GATED, FP16, true>(p, forward, s) : launch<ACT, GATED, FP16, false>(p, forward, s);
+cudaError_t pick_wide(const bsg::ActParams& p, bool wide, bool forward, cudaStream_t s) {
+  return wide ? launch<ACT, GATED, FP16, true>(p, forward, s) : launch<ACT, GATED, FP16, false>(p, forward, s);
 }
 template <int ACT>
-void pick(const bsg::ActParams& p, bool gated, bool fp16, bool wide, bool forward, cudaStream_t s) {
-  if (gated) fp16 ? pick_wide<ACT, true, true>(p, wide, forward, s) : pick_wide<ACT, true, false>(p, wide, forward, s);
-  else fp16 ? pick_wide<ACT, false, true>(p, wide, forward, s) : pick_wide<ACT, false, false>(p, wide, forward, s);
+cudaError_t pick(const bsg::ActParams& p, bool gated, bool fp16, bool wide, bool forward, cudaStream_t s) {
+  if (gated) return fp16 ? pick_wide<ACT, true, true>(p, wide, forward, s) : pick_wide<ACT, true, false>(p, wide, forward, s);
+  return fp16 ? pick_wide<ACT, false, true>(p, wide, forward, s) : pick_wide<ACT, false, false>(p, wide, forward, s);
 }
 
 int32_t run(const bsg_act_args* a, bool forward, void* stream) {
@@ -74,13 +74,13 @@ int32_t run(const bsg_act_args* a, bool forward, void* stream) {
   const bool wide = a->width % 8 == 0 && host_aligned(a->in, 16) && a->ld_in % 8 == 0 && host_aligned(a->out, 16) && a->ld_out % 8 == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool fp16 = a->type == BSG_OUT_F16;
+  cudaError_t e;
   switch (a->activation) {
-    case BSG_ACT_RELU: pick<bsg::kActRelu>(p, a->gated, fp16, wide, forward, s); break;
-    case BSG_ACT_GELU: pick<bsg::kActGelu>(p, a->gated, fp16, wide, forward, s); break;
-    case BSG_ACT_SILU: pick<bsg::kActSilu>(p, a->gated, fp16, wide, forward, s); break;
-    default: pick<bsg::kActIdentity>(p, a->gated, fp16, wide, forward, s); break;
+    case BSG_ACT_RELU: e = pick<bsg::kActRelu>(p, a->gated, fp16, wide, forward, s); break;
+    case BSG_ACT_GELU: e = pick<bsg::kActGelu>(p, a->gated, fp16, wide, forward, s); break;
+    case BSG_ACT_SILU: e = pick<bsg::kActSilu>(p, a->gated, fp16, wide, forward, s); break;
+    default: e = pick<bsg::kActIdentity>(p, a->gated, fp16, wide, forward, s); break;
   }
-  cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "activation launch: %s", cudaGetErrorString(e));
   return BSG_OK;
 }

@@ -194,6 +194,8 @@ __device__ __forceinline__ ActItem<LANES> act_item(const ActParams& p) {
 template <int ACT, bool GATED, bool FP16, bool WIDE>
 __global__ void __launch_bounds__(kActThreads) bsg_act_forward_kernel(const ActParams p) {
   constexpr int kParts = GATED ? 2 : 1;
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   const ActItem<kActForwardLanes> it = act_item<kActForwardLanes>(p);
   const int sub = threadIdx.x % kActForwardLanes;
   const int32_t F = it.ok ? p.F : 0;
@@ -256,6 +258,8 @@ __device__ __forceinline__ void act_dequant4(uint32_t q, float s, float* x) {
 template <int ACT, bool GATED, bool FP16, bool WIDE>
 __global__ void __launch_bounds__(kActThreads) bsg_act_backward_kernel(const ActParams p) {
   constexpr int kParts = GATED ? 2 : 1;
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   const ActItem<kActBackwardLanes> it = act_item<kActBackwardLanes>(p);
   const int sub = threadIdx.x % kActBackwardLanes;
   const bool live = it.ok && it.k < p.F;
@@ -265,13 +269,13 @@ __global__ void __launch_bounds__(kActThreads) bsg_act_backward_kernel(const Act
   const I8Raw rd = i8_raw8<WIDE>(grad, k, live ? p.F : 0);
   const int8_t* q = p.Q + int64_t(it.row) * kParts * p.pitch + k;
   const float* scale = p.scale + int64_t(it.row) * kParts * p.blocks + it.block;
-  const uint2 qg = __ldg(reinterpret_cast<const uint2*>(q));
-  const float sg = __ldg(scale);
+  const uint2 qg = *reinterpret_cast<const uint2*>(q);
+  const float sg = *scale;
   uint2 qu = make_uint2(0, 0);
   float su = 0.0f;
   if constexpr (GATED) {
-    qu = __ldg(reinterpret_cast<const uint2*>(q + p.pitch));
-    su = __ldg(scale + p.blocks);
+    qu = *reinterpret_cast<const uint2*>(q + p.pitch);
+    su = scale[p.blocks];
   }
   float d[8], g[8], u[8], dg[8], du[8];
   act_unpack<FP16>(i8_fix8<WIDE>(rd, grad, k, live ? p.F : 0), d);

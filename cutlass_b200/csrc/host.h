@@ -3,6 +3,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cstdint>
+#include <cstring>
 
 namespace bsg {
 
@@ -20,5 +21,23 @@ inline bool host_aligned(const void* p, uintptr_t bytes) { return (reinterpret_c
 
 // Current device and its SM count; refuses devices that are not sm_100.
 BSG_HIDDEN int32_t host_device(int32_t not_sm100, int32_t cuda_error, int* dev, int* sms);
+
+// Launch with programmatic stream serialisation: the kernel's CTAs are set up while what runs before on the stream ends, and wait
+// for its end and its writes (griddepcontrol.wait) before they touch global memory.
+template <class... P>
+cudaError_t host_launch(void (*kernel)(P...), unsigned grid, unsigned threads, size_t shared, cudaStream_t s, const P&... args) {
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 }  // namespace bsg

@@ -138,11 +138,11 @@ struct SmemOnce {
 template <bool FP16, bool WIDE>
 int32_t launch_quantise(const bsg::I8QuantParams& p, cudaStream_t s) {
   // A thread keeps up to 64 values, so these rows are read once; one warp per row needs no shared memory.
-  if (p.K <= 32 * 64) bsg::bsg_i8_quant_kernel<32, FP16, WIDE><<<(p.rows + 7) / 8, 256, 0, s>>>(p);
-  else if (p.K <= 64 * 64) bsg::bsg_i8_quant_kernel<64, FP16, WIDE><<<(p.rows + 3) / 4, 256, 0, s>>>(p);
-  else if (p.K <= 128 * 64) bsg::bsg_i8_quant_kernel<128, FP16, WIDE><<<(p.rows + 1) / 2, 256, 0, s>>>(p);
-  else bsg::bsg_i8_quant_kernel<512, FP16, WIDE><<<p.rows, 512, 0, s>>>(p);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  if (p.K <= 32 * 64) e = bsg::host_launch(bsg::bsg_i8_quant_kernel<32, FP16, WIDE>, unsigned(p.rows + 7) / 8, 256, 0, s, p);
+  else if (p.K <= 64 * 64) e = bsg::host_launch(bsg::bsg_i8_quant_kernel<64, FP16, WIDE>, unsigned(p.rows + 3) / 4, 256, 0, s, p);
+  else if (p.K <= 128 * 64) e = bsg::host_launch(bsg::bsg_i8_quant_kernel<128, FP16, WIDE>, unsigned(p.rows + 1) / 2, 256, 0, s, p);
+  else e = bsg::host_launch(bsg::bsg_i8_quant_kernel<512, FP16, WIDE>, unsigned(p.rows), 512, 0, s, p);
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "quantiser launch: %s", cudaGetErrorString(e));
   return BSG_OK;
 }
@@ -167,12 +167,7 @@ int32_t copy_rows(const bsg_int8_args& a, const void* q, const float* scale, cud
   bsg::I8CopyParams p;
   p.Q = static_cast<const int8_t*>(q); p.scale = scale; p.index = a.index; p.out = static_cast<int8_t*>(a.Q); p.out_scale = a.q_scale;
   p.rows = int32_t(a.rows); p.tokens = int32_t(a.tokens); p.pitch = int32_t(a.ldq); p.words = int32_t((a.K + 15) / 16);
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(unsigned((a.rows + 7) / 8), 1, 1);
-  cfg.blockDim = dim3(256, 1, 1);
-  cfg.stream = s;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, bsg::bsg_i8_copy_rows_kernel, p);
+  cudaError_t e = bsg::host_launch(bsg::bsg_i8_copy_rows_kernel, unsigned((a.rows + 7) / 8), 256, 0, s, p);
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   return BSG_OK;
 }
@@ -277,8 +272,7 @@ int32_t launch_token(const bsg::I8TokenParams& p, cudaStream_t s, int sms, int d
   int32_t rc = once.set(reinterpret_cast<const void*>(kernel), bsg::kI8TokenShared, dev);
   if (rc != BSG_OK) return rc;
   const int groups = int((int64_t(p.N) * p.parts + 15) / 16), grid = groups < 2 * sms ? groups : 2 * sms;      // two CTAs fit an SM
-  kernel<<<grid, bsg::kI8TokenThreads, MT * ((p.K + 15) / 16 * 16), s>>>(p);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = bsg::host_launch(kernel, unsigned(grid), bsg::kI8TokenThreads, size_t(MT) * ((p.K + 15) / 16 * 16), s, p);
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   return BSG_OK;
 }

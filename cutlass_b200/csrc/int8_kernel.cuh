@@ -12,7 +12,7 @@
 //                         tile carries no padding rows; bound by reading the weights (32 rows in 64 experts, 7168 x 2048:
 //                         61 us, 6.1 TB/s), for one dense tile per CTA by latency (17 x 14336 x 4096: 14 us, 4.2 TB/s)
 //   bsg_i8_token_kernel   up to four tokens, quantised on the way; bound by reading the weights and by latency (one token,
-//                         4096 x 4096: 5.2 us, 3.2 TB/s)
+//                         4096 x 4096: 4.9 us a call, 3.4 TB/s)
 //
 // The two products are dense (one group of rows) or grouped (ragged rows per group, end rows on the device).
 #pragma once
@@ -99,18 +99,19 @@ __device__ __forceinline__ uint4 i8_shift16(const uint4& lo, const uint4& hi, ui
 // looked at.  WIDE: rows start on 16 bytes and K is a multiple of 8 where it ends inside a group.  Otherwise the one or two
 // aligned 16-byte words that hold the values are read whole: a word with at least one value of the row lies in the row's
 // allocation (and on its page), whose bounds are multiples of 16.
+// (Ordinary loads: what a kernel reads may be written by the one before it until it has waited for that one.)
 struct I8Raw { uint4 lo, hi; };
 template <bool WIDE>
 __device__ __forceinline__ I8Raw i8_raw8(const uint16_t* row, int32_t k, int32_t K) {
   I8Raw r;
   r.lo = r.hi = make_uint4(0, 0, 0, 0);
   if constexpr (WIDE) {
-    if (k < K) r.lo = __ldg(reinterpret_cast<const uint4*>(row + k));
+    if (k < K) r.lo = *reinterpret_cast<const uint4*>(row + k);
   } else {
     const uintptr_t a = reinterpret_cast<uintptr_t>(row + k);
     const uint4* at = reinterpret_cast<const uint4*>(a & ~uintptr_t(15));
-    if (k < K) r.lo = __ldg(at);
-    if (k < K && reinterpret_cast<const uint16_t*>(at + 1) < row + K) r.hi = __ldg(at + 1);
+    if (k < K) r.lo = *at;
+    if (k < K && reinterpret_cast<const uint16_t*>(at + 1) < row + K) r.hi = at[1];
   }
   return r;
 }
@@ -168,12 +169,13 @@ __global__ void __launch_bounds__(TPR > kI8QuantThreads ? TPR : kI8QuantThreads)
   const int t = threadIdx.x % TPR;
   const int32_t r = blockIdx.x * kRows + threadIdx.x / TPR;
   __shared__ float s_max[kThreads / 32];
-  // The product behind may start its set-up now (and fetch weights: what it reads besides this kernel's results is older).
+  // The product behind may start its set-up now (and fetch weights: what it reads besides this kernel's results is older, and
+  // complete, since this kernel has waited first).
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
   const bool row_ok = r < p.rows;
   int32_t src = r;
-  if (row_ok && p.index) src = __ldg(p.index + r);
+  if (row_ok && p.index) src = p.index[r];
   const bool src_ok = row_ok && src >= 0 && src < p.tokens;
   const uint16_t* row = p.X + (src_ok ? int64_t(src) * p.ldx : 0);
   const int32_t K = src_ok ? p.K : 0;
@@ -242,7 +244,7 @@ static __global__ void __launch_bounds__(256) bsg_i8_copy_rows_kernel(const I8Co
   ptx::grid_launch_dependents();
   const int32_t r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (r >= p.rows) return;
-  const int32_t at = __ldg(p.index + r);
+  const int32_t at = p.index[r];
   const bool ok = at >= 0 && at < p.tokens;
   const uint4* src = reinterpret_cast<const uint4*>(p.Q + (ok ? int64_t(at) * p.pitch : 0));
   uint4* dst = reinterpret_cast<uint4*>(p.out + int64_t(r) * p.pitch);
@@ -1151,7 +1153,7 @@ struct I8TokenParams {
 __device__ __forceinline__ uint4 i8_weights16(const int8_t* row, int32_t k, int32_t K) {
   if (k + 16 <= K) {
     uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(row + k));
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(row + k));
     return v;
   }
   uint32_t w[4] = {0, 0, 0, 0};
@@ -1186,9 +1188,9 @@ __global__ void __launch_bounds__(kI8TokenThreads, 2) bsg_i8_token_kernel(const 
       }
     }
   };
-  fetch(w, blockIdx.x, 0);      // the weights are read-only for this kernel's whole life
   ptx::grid_dependency_wait();
   ptx::grid_launch_dependents();
+  fetch(w, blockIdx.x, 0);
 
   {
     const int m = threadIdx.x / kPerToken, t = threadIdx.x % kPerToken;
@@ -1268,7 +1270,7 @@ __global__ void __launch_bounds__(kI8TokenThreads, 2) bsg_i8_token_kernel(const 
       }
       const int32_t n = grp * per_group + n_warp + lane / MT, m = lane % MT;
       if (finish && n < p.N && m < p.M) {
-        float x[1] = {i8_finish(uint32_t(mine), s_scale[m], __ldg(p.sb + n), p.bias ? __ldg(p.bias + n) : 0.0f)};
+        float x[1] = {i8_finish(uint32_t(mine), s_scale[m], p.sb[n], p.bias ? p.bias[n] : 0.0f)};
         i8_activate(x, p.activation);
         const int64_t at = int64_t(m) * p.ldd + n;
         if (p.out_kind == kOutBf16) reinterpret_cast<__nv_bfloat16*>(p.D)[at] = __float2bfloat16_rn(x[0]);

@@ -88,21 +88,6 @@ struct SmemOnce {
   }
 };
 
-template <class... Args>
-cudaError_t launch_behind(void (*kernel)(Args...), unsigned grid, unsigned threads, cudaStream_t s, const bsg::RouteParams& p) {
-  cudaLaunchConfig_t cfg;
-  memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(threads, 1, 1);
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 template <int TYPE, int V, int ROUNDS>
 int32_t forward_v(const bsg::RouteParams& p, int dev, cudaStream_t s) {
   cudaError_t e;
@@ -112,8 +97,7 @@ int32_t forward_v(const bsg::RouteParams& p, int dev, cudaStream_t s) {
     const int shared = 2 * bsg::kRouteOneWarps * p.experts * 4;
     int32_t rc = once.set(reinterpret_cast<const void*>(kernel), shared, dev);
     if (rc != BSG_OK) return rc;
-    kernel<<<1, bsg::kRouteOneWarps * 32, shared, s>>>(p);
-    e = cudaGetLastError();
+    e = bsg::host_launch(kernel, 1, bsg::kRouteOneWarps * 32, size_t(shared), s, p);
   } else if (p.tokens <= bsg::kRouteClusterTokens) {
     static SmemOnce once;
     auto kernel = bsg::bsg_route_tokens_kernel<TYPE, V, bsg::kRouteOneWarps, bsg::kRouteClusterCtas, ROUNDS>;
@@ -126,11 +110,13 @@ int32_t forward_v(const bsg::RouteParams& p, int dev, cudaStream_t s) {
     cfg.blockDim = dim3(bsg::kRouteOneWarps * 32, 1, 1);
     cfg.dynamicSmemBytes = size_t(shared);
     cfg.stream = s;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = bsg::kRouteClusterCtas; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = bsg::kRouteClusterCtas; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
     e = cudaLaunchKernelEx(&cfg, kernel, p);
   } else {
     static SmemOnce once;
@@ -138,10 +124,9 @@ int32_t forward_v(const bsg::RouteParams& p, int dev, cudaStream_t s) {
     const int shared = 2 * bsg::kRouteWarps * p.experts * 4;
     int32_t rc = once.set(reinterpret_cast<const void*>(kernel), shared, dev);
     if (rc != BSG_OK) return rc;
-    kernel<<<p.blocks, bsg::kRouteThreads, shared, s>>>(p);
-    e = cudaGetLastError();
-    if (e == cudaSuccess) e = launch_behind(bsg::bsg_route_scan_kernel, (p.experts + 1 + 3) / 4, 128, s, p);
-    if (e == cudaSuccess) e = launch_behind(bsg::bsg_route_order_kernel, p.blocks, bsg::kRouteThreads, s, p);
+    e = bsg::host_launch(kernel, unsigned(p.blocks), bsg::kRouteThreads, size_t(shared), s, p);
+    if (e == cudaSuccess) e = bsg::host_launch(bsg::bsg_route_scan_kernel, unsigned(p.experts + 1 + 3) / 4, 128, 0, s, p);
+    if (e == cudaSuccess) e = bsg::host_launch(bsg::bsg_route_order_kernel, unsigned(p.blocks), bsg::kRouteThreads, 0, s, p);
   }
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "router launch: %s", cudaGetErrorString(e));
   return BSG_OK;
@@ -168,8 +153,7 @@ int32_t backward_v(const bsg::RouteParams& p, int sms, cudaStream_t s) {
     per_sm.store(n, std::memory_order_relaxed);
   }
   const int64_t want = (int64_t(p.tokens) + bsg::kRouteWarps - 1) / bsg::kRouteWarps, most = int64_t(n) * sms;
-  kernel<<<unsigned(want < most ? want : most), bsg::kRouteThreads, shared, s>>>(p);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = bsg::host_launch(kernel, unsigned(want < most ? want : most), bsg::kRouteThreads, shared, s, p);
   if (e != cudaSuccess) return host_fail(BSG_ERR_CUDA, "router launch: %s", cudaGetErrorString(e));
   return BSG_OK;
 }

@@ -103,7 +103,7 @@ __device__ __forceinline__ void route_load(RouteRow<TYPE, V>& r, const void* bas
       if (wide && e0 + C <= E) {
 #pragma unroll
         for (int h = 0; h < C / kPer; ++h) {
-          const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + e0) + h);
+          const uint4 u = reinterpret_cast<const uint4*>(row + e0)[h];
           uint32_t* to = r.w + (g * C + h * kPer) * int(sizeof(T)) / 4;
           to[0] = u.x; to[1] = u.y; to[2] = u.z; to[3] = u.w;
         }
@@ -115,8 +115,8 @@ __device__ __forceinline__ void route_load(RouteRow<TYPE, V>& r, const void* bas
     for (int j = 0; j < C; ++j) {
       bits[j] = kNone;
       if (e0 + j < E) {
-        if constexpr (TYPE == kRouteF32) bits[j] = __float_as_uint(__ldg(row + e0 + j));
-        else bits[j] = __ldg(row + e0 + j);
+        if constexpr (TYPE == kRouteF32) bits[j] = __float_as_uint(row[e0 + j]);
+        else bits[j] = row[e0 + j];
       }
     }
     if constexpr (TYPE == kRouteF32) {
@@ -385,6 +385,7 @@ __global__ void __launch_bounds__(WARPS * 32) bsg_route_tokens_kernel(const Rout
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int e = threadIdx.x; e < WARPS * E; e += WARPS * 32) s_count[e] = 0;
   __syncthreads();
+  ptx::grid_dependency_wait();
   int32_t* my_count = s_count + warp * E;
   float acc[V];
 #pragma unroll
@@ -632,6 +633,7 @@ static __global__ void __launch_bounds__(kRouteThreads) bsg_route_order_kernel(c
   __shared__ int32_t s_scan[kRouteWarps];
   __shared__ float s_part[kRouteWarps];
   ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   const int E = p.experts, K = p.k;
   const int64_t slots = int64_t(p.tokens) * K;
   const int64_t i0 = min(int64_t(blockIdx.x) * p.per_block * K, slots), i1 = min(i0 + int64_t(p.per_block) * K, slots);
@@ -681,6 +683,8 @@ __global__ void __launch_bounds__(kRouteThreads) bsg_route_backward_kernel(const
   __syncwarp();
   int k_lanes = 1;
   while (k_lanes < K) k_lanes <<= 1;
+  ptx::grid_dependency_wait();
+  ptx::grid_launch_dependents();
   const float n = float(max(*p.live, 1));
   const float c = p.grad_loss ? *p.grad_loss * (float(E) / n) : 0.0f;
   float f[V];

@@ -303,7 +303,9 @@ int32_t bsg_ptr_array_run(const bsg_ptr_array_args* args, void* workspace, size_
  * bsg_grouped_args (W, w_scale and bias per group); rows of D at or behind the last end row are not written.
  *
  * Rows of Q and W start on 16-byte boundaries (on 128-byte ones a copy of 128 bytes of a row is one line of L2: faster);
- * K, N, ldd and the alignment of X, D, bias and the scales are free (whole elements).  Nothing is allocated.
+ * K, N, ldd and the alignment of X, D, bias and the scales are free (whole elements).  Nothing is allocated.  These kernels,
+ * like those of bsg_act_* and bsg_route_*, are launched with programmatic stream serialisation: they are set up while what runs
+ * before them on the stream ends, and wait for its end before they read or write.
  */
 typedef struct bsg_int8_args {
   int32_t in_kind;          /* type of X: BSG_OUT_BF16 or BSG_OUT_F16 */

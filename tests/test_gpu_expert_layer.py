@@ -291,3 +291,47 @@ def test_two_streams_at_once(cuda_lib):
     for a, b in zip(want, got):
         for x, y in zip(a, b):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("T,D,F", [(400, 512, 264), (300, 200, 130), (3, 256, 128)])
+def test_each_call_sees_what_the_call_before_it_wrote(cuda_lib, T, D, F):
+    """A long row of calls into the same buffers, each of which reads what the one in front of it has just written, against the
+    same calls with a wait after each: kernels are set up while the ones before them end."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    E, k, steps = 16, 2, 12
+    wide = torch.randn((steps, T, 2 * F), device="cuda", generator=g).to(BF16)
+    w, ws = product_tests.weights((D,), F, seed=1)
+    w2, ws2 = product_tests.weights((E,), D, seed=2)
+    w3, ws3 = product_tests.weights((E, 2 * F), D, seed=3)
+    x, h, y, logits, dx = (torch.zeros(s, dtype=BF16, device="cuda") for s in ((T, 2 * F), (T, F), (T, D), (T, E), (T, 2 * F)))
+    up = torch.zeros((T * k, 2 * F), dtype=BF16, device="cuda")
+
+    def run(wait):
+        made = []
+        done = torch.cuda.synchronize if wait else lambda: None
+        for i in range(steps):
+            x.copy_(wide[i])
+            _, kept = ops.checkpoint_activation(x, "gelu", out=h)
+            done()
+            dx_ = ops.checkpoint_activation_backward(h, kept, out=dx)
+            done()
+            q = ops.quantize_int8(h)
+            done()
+            ops.int8_linear(h, w, ws * 0.01, out=y)
+            done()
+            ops.int8_linear(y, w2, ws2, out=logits)
+            done()
+            r = ops.route_tokens(logits, k)
+            done()
+            d = ops.route_tokens_backward(logits, r, r.weights, r.balance_loss)
+            done()
+            ops.int8_linear(y, w3, ws3, offsets=r.offsets, rows=r.rows, out=up)
+            done()
+            h2, _ = ops.checkpoint_activation(up, "silu")
+            x.zero_()
+            made.append([t.clone() for t in (h, dx_, q.quantized.tensor, q.scale.tensor, y, logits, r.experts, r.rows, r.balance_loss, d, up, h2)])
+        torch.cuda.synchronize()
+        return made
+    for a, b in zip(run(True), run(False)):
+        for s, t in zip(a, b):
+            assert torch.equal(torch.nan_to_num(s.float()), torch.nan_to_num(t.float()))
