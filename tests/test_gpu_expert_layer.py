@@ -335,3 +335,32 @@ def test_each_call_sees_what_the_call_before_it_wrote(cuda_lib, T, D, F):
     for a, b in zip(run(True), run(False)):
         for s, t in zip(a, b):
             assert torch.equal(torch.nan_to_num(s.float()), torch.nan_to_num(t.float()))
+
+
+def test_an_event_of_another_stream_is_waited_for(cuda_lib):
+    """The stream's last call is ours, then comes a wait for another stream that is still busy making the input."""
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    inputs = torch.randn((8, 64, 512), device="cuda", generator=g).to(BF16)
+    want = [(ops.quantize_int8(x).quantized.tensor.clone(), ops.checkpoint_activation(x)[0].clone(), ops.route_tokens(x[:, :64], 3).experts.clone()) for x in inputs]
+    big = torch.randn((4096, 4096), device="cuda", generator=g)
+    x, other = torch.zeros((64, 512), dtype=BF16, device="cuda"), inputs[0].clone()
+    torch.cuda.synchronize()
+    got = []
+    for i in range(8):
+        with torch.cuda.stream(a):
+            a.wait_stream(b)
+            x.zero_()
+            for _ in range(3):
+                big @ big
+            x.copy_(inputs[i])
+            made = a.record_event()
+        with torch.cuda.stream(b):
+            b.wait_stream(a) if i == 0 else None
+            for call in (lambda t: ops.quantize_int8(t).quantized.tensor, lambda t: ops.checkpoint_activation(t)[0], lambda t: ops.route_tokens(t[:, :64], 3).experts):
+                call(other)
+                b.wait_event(made)
+                got.append(call(x).clone())
+    torch.cuda.synchronize()
+    for y, z in zip(got, [t for w in want for t in w]):
+        assert torch.equal(y, z)
