@@ -2,6 +2,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstring>
 #include <mutex>
 
@@ -41,6 +42,10 @@ struct I8Plan {
 // Both sides of some choices: 777 x 5000 x 8192: 128-token tiles 34.3 us, 256 x 256 40.4, 64-token tiles 43.9; 2000 x 5000 x
 // 8192: 256 x 256 60.3, 256 x 128 68.8, 128-token tiles 78.8; 777 x 512 x 512: 32-token tiles 4.6, 16 4.9, 64 6.2, 128 8.1.  Over
 // 85 other problems, drawn at random, the choice took 1.04 times the time of the best variant in the geometric mean, 1.21 at most.
+// Grouped, reading the weights and the rest are added as squares: small tiles read them several times (900 rows in 30 groups,
+// 3001 x 1000: 32-token tiles 17.1 us, 16-token tiles 20.5), which over 36 problems brings the choice from 1.057 to 1.018 times the
+// best.  Results whose rows are no whole 16-byte pieces leave row by row and take the kernel of many rows twice as long (9000 rows
+// in 5 groups, 1500 x 700: 256 x 128 33.4 us, 128-token tiles 22.7).
 struct Variant {
   bool few;
   int32_t tile;
@@ -57,6 +62,8 @@ int32_t choose(const bsg_int8_args& a, I8Plan* plan) {
   const int64_t k_tiles = (a.K + 127) / 128;
   const int64_t active = a.rows < a.num_groups ? a.rows : a.num_groups;      // groups that can have rows
   const double weights = double(a.N) * double(a.K) * double(active > 0 ? active : 1) / kHbmBytesPerUs;
+  const int64_t esz = a.out_kind == BSG_OUT_F32 ? 4 : 2;
+  const bool whole_rows = host_aligned(a.D, 16) && a.ldd * esz % 16 == 0;      // results leave by TMA
   double best = 1e300;
   bool found = false;
   for (const Variant& of : kVariants) {
@@ -78,9 +85,11 @@ int32_t choose(const bsg_int8_args& a, I8Plan* plan) {
       const double tail = tiles * split - waves * slots;
       if (tail > 0.0) waves += !v.few && v.tile == 256 && waves > 0.0 && 2.0 * tail <= slots ? 0.6 : 1.0;      // a thin last wave is split
       double tile_time = double((k_tiles + split - 1) / split) * v.per_k_tile;
-      if (waves > 1.0 && tile_time < v.least) tile_time = v.least;      // (the first tile's epilogue is in `fixed`)
+      const double least = v.few || &v == &kTurned || whole_rows ? v.least : 2.0 * v.least;
+      if (waves > 1.0 && tile_time < least) tile_time = least;      // (the first tile's epilogue is in `fixed`)
       double t = waves * tile_time;
-      if (t < weights) t = weights;
+      if (a.offsets) t = sqrt(t * t + weights * weights);
+      else if (t < weights) t = weights;
       t += v.fixed + (split > 1 ? 0.8 + 0.02 * v.tile : 0.0);      // the cluster's barrier and the exchange of partial sums
       if (t < best) {
         best = t;
