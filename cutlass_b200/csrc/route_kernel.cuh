@@ -12,8 +12,10 @@
 // registers too and leave once per warp; they are added in a fixed order (warp, then block), so results do not change from run
 // to run.  The row order is a stable counting sort: blocks, and warps inside them, own consecutive tokens, and the k experts of
 // a token differ, so a warp counts its rows per expert without atomics and knows the rank of each at once; (1) ranks inside a
-// block and counts per block and expert, (2) prefix over blocks, (3) rows.  A batch of up to 128 tokens is one block, which
-// does all three in one launch.
+// block and counts per block and expert, (2) prefix over blocks, (3) rows.  Up to 16 tokens are one block and up
+// to 512 a cluster of eight, which do all three in one launch: a token to a warp, or four, since a token's latency (1 us with 256
+// experts) is what counts there.  128 tokens, 256 experts, k = 8: 8.2 us a call, 16.4 in one block; 512 tokens: 12.3, 14 in three
+// launches; 1024 tokens: 19.4 and 14.
 // 65536 tokens, 256 experts, k = 8, bf16: (1) 32 us (bound by issue; 34 MB are read, 5 us), (2) and (3), which start while it ends,
 // 9 more; the gradient 23 us (67 MB, 10 us).  16 tokens, 64 experts: 3.6 and 2.5 us.
 #pragma once
@@ -28,7 +30,7 @@ namespace bsg {
 constexpr int kRouteThreads = 256;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kRouteOneWarps = 16;           // warps of the block that does a small batch alone
-constexpr int kRouteOneTokens = 16;
+constexpr int kRouteOneTokens = 16;          // one to a warp
 constexpr int kRouteClusterCtas = 8;         // such blocks, in one cluster, that do a batch together
 constexpr int kRouteClusterTokens = 512;
 constexpr int kRouteBlocksMax = 740;         // five blocks for each of 148 SMs
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(WARPS * 32) bsg_route_tokens_kernel(const Rout
       *p.live = live_all;
     }
   }
-  // this warp's slots: rank in the block, or, in the only block, the row
+  // this warp's slots: rank in the block, or, where this launch is all, the row
   for (int64_t i = int64_t(a) * K + lane; i < int64_t(b) * K; i += 32) {
     const int32_t e = p.chosen[i];
     if (e >= 0) {
