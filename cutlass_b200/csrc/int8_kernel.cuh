@@ -821,10 +821,11 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         }
         i8_activate(x, act);
         // 128 bytes of a row at a time: 32 columns of 32 bits, or two steps of 32 columns of 16 bits (TMA moves a row of a box in
-        // about seven cycles, whatever its length).  Staging: 16-byte piece c of row r at piece c ^ (r & 7).
+        // about seven cycles, whatever its length).  Staging: 16-byte piece c of row r at piece c ^ (r & 7).  Before it is written
+        // again the last copy out of it has to have read it, whatever way this tile goes: the copy may be the tile before's.
         const int second = f32 ? 0 : (c0 >> 5) & 1;
         if (second == 0) {
-          if (tma && lane == 0) ptx::bulk_wait_group_read<0>();
+          if (lane == 0) ptx::bulk_wait_group_read<0>();
           __syncwarp();
         }
         if (f32) {

@@ -212,6 +212,43 @@ def test_more_tiles_than_pairs_of_sms(cuda_lib, M, N, dtype):
     check(out, x, w, ws)
 
 
+@pytest.mark.parametrize("sizes,N,tile,dtype", [((4099,), 2048, 256, BF16), ((4220,), 2048, 256, F32), ((4099,), 2048, 128, BF16), ((4220,), 2048, 128, F16), ((3920,), 11968, 256, BF16),
+                                                ((1000, 517, 0, 333, 2050, 77, 1500), 1024, 128, BF16), ((1000, 517, 0, 333, 2050, 77, 1500), 1024, 128, F32)])
+def test_a_groups_last_rows_behind_whole_tiles(cuda_lib, sizes, N, tile, dtype):
+    """A pair of SMs goes from a tile whose rows leave by asynchronous copies to one that holds a matrix' or a group's last rows,
+    which are stored by threads, with so little to add up that the second tile is ready at once: every value equals that of the
+    kernel for few rows, whose results leave another way."""
+    import ctypes as C
+    M, E, K = sum(sizes), len(sizes), 64
+    x = tokens(M, K, BF16, seed=1)
+    w, ws = weights((E, N), K, seed=2)
+    ws = ws * 0.001
+    A = ops.quantize_int8(x)
+    ends = torch.tensor(sizes, device="cuda").cumsum(0).to(torch.int32)
+    out = torch.full((M, N), math.nan, dtype=dtype, device="cuda")
+    if E > 1:
+        args = ops.GroupedGemmArguments(A, ops.ScaledOperand(w.transpose(1, 2), ws, (1, 1, K), ops.ScaleSwizzleMode.SwizzleNone), out, torch.int32, offsets=ends)
+    else:
+        args = ops.GemmArguments(A, ops.ScaledOperand(w[0].t(), ws[0], (1, 1, K), ops.ScaleSwizzleMode.SwizzleNone), out, torch.int32)
+    a = ops.get_operators(args)[0].build_args(args)
+    workspace = torch.zeros(16, dtype=torch.uint8, device="cuda")
+
+    def product(kernel, tile):
+        out.fill_(math.nan)
+        a.kernel, a.tile = kernel, tile
+        L.check(L.load().bsg_int8_gemm_run(C.byref(a), workspace.data_ptr(), 16, torch.cuda.current_stream().cuda_stream))
+        return out.clone()
+    want = product(1, 64)
+    for _ in range(8):
+        assert torch.equal(product(2, tile), want)
+    L.check(L.load().bsg_read_device_status(workspace.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    begin = 0
+    for e, n in enumerate(sizes):
+        if n:
+            check(want[begin:begin + n], x[begin:begin + n], w[e], ws[e])
+        begin += n
+
+
 def test_the_longest_sum_is_exact(cuda_lib):
     """All products 127 * 127 at the largest K: the sum comes within 2^-9 of the 32-bit range."""
     K = 131071
