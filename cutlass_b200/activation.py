@@ -14,7 +14,7 @@ import torch
 
 from . import lib as L
 from .arguments import ACTIVATIONS
-from .int8 import _IN_KINDS, _launch, _matrix, _no_gradient
+from .int8 import _IN_KINDS, _elsewhere, _launch, _matrix, _no_gradient, _other_stream
 
 BLOCK = 128      # columns of a row that share one scale
 
@@ -63,6 +63,9 @@ def checkpoint_activation(x, activation: str = "silu", *, gated: bool = True, ou
         done = L.binding().act_forward(x, activation, gated)
         if done is not None:
             return done
+    other = _other_stream(x, stream)
+    if other is not None:
+        return _elsewhere(other, checkpoint_activation, x, activation, gated=gated, out=out)
     gated = bool(gated)
     act = ACTIVATIONS.get(activation)
     if act is None:
@@ -76,13 +79,11 @@ def checkpoint_activation(x, activation: str = "silu", *, gated: bool = True, ou
     data = x.new_empty(split + 4 * T * parts * ((F + BLOCK - 1) // BLOCK), dtype=torch.int8)
     if out is None:
         out, ldh = x.new_empty((T, F)), F
-        made = (data, out)
     else:
         ldh = _given("out", out, kind, device, T, F)
-        made = (data,)
     q = data.data_ptr()
     pack, call = L.direct("bsg_act_forward", L.ACT_LAYOUT)
-    _launch(device, stream, made, call, pack(kind, act, parts - 1, 0, T, F, x.data_ptr(), ldx, out.data_ptr(), ldh, q, q + split))
+    _launch(device, call, pack(kind, act, parts - 1, 0, T, F, x.data_ptr(), ldx, out.data_ptr(), ldh, q, q + split))
     return out, ActivationCheckpoint(data, activation, gated, T, F, x.dtype)
 
 
@@ -93,18 +94,20 @@ def checkpoint_activation_backward(grad, kept: ActivationCheckpoint, *, out=None
         dx = L.binding().act_backward(grad, kept)
         if dx is not None:
             return dx
+    other = _other_stream(grad, stream)
+    if other is not None:
+        return _elsewhere(other, checkpoint_activation_backward, grad, kept, out=out)
     data, T, F, parts = kept.data, kept.rows, kept.width, 2 if kept.gated else 1
     kind, device, q = _IN_KINDS[kept.dtype], data.get_device(), data.data_ptr()
     ldg = _given("grad", grad, kind, device, T, F)
     _no_gradient("checkpoint_activation_backward", grad)
     if out is None:
         out, ldx = grad.new_empty((T, parts * F)), parts * F
-        made = (out,)
     else:
-        ldx, made = _given("out", out, kind, device, T, parts * F), ()
+        ldx = _given("out", out, kind, device, T, parts * F)
     pack, call = L.direct("bsg_act_backward", L.ACT_LAYOUT)
-    _launch(device, stream, made, call, pack(kind, ACTIVATIONS[kept.activation], parts - 1, 0, T, F, grad.data_ptr(), ldg, out.data_ptr(), ldx,
-                                             q, q + kept._split()))
+    _launch(device, call, pack(kind, ACTIVATIONS[kept.activation], parts - 1, 0, T, F, grad.data_ptr(), ldg, out.data_ptr(), ldx,
+                               q, q + kept._split()))
     return out
 
 

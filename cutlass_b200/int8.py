@@ -23,24 +23,45 @@ _POWER = (1, 1, 2, 4, 4)       # number of tokens -> the next power of two
 _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
-def _launch(device: int, stream, made, call, *args) -> None:
-    """``call(*args, handle)`` with ``device`` current and the raw handle of ``stream`` (None: torch's current stream of that
-    device).  ``made`` are tensors that were allocated for the call on the current stream: if it runs on another one, the
-    allocator is told."""
+def _launch(device: int, call, *args) -> None:
+    """``call(*args, handle)`` with ``device`` current and the raw handle of torch's current stream of that device."""
     if device != _current_device():
         with torch.cuda.device(device):
-            return _launch(device, stream, made, call, *args)
-    handle = _current_stream(device)
-    if stream is not None:
-        other = to_cuda_stream(stream)
-        if other != handle:
-            s = torch.cuda.ExternalStream(other, device=device) if other else torch.cuda.default_stream(device)
-            for t in made:
-                t.record_stream(s)
-            handle = other
-    code = call(*args, handle)
+            return _launch(device, call, *args)
+    code = call(*args, _current_stream(device))
     if code:
         L.check(code)
+
+
+def _other_stream(x, stream):
+    """``stream`` as a torch stream, where it is another one than torch's current stream of the device of ``x``; else None."""
+    device = x.get_device()
+    if stream is None or device < 0:
+        return None
+    handle = to_cuda_stream(stream)
+    if handle == _current_stream(device):
+        return None
+    return torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+
+
+def _elsewhere(other, call, *args, out=None, **more):
+    """``call`` with ``other`` as torch's current stream, so that what it allocates is memory of that stream: a block that the
+    current stream has given back may still be in use by work queued there, for which ``other`` does not wait.  What is returned
+    is not reused before the work that the stream of the caller has queued by the time it is freed."""
+    here = torch.cuda.current_stream(other.device)
+    with torch.cuda.stream(other):
+        made = call(*args, **more) if out is None else call(*args, out=out, **more)
+
+    def keep(t):
+        if isinstance(t, ScaledOperand):
+            t = (t.quantized.tensor, t.scale.tensor)
+        if isinstance(t, tuple):
+            for part in t:
+                keep(part)
+        elif isinstance(t, torch.Tensor) and t is not out:
+            t.record_stream(here)
+    keep(made)
+    return made
 
 
 def _pitch(K: int) -> int:
@@ -89,24 +110,24 @@ def quantize_int8(x, *, rows=None, out=None, scale_out=None, stream=None) -> Sca
     scale NaN), as a grouped product wants its tokens.  The result's rows start on 128-byte boundaries (up to K = 128: 16-byte).
     ``out`` (R, K) int8 with rows on 16-byte boundaries and ``scale_out`` (R,) fp32 may be given.  Asynchronous on ``stream`` (None: torch's
     current stream)."""
+    other = _other_stream(x, stream)
+    if other is not None:
+        return _elsewhere(other, quantize_int8, x, rows=rows, out=out, scale_out=scale_out)
     kind, device, M, K, ldx = _matrix("x", x, _IN_KINDS)
     _no_gradient("quantize_int8", x)
     R = M if rows is None else _check_rows(rows, device)
-    made = []
     if out is None:
-        made.append(torch.empty((R, _pitch(K)), dtype=torch.int8, device=x.device))
-        out = made[-1][:, :K]
+        out = torch.empty((R, _pitch(K)), dtype=torch.int8, device=x.device)[:, :K]
     elif tuple(out.shape) != (R, K) or out.dtype != torch.int8 or out.device != x.device or (K > 1 and out.stride(1) != 1) \
             or (R > 1 and (out.stride(0) < K or out.stride(0) % 16 != 0)) or out.data_ptr() % 16 != 0:
         raise ValueError(f"out must be an int8 tensor of shape {(R, K)} on {x.device} whose rows start on 16-byte boundaries")
     if scale_out is None:
         scale_out = torch.empty(R, dtype=torch.float32, device=x.device)
-        made.append(scale_out)
     _check_array("scale_out", scale_out, torch.float32, (R,), device)
     pack, call = L.direct("bsg_int8_quantize", L.INT8_LAYOUT)
     args = pack(kind, 0, 1, 0, R, M, 1, K, x.data_ptr(), ldx, 0 if rows is None else rows.data_ptr(), out.data_ptr(),
                 out.stride(0) if R > 1 else _pitch(K), scale_out.data_ptr(), 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
-    _launch(device, stream, made, call, args)
+    _launch(device, call, args)
     return ScaledOperand(out, scale_out, (1, 1, K), ScaleSwizzleMode.SwizzleNone)
 
 
@@ -127,6 +148,9 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
         y = L.binding().int8_linear(x, weight, weight_scale, bias, activation, offsets, rows, out_dtype)
         if y is not None:
             return y
+    other = _other_stream(x, stream)
+    if other is not None:
+        return _elsewhere(other, int8_linear, x, weight, weight_scale, bias, activation=activation, offsets=offsets, rows=rows, out=out, out_dtype=out_dtype)
     in_kind, device, M, K, ldx = _matrix("x", x, _IN_KINDS)
     _no_gradient("int8_linear", x, weight_scale, bias)
     shape, strides, w = weight.shape, weight.stride(), weight.data_ptr()
@@ -157,10 +181,8 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r}: one of {sorted(ACTIVATIONS)}")
-    made = []
     if out is None:
         out, ldd = x.new_empty((R, N), dtype=out_dtype), N
-        made.append(out)
         out_kind = _OUT_KINDS.get(out.dtype)
     else:
         out_kind, out_device, out_rows, out_cols, ldd = _matrix("out", out, _OUT_KINDS)
@@ -179,7 +201,6 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
             L.check(L.load().bsg_int8_scratch_rows(C.byref(L.Int8Args(rows=R, tokens=M, K=K, index=rows.data_ptr())), C.byref(count)))
             held = count.value
         scratch = x.new_empty(held * (pitch + 4), dtype=torch.int8)       # 8-bit tokens, then their scales
-        made.append(scratch)
         q = scratch.data_ptr()
         q_scale = q + held * pitch
     status = _default_workspaces.get(device)
@@ -189,5 +210,5 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
     args = pack(in_kind, out_kind, experts, act, R, M, N, K, x.data_ptr(), ldx, 0 if rows is None else rows.data_ptr(), q, pitch,
                 q_scale, w, ldw, group_stride, weight_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
                 0 if offsets is None else offsets.data_ptr(), out.data_ptr(), ldd, 0, 0, 0, 0)
-    _launch(device, stream, made, call, args, status.data_ptr(), 16)
+    _launch(device, call, args, status.data_ptr(), 16)
     return out

@@ -15,7 +15,7 @@ import torch
 
 from . import lib as L
 from .int8 import _OUT_KINDS as _KINDS
-from .int8 import _check_array, _launch, _matrix
+from .int8 import _check_array, _elsewhere, _launch, _matrix, _other_stream
 
 MAX_EXPERTS, MAX_TOP_K = 1024, 32
 
@@ -76,9 +76,9 @@ def _forward(logits, top_k, token_mask, normalize, stream) -> Routing:
     words = _scratch_words(T, E)
     if words:
         scratch = logits.new_empty(words, dtype=torch.int32)
-        _launch(device, stream, (whole, weights, loss, scratch), call, args, scratch.data_ptr(), 4 * words)
+        _launch(device, call, args, scratch.data_ptr(), 4 * words)
     else:
-        _launch(device, stream, (whole, weights, loss), call, args, 0, 0)
+        _launch(device, call, args, 0, 0)
     softmax, experts, rows, positions, counts, offsets, live = whole.split_with_sizes((2 * T, n, n, n, E, E, 1))
     return Routing(experts.view(T, top_k), weights, counts, offsets, rows, positions.view(T, top_k), loss, live, softmax, normalize)
 
@@ -91,6 +91,9 @@ def route_tokens_backward(logits, routing: Routing, grad_weights=None, grad_bala
         d = L.binding().route_backward(logits, routing, grad_weights, grad_balance_loss)
         if d is not None:
             return d
+    other = _other_stream(logits, stream)
+    if other is not None:
+        return _elsewhere(other, route_tokens_backward, logits, routing, grad_weights, grad_balance_loss)
     experts, counts = routing.experts, routing.counts
     k = experts.shape[1]
     kind, device, T, E, ld = _check_logits(logits, k)
@@ -106,7 +109,7 @@ def route_tokens_backward(logits, routing: Routing, grad_weights=None, grad_bala
     args = pack(kind, E, k, routing.normalize, T, logits.data_ptr(), ld, 0, experts.data_ptr(), routing.weights.data_ptr(),
                 counts.data_ptr(), routing.num_tokens.data_ptr(), routing.softmax.data_ptr(), 0, 0, 0, 0, 0 if grad_weights is None else grad_weights.data_ptr(),
                 0 if grad_balance_loss is None else grad_balance_loss.data_ptr(), out.data_ptr(), E)
-    _launch(device, stream, (out,), call, args)
+    _launch(device, call, args)
     return out
 
 
@@ -142,11 +145,14 @@ def route_tokens(logits, top_k: int, *, token_mask=None, normalize: bool = True,
     e and P_e the mean probability over the n tokens that count: 1 when balanced, 0 when n = 0.
 
     E is at most 1024 and k at most 32.  Results do not depend on the order in which anything runs.  Asynchronous on ``stream``
-    (None: torch's current stream); the backward pass runs on the stream that autograd makes current."""
+    (None: torch's current stream); autograd runs the backward pass on the same one."""
     if stream is None and logits.is_cuda:      # (None for logits that want a gradient, too)
         r = L.binding().route_forward(logits, top_k, token_mask, normalize)
         if r is not None:
             return r
+    other = _other_stream(logits, stream)
+    if other is not None:
+        return _elsewhere(other, route_tokens, logits, top_k, token_mask=token_mask, normalize=normalize)
     if not (torch.is_grad_enabled() and logits.requires_grad):
         return _forward(logits, top_k, token_mask, normalize, stream)
     weights, loss, experts, counts, offsets, rows, positions, live, softmax = _Route.apply(logits, top_k, token_mask, normalize, stream)

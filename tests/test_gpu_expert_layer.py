@@ -364,3 +364,72 @@ def test_an_event_of_another_stream_is_waited_for(cuda_lib):
     torch.cuda.synchronize()
     for y, z in zip(got, [t for w in want for t in w]):
         assert torch.equal(y, z)
+
+
+# ------------------------------------------------------------------------------------------------------ memory of two streams
+def _calls(seed):
+    """Every operator once, as functions of the stream; inputs of their own."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((600, 512), device="cuda", generator=g).to(BF16)
+    w, ws = product_tests.weights((256,), 512, seed=1)
+    w3, ws3 = product_tests.weights((2, 256), 512, seed=2)
+    ends = torch.tensor([250, 600], dtype=torch.int32, device="cuda")
+    index = torch.randperm(600, device="cuda", generator=g).to(torch.int32)
+    logits = torch.randn((600, 64), device="cuda", generator=g)
+    _, kept = ops.checkpoint_activation(x)
+    r = ops.route_tokens(logits, 4)
+    return [lambda s: [ops.quantize_int8(x, stream=s).quantized.tensor], lambda s: [ops.int8_linear(x, w, ws, stream=s)],
+            lambda s: [ops.int8_linear(x, w3, ws3, offsets=ends, rows=index, stream=s)],
+            lambda s: list(ops.checkpoint_activation(x, stream=s)[:1]), lambda s: [ops.checkpoint_activation_backward(x[:, :256], kept, stream=s)],
+            lambda s: list(ops.route_tokens(logits, 4, stream=s)[:7]), lambda s: [ops.route_tokens_backward(logits, r, r.weights, None, stream=s)]]
+
+
+def test_a_given_stream_gets_memory_of_its_own(cuda_lib):
+    """A block that the current stream has just given back may still be in use by work queued there: a call on another stream,
+    which does not wait for that work, gets none of it."""
+    side = torch.cuda.Stream()
+    for call in _calls(3):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        sizes = sorted({t.untyped_storage().nbytes() for t in call(None)})
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        held = [torch.empty(n, dtype=torch.int8, device="cuda") for n in sizes for _ in range(12)]
+        given_back = [(t.data_ptr(), t.data_ptr() + t.numel()) for t in held]
+        del held
+        for t in call(side):
+            at = t.untyped_storage().data_ptr()
+            assert not any(a <= at < b for a, b in given_back)
+        side.synchronize()
+
+
+def test_calls_on_two_streams_by_turns(cuda_lib):
+    """Calls of the same sizes on the current stream and, by argument, on another one, many of them without waiting, and their
+    temporaries given back at once."""
+    side = torch.cuda.Stream()
+    here, there = _calls(4), _calls(5)
+    want = [[[t.clone() for t in call(None)] for call in calls] for calls in (here, there)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = [[], []]
+        for a, b in zip(here, there):
+            got[0].append(a(None))
+            got[1].append(b(side))
+        torch.cuda.synchronize()
+        for w, g in zip(want, got):
+            for s, t in zip(w, g):
+                for y, z in zip(s, t):
+                    assert torch.equal(y, z)
+
+
+def test_the_gradient_of_a_routing_on_a_given_stream(cuda_lib):
+    logits = torch.randn((700, 32), device="cuda")
+    a, b = logits.clone().requires_grad_(), logits.clone().requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    r, s = ops.route_tokens(a, 3, stream=side), ops.route_tokens(b, 3)
+    torch.cuda.current_stream().wait_stream(side)
+    for q in (r, s):
+        (q.weights.square().sum() + q.balance_loss).backward()
+    torch.cuda.synchronize()
+    assert torch.equal(r.weights, s.weights) and torch.equal(a.grad, b.grad)
