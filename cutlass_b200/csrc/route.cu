@@ -72,12 +72,12 @@ bsg::RouteParams params(const bsg_route_args* a, void* scratch) {
   return p;
 }
 
-// Kernels that use more than 48 KB of shared memory (more than 768 or 384 experts) are allowed to once per device.
+// Kernels that use more than 48 KB of shared memory, their few hundred static bytes included, are allowed to once per device.
 struct SmemOnce {
   std::mutex mu;
   bool done[64] = {};
   int32_t set(const void* kernel, int bytes, int dev) {
-    if (bytes <= 48 * 1024) return BSG_OK;
+    if (bytes <= 48 * 1024 - kStaticMost) return BSG_OK;
     if (dev < 0 || dev >= 64) return host_fail(BSG_ERR_NOT_SUPPORTED, "device ordinal %d is outside [0, 64)", dev);
     std::lock_guard<std::mutex> lock(mu);
     if (done[dev]) return BSG_OK;
@@ -86,6 +86,7 @@ struct SmemOnce {
     done[dev] = true;
     return BSG_OK;
   }
+  static constexpr int kStaticMost = 1024;      // the arrays of one entry per warp take up to 208
 };
 
 template <int TYPE, int V, int ROUNDS>

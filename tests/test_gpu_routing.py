@@ -265,3 +265,16 @@ def test_streams_and_graphs(cuda_lib):
         for _, q, d, k in graphs:
             want = check(logits, k, mask, True, q)
             check_grad(d, want, k, True, torch.zeros_like(q.weights), float(q.balance_loss), BF16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("E", [383, 384, 385, 767, 768, 769])
+@pytest.mark.parametrize("T", [9, 100, 600])
+def test_expert_counts_around_48_kilobytes_of_shared_memory(cuda_lib, T, E, dtype):
+    """Static and dynamic shared memory count together: one block, a cluster and many blocks, on both sides of what needs no
+    permission."""
+    logits, mask = make(T, E, dtype, seed=E, masked=0.1, padded=0.1)
+    r = ops.route_tokens(logits, 8, token_mask=mask)
+    want = check(logits, 8, mask, True, r)
+    gw, gl = torch.randn((T, 8), device="cuda"), torch.tensor(0.7, device="cuda")
+    check_grad(ops.route_tokens_backward(logits, r, gw, gl), want, 8, True, gw, gl, dtype)
