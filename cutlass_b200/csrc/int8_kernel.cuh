@@ -266,6 +266,7 @@ static __global__ void __launch_bounds__(256) bsg_i8_copy_rows_kernel(const I8Co
 }
 
 // ------------------------------------------------------------------------------------------------ products
+// Barriers and loads of tensor memory are instructions of whole warps (.aligned): a __syncwarp stands before each.
 struct I8GemmParams {
   int32_t num_groups;         // 1 for a dense product
   int32_t total_rows, N, K;
@@ -728,6 +729,7 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       float* sa = sCol + acc * 256;
       sa[epi * 32 + lane] = d.sa;
       if (t + num_clusters < total_work) need = need_of(t + num_clusters);
+      __syncwarp();
       asm volatile("bar.sync 1, 256;" ::: "memory");
       i8_wait(tfull0 + acc * 8, uint32_t(it >> 1) & 1u, ctl, dead);
       __syncwarp();
@@ -736,6 +738,7 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll 1
       for (int c0 = half * 32; c0 < d.height; c0 += 64) {
         uint32_t v[32];
+        __syncwarp();
         ptx::tmem_ld_32x32b_x32(lane_addr + c0, v);
         ptx::tmem_ld_wait();
         if (d.n < p.N && c0 < d.rows) i8_put(p, v, sa + c0, min(32, d.rows - c0), d.sb, d.bias, int64_t(d.row0 + c0) * p.ldd + d.n);
@@ -786,6 +789,7 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         cs[BN + epi * 32 + lane] = need.bias;
       }
       if (t + num_clusters < total_work) need = need_of(t + num_clusters);
+      __syncwarp();
       asm volatile("bar.sync 1, 256;" ::: "memory");
       i8_wait(tfull0 + acc * 8, uint32_t(it >> 1) & 1u, ctl, dead);
       __syncwarp();
@@ -798,6 +802,7 @@ bsg_i8_rows_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll 1
       for (int c0 = half * (cols / 2); c0 < c_end; c0 += 32) {
         uint32_t v[32];
+        __syncwarp();
         ptx::tmem_ld_32x32b_x32(lane_addr + c0, v);
         ptx::tmem_ld_wait();
         if (c0 + 32 == c_end) {
@@ -1059,6 +1064,7 @@ bsg_i8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
       const int32_t cols = min(BT, ti.row_end - ti.row0);
       float* sa = sSa + acc * BT;
       if (threadIdx.x < BT) sa[threadIdx.x] = int32_t(threadIdx.x) < cols ? __ldcg(p.sa + ti.row0 + threadIdx.x) : 0.0f;
+      __syncwarp();
       asm volatile("bar.sync 1, 128;" ::: "memory");
       i8_wait(tfull0 + acc * 8, uint32_t(it >> 1) & 1u, ctl, dead);
       __syncwarp();
@@ -1067,6 +1073,7 @@ bsg_i8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant
 #pragma unroll 1
       for (int c0 = 0; c0 < BT; c0 += kChunk) {
         uint32_t v[kChunk];
+        __syncwarp();
         if constexpr (kChunk == 32) ptx::tmem_ld_32x32b_x32(lane_addr + c0, v);
         else i8_tmem_ld_x16(lane_addr + c0, v);
         ptx::tmem_ld_wait();

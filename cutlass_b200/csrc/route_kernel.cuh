@@ -510,6 +510,7 @@ __global__ void __launch_bounds__(WARPS * 32) bsg_route_tokens_kernel(const Rout
         }
       }
       if (threadIdx.x == 0) s_live_mine = live_all;
+      __syncwarp();      // (the barrier's instructions want a whole warp at once, also below)
       ptx::cluster_arrive();
       ptx::cluster_wait();
       live_all = 0;
@@ -536,6 +537,7 @@ __global__ void __launch_bounds__(WARPS * 32) bsg_route_tokens_kernel(const Rout
           }
         }
       }
+      __syncwarp();
       ptx::cluster_arrive();      // what this block needed of the others it has; it leaves when they have theirs
     }
 #pragma unroll
@@ -581,7 +583,10 @@ __global__ void __launch_bounds__(WARPS * 32) bsg_route_tokens_kernel(const Rout
   }
   if constexpr (ONE) {
     for (int64_t r = total + int64_t(blockIdx.x) * WARPS * 32 + threadIdx.x; r < int64_t(p.tokens) * K; r += CTAS * WARPS * 32) p.rows[r] = -1;
-    if constexpr (CTAS > 1) ptx::cluster_wait();
+    if constexpr (CTAS > 1) {
+      __syncwarp();
+      ptx::cluster_wait();
+    }
   }
 }
 
