@@ -14,7 +14,7 @@ import torch
 
 from . import lib as L
 from .arguments import ACTIVATIONS
-from .int8 import _IN_KINDS, _elsewhere, _launch, _matrix, _no_gradient, _other_stream
+from .int8 import _IN_KINDS, _check_array, _elsewhere, _launch, _matrix, _no_gradient, _other_stream
 
 BLOCK = 128      # columns of a row that share one scale
 
@@ -98,7 +98,11 @@ def checkpoint_activation_backward(grad, kept: ActivationCheckpoint, *, out=None
     if other is not None:
         return _elsewhere(other, checkpoint_activation_backward, grad, kept, out=out)
     data, T, F, parts = kept.data, kept.rows, kept.width, 2 if kept.gated else 1
-    kind, device, q = _IN_KINDS[kept.dtype], data.get_device(), data.data_ptr()
+    kind, act, device = _IN_KINDS.get(kept.dtype), ACTIVATIONS.get(kept.activation), data.get_device()
+    if kind is None or act is None or type(T) is not int or type(F) is not int or T < 0 or F < 1:
+        raise ValueError(f"kept is no checkpoint: activation {kept.activation!r}, {T!r} rows of {F!r} values of {kept.dtype}")
+    _check_array("kept.data", data, torch.int8, (kept._split() + 4 * T * parts * -(-F // BLOCK),), device)
+    q = data.data_ptr()
     ldg = _given("grad", grad, kind, device, T, F)
     _no_gradient("checkpoint_activation_backward", grad)
     if out is None:
@@ -106,7 +110,7 @@ def checkpoint_activation_backward(grad, kept: ActivationCheckpoint, *, out=None
     else:
         ldx = _given("out", out, kind, device, T, parts * F)
     pack, call = L.direct("bsg_act_backward", L.ACT_LAYOUT)
-    _launch(device, call, pack(kind, ACTIVATIONS[kept.activation], parts - 1, 0, T, F, grad.data_ptr(), ldg, out.data_ptr(), ldx,
+    _launch(device, call, pack(kind, act, parts - 1, 0, T, F, grad.data_ptr(), ldg, out.data_ptr(), ldx,
                                q, q + kept._split()))
     return out
 

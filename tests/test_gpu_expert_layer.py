@@ -433,3 +433,17 @@ def test_the_gradient_of_a_routing_on_a_given_stream(cuda_lib):
         (q.weights.square().sum() + q.balance_loss).backward()
     torch.cuda.synchronize()
     assert torch.equal(r.weights, s.weights) and torch.equal(a.grad, b.grad)
+
+
+def test_refusals_of_a_checkpoint_that_does_not_fit(cuda_lib):
+    """The checkpoint is looked at field by field, whichever way the call goes (a stream or an output given, or neither)."""
+    x = torch.randn((6, 400), device="cuda").to(BF16)
+    h, kept = ops.checkpoint_activation(x)
+    stream, out = torch.cuda.current_stream(), torch.empty_like(x)
+    bad = [dict(data=kept.data[:-16]), dict(data=kept.data[:0]), dict(data=torch.cat([kept.data, kept.data])), dict(data=kept.data.view(torch.uint8)), dict(data=kept.data[None]),
+           dict(data=kept.data.cpu()), dict(data=torch.zeros(2 * kept.data.numel(), dtype=torch.int8, device="cuda")[::2]), dict(rows=7), dict(width=201), dict(rows=6.0), dict(rows=-1),
+           dict(gated=False), dict(activation="tanh"), dict(dtype=F32), dict(dtype=F16)]
+    for change in bad:
+        for how in (dict(), dict(stream=stream), dict(out=out)):
+            with pytest.raises(ValueError):
+                ops.checkpoint_activation_backward(h, kept._replace(**change), **how)
