@@ -705,6 +705,7 @@ __global__ void __launch_bounds__(kRouteThreads) bsg_route_backward_kernel(const
   auto slot_of = [&](int t) {
     Slot s;
     s.e = lane < K ? p.chosen[int64_t(t) * K + lane] : -1;
+    if (s.e >= E) s.e = -1;      // (none that the forward pass writes: an index behind this warp's part of shared memory)
     s.w = lane < K ? p.weights[int64_t(t) * K + lane] : 0.0f;
     s.gw = lane < K && p.grad_weights ? p.grad_weights[int64_t(t) * K + lane] : 0.0f;
     s.soft = p.softmax[t];

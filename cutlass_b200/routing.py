@@ -95,10 +95,13 @@ def route_tokens_backward(logits, routing: Routing, grad_weights=None, grad_bala
     if other is not None:
         return _elsewhere(other, route_tokens_backward, logits, routing, grad_weights, grad_balance_loss)
     experts, counts = routing.experts, routing.counts
+    if experts.dim() != 2:
+        raise ValueError(f"routing.experts must be (tokens, k), got {tuple(experts.shape)}")
     k = experts.shape[1]
     kind, device, T, E, ld = _check_logits(logits, k)
-    if experts.shape[0] != T or counts.shape[0] != E or experts.get_device() != device:
-        raise ValueError("routing does not belong to these logits")
+    for name, dtype, shape in (("experts", torch.int32, (T, k)), ("weights", torch.float32, (T, k)), ("counts", torch.int32, (E,)),
+                               ("num_tokens", torch.int32, (1,)), ("softmax", torch.int32, (2 * T,))):
+        _check_array("routing." + name, getattr(routing, name), dtype, shape, device)
     if grad_weights is not None:
         _check_array("grad_weights", grad_weights, torch.float32, experts.shape, device)
     if grad_balance_loss is not None and (grad_balance_loss.dtype != torch.float32 or grad_balance_loss.numel() != 1

@@ -447,3 +447,28 @@ def test_refusals_of_a_checkpoint_that_does_not_fit(cuda_lib):
         for how in (dict(), dict(stream=stream), dict(out=out)):
             with pytest.raises(ValueError):
                 ops.checkpoint_activation_backward(h, kept._replace(**change), **how)
+
+
+def test_refusals_of_a_routing_that_does_not_fit(cuda_lib):
+    stream = torch.cuda.current_stream()
+    logits = torch.randn((6, 8), device="cuda")
+    r = ops.route_tokens(logits, 2)
+    for change in (dict(experts=r.experts[:, :1]), dict(experts=r.experts.t().contiguous().t()), dict(experts=r.experts.long()), dict(experts=r.experts.reshape(-1)), dict(weights=r.weights[:5]),
+                   dict(weights=r.weights.half()), dict(weights=r.weights.cpu()), dict(weights=torch.zeros((6, 4), device="cuda")[:, ::2]), dict(counts=r.counts[:7]), dict(counts=r.counts.float()),
+                   dict(num_tokens=r.num_tokens[:0]), dict(num_tokens=r.num_tokens.long()), dict(softmax=r.softmax[:-1]), dict(softmax=r.softmax.view(F32)), dict(softmax=r.softmax.view(6, 2)),
+                   dict(softmax=r.softmax.cpu())):
+        for how in (dict(), dict(stream=stream)):
+            with pytest.raises(ValueError):
+                ops.route_tokens_backward(logits, r._replace(**change), torch.ones((6, r.weights.shape[1]), device="cuda"), None, **how)
+
+
+def test_choices_that_are_no_experts_have_no_gradient(cuda_lib):
+    """A choice outside the experts reads and writes nothing: the slot counts as one that chose nothing."""
+    logits = torch.randn((50, 8), device="cuda")
+    r = ops.route_tokens(logits, 3)
+    gw = torch.randn((50, 3), device="cuda")
+    none, outside = r.experts.clone(), r.experts.clone()
+    none[::3, 1:], outside[::3, 1:] = -1, 1 << 20
+    none[1, 2], outside[1, 2] = -1, 8
+    gl = torch.ones((), device="cuda")
+    assert torch.equal(ops.route_tokens_backward(logits, r._replace(experts=outside), gw, gl), ops.route_tokens_backward(logits, r._replace(experts=none), gw, gl))
