@@ -392,9 +392,10 @@ __global__ void __launch_bounds__(WARPS * 32) bsg_route_tokens_kernel(const Rout
   float acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-  const int t0 = blockIdx.x * p.per_block, t1 = min(t0 + p.per_block, p.tokens);
-  const int per_warp = (t1 - t0 + WARPS - 1) / WARPS;
-  const int a = min(t0 + warp * per_warp, t1), b = min(a + per_warp, t1);
+  // (no sum passes the number of tokens, which may be 2^31 - 1)
+  const int t0 = blockIdx.x * p.per_block, mine_all = min(p.per_block, p.tokens - t0);
+  const int per_warp = (mine_all + WARPS - 1) / WARPS;
+  const int a = t0 + min(warp * per_warp, mine_all), b = a + min(per_warp, t0 + mine_all - a);
   constexpr bool kAhead = V <= 8;             // the next token's logits are asked for before this one's are used
   int k_lanes = ROUNDS > 0 ? ROUNDS : 1;       // a power of two, at least k
   if constexpr (ROUNDS == 0) {
@@ -720,9 +721,12 @@ __global__ void __launch_bounds__(kRouteThreads) bsg_route_backward_kernel(const
     route_load<TYPE, V>(raw, p.logits, int64_t(t) * p.ld, lane, E, p.wide != 0);
     slot = slot_of(t);
   }
-  for (; t < p.tokens; t += step) {
+  const int before_last = p.tokens - step;      // t < before_last: there is a next token (t + step may pass 2^31)
+  bool more = t < p.tokens;
+  while (more) {
+    more = t < before_last;
     if constexpr (kAhead) {
-      if (t + step < p.tokens) {
+      if (more) {
         route_load<TYPE, V>(next, p.logits, int64_t(t + step) * p.ld, lane, E, p.wide != 0);
         next_slot = slot_of(t + step);
       }
@@ -785,10 +789,11 @@ __global__ void __launch_bounds__(kRouteThreads) bsg_route_backward_kernel(const
     if constexpr (kAhead) {
       raw = next;
       slot = next_slot;
-    } else if (t + step < p.tokens) {
+    } else if (more) {
       route_load<TYPE, V>(raw, p.logits, int64_t(t + step) * p.ld, lane, E, p.wide != 0);
       slot = slot_of(t + step);
     }
+    if (more) t += step;
   }
 }
 

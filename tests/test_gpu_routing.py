@@ -278,3 +278,47 @@ def test_expert_counts_around_48_kilobytes_of_shared_memory(cuda_lib, T, E, dtyp
     want = check(logits, 8, mask, True, r)
     gw, gl = torch.randn((T, 8), device="cuda"), torch.tensor(0.7, device="cuda")
     check_grad(ops.route_tokens_backward(logits, r, gw, gl), want, 8, True, gw, gl, dtype)
+
+
+def test_as_many_tokens_as_31_bits_count(cuda_lib):
+    """2^31 - 1 tokens, the largest number that is taken: all but the last 300 have equal logits and choose the first expert."""
+    T, n = (1 << 31) - 1, 300
+    if torch.cuda.mem_get_info()[0] < 110 << 30:
+        pytest.skip("needs 110 GiB of device memory")
+    torch.cuda.empty_cache()
+    logits = torch.zeros((T, 2), dtype=BF16, device="cuda")
+    logits[-n:], _ = make(n, 2, BF16, seed=11)
+    tail = logits[-n:].double().cpu()
+    pick = (tail[:, 1] > tail[:, 0]).long()
+    r = ops.route_tokens(logits, 1, normalize=False)
+    second = int(pick.sum())
+    assert r.counts.tolist() == [T - second, second] and r.offsets.tolist() == [T - second, T] and int(r.num_tokens) == T
+    step = 1 << 28
+    for lo in range(0, T - n, step):
+        hi = min(lo + step, T - n)
+        at = torch.arange(lo, hi, dtype=torch.int32, device="cuda")
+        assert not bool(r.experts[lo:hi].any()) and bool((r.weights[lo:hi] == 0.5).all())
+        assert torch.equal(r.rows[lo:hi], at) and torch.equal(r.positions[lo:hi, 0], at)
+    token = torch.arange(T - n, T)
+    assert torch.equal(r.experts[-n:, 0].cpu().long(), pick)
+    assert torch.equal(r.rows[T - n:].cpu().long(), torch.cat([token[pick == 0], token[pick == 1]]))
+    place = torch.where(pick == 0, T - n + (pick == 0).long().cumsum(0) - 1, T - second + pick.cumsum(0) - 1)
+    assert torch.equal(r.positions[-n:, 0].cpu().long(), place)
+    p = torch.softmax(tail, 1)
+    w = p.gather(1, pick[:, None])
+    assert bool(((r.weights[-n:].cpu().double() - w).abs() <= 2.0 ** -17 * w).all())
+    want = 2 * ((T - second) / T * (0.5 * (T - n) + float(p[:, 0].sum())) / T + second / T * (0.5 * (T - n) + float(p[:, 1].sum())) / T)
+    assert abs(float(r.balance_loss) - want) <= 2.0 ** -16 * want
+    gw = torch.zeros((T, 1), device="cuda")
+    gw[-n:] = torch.randn((n, 1), device="cuda")
+    d = ops.route_tokens_backward(logits, r, gw, None)
+    for lo in range(0, T - n, step):
+        assert not bool(d[lo:min(lo + step, T - n)].any())
+    part = w * gw[-n:].cpu().double()
+    ref = torch.zeros_like(p).scatter_(1, pick[:, None], part) - p * part
+    size = torch.zeros_like(p).scatter_(1, pick[:, None], part.abs()) + p * part.abs()
+    tol = 4 * 2.0 ** -17 * size
+    tol = tol + torch.finfo(BF16).eps / 2 * (ref.abs() + tol)
+    assert bool(((d[-n:].cpu().double() - ref).abs() <= tol).all())
+    del logits, r, gw, d
+    torch.cuda.empty_cache()
