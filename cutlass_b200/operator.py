@@ -556,7 +556,17 @@ class Int8GemmOperator(Operator):
         return a
 
     def _run(self, args, artifact: CompiledArtifact, stream: int, workspace) -> None:
-        ws = self._resolve_workspace(workspace, args.out.tensor.device)
+        device = args.out.tensor.device
+        bias = args.epilogue.bias if args.epilogue else None
+        for name, t in (("A", args.A.quantized), ("the scale of A", args.A.scale), ("B", args.B.quantized), ("the scale of B", args.B.scale), ("bias", bias),
+                        ("offsets", getattr(args, "offsets", None))):
+            t = t.tensor if isinstance(t, DenseTensor) else t
+            if t is not None and (not t.is_cuda or t.device != device):
+                raise ValueError(f"{name} must be on the CUDA device of out, got {t.device} and {device}")
+        if device.index != torch.cuda.current_device():
+            with torch.cuda.device(device):
+                return self._run(args, artifact, stream, workspace)
+        ws = self._resolve_workspace(workspace, device)
         a = self.build_args(args)
         L.check(artifact.library.bsg_int8_gemm_run(C.byref(a), ws.data_ptr(), ws.numel() * ws.element_size(), stream))
 

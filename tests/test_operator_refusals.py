@@ -163,3 +163,37 @@ def test_operators_are_found_by_their_operands():
     grouped = ops.GroupedGemmArguments(operand(M, K), ops.ScaledOperand(q.transpose(1, 2), torch.ones((E, N)), (1, 1, K), ops.ScaleSwizzleMode.SwizzleNone), out, torch.int32,
                                        offsets=torch.zeros(E, dtype=torch.int32))
     assert [o.metadata.grouped for o in ops.get_operators(grouped)] == [True]
+
+
+def _int8_arguments(device, **moved):
+    """Dense and grouped arguments on ``device``; ``moved``: names of tensors -> the device they are on instead."""
+    at = lambda name: moved.get(name, device)  # noqa: E731
+    M, N, K, E = 6, 16, 48, 3
+    A = ops.ScaledOperand(torch.zeros((M, K), dtype=torch.int8, device=at("a")), torch.ones(M, device=at("a_scale")), (1, 1, K), ops.ScaleSwizzleMode.SwizzleNone)
+    made = []
+    for shape in ((N,), (E, N)):
+        q = torch.zeros(shape + (K,), dtype=torch.int8, device=at("b")).transpose(-1, -2)
+        B = ops.ScaledOperand(q, torch.ones(shape, device=at("b_scale")), (1, 1, K), ops.ScaleSwizzleMode.SwizzleNone)
+        out = torch.zeros((M, N), dtype=BF16, device=at("out"))
+        epilogue = ops.EpilogueDescriptor(bias=torch.zeros(shape, device=at("bias")))
+        made.append(ops.GroupedGemmArguments(A, B, out, torch.int32, offsets=torch.full((E,), M, dtype=torch.int32, device=at("offsets")), epilogue=epilogue) if len(shape) == 2
+                    else ops.GemmArguments(A, B, out, torch.int32, epilogue))
+    return made
+
+
+def test_operators_run_on_cuda_tensors_only():
+    for args in _int8_arguments("cpu"):
+        with pytest.raises(ValueError, match="CUDA device"):
+            ops.get_operators(args)[0].run(args)
+
+
+@pytest.mark.gpu
+def test_operators_want_all_tensors_on_one_device(cuda_lib):
+    for args in _int8_arguments("cuda"):
+        ops.get_operators(args)[0].run(args)
+    for name in ("a", "a_scale", "b", "b_scale", "out", "bias", "offsets"):
+        dense, grouped = _int8_arguments("cuda", **{name: "cpu"})
+        for args in [grouped] if name == "offsets" else [dense, grouped]:
+            with pytest.raises(ValueError, match="CUDA device"):
+                ops.get_operators(args)[0].run(args)
+    torch.cuda.synchronize()
