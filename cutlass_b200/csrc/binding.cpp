@@ -9,6 +9,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -72,7 +73,8 @@ bool matrix(PyObject* o, bool with_f32, Matrix* m) {
   m->pitch = m->rows > 1 ? m->t->stride(0) : m->cols;
   return m->kind >= 0 && m->device == c10::cuda::current_device() && m->cols >= 1 && (m->cols == 1 || m->t->stride(1) == 1) && m->pitch >= m->cols;
 }
-bool wants_gradient(const at::Tensor* t) { return t && t->requires_grad() && at::GradMode::is_enabled(); }
+bool has_tangent(const at::Tensor* t) { return t && c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined(); }
+bool wants_gradient(const at::Tensor* t) { return t && ((t->requires_grad() && at::GradMode::is_enabled()) || has_tangent(t)); }
 
 at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) { return at::Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt)); }
 
@@ -285,6 +287,7 @@ PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor* gw = a[2] == Py_None ? nullptr : array(a[2], at::kFloat, {T, k}, l.device);
     const at::Tensor* gl = a[3] == Py_None ? nullptr : tensor(a[3]);
     if (!experts || !weights || !counts || !live || !soft || (a[2] != Py_None && !gw)) Py_RETURN_NONE;
+    if (has_tangent(l.t) || has_tangent(weights) || has_tangent(gw) || has_tangent(gl)) Py_RETURN_NONE;
     if (a[3] != Py_None && (!gl || gl->scalar_type() != at::kFloat || gl->numel() != 1 || gl->get_device() != l.device)) Py_RETURN_NONE;
     at::Tensor d = empty({T, E}, l.t->scalar_type(), *l.t);
     bsg_route_args c{};

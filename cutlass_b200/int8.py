@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from . import lib as L
 from .arguments import ACTIVATIONS, ScaledOperand, ScaleSwizzleMode
@@ -71,11 +72,19 @@ def _pitch(K: int) -> int:
     return (K + 15) & ~15 if K <= 128 else (K + 127) & ~127
 
 
+def _no_tangent(name, *tensors) -> None:
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled():
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has no forward-mode derivative: its inputs must not carry tangents")
+
+
 def _no_gradient(name, *tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{name} has no gradient: call it under torch.no_grad() or detach its inputs")
+    _no_tangent(name, *tensors)
 
 
 def _matrix(name, t, kinds):

@@ -15,7 +15,7 @@ import torch
 
 from . import lib as L
 from .int8 import _OUT_KINDS as _KINDS
-from .int8 import _check_array, _elsewhere, _launch, _matrix, _other_stream
+from .int8 import _check_array, _elsewhere, _launch, _matrix, _no_tangent, _other_stream
 
 MAX_EXPERTS, MAX_TOP_K = 1024, 32
 
@@ -94,6 +94,7 @@ def route_tokens_backward(logits, routing: Routing, grad_weights=None, grad_bala
     other = _other_stream(logits, stream)
     if other is not None:
         return _elsewhere(other, route_tokens_backward, logits, routing, grad_weights, grad_balance_loss)
+    _no_tangent("route_tokens_backward", logits, routing.weights, grad_weights, grad_balance_loss)
     experts, counts = routing.experts, routing.counts
     if experts.dim() != 2:
         raise ValueError(f"routing.experts must be (tokens, k), got {tuple(experts.shape)}")
@@ -156,6 +157,7 @@ def route_tokens(logits, top_k: int, *, token_mask=None, normalize: bool = True,
     other = _other_stream(logits, stream)
     if other is not None:
         return _elsewhere(other, route_tokens, logits, top_k, token_mask=token_mask, normalize=normalize)
+    _no_tangent("route_tokens", logits)
     if not (torch.is_grad_enabled() and logits.requires_grad):
         return _forward(logits, top_k, token_mask, normalize, stream)
     weights, loss, experts, counts, offsets, rows, positions, live, softmax = _Route.apply(logits, top_k, token_mask, normalize, stream)

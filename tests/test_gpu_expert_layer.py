@@ -472,3 +472,35 @@ def test_choices_that_are_no_experts_have_no_gradient(cuda_lib):
     none[1, 2], outside[1, 2] = -1, 8
     gl = torch.ones((), device="cuda")
     assert torch.equal(ops.route_tokens_backward(logits, r._replace(experts=outside), gw, gl), ops.route_tokens_backward(logits, r._replace(experts=none), gw, gl))
+
+
+def test_tangents_are_refused(cuda_lib):
+    """Forward-mode derivatives exist nowhere here: a tensor that carries a tangent is refused, not stripped of it."""
+    fa = torch.autograd.forward_ad
+    x, logits = torch.randn((6, 64), device="cuda").to(BF16), torch.randn((6, 8), device="cuda")
+    w, ws = product_tests.weights((24,), 64, seed=1)
+    bias = torch.zeros(24, device="cuda")
+    h, kept = ops.checkpoint_activation(x)
+    r = ops.route_tokens(logits, 2)
+    gl = torch.ones((), device="cuda")
+    stream = torch.cuda.current_stream()
+    with fa.dual_level():
+        dual = lambda t: fa.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for how in (dict(), dict(stream=stream)):
+            for call in (lambda: ops.quantize_int8(dual(x), **how), lambda: ops.int8_linear(dual(x), w, ws, **how), lambda: ops.int8_linear(x, w, dual(ws), **how),
+                         lambda: ops.int8_linear(x, w, ws, dual(bias), **how), lambda: ops.checkpoint_activation(dual(x), **how),
+                         lambda: ops.checkpoint_activation_backward(dual(h), kept, **how), lambda: ops.route_tokens(dual(logits), 2, **how),
+                         lambda: ops.route_tokens_backward(dual(logits), r, r.weights, gl, **how), lambda: ops.route_tokens_backward(logits, r, dual(r.weights), gl, **how),
+                         lambda: ops.route_tokens_backward(logits, r, None, dual(gl), **how)):
+                with pytest.raises(ValueError, match="forward-mode"):
+                    call()
+                with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+                    call()
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            ops.checkpointed_activation(dual(x))
+        ops.int8_linear(x, w, ws)      # others go on
+    for call in (lambda t: ops.route_tokens(t, 2).weights, lambda t: ops.int8_linear(t.to(BF16), w[:, :8].contiguous(), ws)):
+        with pytest.raises((ValueError, RuntimeError)):
+            torch.func.jvp(call, (logits,), (logits,))
+        with pytest.raises((ValueError, RuntimeError)):
+            torch.vmap(call)(logits.expand(3, 6, 8))
