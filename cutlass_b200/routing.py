@@ -22,7 +22,11 @@ MAX_EXPERTS, MAX_TOP_K = 1024, 32
 
 class Routing(NamedTuple):
     """What ``route_tokens`` returns.  A slot that chose nothing (a token that does not count, or fewer than k logits above
-    -inf) has expert -1, weight 0 and position -1; rows at or behind ``offsets[-1]`` name token -1."""
+    -inf) has expert -1, weight 0 and position -1, which is no row: what is taken at positions has to be masked there (the rows of
+    a grouped product behind the last end row are not written and may hold anything, also NaN).  Rows at or behind
+    ``offsets[-1]`` name token -1.
+
+    Without gradients the tensors are parts of one buffer: keeping any of them keeps the memory of all."""
 
     experts: torch.Tensor         # (T, k) int32, largest logit first
     weights: torch.Tensor         # (T, k) fp32
