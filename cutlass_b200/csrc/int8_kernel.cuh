@@ -58,19 +58,20 @@ __device__ __forceinline__ uint32_t i8_maxabs2(uint32_t a, uint32_t b) {
 // that of one fused multiply-add with 1.5 * 2^23, whose last byte is then the level in two's complement.
 struct I8Scale {
   float inv;       // 127 / (amax * pre), enlarged; 0 for a row of zeros
-  float pre;       // 2^64 for rows so small that 127 / amax leaves fp32's range, else 1
+  float pre;       // 2^64 for rows so small that 127 / amax leaves fp32's range, 2^-64 for rows so large that 1 / amax may be
+                   // subnormal, which has fewer bits, else 1
   uint32_t keep;   // all ones; 0 for a row that holds a NaN or an infinity, whose levels are 0
 };
 __device__ __forceinline__ float i8_rcp(float x) {
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));      // off by at most 2^-23 between 2^-64 and 2^128
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));      // off by at most 2^-23 where the result is normal (x up to 2^126)
   return r;
 }
 __device__ __forceinline__ I8Scale i8_scale(float amax) {
   I8Scale s;
   const bool finite = amax < __uint_as_float(0x7F800000u);
   s.keep = finite ? 0xFFFFFFFFu : 0u;
-  s.pre = amax < 0x1p-64f ? 0x1p64f : 1.0f;
+  s.pre = amax < 0x1p-64f ? 0x1p64f : amax > 0x1p64f ? 0x1p-64f : 1.0f;
   s.inv = amax > 0.0f && finite ? __fmul_rn(i8_rcp(__fmul_rn(amax, s.pre)), 127.0f * (1.0f + 0x1p-21f)) : 0.0f;
   return s;
 }

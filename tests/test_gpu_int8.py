@@ -434,3 +434,27 @@ def test_empty_inputs(cuda_lib):
     w, ws = weights((8,), 16, seed=0)
     assert ops.int8_linear(torch.empty((0, 16), dtype=BF16, device="cuda"), w, ws).shape == (0, 8)
     assert ops.quantize_int8(torch.empty((0, 16), dtype=BF16, device="cuda")).quantized.tensor.shape == (0, 16)
+
+
+@pytest.mark.parametrize("exponent", [-126, -110, -72, -71, -70, 56, 57, 58, 100, 117, 118, 119, 120])
+def test_halves_round_outwards_at_the_ends_of_the_range(cuda_lib, exponent):
+    """Every mantissa of the maximum, the rows scaled to where a reciprocal or a level factor leaves fp32's normal range or a row is
+    scaled on its way, against values on and next to each half."""
+    amax = (torch.arange(128, 256, device="cuda").double() * 2.0 ** exponent).to(BF16)
+    half = (torch.arange(127, device="cuda").double() + 0.5)[None] * amax.double()[:, None] / 127.0
+    near = half.to(BF16)
+    bits = near.view(torch.int16)
+    x = torch.cat([amax[:, None], near, (bits - 1).view(BF16), -(bits + 1).view(BF16), -near, amax[:, None] / 2], 1).clamp(-amax[:, None], amax[:, None]).contiguous()
+    q, s = levels(x)
+    r = ops.quantize_int8(x)
+    assert torch.equal(r.quantized.tensor.double(), q) and torch.equal(r.scale.tensor, s.float())
+    for rows in (1, 3):
+        for i in range(0, 128, 17):
+            few = x[i:i + rows].contiguous()
+            eye = torch.zeros((16, 512), dtype=torch.int8, device="cuda")[:, :few.shape[1]]
+            eye[torch.arange(16), torch.arange(16) * 31] = 1
+            got = ops.int8_linear(few, eye, torch.full((16,), 2.0 ** 100 if exponent < 0 else 2.0 ** -100, device="cuda"), out_dtype=F32)
+            n = few.shape[0]
+            want = q[i:i + n, torch.arange(16, device="cuda") * 31] * s[i:i + n].float().double()[:, None]
+            tol = 3 * 2.0 ** -24 * want.abs() + 2.0 ** -149 * 0.5
+            assert bool(((got.double() * (2.0 ** -100 if exponent < 0 else 2.0 ** 100) - want).abs() <= tol).all())
