@@ -355,7 +355,9 @@ int32_t bsg_int8_linear_run(const bsg_int8_args* args, void* workspace, size_t w
  *     forward   h = act(g) u (or act(g)); kept: per row and block of 128 columns of g and of u
  *               s = max|.| / 127, q = sign(.) floor(127 |.| / max|.| + 1/2)
  *     backward  with g^ = s q, u^ = s q:  dg = dh u^ act'(g^), du = dh act(g^)  (or dg = dh act'(g^))
- * A block with a NaN or an infinity is kept as NaN.  act and its order of operations: BSG_ACT_*.
+ * A block with a NaN or an infinity is kept as NaN.  act is that of BSG_ACT_* in formulas of its own: before the last rounding gelu and
+ * silu are off by a few 2^-22 and, in the tail, by 2^-17 + x^2 2^-23 of their value, so that they may differ from the activations
+ * behind a product by that rounding.
  */
 typedef struct bsg_act_args {
   int32_t type;             /* BSG_OUT_BF16 or BSG_OUT_F16: X, h and their gradients */

@@ -190,3 +190,43 @@ def test_empty(cuda_lib):
     h, kept = ops.checkpoint_activation(torch.empty((0, 32), dtype=BF16, device="cuda"))
     assert h.shape == (0, 16)
     assert ops.checkpoint_activation_backward(torch.empty((0, 16), dtype=BF16, device="cuda"), kept).shape == (0, 32)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_the_tail_of_gelu_keeps_its_relative_precision(cuda_lib, dtype):
+    """Every value of the type between 2^-6 and 13 in magnitude, a block of 128 of each.  With y = |x| the lower tail P(-y) is
+    exp(-y^2 / 2) times a polynomial of t = 1 / (1 + c y): off by 2^-17 (the fit, 5.3e-6), by y^2 / 2 times 2.5 * 2^-24 (argument of
+    the exponential: the square, its product with log2 e, that constant) and by 48 * 2^-24 for the rest (exponential 4, the
+    reciprocal 2, seven steps of the polynomial whose terms add up to twice its value, two products).  gelu(x) = x P(x) takes two
+    roundings more, its slope P(x) + x p(x) those of p as well; the kept value is off by the roundings of its scale and of
+    their product, 2 * 2^-24 of it, which its function passes on by its slope.  Last half a step of the type."""
+    bits = torch.arange(1, 1 << 15, device="cuda", dtype=torch.int32).to(torch.int16).view(dtype)
+    pos = bits[(bits >= 2.0 ** -6) & (bits <= 13)]
+    v = torch.cat([-pos, pos])
+    x = v[:, None].expand(-1, 128).contiguous()
+    z = v.double()
+    y = z.abs()
+    tail, p = 0.5 * torch.erfc(y / math.sqrt(2)), torch.exp(-y * y / 2) / math.sqrt(2 * math.pi)
+    exponent = y * y / 2 * 2.5 * 2.0 ** -24
+    off = 2.0 ** -17 + exponent + 48 * 2.0 ** -24
+    one = torch.ones_like(x)
+
+    def near(got, want, inner):
+        info = torch.finfo(dtype)
+        tol = inner + info.eps / 2 * (want.abs() + inner) + info.smallest_normal * info.eps
+        err = (got.double() - want[:, None]).abs() - tol[:, None]
+        worst = int(err.amax(1).argmax())
+        assert float(err.max()) <= 0, f"at {float(v[worst])}: {float(got[worst, 0])} instead of {float(want[worst])}"
+
+    value, slope = act64(z, "gelu")
+    value_off = y * tail * off + 2.0 ** -22 * value.abs()
+    h, kept = ops.checkpoint_activation(x, "gelu", gated=False)
+    near(h, value, value_off)
+    kept_off = 2.0 ** -23 * y
+    slope_off = tail * off + y * p * (exponent + 8 * 2.0 ** -24) + 2.0 ** -22 * (tail + y * p) + 2.0 ** -23 * (z > 0) + p * (2 - y * y).abs() * kept_off
+    near(ops.checkpoint_activation_backward(one, kept), slope, slope_off)
+    h, kept = ops.checkpoint_activation(torch.cat([x, one], 1), "gelu")
+    near(h, value, value_off)
+    dx = ops.checkpoint_activation_backward(one, kept)
+    near(dx[:, :128], slope, slope_off + 2.0 ** -22 * slope.abs())
+    near(dx[:, 128:], value, value_off + (tail + y * p) * kept_off * (z < 0) + 1.13 * kept_off * (z > 0))
