@@ -99,6 +99,22 @@ def _matrix(name, t, kinds):
     return kind, device, rows, cols, (pitch if rows > 1 else cols)
 
 
+def _share_memory(a, b) -> bool:
+    """Whether two row-major matrices have a byte in common (or may have: pitches that differ)."""
+    spans = []
+    for t in (a, b):
+        size = t.element_size()
+        pitch = (t.stride(0) if t.shape[0] > 1 else t.shape[1]) * size
+        spans.append((t.data_ptr(), pitch, t.shape[1] * size, (t.shape[0] - 1) * pitch + t.shape[1] * size if t.numel() else 0))
+    (p, p_pitch, p_row, p_all), (q, q_pitch, q_row, q_all) = spans
+    if p + p_all <= q or q + q_all <= p or not p_all or not q_all:
+        return False
+    if a.shape[0] > 1 and b.shape[0] > 1 and p_pitch == q_pitch:
+        behind = (q - p) % p_pitch      # columns of one buffer, side by side
+        return behind < p_row or behind + q_row > p_pitch
+    return True
+
+
 def _check_array(name, t, dtype, shape, device) -> None:
     if t.dtype != dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on CUDA device {device}, "
@@ -152,7 +168,7 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
     copied into expert order first (``route_tokens`` makes both).  Rows of the result at or behind the last end row are not
     written.  Offsets that fall or leave the rows are clamped and reported by ``check_device_status`` of an operator.
 
-    No gradient is kept.  Asynchronous on ``stream`` (None: torch's current stream)."""
+    ``out`` may share memory with ``x``.  No gradient is kept.  Asynchronous on ``stream`` (None: torch's current stream)."""
     if out is None and stream is None and x.is_cuda:
         y = L.binding().int8_linear(x, weight, weight_scale, bias, activation, offsets, rows, out_dtype)
         if y is not None:
@@ -201,8 +217,8 @@ def int8_linear(x, weight, weight_scale, bias=None, *, activation="identity", of
         raise ValueError(f"out dtype {out.dtype} is not supported (bf16, fp16 or fp32)")
     if R == 0:
         return out
-    if offsets is None and R <= 4 and _POWER[R] * whole <= 65536:      # quantised inside the product's kernel
-        q = q_scale = 0
+    if offsets is None and R <= 4 and _POWER[R] * whole <= 65536 and not _share_memory(x, out):
+        q = q_scale = 0      # quantised inside the product's kernel, whose blocks read x while others already write
     else:
         held = R
         if rows is not None:      # tokens that several rows use may be held twice: as they come, and in the order of the rows

@@ -346,7 +346,7 @@ int32_t bsg_int8_quantize(const bsg_int8_args* args, void* cuda_stream);
 int32_t bsg_int8_gemm_run(const bsg_int8_args* args, void* workspace, size_t workspace_bytes, void* cuda_stream);
 /* Both steps; the product's set-up and its first weights overlap the quantiser.  With Q and q_scale NULL the tokens are
  * quantised inside the product's kernel: dense, without an index, at most 4 rows, which in 8 bits (their number rounded up to
- * a power of two times K rounded up to 16) take at most 64 KB. */
+ * a power of two times K rounded up to 16) take at most 64 KB; D must not overlap X then. */
 int32_t bsg_int8_linear_run(const bsg_int8_args* args, void* workspace, size_t workspace_bytes, void* cuda_stream);
 
 /*

@@ -458,3 +458,21 @@ def test_halves_round_outwards_at_the_ends_of_the_range(cuda_lib, exponent):
             want = q[i:i + n, torch.arange(16, device="cuda") * 31] * s[i:i + n].float().double()[:, None]
             tol = 3 * 2.0 ** -24 * want.abs() + 2.0 ** -149 * 0.5
             assert bool(((got.double() * (2.0 ** -100 if exponent < 0 else 2.0 ** 100) - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("M", [1, 2, 4, 5, 300])
+def test_results_in_the_place_of_the_tokens(cuda_lib, M):
+    """``out`` is ``x`` itself, or its columns further on; columns beside those of x in one buffer are no overlap."""
+    K = 2048
+    w, ws = weights((K,), K, seed=1)
+    ws = ws / math.sqrt(K)
+    x = tokens(M, K, BF16, seed=M)
+    want = ops.int8_linear(x, w, ws)
+    for _ in range(5):
+        for shift in (0, 3, 8, K):
+            buf = torch.zeros((M, 2 * K), dtype=BF16, device="cuda")
+            buf[:, :K] = x
+            ops.int8_linear(buf[:, :K], w, ws, out=buf[:, shift:shift + K])
+            assert torch.equal(buf[:, shift:shift + K], want)
+            if shift == K:
+                assert torch.equal(buf[:, :K], x)
