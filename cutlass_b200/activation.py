@@ -14,7 +14,7 @@ import torch
 
 from . import lib as L
 from .arguments import ACTIVATIONS
-from .int8 import _IN_KINDS, _check_array, _elsewhere, _launch, _matrix, _no_gradient, _other_stream
+from .int8 import _IN_KINDS, _check_array, _elsewhere, _launch, _matrix, _no_gradient, _other_stream, _share_memory
 
 BLOCK = 128      # columns of a row that share one scale
 
@@ -54,10 +54,16 @@ def _given(name, t, kind, device, rows, cols) -> int:
     return pitch
 
 
+def _check_place(out, inp, ld_out, ld_in) -> None:
+    """A result may lie where its input lies, value on value (every value is read before its place is written), or elsewhere."""
+    if _share_memory(out, inp) and (out.data_ptr() != inp.data_ptr() or (ld_out != ld_in and out.shape[0] > 1)):
+        raise ValueError("out must begin where the input begins, with the same distance between rows, or share no memory with it")
+
+
 def checkpoint_activation(x, activation: str = "silu", *, gated: bool = True, out=None, stream=None):
     """``(h, kept)``: ``h = act(x[:, :F]) * x[:, F:]`` for ``gated`` (x has 2F columns), else ``act(x)``, computed from ``x``
     itself, and the ``ActivationCheckpoint`` that ``checkpoint_activation_backward`` takes.  ``x`` is (T, 2F) or (T, F) bf16 /
-    fp16; ``activation``: "identity", "relu", "gelu" (erf form) or "silu"; ``out`` (T, F) may be given.  A block of 128 values
+    fp16; ``activation``: "identity", "relu", "gelu" (erf form) or "silu"; ``out`` (T, F) may be given, also the columns of ``x`` that it begins with.  A block of 128 values
     with a NaN or an infinity is kept as NaN.  Asynchronous on ``stream`` (None: torch's current stream)."""
     if out is None and stream is None and x.is_cuda:
         done = L.binding().act_forward(x, activation, gated)
@@ -81,6 +87,7 @@ def checkpoint_activation(x, activation: str = "silu", *, gated: bool = True, ou
         out, ldh = x.new_empty((T, F)), F
     else:
         ldh = _given("out", out, kind, device, T, F)
+        _check_place(out, x, ldh, ldx)
     q = data.data_ptr()
     pack, call = L.direct("bsg_act_forward", L.ACT_LAYOUT)
     _launch(device, call, pack(kind, act, parts - 1, 0, T, F, x.data_ptr(), ldx, out.data_ptr(), ldh, q, q + split))
@@ -109,6 +116,7 @@ def checkpoint_activation_backward(grad, kept: ActivationCheckpoint, *, out=None
         out, ldx = grad.new_empty((T, parts * F)), parts * F
     else:
         ldx = _given("out", out, kind, device, T, parts * F)
+        _check_place(out, grad, ldx, ldg)
     pack, call = L.direct("bsg_act_backward", L.ACT_LAYOUT)
     _launch(device, call, pack(kind, act, parts - 1, 0, T, F, grad.data_ptr(), ldg, out.data_ptr(), ldx,
                                q, q + kept._split()))

@@ -230,3 +230,27 @@ def test_the_tail_of_gelu_keeps_its_relative_precision(cuda_lib, dtype):
     dx = ops.checkpoint_activation_backward(one, kept)
     near(dx[:, :128], slope, slope_off + 2.0 ** -22 * slope.abs())
     near(dx[:, 128:], value, value_off + (tail + y * p) * kept_off * (z < 0) + 1.13 * kept_off * (z > 0))
+
+
+@pytest.mark.parametrize("gated", [True, False])
+@pytest.mark.parametrize("T,F,pad", [(1, 300, 0), (40, 1024, 0), (33, 515, 3), (600, 136, 8)])
+def test_results_in_the_place_of_the_input(cuda_lib, T, F, pad, gated):
+    """h over the first columns of x and the gradient of x over that of h, value on value; any other overlap is refused."""
+    x, dh = make(T, F, BF16, gated, seed=1, pad=pad)
+    h, kept = ops.checkpoint_activation(x, "gelu", gated=gated)
+    dx = ops.checkpoint_activation_backward(dh, kept)
+    buf = x.new_zeros((T, 2 * F + pad + 1))
+    cols = x.shape[1]
+    buf[:, :cols] = x
+    _, again = ops.checkpoint_activation(buf[:, :cols], "gelu", gated=gated, out=buf[:, :F])
+    assert torch.equal(buf[:, :F], h) and torch.equal(again.scale, kept.scale) and torch.equal(again.quantized[..., :F], kept.quantized[..., :F])
+    buf[:, :F] = dh
+    ops.checkpoint_activation_backward(buf[:, :F], kept, out=buf[:, :cols])
+    assert torch.equal(buf[:, :cols], dx)
+    with pytest.raises(ValueError):
+        ops.checkpoint_activation(buf[:, :cols], "gelu", gated=gated, out=buf[:, 1:1 + F])
+    with pytest.raises(ValueError):
+        ops.checkpoint_activation_backward(buf[:, 1:1 + F], kept, out=buf[:, :cols])
+    wide = x.new_zeros((T, cols + F))
+    wide[:, :cols] = x
+    assert torch.equal(ops.checkpoint_activation(wide[:, :cols], "gelu", gated=gated, out=wide[:, cols:])[0], h)      # columns side by side
