@@ -7,6 +7,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -20,6 +21,7 @@ def lib_name(profile: bool) -> str:
 
 OUT = os.path.join(_HERE, "lib", lib_name(PROFILE))
 BINDING = os.path.join(_HERE, "lib", "_binding.so")
+BINDING_STAMP = os.path.join(_HERE, "build", "binding.for")      # what it was made for
 SOURCES = {      # translation unit -> the headers it includes
     "bsgemm.cu": ["gemm_kernel.cuh", "quant_kernel.cuh", "ptx.cuh", "host.h"],
     "int8.cu": ["int8_kernel.cuh", "gemm_kernel.cuh", "ptx.cuh", "host.h"],
@@ -58,34 +60,52 @@ def _nvcc(args: list[str]) -> str:
     return proc.stderr
 
 
-def _build_binding(force: bool) -> None:
-    """The Python module of csrc/binding.cpp (host code; needs torch's headers)."""
-    src = os.path.join(CSRC, "binding.cpp")
-    if not force and os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in (src, os.path.join(CSRC, ABI_HEADER))):
-        return
+def _binding_for() -> str:
+    import torch
+    return f"python {sys.version_info[0]}.{sys.version_info[1]} torch {torch.__version__}"
+
+
+def _compile_binding() -> None:
     import sysconfig
 
     import torch
     root = os.path.dirname(torch.__file__)
     cuda = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DBSG_BINDING_FOR="{_binding_for()}"',
            "-isystem" + os.path.join(root, "include"), "-isystem" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
-           "-isystem" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], src, "-o", BINDING,
+           "-isystem" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], os.path.join(CSRC, "binding.cpp"), "-o", BINDING,
            "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError("the compiler failed:\n" + proc.stdout + proc.stderr)
 
 
+def _build_binding(force: bool) -> None:
+    """The Python module of csrc/binding.cpp (host code; needs a C++ compiler, Python's and torch's headers), if it is missing, older
+    than its source or made for another Python or torch.  Where it cannot be made the package works without it, so that is a
+    warning."""
+    deps = (os.path.join(CSRC, "binding.cpp"), os.path.join(CSRC, ABI_HEADER))
+    try:
+        made_for = open(BINDING_STAMP).read() if os.path.exists(BINDING_STAMP) else None
+        if not force and os.path.exists(BINDING) and made_for == _binding_for() and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
+            return
+        _compile_binding()
+        with open(BINDING_STAMP, "w") as f:
+            f.write(_binding_for())
+    except (OSError, ImportError, RuntimeError) as error:
+        warnings.warn(f"the binding of the short calls was not built; they take more host time without it: {error}", RuntimeWarning)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compile the CUDA library, and the Python binding of its short calls, if they are missing or older than their sources;
     return the library's path.  Translation units are compiled side by side, and only those whose sources changed."""
     os.makedirs(os.path.dirname(OUT), exist_ok=True)
+    os.makedirs(os.path.join(_HERE, "build"), exist_ok=True)
     if not force and not _stale():
         _build_binding(False)
         return OUT
     units = _objects()
-    os.makedirs(os.path.join(_HERE, "build"), exist_ok=True)
     extra = (["-DBSG_PROFILE"] if PROFILE else []) + (["-Xptxas", "-v"] if verbose else [])
     with ThreadPoolExecutor() as pool:
         binding = pool.submit(_build_binding, force)

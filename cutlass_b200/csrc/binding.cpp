@@ -337,4 +337,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, n
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__binding() { return PyModule_Create(&module); }
+#ifndef BSG_BINDING_FOR
+#error "BSG_BINDING_FOR names the Python and the torch that this is compiled for"
+#endif
+PyMODINIT_FUNC PyInit__binding() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "made_for", BSG_BINDING_FOR) != 0) Py_CLEAR(m);
+  return m;
+}

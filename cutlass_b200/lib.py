@@ -11,6 +11,7 @@ import importlib.machinery
 import importlib.util
 import os
 import struct
+import warnings
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # BSG_PROFILE=1 selects the instrumented build (python -m cutlass_b200.build with the same variable set).
@@ -194,17 +195,38 @@ BOUND = ("bsg_int8_linear_run", "bsg_int8_scratch_rows", "bsg_act_forward", "bsg
 _binding = None
 
 
+class _NoBinding:
+    """Stands in for the binding: every call is left to the Python around it."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def _load_binding():
+    if not os.path.exists(BINDING_PATH):
+        raise ImportError(f"{BINDING_PATH} is missing")
+    from .build import _binding_for
+    loader = importlib.machinery.ExtensionFileLoader("_binding", BINDING_PATH)
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
+    loader.exec_module(module)
+    if module.made_for != _binding_for():
+        raise ImportError(f"{BINDING_PATH} was made for {module.made_for}, this is {_binding_for()}")
+    return module
+
+
 def binding():
     """The module of ``csrc/binding.cpp``: whole calls with little host time.  Each of its functions returns None, having done
-    nothing, for a call that is not the plain case; the Python around it then does the work or says what is wrong."""
+    nothing, for a call that is not the plain case; the Python around it then does the work or says what is wrong.  Where the module
+    is missing, or was made for another Python or torch, that Python makes every call, and a warning says so once."""
     global _binding
     if _binding is None:
-        if not os.path.exists(BINDING_PATH):
-            raise FileNotFoundError(f"{BINDING_PATH} is missing: build it with `python -m cutlass_b200.build`")
         lib = load()
-        loader = importlib.machinery.ExtensionFileLoader("_binding", BINDING_PATH)
-        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_binding", loader))
-        loader.exec_module(module)
+        try:
+            module = _load_binding()
+        except ImportError as error:
+            warnings.warn(f"{error}: calls take more host time without the binding; build it with `python -m cutlass_b200.build`", RuntimeWarning)
+            _binding = _NoBinding()
+            return _binding
         from .activation import ActivationCheckpoint
         from .arguments import ACTIVATIONS
         from .operator import _default_workspaces

@@ -75,3 +75,70 @@ def test_results_are_tensors_of_their_own(cuda_lib):
     again = ops.route_tokens(l.detach(), 2)
     want = ops.route_tokens_backward(l.detach(), again, torch.ones_like(again.weights), torch.ones((), device="cuda"))
     assert torch.equal(l.grad, want)
+
+
+@pytest.fixture
+def unloaded(monkeypatch):
+    monkeypatch.setattr(L, "_binding", None)
+    return monkeypatch
+
+
+def test_without_the_binding_python_makes_the_calls(unloaded, tmp_path):
+    """Missing, not loadable, or made for another torch: a warning, and every call is left to the Python around it."""
+    import cutlass_b200.build as B
+    broken = tmp_path / "_binding.so"
+    broken.write_bytes(b"no library")
+    for change in (lambda m: m.setattr(L, "BINDING_PATH", str(tmp_path / "nothing.so")), lambda m: m.setattr(L, "BINDING_PATH", str(broken)),
+                   lambda m: m.setattr(B, "_binding_for", lambda: "python 3.0 torch 0.1")):
+        with unloaded.context() as m:
+            m.setattr(L, "_binding", None)
+            change(m)
+            with pytest.warns(RuntimeWarning, match="binding"):
+                b = L.binding()
+            assert L.binding() is b
+            assert b.int8_linear(1, 2, 3) is None and b.route_forward(None, 2, None, True) is None and b.act_backward(None, None) is None
+    unloaded.setattr(L, "_binding", None)
+    assert L.binding().made_for == B._binding_for()
+
+
+def test_a_binding_that_cannot_be_built_is_a_warning(monkeypatch, tmp_path):
+    """A host without a C++ compiler builds the library; a binding made for another torch is made again."""
+    import cutlass_b200.build as B
+    made = []
+    monkeypatch.setattr(B, "BINDING", str(tmp_path / "_binding.so"))
+    monkeypatch.setattr(B, "BINDING_STAMP", str(tmp_path / "binding.for"))
+    with monkeypatch.context() as m:
+        m.setenv("CXX", str(tmp_path / "no-such-compiler"))
+        with pytest.warns(RuntimeWarning, match="not built"):
+            assert B.build() == B.OUT
+    monkeypatch.setattr(B, "_compile_binding", lambda: (made.append(1), open(B.BINDING, "w").close()))
+    for _ in range(2):
+        B._build_binding(False)
+    assert len(made) == 1
+    monkeypatch.setattr(B, "_binding_for", lambda: "python 3.0 torch 0.1")
+    B._build_binding(False)
+    assert len(made) == 2
+
+
+@pytest.mark.gpu
+def test_the_calls_work_without_the_binding(cuda_lib, unloaded):
+    x = torch.randn((50, 128), device="cuda").to(torch.bfloat16)
+    w = ops.quantize_int8(torch.randn((64, 128), device="cuda").to(torch.bfloat16))
+    logits = torch.randn((50, 16), device="cuda")
+
+    def calls():
+        h, kept = ops.checkpoint_activation(x)
+        leaf, up = logits.clone().requires_grad_(), x.clone().requires_grad_()
+        r = ops.route_tokens(leaf, 2)
+        (r.weights.square().sum() + r.balance_loss).backward()
+        ops.checkpointed_activation(up).square().sum().backward()
+        r2 = ops.route_tokens(logits, 2)
+        return [ops.int8_linear(x, w.quantized.tensor, w.scale.tensor), ops.int8_linear(x[:2], w.quantized.tensor, w.scale.tensor), h, kept.scale,
+                ops.checkpoint_activation_backward(h, kept), leaf.grad, up.grad, r2.rows, r2.weights, ops.route_tokens_backward(logits, r2, r2.weights, r2.balance_loss)]
+    want = calls()
+    unloaded.setattr(L, "_binding", None)
+    unloaded.setattr(L, "BINDING_PATH", "nothing.so")
+    with pytest.warns(RuntimeWarning):
+        got = calls()
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
