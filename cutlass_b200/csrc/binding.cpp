@@ -109,6 +109,19 @@ int32_t activation_of(PyObject* name) {
   return code ? int32_t(PyLong_AsLong(code)) : -1;
 }
 
+// The interpreter's lock is given up while memory is allocated and kernels are launched: both may wait, for the device or for a full
+// queue, and other Python threads go on.  (The arguments are the caller's and stay alive.)
+class Unlocked {
+ public:
+  Unlocked() : state_(PyEval_SaveThread()) {}
+  ~Unlocked() { PyEval_RestoreThread(state_); }
+  Unlocked(const Unlocked&) = delete;
+  Unlocked& operator=(const Unlocked&) = delete;
+
+ private:
+  PyThreadState* state_;
+};
+
 template <class F>
 PyObject* guarded(F body) {
   try {
@@ -163,17 +176,22 @@ PyObject* int8_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
     c.W = w->const_data_ptr(); c.ldw = ldw; c.group_stride_w = group_stride; c.w_scale = ws->const_data_ptr<float>();
     c.bias = bias ? bias->const_data_ptr<float>() : nullptr; c.offsets = offsets ? offsets->const_data_ptr<int32_t>() : nullptr;
     c.ldd = N;
-    at::Tensor scratch;
-    if (grouped || R > 4 || (R <= 2 ? R : 4) * whole > 65536) {      // else the tokens are quantised inside the product's kernel
-      int64_t held = R;
-      if (rows && g.int8_scratch_rows(&c, &held) != BSG_OK) Py_RETURN_NONE;
-      scratch = empty({held * (pitch + 4)}, at::kChar, *x.t);        // 8-bit tokens, then their scales
-      c.Q = scratch.mutable_data_ptr();
-      c.q_scale = reinterpret_cast<float*>(static_cast<char*>(c.Q) + held * pitch);
+    at::Tensor scratch, y;
+    void* const status_words = status->mutable_data_ptr();
+    int32_t code;
+    {
+      Unlocked unlocked;
+      if (grouped || R > 4 || (R <= 2 ? R : 4) * whole > 65536) {      // else the tokens are quantised inside the product's kernel
+        int64_t held = R;
+        if (rows) g.int8_scratch_rows(&c, &held);
+        scratch = empty({held * (pitch + 4)}, at::kChar, *x.t);        // 8-bit tokens, then their scales
+        c.Q = scratch.mutable_data_ptr();
+        c.q_scale = reinterpret_cast<float*>(static_cast<char*>(c.Q) + held * pitch);
+      }
+      y = empty({R, N}, out_type, *x.t);
+      c.D = y.mutable_data_ptr();
+      code = g.int8_linear_run(&c, status_words, 16, current_stream(dev));
     }
-    at::Tensor y = empty({R, N}, out_type, *x.t);
-    c.D = y.mutable_data_ptr();
-    const int32_t code = g.int8_linear_run(&c, status->mutable_data_ptr(), 16, current_stream(dev));
     return code ? failed(code) : THPVariable_Wrap(std::move(y));
   });
 }
@@ -187,13 +205,19 @@ PyObject* act_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const bool gated = a[2] == Py_True;
     if (act < 0 || (!gated && a[2] != Py_False) || (gated && x.cols % 2 != 0)) Py_RETURN_NONE;
     const int64_t parts = gated ? 2 : 1, T = x.rows, F = x.cols / parts, split = T * parts * ((F + 15) & ~int64_t(15));
-    at::Tensor data = empty({split + 4 * T * parts * ((F + 127) / 128)}, at::kChar, *x.t);
-    at::Tensor h = empty({T, F}, x.t->scalar_type(), *x.t);
+    at::Tensor data, h;
     bsg_act_args c{};
     c.type = x.kind; c.activation = act; c.gated = gated; c.rows = T; c.width = F;
-    c.in = x.t->const_data_ptr(); c.ld_in = x.pitch; c.out = h.mutable_data_ptr(); c.ld_out = F;
-    c.kept = data.mutable_data_ptr(); c.kept_scale = reinterpret_cast<float*>(static_cast<char*>(c.kept) + split);
-    const int32_t code = g.act_forward(&c, current_stream(x.device));
+    c.in = x.t->const_data_ptr(); c.ld_in = x.pitch; c.ld_out = F;
+    int32_t code;
+    {
+      Unlocked unlocked;
+      data = empty({split + 4 * T * parts * ((F + 127) / 128)}, at::kChar, *x.t);
+      h = empty({T, F}, x.t->scalar_type(), *x.t);
+      c.out = h.mutable_data_ptr();
+      c.kept = data.mutable_data_ptr(); c.kept_scale = reinterpret_cast<float*>(static_cast<char*>(c.kept) + split);
+      code = g.act_forward(&c, current_stream(x.device));
+    }
     if (code) return failed(code);
     PyObject* dtype = reinterpret_cast<PyObject*>(torch::getTHPDtype(x.t->scalar_type()));
     Py_INCREF(a[1]);
@@ -220,13 +244,19 @@ PyObject* act_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     const at::Tensor* data = array(kept[0], at::kChar, {split + 4 * T * parts * ((F + 127) / 128)}, d.device);
     if (!data) Py_RETURN_NONE;
-    at::Tensor dx = empty({T, parts * F}, d.t->scalar_type(), *d.t);
+    at::Tensor dx;
     bsg_act_args c{};
     c.type = d.kind; c.activation = act; c.gated = gated; c.rows = T; c.width = F;
-    c.in = d.t->const_data_ptr(); c.ld_in = d.pitch; c.out = dx.mutable_data_ptr(); c.ld_out = parts * F;
+    c.in = d.t->const_data_ptr(); c.ld_in = d.pitch; c.ld_out = parts * F;
     c.kept = const_cast<void*>(data->const_data_ptr());
     c.kept_scale = reinterpret_cast<float*>(static_cast<char*>(c.kept) + split);
-    const int32_t code = g.act_backward(&c, current_stream(d.device));
+    int32_t code;
+    {
+      Unlocked unlocked;
+      dx = empty({T, parts * F}, d.t->scalar_type(), *d.t);
+      c.out = dx.mutable_data_ptr();
+      code = g.act_backward(&c, current_stream(d.device));
+    }
     return code ? failed(code) : THPVariable_Wrap(std::move(dx));
   });
 }
@@ -244,8 +274,6 @@ PyObject* route_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (a[2] != Py_None && !mask) Py_RETURN_NONE;
     const int64_t slots = T * k;
     // one allocation: softmax (2 T), experts, rows, positions, weights (slots each), counts, offsets (E each), live, loss
-    at::Tensor all = empty({2 * T + 4 * slots + 2 * E + 2}, at::kInt, *l.t);
-    int32_t* p = static_cast<int32_t*>(all.mutable_data_ptr());
     int64_t at_ = 0;
     auto take = [&](int64_t count) { const int64_t o = at_; at_ += count; return o; };
     const int64_t soft = take(2 * T), experts = take(slots), rows = take(slots), positions = take(slots), weights = take(slots), counts = take(E), offsets = take(E),
@@ -253,14 +281,20 @@ PyObject* route_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     bsg_route_args c{};
     c.type = l.kind; c.experts = int32_t(E); c.k = int32_t(k); c.normalize = a[3] == Py_True; c.tokens = T;
     c.logits = l.t->const_data_ptr(); c.ld = l.pitch; c.mask = mask ? static_cast<const uint8_t*>(mask->const_data_ptr()) : nullptr;
-    c.chosen = p + experts; c.weights = reinterpret_cast<float*>(p + weights); c.counts = p + counts; c.live = p + live;
-    c.softmax = reinterpret_cast<float*>(p + soft); c.offsets = p + offsets; c.rows = p + rows; c.positions = p + positions;
-    c.loss = reinterpret_cast<float*>(p + loss);
     size_t bytes = 0;
     if (g.route_scratch_size(&c, &bytes) != BSG_OK) Py_RETURN_NONE;
-    at::Tensor scratch;
-    if (bytes) scratch = empty({int64_t(bytes)}, at::kByte, *l.t);
-    const int32_t code = g.route_forward(&c, bytes ? scratch.mutable_data_ptr() : nullptr, bytes, current_stream(l.device));
+    at::Tensor all, scratch;
+    int32_t code;
+    {
+      Unlocked unlocked;
+      all = empty({at_}, at::kInt, *l.t);
+      int32_t* p = static_cast<int32_t*>(all.mutable_data_ptr());
+      c.chosen = p + experts; c.weights = reinterpret_cast<float*>(p + weights); c.counts = p + counts; c.live = p + live;
+      c.softmax = reinterpret_cast<float*>(p + soft); c.offsets = p + offsets; c.rows = p + rows; c.positions = p + positions;
+      c.loss = reinterpret_cast<float*>(p + loss);
+      if (bytes) scratch = empty({int64_t(bytes)}, at::kByte, *l.t);
+      code = g.route_forward(&c, bytes ? scratch.mutable_data_ptr() : nullptr, bytes, current_stream(l.device));
+    }
     if (code) return failed(code);
     auto ints = [&](int64_t o, at::IntArrayRef s) { return THPVariable_Wrap(part(all, at::kInt, o, s)); };
     auto reals = [&](int64_t o, at::IntArrayRef s) { return THPVariable_Wrap(part(all, at::kFloat, o, s)); };
@@ -289,7 +323,7 @@ PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!experts || !weights || !counts || !live || !soft || (a[2] != Py_None && !gw)) Py_RETURN_NONE;
     if (has_tangent(l.t) || has_tangent(weights) || has_tangent(gw) || has_tangent(gl)) Py_RETURN_NONE;
     if (a[3] != Py_None && (!gl || gl->scalar_type() != at::kFloat || gl->numel() != 1 || gl->get_device() != l.device)) Py_RETURN_NONE;
-    at::Tensor d = empty({T, E}, l.t->scalar_type(), *l.t);
+    at::Tensor d;
     bsg_route_args c{};
     c.type = l.kind; c.experts = int32_t(E); c.k = int32_t(k); c.normalize = r[9] == Py_True; c.tokens = T;
     c.logits = l.t->const_data_ptr(); c.ld = l.pitch;
@@ -297,8 +331,14 @@ PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     c.counts = const_cast<int32_t*>(counts->const_data_ptr<int32_t>()); c.live = const_cast<int32_t*>(live->const_data_ptr<int32_t>());
     c.softmax = reinterpret_cast<float*>(const_cast<int32_t*>(soft->const_data_ptr<int32_t>()));
     c.grad_weights = gw ? gw->const_data_ptr<float>() : nullptr; c.grad_loss = gl ? gl->const_data_ptr<float>() : nullptr;
-    c.grad_logits = d.mutable_data_ptr(); c.ld_grad = E;
-    const int32_t code = g.route_backward(&c, current_stream(l.device));
+    c.ld_grad = E;
+    int32_t code;
+    {
+      Unlocked unlocked;
+      d = empty({T, E}, l.t->scalar_type(), *l.t);
+      c.grad_logits = d.mutable_data_ptr();
+      code = g.route_backward(&c, current_stream(l.device));
+    }
     return code ? failed(code) : THPVariable_Wrap(std::move(d));
   });
 }

@@ -142,3 +142,40 @@ def test_the_calls_work_without_the_binding(cuda_lib, unloaded):
         got = calls()
     for a, b in zip(want, got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_other_threads_run_while_a_call_waits(cuda_lib):
+    """A launch waits where the queue of the device is full; another Python thread goes on meanwhile."""
+    import threading
+    import time
+    x = torch.randn((40, 128), device="cuda").to(torch.bfloat16)
+    w = ops.quantize_int8(torch.randn((64, 128), device="cuda").to(torch.bfloat16))
+    logits = torch.randn((8, 16), device="cuda")
+    h, kept = ops.checkpoint_activation(x)
+    r = ops.route_tokens(logits, 2)
+    gl = torch.ones((), device="cuda")
+    for call in (lambda: ops.int8_linear(x, w.quantized.tensor, w.scale.tensor), lambda: ops.checkpoint_activation(x), lambda: ops.checkpoint_activation_backward(h, kept),
+                 lambda: ops.route_tokens(logits, 2), lambda: ops.route_tokens_backward(logits, r, r.weights, gl)):
+        for _ in range(3):
+            call()
+        torch.cuda.synchronize()
+        torch.cuda._sleep(2_500_000_000)      # more than a second
+        took = []
+
+        def queue():
+            start = time.perf_counter()
+            for _ in range(3000):
+                call()
+            took.append(time.perf_counter() - start)
+        worker = threading.Thread(target=queue)
+        worker.start()
+        longest, last = 0.0, time.perf_counter()
+        while worker.is_alive():
+            time.sleep(0.002)
+            now = time.perf_counter()
+            longest, last = max(longest, now - last), now
+        worker.join()
+        torch.cuda.synchronize()
+        assert took[0] > 0.8, "the queue did not fill"
+        assert longest < 0.4, f"another thread stood still for {longest:.2f} s"
