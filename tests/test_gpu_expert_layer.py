@@ -504,3 +504,33 @@ def test_tangents_are_refused(cuda_lib):
             torch.func.jvp(call, (logits,), (logits,))
         with pytest.raises((ValueError, RuntimeError)):
             torch.vmap(call)(logits.expand(3, 6, 8))
+
+
+def test_captured_calls_on_a_given_stream(cuda_lib):
+    """Calls on another stream that has joined a capture: their memory belongs to the graph, replays follow their inputs, and
+    eager calls of the same sizes between the replays change nothing."""
+    side = torch.cuda.Stream()
+    x = torch.randn((600, 512), device="cuda").to(BF16)
+    logits = torch.randn((600, 64), device="cuda")
+    w, ws = product_tests.weights((256,), 512, seed=1)
+
+    def calls(s):
+        h, kept = ops.checkpoint_activation(x, stream=s)
+        r = ops.route_tokens(logits, 4, stream=s)
+        return [ops.int8_linear(x, w, ws, stream=s), h, kept.scale, ops.checkpoint_activation_backward(h, kept, stream=s), r.rows, r.weights,
+                ops.route_tokens_backward(logits, r, r.weights, None, stream=s)]
+    calls(None)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        got = calls(side)
+        torch.cuda.current_stream().wait_stream(side)
+    for seed in range(3):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x.copy_(torch.randn((600, 512), device="cuda", generator=g))
+        logits.copy_(torch.randn((600, 64), device="cuda", generator=g))
+        want = calls(None)
+        graph.replay()
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)
