@@ -135,6 +135,7 @@ class _CheckpointedActivation(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         kept = ActivationCheckpoint(*ctx.saved_tensors, *ctx.how)
+        grad = grad.resolve_neg()
         if grad.stride(1) != 1 or (grad.shape[0] > 1 and grad.stride(0) < grad.shape[1]):      # e.g. an expanded gradient
             grad = grad.contiguous()
         return checkpoint_activation_backward(grad, kept), None, None

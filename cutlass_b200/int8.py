@@ -87,11 +87,17 @@ def _no_gradient(name, *tensors) -> None:
     _no_tangent(name, *tensors)
 
 
+def _no_lazy_sign(name, t) -> None:
+    if t.is_neg():
+        raise ValueError(f"{name} is a view with its sign turned, which its memory does not show: pass {name}.resolve_neg()")
+
+
 def _matrix(name, t, kinds):
     """(kind, device index, rows, columns, row pitch) of a row-major CUDA matrix; columns that do not overlap."""
     shape, kind, device = t.shape, kinds.get(t.dtype), t.get_device()
     if len(shape) != 2 or kind is None or device < 0:
         raise ValueError(f"{name} must be a 2-D CUDA tensor of type {', '.join(str(k) for k in kinds)}, got {t.dtype} {tuple(shape)} on {t.device}")
+    _no_lazy_sign(name, t)
     rows, cols = shape
     pitch, step = t.stride()
     if cols < 1 or (step != 1 and cols > 1 and rows > 0) or (rows > 1 and pitch < cols):
@@ -119,6 +125,7 @@ def _check_array(name, t, dtype, shape, device) -> None:
     if t.dtype != dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on CUDA device {device}, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+    _no_lazy_sign(name, t)
 
 
 def _check_rows(rows, device) -> int:

@@ -15,7 +15,7 @@ import torch
 
 from . import lib as L
 from .int8 import _OUT_KINDS as _KINDS
-from .int8 import _check_array, _elsewhere, _launch, _matrix, _no_tangent, _other_stream
+from .int8 import _check_array, _elsewhere, _launch, _matrix, _no_lazy_sign, _no_tangent, _other_stream
 
 MAX_EXPERTS, MAX_TOP_K = 1024, 32
 
@@ -112,6 +112,8 @@ def route_tokens_backward(logits, routing: Routing, grad_weights=None, grad_bala
     if grad_balance_loss is not None and (grad_balance_loss.dtype != torch.float32 or grad_balance_loss.numel() != 1
                                           or grad_balance_loss.get_device() != device):
         raise ValueError(f"grad_balance_loss must be a one-element fp32 tensor on CUDA device {device}")
+    if grad_balance_loss is not None:
+        _no_lazy_sign("grad_balance_loss", grad_balance_loss)
     out = logits.new_empty((T, E))
     pack, call = L.direct("bsg_route_backward", L.ROUTE_LAYOUT)
     args = pack(kind, E, k, routing.normalize, T, logits.data_ptr(), ld, 0, experts.data_ptr(), routing.weights.data_ptr(),
@@ -139,7 +141,7 @@ class _Route(torch.autograd.Function):
         if grad_weights is None and grad_loss is None:
             return None, None, None, None, None
         r = Routing(experts, weights, counts, None, None, None, None, live, softmax, ctx.normalize)
-        grad = route_tokens_backward(logits, r, grad_weights.contiguous() if grad_weights is not None else None, grad_loss)
+        grad = route_tokens_backward(logits, r, None if grad_weights is None else grad_weights.resolve_neg().contiguous(), None if grad_loss is None else grad_loss.resolve_neg())
         return grad, None, None, None, None
 
 

@@ -534,3 +534,24 @@ def test_captured_calls_on_a_given_stream(cuda_lib):
         graph.replay()
         for a, b in zip(want, got):
             assert torch.equal(a, b)
+
+
+def test_views_with_their_sign_turned(cuda_lib):
+    """torch may keep a sign beside a tensor instead of in its memory: such a view is refused as an argument and heeded as a gradient."""
+    neg = torch._neg_view
+    x, logits = torch.randn((6, 64), device="cuda").to(BF16), torch.randn((6, 8), device="cuda")
+    w, ws = product_tests.weights((24,), 64, seed=1)
+    h, kept = ops.checkpoint_activation(x)
+    r = ops.route_tokens(logits, 2)
+    gl = torch.ones((), device="cuda")
+    for call in (lambda: ops.quantize_int8(neg(x)), lambda: ops.int8_linear(neg(x), w, ws), lambda: ops.int8_linear(x, w, neg(ws)), lambda: ops.checkpoint_activation(neg(x)),
+                 lambda: ops.checkpoint_activation_backward(neg(h), kept), lambda: ops.route_tokens(neg(logits), 2), lambda: ops.route_tokens_backward(neg(logits), r, r.weights, gl),
+                 lambda: ops.route_tokens_backward(logits, r, neg(r.weights), gl), lambda: ops.route_tokens_backward(logits, r, r.weights, neg(gl))):
+        with pytest.raises(ValueError, match="sign"):
+            call()
+    up, leaf = x.clone().requires_grad_(), logits.clone().requires_grad_()
+    ops.checkpointed_activation(up).backward(neg(h))
+    assert torch.equal(up.grad, ops.checkpoint_activation_backward(-h, kept))
+    q = ops.route_tokens(leaf, 2)
+    torch.autograd.backward([q.weights, q.balance_loss], [neg(r.weights), neg(gl)])
+    assert torch.equal(leaf.grad, ops.route_tokens_backward(logits, r, -r.weights, -gl))
