@@ -392,10 +392,10 @@ __global__ void __launch_bounds__(WARPS * 32) bsg_route_tokens_kernel(const Rout
   float acc[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.0f;
-  // (no sum passes the number of tokens, which may be 2^31 - 1)
-  const int t0 = blockIdx.x * p.per_block, mine_all = min(p.per_block, p.tokens - t0);
-  const int per_warp = (mine_all + WARPS - 1) / WARPS;
-  const int a = t0 + min(warp * per_warp, mine_all), b = a + min(per_warp, t0 + mine_all - a);
+  // (sums of token numbers, of which there may be 2^31 - 1, are unsigned)
+  const uint32_t all = p.tokens, t0 = min(blockIdx.x * uint32_t(p.per_block), all), t1 = min(t0 + p.per_block, all);
+  const uint32_t per_warp = (t1 - t0 + WARPS - 1) / WARPS;
+  const int a = min(t0 + warp * per_warp, t1), b = min(a + per_warp, t1);
   constexpr bool kAhead = V <= 8;             // the next token's logits are asked for before this one's are used
   int k_lanes = ROUNDS > 0 ? ROUNDS : 1;       // a power of two, at least k
   if constexpr (ROUNDS == 0) {
@@ -703,35 +703,31 @@ __global__ void __launch_bounds__(kRouteThreads) bsg_route_backward_kernel(const
   }
   // what a token needs, asked for one token ahead
   struct Slot { int32_t e; float w, gw; float2 soft; };
-  auto slot_of = [&](int t) {
+  auto slot_of = [&](uint32_t t) {
     Slot s;
     s.e = lane < K ? p.chosen[int64_t(t) * K + lane] : -1;
-    if (s.e >= E) s.e = -1;      // (none that the forward pass writes: an index behind this warp's part of shared memory)
     s.w = lane < K ? p.weights[int64_t(t) * K + lane] : 0.0f;
     s.gw = lane < K && p.grad_weights ? p.grad_weights[int64_t(t) * K + lane] : 0.0f;
     s.soft = p.softmax[t];
     return s;
   };
   constexpr bool kAhead = V <= 8;
-  const int step = int(gridDim.x) * kRouteWarps;
-  int t = blockIdx.x * kRouteWarps + warp;
+  const uint32_t tokens = p.tokens, step = gridDim.x * kRouteWarps;      // (t + step may pass 2^31)
+  uint32_t t = blockIdx.x * kRouteWarps + warp;
   RouteRow<TYPE, V> raw, next;
   Slot slot{}, next_slot{};
-  if (t < p.tokens) {
+  if (t < tokens) {
     route_load<TYPE, V>(raw, p.logits, int64_t(t) * p.ld, lane, E, p.wide != 0);
     slot = slot_of(t);
   }
-  const int before_last = p.tokens - step;      // t < before_last: there is a next token (t + step may pass 2^31)
-  bool more = t < p.tokens;
-  while (more) {
-    more = t < before_last;
+  for (; t < tokens; t += step) {
     if constexpr (kAhead) {
-      if (more) {
+      if (t + step < tokens) {
         route_load<TYPE, V>(next, p.logits, int64_t(t + step) * p.ld, lane, E, p.wide != 0);
         next_slot = slot_of(t + step);
       }
     }
-    const int32_t e = slot.e;
+    const int32_t e = slot.e < E ? slot.e : -1;      // (none behind the experts that the forward pass writes: `part` ends there)
     const float w = e >= 0 ? slot.w : 0.0f, gw = e >= 0 ? slot.gw : 0.0f;
     const float2 soft = slot.soft;
     const bool live = __shfl_sync(0xffffffffu, e, 0) >= 0;
@@ -789,11 +785,10 @@ __global__ void __launch_bounds__(kRouteThreads) bsg_route_backward_kernel(const
     if constexpr (kAhead) {
       raw = next;
       slot = next_slot;
-    } else if (more) {
+    } else if (t + step < tokens) {
       route_load<TYPE, V>(raw, p.logits, int64_t(t + step) * p.ld, lane, E, p.wide != 0);
       slot = slot_of(t + step);
     }
-    if (more) t += step;
   }
 }
 
