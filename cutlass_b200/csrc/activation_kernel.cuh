@@ -10,7 +10,7 @@
 // everything else stays in registers.  Backward there is no such cost, and sixteen lanes with eight values each, whose rows leave
 // 256 bytes at a time, are faster (eight lanes: 1.2 times as long).
 // 8192 x 14336 gated silu, bf16: forward 138 us, backward 137, each 0.95 GB (6.9 TB/s; the issue slots 70 to 74 % taken); gelu
-// 156 and 153.  2051 x 5003 gelu, fp16, rows on any 2-byte boundary, in L2: 19 and 22 us, bound by the instructions (78 and 82 %).
+// 157 and 153.  2051 x 5003 gelu, fp16, rows on any 2-byte boundary, in L2: 19 and 21 us, bound by the instructions (78 and 83 %).
 // h is computed from x itself, not from what is kept.
 #pragma once
 #include <cuda_bf16.h>

@@ -3,7 +3,7 @@
 //   q[m,k] = sign(x) floor(127 |x[m,k]| / a_m + 1/2),  a_m = max_k |x[m,k]|,  sa[m] = a_m / 127
 //   D[m,n] = act(sa[m] * sb[n] * sum_k q[m,k] w[n,k] + bias[n])
 //
-// The sum is a 32-bit integer and exact (K <= 131071: 127 * 127 * K < 2^31), so neither the order of the additions nor
+// The sum is a 32-bit integer and exact (K <= 131071: 127 * 128 * K < 2^31), so neither the order of the additions nor
 // a split of K changes a result.  The kernels:
 //
 //   bsg_i8_quant_kernel   tokens -> 8 bits; bound by HBM (8192 x 8192: 34 us, 5.9 TB/s)

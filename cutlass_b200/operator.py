@@ -69,7 +69,7 @@ class CompiledArtifact:
 
 
 _WORKSPACE_BYTES = 16
-MAX_INT8_K = 131071       # 127 * 127 * K stays below 2^31
+MAX_INT8_K = 131071       # 127 * 128 * K stays below 2^31 (levels up to 127, weights down to -128)
 _default_workspaces: dict[int, torch.Tensor] = {}
 
 
