@@ -178,4 +178,4 @@ def test_other_threads_run_while_a_call_waits(cuda_lib):
         worker.join()
         torch.cuda.synchronize()
         assert took[0] > 0.8, "the queue did not fill"
-        assert longest < 0.4, f"another thread stood still for {longest:.2f} s"
+        assert longest < 0.6, f"another thread stood still for {longest:.2f} s"

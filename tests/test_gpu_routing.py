@@ -283,9 +283,9 @@ def test_expert_counts_around_48_kilobytes_of_shared_memory(cuda_lib, T, E, dtyp
 def test_as_many_tokens_as_31_bits_count(cuda_lib):
     """2^31 - 1 tokens, the largest number that is taken: all but the last 300 have equal logits and choose the first expert."""
     T, n = (1 << 31) - 1, 300
+    torch.cuda.empty_cache()
     if torch.cuda.mem_get_info()[0] < 110 << 30:
         pytest.skip("needs 110 GiB of device memory")
-    torch.cuda.empty_cache()
     logits = torch.zeros((T, 2), dtype=BF16, device="cuda")
     logits[-n:], _ = make(n, 2, BF16, seed=11)
     tail = logits[-n:].double().cpu()
